@@ -467,6 +467,78 @@ int kvq_fp8_pth_decode_attn(const void* query, int dtype, int64_t batch, int64_t
                             int block_index_type, int64_t max_blocks, const int64_t* seq_lens,
                             void* workspace, int64_t workspace_bytes, void* out, void* stream);
 
+/* Causal attention of each request's last query_lens[b] of its seq_lens[b] cached
+ * positions straight over the paged E4M3 codes, K = float(code) * k_scale[token,
+ * head] and V likewise, not rounded to `dtype`; softmax in fp32.  A row at position
+ * p sees j <= p and, with window > 0, of those j > p - window or j < sinks
+ * (window 0: all).  A row that sees nothing gives zeros.
+ *   query [>= sum query_lens, num_heads, D] of `dtype`, its rows query_stride
+ *   elements apart (heads and dims contiguous); out contiguous; rows behind the
+ *   last request's are left alone.  D % 4 == 0, D <= 512, codes on 4-byte bounds.
+ *   Pages nobody sees any more may have any id; others are checked on the host
+ *   (kvq_fp8_pth_window_check) and ids outside the cache read a page inside it.
+ * weights_in / weights_out (both or neither, may be the same array) fp32 [rows,
+ * KVH, weight_cols]: for request b, row weight_rows[b] (host int64, distinct) and
+ * every cached position j,
+ *   weights_out = (j < seq_lens[b] - query_lens[b] ? weights_in : 0)
+ *                 + the sum of its attention weights over the request's rows and
+ *                   the heads of the kv head's group,
+ * positions behind seq_lens[b] and requests without rows untouched.
+ * The lengths (host int64 [batch]) are read during the call and travel with the
+ * launches.  `workspace` holds kvq_fp8_pth_window_attn_workspace_bytes for the
+ * same arguments and device; a smaller one returns KVQ_ERR_INVALID before
+ * anything is launched.  No counterpart in the reference, whose fp8 scheme stops
+ * at the store. */
+int64_t kvq_fp8_pth_window_attn_workspace_bytes(const int64_t* seq_lens, const int64_t* query_lens,
+                                                int64_t batch, int dtype, int num_heads,
+                                                int num_kv_heads, int head_size, int block_size,
+                                                int64_t window, int64_t sinks, int with_weights);
+int kvq_fp8_pth_window_attn(const void* query, int dtype, int64_t query_stride,
+                            const int64_t* seq_lens, const int64_t* query_lens, int64_t batch,
+                            int num_heads, int num_kv_heads, int head_size, float scale,
+                            int64_t window, int64_t sinks, const uint8_t* k_data,
+                            const float* k_scale, const uint8_t* v_data, const float* v_scale,
+                            int64_t num_blocks, int block_size, const void* block_table,
+                            int block_index_type, int64_t max_blocks, const float* weights_in,
+                            float* weights_out, const int64_t* weight_rows, int64_t weight_cols,
+                            void* workspace, int64_t workspace_bytes, void* out, void* stream);
+
+/* Host-side (no GPU call): every page of `block_table` (host, [batch, max_blocks])
+ * that some row of kvq_fp8_pth_window_attn sees lies in [0, num_blocks).  Returns
+ * 0, b + 1 for the first request with one that does not, KVQ_ERR_CAPACITY when the
+ * table does not cover a length, or KVQ_ERR_INVALID. */
+int64_t kvq_fp8_pth_window_check(const void* block_table, int block_index_type, int64_t max_blocks,
+                                 const int64_t* seq_lens, const int64_t* query_lens, int64_t batch,
+                                 int64_t num_blocks, int block_size, int64_t window, int64_t sinks);
+
+/* Eviction by running weight.  A request with seq_lens[b] > keep[b] (host int64)
+ * keeps, per kv head, its first `sinks` rows, its last `recent` and the heaviest of
+ * the rest, keep[b] in all (equal weights: the earliest; NaN is heaviest), in the
+ * order of their positions; other requests keep every row.  Row kept[b, h, r]
+ * becomes row r: codes and scales of both sides within the request's pages, or,
+ * given out_block_table, into those pages; weights (fp32 [rows, KVH, weight_cols],
+ * row weight_rows[b]) into weights_out, which may be weights_in.  kept int32
+ * [batch, KVH, kept_cols], -1 behind a request's rows.  What lies behind the rows
+ * kept stays as it was.  Pages are checked on the host (kvq_fp8_pth_evict_check).
+ * D % 4 == 0, D <= 512, codes on 4-byte bounds.  No counterpart in the reference. */
+int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_data, float* v_scale,
+                      int64_t num_blocks, int block_size, int num_kv_heads, int head_size,
+                      const void* block_table, const void* out_block_table, int block_index_type,
+                      int64_t max_blocks, int64_t out_max_blocks, const int64_t* seq_lens,
+                      const int64_t* keep, int64_t batch, int64_t sinks, int64_t recent,
+                      const float* weights_in, float* weights_out, const int64_t* weight_rows,
+                      int64_t weight_cols, int32_t* kept, int64_t kept_cols, void* stream);
+
+/* Host-side (no GPU call), over the host's copies of the tables: 0 when every live
+ * page lies in [0, num_blocks) and no page whose rows move (in place), or that rows
+ * move to, is any other request's or row's; 2 b + 1 for request b's page outside the
+ * cache, 2 b + 2 for a page of request b in use twice, KVQ_ERR_CAPACITY when a
+ * table does not cover the rows, or KVQ_ERR_INVALID. */
+int64_t kvq_fp8_pth_evict_check(const void* block_table, const void* out_block_table,
+                                int block_index_type, int64_t max_blocks, int64_t out_max_blocks,
+                                const int64_t* seq_lens, const int64_t* keep, int64_t batch,
+                                int64_t num_blocks, int block_size);
+
 /* ---- self-test ---------------------------------------------------------- */
 
 /* One v_mfma_f32_16x16x32_f16 with the operand/result lane mapping the decode

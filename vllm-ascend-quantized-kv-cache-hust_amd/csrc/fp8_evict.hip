@@ -1,0 +1,468 @@
+// SPDX-License-Identifier: Apache-2.0
+// Eviction from the paged E4M3 cache by running attention weight.
+//
+// A request of L cached rows with a budget of `keep` < L keeps, per kv head, its
+// first `sinks` rows, its last `recent` and the keep - sinks - recent heaviest of
+// the rest (of equal weights the earliest), in the order of their positions: row
+// kept[r] becomes row r, in codes, scales and weights.  The cached row of a
+// (token, head) stands by itself (its scale is its own), so heads keep rows of
+// their own.  A request within its budget keeps all.
+//
+// evict_select_kernel: one workgroup per (request, kv head).  The weights' bits
+//   become integers in their order (NaN above all, -0 as 0); three rounds of
+//   histograms over 11, 11 and 10 bits find the threshold (the top 11 bits of a
+//   float, its sign, exponent and two bits of fraction, spread weights of similar
+//   size over many more counters than its top byte would), then each wave counts,
+//   and after one barrier writes, the survivors of a run of positions of its own.
+// evict_move_kernel: a workgroup copies kMoveRows ranks of a request, all kv
+//   heads: their rows lie side by side in the destination pages.
+// evict_compact_kernel: in place.  kept[r] >= r and kept is increasing, so what a
+//   chunk of ranks reads is nothing that an earlier chunk has written; one
+//   workgroup per (request, kv head, side) walks its chunks in order, and within
+//   a chunk every load has returned before the first store.
+#include <vector>
+
+#include "fp8_window.h"
+
+namespace {
+
+using namespace kvq;
+
+struct EvictReq {
+  int32_t len, keep;
+  int32_t table;  // row of both block tables and of kept
+  int32_t wrow;   // row of the running weights
+  int32_t first;  // units of the requests before it
+};
+constexpr int kEvictReqs = 160;
+struct EvictArg {
+  EvictReq r[kEvictReqs];
+};
+
+__device__ __forceinline__ EvictReq evict_req(int count, int unit) {
+  win_cint* a = (win_cint*)__builtin_amdgcn_kernarg_segment_ptr();
+  const int lane = threadIdx.x & 63;
+  int at = 0;
+  for (int c = 0; c < count; c += 64) {
+    const bool on = c + lane < count && a[5 * (c + lane) + 4] <= unit;
+    at += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on));
+  }
+  win_cint* r = a + 5 * __builtin_amdgcn_readfirstlane(at - 1);
+  return EvictReq{r[0], r[1], r[2], r[3], r[4]};
+}
+
+// ---- selection ------------------------------------------------------------------
+
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
+constexpr int kBins = 2048;
+constexpr int kCachedRow = 32768;  // weights of a row that the workgroup keeps in LDS
+
+// Unsigned integers in the order of the weights.
+__device__ __forceinline__ uint32_t weight_key(uint32_t bits) {
+  if ((bits & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;  // NaN
+  if (bits == 0x80000000u) bits = 0;
+  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x, int lane) {  // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t y = __shfl_up(x, d, 64);
+    x += lane >= d ? y : 0;
+  }
+  return x;
+}
+
+// A unit is one kv head of a request.
+__global__ void __launch_bounds__(kSelThreads)
+evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const float* w_in,
+                    float* w_out, int64_t w_cols, int32_t* __restrict__ kept, int64_t kept_cols,
+                    int cached) {
+  extern __shared__ uint32_t s_row[];  // the row's bits, where it fits
+  __shared__ uint32_t s_hist[kBins];
+  __shared__ uint32_t s_wave[2][kSelWaves];
+  __shared__ uint32_t s_found[2];
+  const EvictReq r = evict_req(count, blockIdx.x);
+  const int h = static_cast<int>(blockIdx.x) - r.first;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float* in = w_in + (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
+  float* out = w_out + (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
+  int32_t* ids = kept + (static_cast<int64_t>(r.table) * kvh + h) * kept_cols;
+  const int stay = r.len < r.keep ? r.len : r.keep;
+  for (int64_t k = stay + tid; k < kept_cols; k += kSelThreads) ids[k] = -1;
+  if (r.len <= r.keep) {  // uniform
+    for (int k = tid; k < r.len; k += kSelThreads) {
+      ids[k] = k;
+      if (in != out) out[k] = in[k];
+    }
+    return;
+  }
+  if (cached) {
+    for (int k = tid; k < r.len; k += kSelThreads) s_row[k] = __float_as_uint(in[k]);
+  }
+  auto bits = [&](int k) -> uint32_t { return cached ? s_row[k] : __float_as_uint(in[k]); };
+  const int end = r.len - recent;  // the middle is [sinks, end)
+  uint32_t want = static_cast<uint32_t>(r.keep - sinks - recent);
+  uint32_t prefix = 0, mask = 0;
+  // three rounds: `want` survivors among the keys that agree with prefix on mask
+  if (want > 0) {
+#pragma unroll
+    for (int round = 0; round < 3; ++round) {
+      const int shift = round == 0 ? 21 : (round == 1 ? 10 : 0);
+      const uint32_t field = round == 2 ? 0x3ffu : 0x7ffu;
+      for (int k = tid; k < kBins; k += kSelThreads) s_hist[k] = 0;
+      __syncthreads();
+      for (int k = sinks + tid; k < end; k += kSelThreads) {
+        const uint32_t key = weight_key(bits(k));
+        if ((key & mask) == prefix) atomicAdd(&s_hist[(key >> shift) & field], 1u);
+      }
+      __syncthreads();
+      // thread t: bins 2047 - 2t and 2046 - 2t; keys in the bins above them
+      const uint32_t c0 = s_hist[kBins - 1 - 2 * tid], c1 = s_hist[kBins - 2 - 2 * tid];
+      const uint32_t upto = wave_scan(c0 + c1, lane);
+      if (lane == 63) s_wave[0][wave] = upto;
+      __syncthreads();
+      uint32_t above = upto - (c0 + c1);
+      for (int w = 0; w < wave; ++w) above += s_wave[0][w];
+      if (above < want && want <= above + c0 + c1) {  // one thread
+        const bool upper = want <= above + c0;
+        s_found[0] = static_cast<uint32_t>(kBins - 1 - 2 * tid) - (upper ? 0u : 1u);
+        s_found[1] = want - above - (upper ? 0u : c0);
+      }
+      __syncthreads();
+      prefix |= s_found[0] << shift;
+      mask |= field << shift;
+      want = s_found[1];
+      __syncthreads();  // s_found and s_wave are read before the next round writes them
+    }
+  } else {
+    __syncthreads();  // the row in LDS
+  }
+  const bool some = r.keep - sinks - recent > 0;
+  // keys above `prefix` stay, and the first `want` that equal it
+  const int per = ((end - sinks + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
+  const int begin = sinks + wave * per;
+  const int stop = begin + per < end ? begin + per : end;
+  uint32_t more = 0, same = 0;  // of this wave's run
+  if (some) {
+    for (int k = begin + lane; k - lane < stop; k += 64) {
+      const uint32_t key = k < stop ? weight_key(bits(k)) : 0u;
+      more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k < stop && key > prefix));
+      same += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k < stop && key == prefix));
+    }
+  }
+  if (lane == 0) {
+    s_wave[0][wave] = more;
+    s_wave[1][wave] = same;
+  }
+  __syncthreads();
+  uint32_t more0 = 0, same0 = 0;
+  for (int w = 0; w < wave; ++w) {
+    more0 += s_wave[0][w];
+    same0 += s_wave[1][w];
+  }
+  // `cached`: the weights move from LDS right here
+  auto put = [&](int rank, int k) {
+    ids[rank] = k;
+    if (cached) out[rank] = __uint_as_float(s_row[k]);
+  };
+  if (some) {
+    uint32_t at = sinks + more0 + (same0 < want ? same0 : want);
+    const uint64_t below = (1ull << lane) - 1;
+    for (int k = begin + lane; k - lane < stop; k += 64) {
+      const uint32_t key = k < stop ? weight_key(bits(k)) : 0u;
+      const uint64_t eq = __builtin_amdgcn_ballot_w64(k < stop && key == prefix);
+      const bool take = k < stop && (key > prefix || (key == prefix &&
+                                     same0 + __builtin_popcountll(eq & below) < want));
+      const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
+      if (take) put(static_cast<int>(at) + __builtin_popcountll(taken & below), k);
+      at += __builtin_popcountll(taken);
+      same0 += __builtin_popcountll(eq);
+    }
+  }
+  for (int k = tid; k < sinks; k += kSelThreads) put(k, k);
+  for (int k = tid; k < recent; k += kSelThreads) put(r.keep - recent + k, end + k);
+  if (cached) return;
+  // long rows: through the list just written (this workgroup's), chunk by chunk;
+  // a chunk reads behind everything that the chunks before it have written
+  __syncthreads();
+  for (int k0 = 0; k0 < r.keep; k0 += kSelThreads) {
+    const int k = k0 + tid;
+    float x = 0.0f;
+    if (k < r.keep) x = in[ids[k]];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (k < r.keep) out[k] = x;
+  }
+}
+
+// ---- moving the rows ----------------------------------------------------------------
+
+struct EvictCache {
+  uint8_t *kd, *vd;
+  float *ks, *vs;
+  const void *src, *dst;  // block tables
+  int64_t src_cols, dst_cols, nb;
+  FastDiv bs, kvh;
+  int bt64, d;
+  __device__ __forceinline__ int64_t slot(const void* table, int64_t cols, int row, int p) const {
+    const uint32_t i = bs.div(static_cast<uint32_t>(p));
+    const int64_t at = static_cast<int64_t>(row) * cols + i;
+    const int64_t b = bt64 ? static_cast<const int64_t*>(table)[at]
+                           : static_cast<int64_t>(static_cast<const int32_t*>(table)[at]);
+    const int64_t page = b < 0 ? 0 : (b >= nb ? nb - 1 : b);  // live ids are checked on the host
+    return page * bs.d + (static_cast<uint32_t>(p) - i * bs.d);
+  }
+};
+
+constexpr int kMoveRows = 32;  // ranks of a workgroup
+
+// W: the words a row moves in.  A unit is kMoveRows ranks.
+template <typename W>
+__global__ void __launch_bounds__(256)
+evict_move_kernel(EvictArg, int count, EvictCache c, const int32_t* __restrict__ kept,
+                  int64_t kept_cols, FastDiv pieces) {
+  const EvictReq r = evict_req(count, blockIdx.x);
+  const int rank0 = (static_cast<int>(blockIdx.x) - r.first) * kMoveRows;
+  const int stay = r.len < r.keep ? r.len : r.keep;
+  const int ranks = stay - rank0 < kMoveRows ? stay - rank0 : kMoveRows;
+  const int kvh = static_cast<int>(c.kvh.d), rows = ranks * kvh;
+  // row x of this unit: rank rank0 + x / kvh, head x % kvh
+  auto source = [&](int x, int& rank, int& h) -> int64_t {
+    const int k = static_cast<int>(c.kvh.div(static_cast<uint32_t>(x)));
+    h = x - k * kvh;
+    rank = rank0 + k;
+    const int p = kept[(static_cast<int64_t>(r.table) * kvh + h) * kept_cols + rank];
+    return c.slot(c.src, c.src_cols, r.table, p) * kvh + h;
+  };
+  const int total = rows * static_cast<int>(pieces.d);
+  for (int e = threadIdx.x; e < total; e += 256) {
+    const int x = static_cast<int>(pieces.div(static_cast<uint32_t>(e)));
+    const int w = e - x * static_cast<int>(pieces.d);
+    int rank, h;
+    const int64_t from = source(x, rank, h);
+    const int64_t to = c.slot(c.dst, c.dst_cols, r.table, rank) * kvh + h;
+    const W a = reinterpret_cast<const W*>(c.kd + from * c.d)[w];
+    const W b = reinterpret_cast<const W*>(c.vd + from * c.d)[w];
+    reinterpret_cast<W*>(c.kd + to * c.d)[w] = a;
+    reinterpret_cast<W*>(c.vd + to * c.d)[w] = b;
+    if (w == 0) {
+      const float s = c.ks[from], t = c.vs[from];
+      c.ks[to] = s;
+      c.vs[to] = t;
+    }
+  }
+}
+
+constexpr int kCompactThreads = 1024;
+constexpr int kCompactDepth = 4;  // words in flight per thread
+
+// In place.  A unit is one side of one kv head.
+template <typename W>
+__global__ void __launch_bounds__(kCompactThreads)
+evict_compact_kernel(EvictArg, int count, EvictCache c, const int32_t* __restrict__ kept,
+                     int64_t kept_cols, FastDiv pieces, int sinks) {
+  const EvictReq r = evict_req(count, blockIdx.x);
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int kvh = static_cast<int>(c.kvh.d);
+  const int h = u >> 1;
+  uint8_t* data = u & 1 ? c.vd : c.kd;
+  float* scale = u & 1 ? c.vs : c.ks;
+  const int32_t* ids = kept + (static_cast<int64_t>(r.table) * kvh + h) * kept_cols;
+  const int64_t total = static_cast<int64_t>(r.keep) * pieces.d;  // words, < 2^31 (host)
+  for (int64_t e0 = static_cast<int64_t>(sinks) * pieces.d; e0 < total;
+       e0 += kCompactThreads * kCompactDepth) {
+    W word[kCompactDepth];
+    float s[kCompactDepth];
+    int64_t to[kCompactDepth];
+    int part[kCompactDepth];
+#pragma unroll
+    for (int k = 0; k < kCompactDepth; ++k) {
+      const int64_t e = e0 + k * kCompactThreads + threadIdx.x;
+      to[k] = -1;
+      if (e < total) {
+        const int rank = static_cast<int>(pieces.div(static_cast<uint32_t>(e)));
+        part[k] = static_cast<int>(e) - rank * static_cast<int>(pieces.d);
+        const int p = ids[rank];
+        if (p != rank) {
+          const int64_t from = c.slot(c.src, c.src_cols, r.table, p) * kvh + h;
+          to[k] = c.slot(c.src, c.src_cols, r.table, rank) * kvh + h;
+          word[k] = reinterpret_cast<const W*>(data + from * c.d)[part[k]];
+          if (part[k] == 0) s[k] = scale[from];
+        }
+      }
+    }
+    // every load of the chunk has returned before any of its rows is overwritten
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kCompactDepth; ++k) {
+      if (to[k] >= 0) {
+        reinterpret_cast<W*>(data + to[k] * c.d)[part[k]] = word[k];
+        if (part[k] == 0) scale[to[k]] = s[k];
+      }
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------
+
+template <typename U, typename G>
+int for_requests(const int64_t* lens, const int64_t* keeps, const int64_t* rows, int64_t batch,
+                 U&& units, G&& go) {
+  EvictArg arg;
+  int count = 0;
+  int64_t total = 0, longest = 0;
+  for (int64_t b = 0; b <= batch; ++b) {
+    if (count == kEvictReqs || (b == batch && count)) {
+      const int rc = go(arg, count, static_cast<unsigned>(total), longest);
+      if (rc != KVQ_OK) return rc;
+      count = 0;
+      total = longest = 0;
+    }
+    if (b == batch) break;
+    const int64_t u = units(b);
+    if (u <= 0) continue;
+    if (total + u > 0x7fffffff) return KVQ_ERR_INVALID;
+    arg.r[count++] = EvictReq{static_cast<int32_t>(lens[b]), static_cast<int32_t>(keeps[b]),
+                              static_cast<int32_t>(b), static_cast<int32_t>(rows[b]),
+                              static_cast<int32_t>(total)};
+    total += u;
+    longest = lens[b] > keeps[b] && lens[b] > longest ? lens[b] : longest;
+  }
+  return KVQ_OK;
+}
+
+int64_t table_id(const void* table, int type, int64_t at) {
+  return type == KVQ_INDEX_I64 ? static_cast<const int64_t*>(table)[at]
+                               : static_cast<const int32_t*>(table)[at];
+}
+
+}  // namespace
+
+extern "C" int64_t kvq_fp8_pth_evict_check(const void* block_table, const void* out_block_table,
+                                           int block_index_type, int64_t max_blocks,
+                                           int64_t out_max_blocks, const int64_t* seq_lens,
+                                           const int64_t* keep, int64_t batch, int64_t num_blocks,
+                                           int block_size) {
+  if (batch < 0 || block_size <= 0 || num_blocks <= 0 || max_blocks < 0 || out_max_blocks < 0 ||
+      (batch > 0 && (!block_table || !seq_lens || !keep)) ||
+      (block_index_type != KVQ_INDEX_I32 && block_index_type != KVQ_INDEX_I64))
+    return KVQ_ERR_INVALID;
+  // 1: a page of some request's rows, 2: of one whose rows move within it (or a
+  // page that rows move to)
+  std::vector<uint8_t> seen(static_cast<size_t>(num_blocks), 0);
+  for (int64_t b = 0; b < batch; ++b) {
+    if (seq_lens[b] < 0 || keep[b] < 0) return KVQ_ERR_INVALID;
+    if (seq_lens[b] > max_blocks * block_size) return KVQ_ERR_CAPACITY;
+    const bool moves = !out_block_table && seq_lens[b] > keep[b];
+    for (int64_t i = 0; i < (seq_lens[b] + block_size - 1) / block_size; ++i) {
+      const int64_t id = table_id(block_table, block_index_type, b * max_blocks + i);
+      if (id < 0 || id >= num_blocks) return 2 * b + 1;
+      if (seen[id] == 2 || (moves && seen[id])) return 2 * b + 2;
+      seen[id] = moves ? 2 : 1;
+    }
+  }
+  if (!out_block_table) return KVQ_OK;
+  for (int64_t b = 0; b < batch; ++b) {
+    const int64_t stay = seq_lens[b] < keep[b] ? seq_lens[b] : keep[b];
+    if (stay > out_max_blocks * block_size) return KVQ_ERR_CAPACITY;
+    for (int64_t i = 0; i < (stay + block_size - 1) / block_size; ++i) {
+      const int64_t id = table_id(out_block_table, block_index_type, b * out_max_blocks + i);
+      if (id < 0 || id >= num_blocks) return 2 * b + 1;
+      if (seen[id]) return 2 * b + 2;
+      seen[id] = 2;
+    }
+  }
+  return KVQ_OK;
+}
+
+extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_data, float* v_scale,
+                                 int64_t num_blocks, int block_size, int num_kv_heads,
+                                 int head_size, const void* block_table,
+                                 const void* out_block_table, int block_index_type,
+                                 int64_t max_blocks, int64_t out_max_blocks,
+                                 const int64_t* seq_lens, const int64_t* keep, int64_t batch,
+                                 int64_t sinks, int64_t recent, const float* weights_in,
+                                 float* weights_out, const int64_t* weight_rows,
+                                 int64_t weight_cols, int32_t* kept, int64_t kept_cols,
+                                 void* stream) {
+  if (batch == 0) return KVQ_OK;
+  if (!k_data || !k_scale || !v_data || !v_scale || !block_table || !seq_lens || !keep ||
+      !weights_in || !weights_out || !weight_rows || !kept || batch < 0 || num_blocks <= 0 ||
+      block_size <= 0 || sinks < 0 || recent < 0 || max_blocks < 0 || out_max_blocks < 0 ||
+      (block_index_type != KVQ_INDEX_I32 && block_index_type != KVQ_INDEX_I64))
+    return KVQ_ERR_INVALID;
+  if (num_kv_heads <= 0 || head_size <= 0 || head_size % 4 || head_size > 512)
+    return KVQ_ERR_GEOMETRY;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(k_data) | reinterpret_cast<uintptr_t>(v_data);
+  if (bits & 3) return KVQ_ERR_GEOMETRY;
+  const bool wide = head_size % 16 == 0 && (bits & 15) == 0;
+  const int pieces = head_size / (wide ? 16 : 4);
+  for (int64_t b = 0; b < batch; ++b) {
+    const int64_t len = seq_lens[b], stay = len < keep[b] ? len : keep[b];
+    if (len < 0 || len > kMaxPositions || keep[b] < 0 || keep[b] > kMaxPositions ||
+        len > max_blocks * block_size || len > weight_cols || stay > kept_cols ||
+        weight_rows[b] < 0 || weight_rows[b] > kMaxPositions ||
+        (out_block_table && stay > out_max_blocks * block_size))
+      return KVQ_ERR_INVALID;
+    if (len > keep[b] && (sinks + recent > keep[b] || keep[b] * pieces > 0x7fffffff))
+      return KVQ_ERR_INVALID;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const EvictCache c{k_data, v_data, k_scale, v_scale, block_table,
+                     out_block_table ? out_block_table : block_table, max_blocks,
+                     out_block_table ? out_max_blocks : max_blocks, num_blocks,
+                     FastDiv::make(static_cast<uint32_t>(block_size)),
+                     FastDiv::make(static_cast<uint32_t>(num_kv_heads)),
+                     block_index_type == KVQ_INDEX_I64, head_size};
+  const FastDiv piece_div = FastDiv::make(static_cast<uint32_t>(pieces));
+  int64_t lds_max = 0;
+  const int lrc = device_lds_max(&lds_max);
+  if (lrc != KVQ_OK) return lrc;
+  int rc = for_requests(
+      seq_lens, keep, weight_rows, batch, [&](int64_t) { return num_kv_heads; },
+      [&](const EvictArg& arg, int count, unsigned blocks, int64_t longest) -> int {
+        const int64_t row_bytes = (4 * longest + 15) / 16 * 16;
+        const int cached = longest <= kCachedRow && row_bytes + 16384 <= lds_max;
+        hipLaunchKernelGGL(evict_select_kernel, dim3(blocks), dim3(kSelThreads),
+                           cached ? static_cast<unsigned>(row_bytes) : 0u, s, arg, count,
+                           num_kv_heads, static_cast<int>(sinks), static_cast<int>(recent),
+                           weights_in, weights_out, weight_cols, kept, kept_cols, cached);
+        KVQ_LAUNCH_CHECK();
+        return KVQ_OK;
+      });
+  if (rc != KVQ_OK) return rc;
+  if (out_block_table) {
+    return for_requests(
+        seq_lens, keep, weight_rows, batch,
+        [&](int64_t b) {
+          return ((seq_lens[b] < keep[b] ? seq_lens[b] : keep[b]) + kMoveRows - 1) / kMoveRows;
+        },
+        [&](const EvictArg& arg, int count, unsigned blocks, int64_t) -> int {
+          if (wide)
+            hipLaunchKernelGGL((evict_move_kernel<uint4>), dim3(blocks), dim3(256), 0, s, arg,
+                               count, c, kept, kept_cols, piece_div);
+          else
+            hipLaunchKernelGGL((evict_move_kernel<uint32_t>), dim3(blocks), dim3(256), 0, s, arg,
+                               count, c, kept, kept_cols, piece_div);
+          KVQ_LAUNCH_CHECK();
+          return KVQ_OK;
+        });
+  }
+  return for_requests(
+      seq_lens, keep, weight_rows, batch,
+      [&](int64_t b) { return seq_lens[b] > keep[b] ? 2 * static_cast<int64_t>(num_kv_heads) : 0; },
+      [&](const EvictArg& arg, int count, unsigned blocks, int64_t) -> int {
+        if (wide)
+          hipLaunchKernelGGL((evict_compact_kernel<uint4>), dim3(blocks), dim3(kCompactThreads), 0,
+                             s, arg, count, c, kept, kept_cols, piece_div,
+                             static_cast<int>(sinks));
+        else
+          hipLaunchKernelGGL((evict_compact_kernel<uint32_t>), dim3(blocks), dim3(kCompactThreads),
+                             0, s, arg, count, c, kept, kept_cols, piece_div,
+                             static_cast<int>(sinks));
+        KVQ_LAUNCH_CHECK();
+        return KVQ_OK;
+      });
+}

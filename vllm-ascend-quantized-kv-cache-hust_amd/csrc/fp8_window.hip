@@ -1,0 +1,354 @@
+// SPDX-License-Identifier: Apache-2.0
+// Causal attention of each request's new rows straight over its paged E4M3
+// rows, with an optional sliding window and sinks, and the running attention
+// weights of the cached positions: the entry points, and the kernels that take
+// any geometry (fp32 queries, any head size the cache has, any page size).
+//
+// K_j = code_k[j] * k_scale[j], V_j = code_v[j] * v_scale[j] per (token, kv head)
+// (the values of pkg/methods/fp8_per_token_head/semantics.py:63-65, not rounded
+// to the query's type), p_ij = softmax over the positions row i sees, out_i =
+// sum_j p_ij V_j.  A row that sees nothing gives zeros.  The running weights:
+// w_j = (j < len - n ? w_j : 0) + sum over the rows i and the heads of the kv
+// head's group of p_ij.
+//
+// The general kernels: one wave per (row, head), 64 positions at a time, a lane
+// a position for the scores and a word of the row for the values, all in fp32
+// with the softmax's running maximum and sum; bound by their lanes' 4-byte loads
+// and by reading each code once per query head.
+#include <vector>
+
+#include "fp8_window.h"
+
+namespace {
+
+using namespace kvq;
+
+__device__ __forceinline__ void codes4(uint32_t w, float (&x)[4]) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
+  x[0] = lo[0];
+  x[1] = lo[1];
+  x[2] = hi[0];
+  x[3] = hi[1];
+}
+
+constexpr int kGenWaves = 4;
+constexpr int kGenMaxD = 512;
+
+// fp32 dot product of the query row in LDS with a row of codes.
+__device__ __forceinline__ float dot_codes(const float* q, const uint8_t* row, int d) {
+  float s = 0.0f;
+  for (int i = 0; i < d; i += 4) {
+    float x[4];
+    codes4(*reinterpret_cast<const uint32_t*>(row + i), x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s = __builtin_fmaf(q[i + k], x[k], s);
+  }
+  return s;
+}
+
+// A unit is one row and kGenWaves heads.
+template <typename T>
+__global__ void __launch_bounds__(64 * kGenWaves)
+win_attn_general_kernel(WinArg, int count, WinCache c, const T* __restrict__ query,
+                        int64_t q_stride, float qscale, T* __restrict__ out,
+                        float* __restrict__ lse) {
+  __shared__ float s_q[kGenWaves][kGenMaxD];
+  const WinReq r = win_req(count, blockIdx.x);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int groups = (c.hq + kGenWaves - 1) / kGenWaves;
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int i = u / groups, head = (u - i * groups) * kGenWaves + wave;
+  if (head >= c.hq) return;  // no barrier below: a wave reads its own part of s_q
+  const int h = static_cast<int>(c.rep.div(static_cast<uint32_t>(head)));
+  const int pos = r.len - r.n + i;
+  const int64_t row = static_cast<int64_t>(r.q0) + i;
+  const T* q = query + row * q_stride + static_cast<int64_t>(head) * c.d;
+  for (int k = lane; k < c.d; k += 64) s_q[wave][k] = to_f32(q[k]);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  float m = -INFINITY, l = 0.0f, acc[2][4] = {};
+  const WinSpan span = pos >= 0 ? WinSpan::of(pos + 1, 1, c.window, c.sinks, 64) : WinSpan{0, 0, 0};
+  for (int g = 0; g < span.groups; ++g) {
+    const int j = span.pos(g, 64) + lane;
+    const bool on = c.sees(pos, j);
+    const int64_t at = (on ? c.slot(r.table, j) : 0) * c.kvh + h;
+    float s = -INFINITY;
+    if (on) s = dot_codes(s_q[wave], c.kd + at * c.d, c.d) * (c.ks[at] * qscale);
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(on);
+    if (!mask) continue;
+    const float top = fmaxf(m, max_wave64(s));
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - base);
+    const float p = on ? __builtin_amdgcn_exp2f(s - base) : 0.0f;
+    m = top;
+    l = l * alpha + sum_wave64(p);
+    const float pv = on ? p * c.vs[at] : 0.0f;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[w][k] *= alpha;
+    for (uint64_t left = mask; left; left &= left - 1) {
+      const int t = __builtin_ctzll(left);
+      const float pt = __shfl(pv, t, 64);
+      const int64_t src = __shfl(at, t, 64);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int col = 4 * (lane + 64 * w);
+        if (col < c.d) {
+          float x[4];
+          codes4(*reinterpret_cast<const uint32_t*>(c.vd + src * c.d + col), x);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[w][k] = __builtin_fmaf(pt, x[k], acc[w][k]);
+        }
+      }
+    }
+  }
+  T* o = out + (row * c.hq + head) * c.d;
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int col = 4 * (lane + 64 * w) + k;
+      // l is 0 only where nothing is seen; a NaN goes through
+      if (col < c.d) o[col] = from_f32<T>(l == 0.0f ? 0.0f : acc[w][k] / l);
+    }
+  // (max, sum) in one number: p = 2^(s - lse)
+  if (lse && lane == 0) lse[row * c.hq + head] = l == 0.0f ? INFINITY : m + __log2f(l);
+}
+
+// Running weights, a thread a position.  A unit is 256 positions of one kv head.
+template <typename T>
+__global__ void __launch_bounds__(256)
+win_weights_general_kernel(WinArg, int count, WinCache c, const T* __restrict__ query,
+                           int64_t q_stride, float qscale, const float* __restrict__ lse,
+                           const float* w_in, float* w_out, int64_t w_cols) {
+  const WinReq r = win_req(count, blockIdx.x);
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int h = u % c.kvh, j0 = u / c.kvh * 256;
+  const int j = j0 + static_cast<int>(threadIdx.x);
+  if (j >= r.len) return;  // no barrier below
+  const int first = r.len - r.n;  // position of row 0
+  const int rep = static_cast<int>(c.rep.d);
+  const int64_t at = c.slot(r.table, j) * c.kvh + h;
+  const uint8_t* key = c.kd + at * c.d;
+  const float scale = c.ks[at] * qscale;
+  float sum = 0.0f;
+  for (int i = j0 > first ? j0 - first : 0; i < r.n; ++i) {
+    if (!c.sees(first + i, j)) continue;
+    const int64_t row = static_cast<int64_t>(r.q0) + i;
+    for (int k = 0; k < rep; ++k) {
+      const int head = h * rep + k;
+      const T* q = query + row * q_stride + static_cast<int64_t>(head) * c.d;
+      float s = 0.0f;
+      for (int e = 0; e < c.d; e += 4) {
+        float x[4];
+        codes4(*reinterpret_cast<const uint32_t*>(key + e), x);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s = __builtin_fmaf(to_f32(q[e + t]), x[t], s);
+      }
+      sum += __builtin_amdgcn_exp2f(s * scale - lse[row * c.hq + head]);
+    }
+  }
+  const int64_t dst = (static_cast<int64_t>(r.wrow) * c.kvh + h) * w_cols + j;
+  w_out[dst] = (j < first ? w_in[dst] : 0.0f) + sum;
+}
+
+// ---- host -----------------------------------------------------------------------
+
+struct Call {
+  const void* query;
+  int dtype;
+  int64_t q_stride;
+  const int64_t *lens, *qlens;
+  int64_t batch;
+  WinCache cache;
+  float qscale;
+  const float* w_in;
+  float* w_out;
+  const int64_t* w_rows;
+  int64_t w_cols;
+  void* out;
+  hipStream_t stream;
+};
+
+// Launches over the requests, kWinReqs at a time: units(b) gives a request's
+// workgroups, go(arg, requests, workgroups) launches them.
+template <typename U, typename G>
+int for_requests(const Call& call, U&& units, G&& go) {
+  WinArg arg;
+  int count = 0;
+  int64_t total = 0, q0 = 0;
+  for (int64_t b = 0; b <= call.batch; ++b) {
+    if (count == kWinReqs || (b == call.batch && count)) {
+      if (total > 0) {
+        const int rc = go(arg, count, static_cast<unsigned>(total));
+        if (rc != KVQ_OK) return rc;
+      }
+      count = 0;
+      total = 0;
+    }
+    if (b == call.batch) break;
+    const int64_t u = units(b);
+    if (u > 0) {
+      if (total + u > 0x7fffffff) return KVQ_ERR_INVALID;
+      arg.r[count++] = WinReq{static_cast<int32_t>(q0), static_cast<int32_t>(call.qlens[b]),
+                              static_cast<int32_t>(call.lens[b]), static_cast<int32_t>(b),
+                              static_cast<int32_t>(total), 1, 0,
+                              static_cast<int32_t>(call.w_rows ? call.w_rows[b] : 0)};
+      total += u;
+    }
+    q0 += call.qlens[b];
+  }
+  return KVQ_OK;
+}
+
+template <typename T>
+int attend_general(const Call& call, float* lse) {
+  const int64_t groups = (call.cache.hq + kGenWaves - 1) / kGenWaves;
+  return for_requests(
+      call, [&](int64_t b) { return call.qlens[b] * groups; },
+      [&](const WinArg& arg, int count, unsigned blocks) -> int {
+        hipLaunchKernelGGL((win_attn_general_kernel<T>), dim3(blocks), dim3(64 * kGenWaves), 0,
+                           call.stream, arg, count, call.cache,
+                           static_cast<const T*>(call.query), call.q_stride, call.qscale,
+                           static_cast<T*>(call.out), lse);
+        KVQ_LAUNCH_CHECK();
+        return KVQ_OK;
+      });
+}
+
+template <typename T>
+int weigh_general(const Call& call, const float* lse) {
+  return for_requests(
+      call,
+      [&](int64_t b) {
+        return call.qlens[b] > 0 ? (call.lens[b] + 255) / 256 * call.cache.kvh : 0;
+      },
+      [&](const WinArg& arg, int count, unsigned blocks) -> int {
+        hipLaunchKernelGGL((win_weights_general_kernel<T>), dim3(blocks), dim3(256), 0, call.stream,
+                           arg, count, call.cache, static_cast<const T*>(call.query),
+                           call.q_stride, call.qscale, lse, call.w_in, call.w_out, call.w_cols);
+        KVQ_LAUNCH_CHECK();
+        return KVQ_OK;
+      });
+}
+
+// Lengths, window and geometry, checked alike by the sizing call and the call.
+int check_shape(const int64_t* lens, const int64_t* qlens, int64_t batch, int dtype, int hq, int kvh,
+                int d, int bs, int64_t window, int64_t sinks) {
+  if (batch < 0 || (batch > 0 && (!lens || !qlens)) || window < 0 || sinks < 0)
+    return KVQ_ERR_INVALID;
+  if (dtype != KVQ_DTYPE_F32 && dtype != KVQ_DTYPE_F16 && dtype != KVQ_DTYPE_BF16)
+    return KVQ_ERR_INVALID;
+  if (kvh <= 0 || hq <= 0 || hq % kvh || d <= 0 || d % 4 || d > kGenMaxD || bs <= 0 || hq > 65536)
+    return KVQ_ERR_GEOMETRY;
+  int64_t rows = 0;
+  for (int64_t b = 0; b < batch; ++b) {
+    if (lens[b] < 0 || lens[b] > kMaxPositions || qlens[b] < 0 || qlens[b] > kMaxPositions)
+      return KVQ_ERR_INVALID;
+    rows += qlens[b];
+    if (rows > kMaxPositions / hq) return KVQ_ERR_INVALID;
+  }
+  return KVQ_OK;
+}
+
+int64_t lse_bytes(const int64_t* qlens, int64_t batch, int hq) {
+  int64_t rows = 0;
+  for (int64_t b = 0; b < batch; ++b) rows += qlens[b];
+  return (4 * rows * hq + 15) / 16 * 16;
+}
+
+}  // namespace
+
+extern "C" int64_t kvq_fp8_pth_window_attn_workspace_bytes(
+    const int64_t* seq_lens, const int64_t* query_lens, int64_t batch, int dtype, int num_heads,
+    int num_kv_heads, int head_size, int block_size, int64_t window, int64_t sinks,
+    int with_weights) {
+  const int rc = check_shape(seq_lens, query_lens, batch, dtype, num_heads, num_kv_heads, head_size,
+                             block_size, window, sinks);
+  if (rc != KVQ_OK) return rc;
+  return with_weights ? lse_bytes(query_lens, batch, num_heads) : 0;
+}
+
+extern "C" int kvq_fp8_pth_window_attn(
+    const void* query, int dtype, int64_t query_stride, const int64_t* seq_lens,
+    const int64_t* query_lens, int64_t batch, int num_heads, int num_kv_heads, int head_size,
+    float scale, int64_t window, int64_t sinks, const uint8_t* k_data, const float* k_scale,
+    const uint8_t* v_data, const float* v_scale, int64_t num_blocks, int block_size,
+    const void* block_table, int block_index_type, int64_t max_blocks, const float* weights_in,
+    float* weights_out, const int64_t* weight_rows, int64_t weight_cols, void* workspace,
+    int64_t workspace_bytes, void* out, void* stream) {
+  const int rc = check_shape(seq_lens, query_lens, batch, dtype, num_heads, num_kv_heads, head_size,
+                             block_size, window, sinks);
+  if (rc != KVQ_OK) return rc;
+  int64_t rows = 0;
+  for (int64_t b = 0; b < batch; ++b) rows += query_lens[b];
+  if (rows == 0) return KVQ_OK;
+  if (!query || !k_data || !k_scale || !v_data || !v_scale || !block_table || !out ||
+      num_blocks <= 0 || max_blocks < 0 || !(scale > 0.0f) ||
+      query_stride < static_cast<int64_t>(num_heads) * head_size)
+    return KVQ_ERR_INVALID;
+  if (block_index_type != KVQ_INDEX_I32 && block_index_type != KVQ_INDEX_I64)
+    return KVQ_ERR_INVALID;
+  if ((reinterpret_cast<uintptr_t>(k_data) | reinterpret_cast<uintptr_t>(v_data)) & 3)
+    return KVQ_ERR_GEOMETRY;  // a row's words
+  const bool weigh = weights_out != nullptr;
+  if (weigh != (weights_in != nullptr) || (weigh && !weight_rows)) return KVQ_ERR_INVALID;
+  for (int64_t b = 0; b < batch; ++b) {
+    if (query_lens[b] == 0) continue;
+    if (seq_lens[b] > max_blocks * block_size) return KVQ_ERR_INVALID;
+    if (weigh && (seq_lens[b] > weight_cols || weight_rows[b] < 0 || weight_rows[b] > kMaxPositions))
+      return KVQ_ERR_INVALID;
+  }
+  const int64_t need = weigh ? lse_bytes(query_lens, batch, num_heads) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return KVQ_ERR_INVALID;
+  Call call{query, dtype, query_stride, seq_lens, query_lens, batch,
+            WinCache{k_data, k_scale, v_data, v_scale, block_table, max_blocks, num_blocks,
+                     FastDiv::make(static_cast<uint32_t>(block_size)),
+                     block_index_type == KVQ_INDEX_I64, num_kv_heads, num_heads, head_size,
+                     FastDiv::make(static_cast<uint32_t>(num_heads / num_kv_heads)),
+                     window > 0 && window < kNoWindow ? static_cast<int>(window) : kNoWindow,
+                     static_cast<int>(window > 0 ? (sinks < kMaxPositions ? sinks : kMaxPositions) : 0)},
+            scale * 1.4426950408889634f, weights_in, weights_out, weight_rows, weight_cols, out,
+            static_cast<hipStream_t>(stream)};
+  float* lse = weigh ? static_cast<float*>(workspace) : nullptr;
+  KVQ_DISPATCH_FLOAT(dtype, T, {
+    int r = attend_general<T>(call, lse);
+    if (r != KVQ_OK) return r;
+    if (weigh) r = weigh_general<T>(call, lse);
+    if (r != KVQ_OK) return r;
+  });
+  return KVQ_OK;
+}
+
+// ---- host checks ------------------------------------------------------------------
+
+extern "C" int64_t kvq_fp8_pth_window_check(const void* block_table, int block_index_type,
+                                            int64_t max_blocks, const int64_t* seq_lens,
+                                            const int64_t* query_lens, int64_t batch,
+                                            int64_t num_blocks, int block_size, int64_t window,
+                                            int64_t sinks) {
+  if (batch < 0 || block_size <= 0 || max_blocks < 0 || (batch > 0 && (!seq_lens || !query_lens)))
+    return KVQ_ERR_INVALID;
+  for (int64_t b = 0; b < batch; ++b) {
+    const int64_t len = seq_lens[b], n = query_lens[b];
+    if (len < 0 || n < 0) return KVQ_ERR_INVALID;
+    if (n == 0 || len == 0) continue;
+    if (len > max_blocks * block_size) return KVQ_ERR_CAPACITY;
+    int64_t low = window > 0 ? len - n - window + 1 : 0;
+    low = low < 0 ? 0 : low;
+    const int64_t sink = window > 0 ? (sinks < low ? sinks : low) : 0;
+    const int64_t sink_pages = (sink + block_size - 1) / block_size;
+    for (int64_t i = 0; i < (len + block_size - 1) / block_size; ++i) {
+      if (i >= sink_pages && (i + 1) * block_size <= low) continue;  // nobody sees it
+      const int64_t at = b * max_blocks + i;
+      const int64_t id = block_index_type == KVQ_INDEX_I64
+                             ? static_cast<const int64_t*>(block_table)[at]
+                             : static_cast<const int32_t*>(block_table)[at];
+      if (id < 0 || id >= num_blocks) return b + 1;
+    }
+  }
+  return KVQ_OK;
+}
