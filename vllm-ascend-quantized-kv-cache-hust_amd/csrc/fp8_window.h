@@ -104,4 +104,165 @@ struct WinSpan {
   }
 };
 
+// ---- operands of the matrix kernels ------------------------------------------------
+typedef float w_f4 __attribute__((ext_vector_type(4)));
+typedef float w_f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t w_u4 __attribute__((ext_vector_type(4)));
+typedef _Float16 w_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 w_h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 w_b8 __attribute__((ext_vector_type(8)));
+
+// Codes (bytes 0, 1 or 2, 3 of x) as a pair of T, exact (NaN codes give NaN).
+template <bool HI>
+__device__ __forceinline__ uint32_t code_pair(uint32_t x, bf16) {
+  return __builtin_bit_cast(
+      uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(x), 1.0f, HI));
+}
+template <bool HI>
+__device__ __forceinline__ uint32_t code_pair(uint32_t x, f16) {
+  return __builtin_bit_cast(
+      uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(x), 1.0f, HI));
+}
+template <typename T>
+__device__ __forceinline__ w_u4 code_op8(uint32_t w0, uint32_t w1) {
+  return w_u4{code_pair<false>(w0, T{}), code_pair<true>(w0, T{}), code_pair<false>(w1, T{}),
+              code_pair<true>(w1, T{})};
+}
+// 0x80 in every byte of x that is a NaN code.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t x) {
+  return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// Two fp32 values as a pair of T (round to nearest even).
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi, bf16) { return bf16x2_bits(lo, hi); }
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi, f16) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((w_f2{lo, hi}), w_h2));
+}
+
+__device__ __forceinline__ w_f4 mfma_op(w_u4 a, w_u4 b, w_f4 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(w_b8, a),
+                                                 __builtin_bit_cast(w_b8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ w_f4 mfma_op(w_u4 a, w_u4 b, w_f4 c, f16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(w_h8, a),
+                                                __builtin_bit_cast(w_h8, b), c, 0, 0, 0);
+}
+
+// Eight consecutive 16-bit elements; `wide` (uniform): on a 16-byte bound.
+template <typename T>
+__device__ __forceinline__ w_u4 load_op8(const T* p, bool wide) {
+  if (wide) return *reinterpret_cast<const w_u4*>(p);
+  w_u4 r;
+  const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = static_cast<uint32_t>(e[2 * i]) | (static_cast<uint32_t>(e[2 * i + 1]) << 16);
+  return r;
+}
+
+// LDS DMA of 16 (4) bytes a lane from base + off (base uniform) to LDS bytes m0 + 16
+// (4) * lane.  Outside the compiler's wait counting: waits are explicit.
+__device__ __forceinline__ void win_dma16(const void* base, uint32_t off, uint32_t m0) {
+  m0 = __builtin_amdgcn_readfirstlane(m0);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "{m0}"(m0)
+               : "memory");
+}
+__device__ __forceinline__ void win_dma4(const void* base, uint32_t off, uint32_t m0) {
+  m0 = __builtin_amdgcn_readfirstlane(m0);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1"
+               :
+               : "v"(off), "s"(base), "{m0}"(m0)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t win_lds(const void* p) {
+  return static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)(p)));
+}
+
+// ---- partial results -----------------------------------------------------------------
+// Row (i, head) of part s of a request: partial row part0 + (s * n + i) * hq + head,
+// o fp32 [D] and (m, l), m in the log2 domain.  A part that sees nothing of the row
+// has m = -inf and its o may be unwritten; m = +inf makes the joined row NaN.
+struct WinParts {
+  float* o;
+  float* ml;
+};
+
+// A call's launches share these.
+struct WinCall {
+  const void* query;
+  int dtype;
+  int64_t q_stride;
+  const int64_t *lens, *qlens;
+  int64_t batch;
+  WinCache cache;
+  float qscale;
+  const float* w_in;
+  float* w_out;
+  const int64_t* w_rows;
+  int64_t w_cols;
+  void* out;
+  float* lse;  // per (row, head), where running weights are kept
+  hipStream_t stream;
+  bool q_wide() const {
+    return (reinterpret_cast<uintptr_t>(query) & 15) == 0 && q_stride % 8 == 0;
+  }
+};
+
+// Launches over some requests of a call, kWinReqs at a time.  shape(b, units, parts):
+// whether request b takes part, its workgroups and its partial results per row;
+// go(arg, requests, workgroups, partial rows).  Partial rows count from 0 in every
+// launch: launches of one stream share the workspace.
+template <typename U, typename G>
+int win_launches(const WinCall& call, U&& shape, G&& go) {
+  WinArg arg;
+  int count = 0;
+  int64_t total = 0, q0 = 0, part0 = 0;
+  for (int64_t b = 0; b <= call.batch; ++b) {
+    if (count == kWinReqs || (b == call.batch && count)) {
+      const int rc = go(arg, count, total, part0);
+      if (rc != KVQ_OK) return rc;
+      count = 0;
+      total = part0 = 0;
+    }
+    if (b == call.batch) break;
+    int64_t units = 0, parts = 1;
+    if (call.qlens[b] > 0 && shape(b, units, parts) && units > 0) {
+      if (total + units > 0x7fffffff) return KVQ_ERR_INVALID;
+      arg.r[count++] = WinReq{static_cast<int32_t>(q0), static_cast<int32_t>(call.qlens[b]),
+                              static_cast<int32_t>(call.lens[b]), static_cast<int32_t>(b),
+                              static_cast<int32_t>(total), static_cast<int32_t>(parts),
+                              static_cast<int32_t>(part0),
+                              static_cast<int32_t>(call.w_rows ? call.w_rows[b] : 0)};
+      total += units;
+      if (parts > 1) part0 += parts * call.qlens[b] * call.cache.hq;
+      if (part0 > 0x7fffffff) return KVQ_ERR_INVALID;
+    }
+    q0 += call.qlens[b];
+  }
+  return KVQ_OK;
+}
+
+inline int64_t win_parts_bytes(int64_t rows, int d) {
+  return rows * (static_cast<int64_t>(d) + 2) * static_cast<int64_t>(sizeof(float));
+}
+
+// Joins the parts of the requests of `arg` that have several (fp8_window.hip).
+int launch_win_join(const WinCall& call, const WinArg& arg, int count, WinParts parts);
+
+// fp8_window_decode.hip: requests of few rows.  _takes: request b is one of them
+// (the geometry is one of the matrix kernels'); _bytes: the partial results.
+bool win_decode_takes(const WinCall& call, int64_t b);
+int64_t win_decode_bytes(const WinCall& call, int* rc);
+int win_decode(const WinCall& call, void* workspace);
+
+// 16-bit queries, head sizes 64, 128 and 256, whole groups of 16 positions a page, at
+// most 16 query heads per kv head, codes on 16-byte bounds.
+inline bool win_matrix_geometry(int dtype, int hq, int kvh, int d, int bs) {
+  return (dtype == KVQ_DTYPE_BF16 || dtype == KVQ_DTYPE_F16) && (d == 64 || d == 128 || d == 256) &&
+         bs % 16 == 0 && hq / kvh <= 16;
+}
+
 }  // namespace kvq

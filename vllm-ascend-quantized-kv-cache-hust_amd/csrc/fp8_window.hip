@@ -15,7 +15,7 @@
 // a position for the scores and a word of the row for the values, all in fp32
 // with the softmax's running maximum and sum; bound by their lanes' 4-byte loads
 // and by reading each code once per query head.
-#include <vector>
+#include <algorithm>
 
 #include "fp8_window.h"
 
@@ -155,81 +155,120 @@ win_weights_general_kernel(WinArg, int count, WinCache c, const T* __restrict__ 
   w_out[dst] = (j < first ? w_in[dst] : 0.0f) + sum;
 }
 
-// ---- host -----------------------------------------------------------------------
+// ---- joining partial results ---------------------------------------------------------
 
-struct Call {
-  const void* query;
-  int dtype;
-  int64_t q_stride;
-  const int64_t *lens, *qlens;
-  int64_t batch;
-  WinCache cache;
-  float qscale;
-  const float* w_in;
-  float* w_out;
-  const int64_t* w_rows;
-  int64_t w_cols;
-  void* out;
-  hipStream_t stream;
-};
+constexpr int kJoinThreads = 256;
 
-// Launches over the requests, kWinReqs at a time: units(b) gives a request's
-// workgroups, go(arg, requests, workgroups) launches them.
-template <typename U, typename G>
-int for_requests(const Call& call, U&& units, G&& go) {
-  WinArg arg;
-  int count = 0;
-  int64_t total = 0, q0 = 0;
-  for (int64_t b = 0; b <= call.batch; ++b) {
-    if (count == kWinReqs || (b == call.batch && count)) {
-      if (total > 0) {
-        const int rc = go(arg, count, static_cast<unsigned>(total));
-        if (rc != KVQ_OK) return rc;
-      }
-      count = 0;
-      total = 0;
-    }
-    if (b == call.batch) break;
-    const int64_t u = units(b);
-    if (u > 0) {
-      if (total + u > 0x7fffffff) return KVQ_ERR_INVALID;
-      arg.r[count++] = WinReq{static_cast<int32_t>(q0), static_cast<int32_t>(call.qlens[b]),
-                              static_cast<int32_t>(call.lens[b]), static_cast<int32_t>(b),
-                              static_cast<int32_t>(total), 1, 0,
-                              static_cast<int32_t>(call.w_rows ? call.w_rows[b] : 0)};
-      total += u;
-    }
-    q0 += call.qlens[b];
+// blockIdx.y: the request, blockIdx.x: row * hq + head.  D / 4 threads hold a part's
+// row, the workgroup several parts at once, joined in LDS in a fixed order.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+win_join_kernel(WinArg, int hq, WinParts parts, T* __restrict__ out, float* __restrict__ lse) {
+  constexpr int LANES = D / 4, SLICES = kJoinThreads / LANES;
+  __shared__ w_f4 s_o[SLICES][LANES];
+  win_cint* a = (win_cint*)__builtin_amdgcn_kernarg_segment_ptr() + 8 * blockIdx.y;
+  const int q0 = a[0], n = a[1], count = a[5], part0 = a[6];
+  const int64_t x = blockIdx.x, stride = static_cast<int64_t>(n) * hq;
+  if (count <= 1 || x >= stride) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const w_f2* ml = reinterpret_cast<const w_f2*>(parts.ml) + part0 + x;
+  float m = -INFINITY;
+  for (int s = lane; s < count; s += 64) m = fmaxf(m, ml[s * stride][0]);
+  m = max_wave64(m);
+  if (m > 0x1.fffffep126f) m = INFINITY;  // the maxima come no higher than FLT_MAX
+  float l = 0.0f;
+  for (int s = lane; s < count; s += 64) {
+    const w_f2 y = ml[s * stride];
+    l += y[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y[0] - m) * y[1];
   }
+  l = sum_wave64(l);
+  const int slice = tid / LANES, k = tid % LANES;
+  w_f4 acc = w_f4{0.f, 0.f, 0.f, 0.f};
+  for (int s = slice; s < count; s += SLICES) {
+    const float ms = ml[s * stride][0];
+    if (ms == -INFINITY) continue;  // sees nothing
+    const w_f4 y = *reinterpret_cast<const w_f4*>(parts.o + (part0 + s * stride + x) * D + 4 * k);
+    acc += __builtin_amdgcn_exp2f(ms - m) * y;
+  }
+  s_o[slice][k] = acc;
+  __syncthreads();
+  if (slice) return;
+#pragma unroll
+  for (int s = 1; s < SLICES; ++s) acc += s_o[s][k];
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t at = static_cast<int64_t>(q0) * hq + x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[at * D + 4 * k + e] = from_f32<T>(acc[e] * inv);
+  if (lse && k == 0) lse[at] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+}  // namespace
+
+namespace kvq {
+
+int launch_win_join(const WinCall& call, const WinArg& arg, int count, WinParts parts) {
+  int64_t rows = 0;
+  for (int i = 0; i < count; ++i)
+    if (arg.r[i].parts > 1) rows = std::max<int64_t>(rows, arg.r[i].n);
+  if (rows == 0) return KVQ_OK;
+  const int hq = call.cache.hq;
+  const dim3 grid(static_cast<unsigned>(rows * hq), static_cast<unsigned>(count));
+#define KVQ_WIN_JOIN(T, D)                                                                    \
+  hipLaunchKernelGGL((win_join_kernel<T, D>), grid, dim3(kJoinThreads), 0, call.stream, arg, hq, \
+                     parts, static_cast<T*>(call.out), call.lse)
+#define KVQ_WIN_JOIN_D(T)                                                              \
+  if (call.cache.d == 64) KVQ_WIN_JOIN(T, 64); else if (call.cache.d == 128)           \
+  KVQ_WIN_JOIN(T, 128); else KVQ_WIN_JOIN(T, 256)
+  if (call.dtype == KVQ_DTYPE_BF16) {
+    KVQ_WIN_JOIN_D(bf16);
+  } else {
+    KVQ_WIN_JOIN_D(f16);
+  }
+#undef KVQ_WIN_JOIN_D
+#undef KVQ_WIN_JOIN
+  KVQ_LAUNCH_CHECK();
   return KVQ_OK;
 }
 
+}  // namespace kvq
+
+namespace {
+
+// ---- host -----------------------------------------------------------------------
+
+// Requests that no matrix kernel takes.
 template <typename T>
-int attend_general(const Call& call, float* lse) {
+int attend_general(const WinCall& call) {
   const int64_t groups = (call.cache.hq + kGenWaves - 1) / kGenWaves;
-  return for_requests(
-      call, [&](int64_t b) { return call.qlens[b] * groups; },
-      [&](const WinArg& arg, int count, unsigned blocks) -> int {
-        hipLaunchKernelGGL((win_attn_general_kernel<T>), dim3(blocks), dim3(64 * kGenWaves), 0,
-                           call.stream, arg, count, call.cache,
+  return win_launches(
+      call,
+      [&](int64_t b, int64_t& units, int64_t&) {
+        units = call.qlens[b] * groups;
+        return !win_decode_takes(call, b);
+      },
+      [&](const WinArg& arg, int count, int64_t blocks, int64_t) -> int {
+        hipLaunchKernelGGL((win_attn_general_kernel<T>), dim3(static_cast<unsigned>(blocks)),
+                           dim3(64 * kGenWaves), 0, call.stream, arg, count, call.cache,
                            static_cast<const T*>(call.query), call.q_stride, call.qscale,
-                           static_cast<T*>(call.out), lse);
+                           static_cast<T*>(call.out), call.lse);
         KVQ_LAUNCH_CHECK();
         return KVQ_OK;
       });
 }
 
 template <typename T>
-int weigh_general(const Call& call, const float* lse) {
-  return for_requests(
+int weigh_general(const WinCall& call) {
+  return win_launches(
       call,
-      [&](int64_t b) {
-        return call.qlens[b] > 0 ? (call.lens[b] + 255) / 256 * call.cache.kvh : 0;
+      [&](int64_t b, int64_t& units, int64_t&) {
+        units = (call.lens[b] + 255) / 256 * call.cache.kvh;
+        return true;
       },
-      [&](const WinArg& arg, int count, unsigned blocks) -> int {
-        hipLaunchKernelGGL((win_weights_general_kernel<T>), dim3(blocks), dim3(256), 0, call.stream,
-                           arg, count, call.cache, static_cast<const T*>(call.query),
-                           call.q_stride, call.qscale, lse, call.w_in, call.w_out, call.w_cols);
+      [&](const WinArg& arg, int count, int64_t blocks, int64_t) -> int {
+        hipLaunchKernelGGL((win_weights_general_kernel<T>), dim3(static_cast<unsigned>(blocks)),
+                           dim3(256), 0, call.stream, arg, count, call.cache,
+                           static_cast<const T*>(call.query), call.q_stride, call.qscale, call.lse,
+                           call.w_in, call.w_out, call.w_cols);
         KVQ_LAUNCH_CHECK();
         return KVQ_OK;
       });
@@ -254,10 +293,41 @@ int check_shape(const int64_t* lens, const int64_t* qlens, int64_t batch, int dt
   return KVQ_OK;
 }
 
-int64_t lse_bytes(const int64_t* qlens, int64_t batch, int hq) {
+int64_t align16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// Bytes of the log-sum-exps (kept for the running weights), before the partial results.
+int64_t lse_bytes(const int64_t* qlens, int64_t batch, int hq, bool weigh) {
+  if (!weigh) return 0;
   int64_t rows = 0;
   for (int64_t b = 0; b < batch; ++b) rows += qlens[b];
-  return (4 * rows * hq + 15) / 16 * 16;
+  return align16(4 * rows * hq);
+}
+
+WinCall make_call(const void* query, int dtype, int64_t query_stride, const int64_t* seq_lens,
+                  const int64_t* query_lens, int64_t batch, int hq, int kvh, int d, float scale,
+                  int64_t window, int64_t sinks, int block_size) {
+  WinCall call{};
+  call.query = query;
+  call.dtype = dtype;
+  call.q_stride = query_stride;
+  call.lens = seq_lens;
+  call.qlens = query_lens;
+  call.batch = batch;
+  call.cache.bs = FastDiv::make(static_cast<uint32_t>(block_size));
+  call.cache.kvh = kvh;
+  call.cache.hq = hq;
+  call.cache.d = d;
+  call.cache.rep = FastDiv::make(static_cast<uint32_t>(hq / kvh));
+  call.cache.window = window > 0 && window < kNoWindow ? static_cast<int>(window) : kNoWindow;
+  call.cache.sinks =
+      static_cast<int>(window > 0 ? std::min<int64_t>(sinks, kMaxPositions) : 0);
+  call.qscale = scale * 1.4426950408889634f;
+  return call;
+}
+
+// Bytes of the partial results: the kernels run one after another and share them.
+int64_t parts_bytes(const WinCall& call, int* rc) {
+  return align16(win_decode_bytes(call, rc));
 }
 
 }  // namespace
@@ -266,10 +336,15 @@ extern "C" int64_t kvq_fp8_pth_window_attn_workspace_bytes(
     const int64_t* seq_lens, const int64_t* query_lens, int64_t batch, int dtype, int num_heads,
     int num_kv_heads, int head_size, int block_size, int64_t window, int64_t sinks,
     int with_weights) {
-  const int rc = check_shape(seq_lens, query_lens, batch, dtype, num_heads, num_kv_heads, head_size,
-                             block_size, window, sinks);
+  int rc = check_shape(seq_lens, query_lens, batch, dtype, num_heads, num_kv_heads, head_size,
+                       block_size, window, sinks);
   if (rc != KVQ_OK) return rc;
-  return with_weights ? lse_bytes(query_lens, batch, num_heads) : 0;
+  // (caches off a 16-byte bound need less: the size does not know the addresses)
+  const WinCall call = make_call(nullptr, dtype, 0, seq_lens, query_lens, batch, num_heads,
+                                 num_kv_heads, head_size, 1.0f, window, sinks, block_size);
+  const int64_t parts = parts_bytes(call, &rc);
+  return rc != KVQ_OK ? KVQ_ERR_INVALID
+                      : lse_bytes(query_lens, batch, num_heads, with_weights != 0) + parts;
 }
 
 extern "C" int kvq_fp8_pth_window_attn(
@@ -280,8 +355,8 @@ extern "C" int kvq_fp8_pth_window_attn(
     const void* block_table, int block_index_type, int64_t max_blocks, const float* weights_in,
     float* weights_out, const int64_t* weight_rows, int64_t weight_cols, void* workspace,
     int64_t workspace_bytes, void* out, void* stream) {
-  const int rc = check_shape(seq_lens, query_lens, batch, dtype, num_heads, num_kv_heads, head_size,
-                             block_size, window, sinks);
+  int rc = check_shape(seq_lens, query_lens, batch, dtype, num_heads, num_kv_heads, head_size,
+                       block_size, window, sinks);
   if (rc != KVQ_OK) return rc;
   int64_t rows = 0;
   for (int64_t b = 0; b < batch; ++b) rows += query_lens[b];
@@ -302,25 +377,36 @@ extern "C" int kvq_fp8_pth_window_attn(
     if (weigh && (seq_lens[b] > weight_cols || weight_rows[b] < 0 || weight_rows[b] > kMaxPositions))
       return KVQ_ERR_INVALID;
   }
-  const int64_t need = weigh ? lse_bytes(query_lens, batch, num_heads) : 0;
-  if (need > 0 && (!workspace || workspace_bytes < need)) return KVQ_ERR_INVALID;
-  Call call{query, dtype, query_stride, seq_lens, query_lens, batch,
-            WinCache{k_data, k_scale, v_data, v_scale, block_table, max_blocks, num_blocks,
-                     FastDiv::make(static_cast<uint32_t>(block_size)),
-                     block_index_type == KVQ_INDEX_I64, num_kv_heads, num_heads, head_size,
-                     FastDiv::make(static_cast<uint32_t>(num_heads / num_kv_heads)),
-                     window > 0 && window < kNoWindow ? static_cast<int>(window) : kNoWindow,
-                     static_cast<int>(window > 0 ? (sinks < kMaxPositions ? sinks : kMaxPositions) : 0)},
-            scale * 1.4426950408889634f, weights_in, weights_out, weight_rows, weight_cols, out,
-            static_cast<hipStream_t>(stream)};
-  float* lse = weigh ? static_cast<float*>(workspace) : nullptr;
+  WinCall call = make_call(query, dtype, query_stride, seq_lens, query_lens, batch, num_heads,
+                           num_kv_heads, head_size, scale, window, sinks, block_size);
+  call.cache.kd = k_data;
+  call.cache.ks = k_scale;
+  call.cache.vd = v_data;
+  call.cache.vs = v_scale;
+  call.cache.table = block_table;
+  call.cache.maxb = max_blocks;
+  call.cache.nb = num_blocks;
+  call.cache.bt64 = block_index_type == KVQ_INDEX_I64;
+  call.w_in = weights_in;
+  call.w_out = weights_out;
+  call.w_rows = weight_rows;
+  call.w_cols = weight_cols;
+  call.out = out;
+  call.stream = static_cast<hipStream_t>(stream);
+  const int64_t lse = lse_bytes(query_lens, batch, num_heads, weigh);
+  const int64_t need = lse + parts_bytes(call, &rc);
+  if (rc != KVQ_OK) return rc;
+  if (need > 0 && (!aligned16(workspace, nullptr) || !workspace || workspace_bytes < need))
+    return KVQ_ERR_INVALID;
+  call.lse = weigh ? static_cast<float*>(workspace) : nullptr;
+  rc = win_decode(call, static_cast<char*>(workspace) + lse);
+  if (rc != KVQ_OK) return rc;
   KVQ_DISPATCH_FLOAT(dtype, T, {
-    int r = attend_general<T>(call, lse);
-    if (r != KVQ_OK) return r;
-    if (weigh) r = weigh_general<T>(call, lse);
-    if (r != KVQ_OK) return r;
+    rc = attend_general<T>(call);
+    if (rc != KVQ_OK) return rc;
+    if (weigh) rc = weigh_general<T>(call);
   });
-  return KVQ_OK;
+  return rc;
 }
 
 // ---- host checks ------------------------------------------------------------------
