@@ -244,7 +244,7 @@ int attend_general(const WinCall& call) {
       call,
       [&](int64_t b, int64_t& units, int64_t&) {
         units = call.qlens[b] * groups;
-        return !win_decode_takes(call, b);
+        return !win_decode_takes(call, b) && !win_chunk_takes(call, b);
       },
       [&](const WinArg& arg, int count, int64_t blocks, int64_t) -> int {
         hipLaunchKernelGGL((win_attn_general_kernel<T>), dim3(static_cast<unsigned>(blocks)),
@@ -327,7 +327,9 @@ WinCall make_call(const void* query, int dtype, int64_t query_stride, const int6
 
 // Bytes of the partial results: the kernels run one after another and share them.
 int64_t parts_bytes(const WinCall& call, int* rc) {
-  return align16(win_decode_bytes(call, rc));
+  const int64_t few = win_decode_bytes(call, rc);
+  if (*rc != KVQ_OK) return 0;
+  return align16(std::max(few, win_chunk_bytes(call, rc)));
 }
 
 }  // namespace
@@ -400,6 +402,8 @@ extern "C" int kvq_fp8_pth_window_attn(
     return KVQ_ERR_INVALID;
   call.lse = weigh ? static_cast<float*>(workspace) : nullptr;
   rc = win_decode(call, static_cast<char*>(workspace) + lse);
+  if (rc != KVQ_OK) return rc;
+  rc = win_chunk(call, static_cast<char*>(workspace) + lse);
   if (rc != KVQ_OK) return rc;
   KVQ_DISPATCH_FLOAT(dtype, T, {
     rc = attend_general<T>(call);
