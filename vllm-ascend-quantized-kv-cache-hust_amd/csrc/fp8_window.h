@@ -263,6 +263,10 @@ bool win_chunk_takes(const WinCall& call, int64_t b);
 int64_t win_chunk_bytes(const WinCall& call, int* rc);
 int win_chunk(const WinCall& call, void* workspace);
 
+// fp8_window_weights.hip: the running weights of the requests of that geometry.
+bool win_weights_takes(const WinCall& call, int64_t b);
+int win_weights(const WinCall& call);
+
 // 16-bit queries, head sizes 64, 128 and 256, whole groups of 16 positions a page, at
 // most 16 query heads per kv head, codes on 16-byte bounds.
 inline bool win_matrix_geometry(int dtype, int hq, int kvh, int d, int bs) {

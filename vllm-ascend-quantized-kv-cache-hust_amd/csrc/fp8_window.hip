@@ -262,7 +262,7 @@ int weigh_general(const WinCall& call) {
       call,
       [&](int64_t b, int64_t& units, int64_t&) {
         units = (call.lens[b] + 255) / 256 * call.cache.kvh;
-        return true;
+        return !win_weights_takes(call, b);
       },
       [&](const WinArg& arg, int count, int64_t blocks, int64_t) -> int {
         hipLaunchKernelGGL((win_weights_general_kernel<T>), dim3(static_cast<unsigned>(blocks)),
@@ -409,6 +409,8 @@ extern "C" int kvq_fp8_pth_window_attn(
     rc = attend_general<T>(call);
     if (rc != KVQ_OK) return rc;
     if (weigh) rc = weigh_general<T>(call);
+    if (rc != KVQ_OK) return rc;
+    if (weigh) rc = win_weights(call);
   });
   return rc;
 }
