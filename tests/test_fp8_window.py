@@ -49,7 +49,7 @@ def _attend(lens=(40, 17), news=(1, 3), hq=4, kvh=2, d=64, edit=None, **kw):
     (dict(out=torch.zeros(5, 4, 64, dtype=torch.bfloat16)), "does not match query"),
     (dict(block_table=torch.zeros(1, 3, dtype=torch.int32)), "2D with a row per request"),
     (dict(block_table=torch.zeros(2, 3)), "int32/int64"),
-    (dict(block_table_host=np.zeros((1, 3))), "the host's copy has 1 rows"),
+    (dict(block_table_host=np.zeros((1, 3))), "the host's copy is \\(1, 3\\)"),
     (dict(weight_rows=[0, 1]), "need weights"),
     (dict(out_weights=torch.zeros(2, 2, 40)), "need weights"),
     (dict(weights=torch.zeros(2, 3, 40)), "weights must be float32"),
@@ -59,7 +59,7 @@ def _attend(lens=(40, 17), news=(1, 3), hq=4, kvh=2, d=64, edit=None, **kw):
     (dict(weights=torch.zeros(2, 2, 40), out_weights=torch.zeros(3, 2, 40)), "does not match"),
     (dict(weights=torch.zeros(2, 2, 40), weight_rows=[1, 1]), "distinct rows"),
     (dict(weights=torch.zeros(2, 2, 40), weight_rows=[0, 2]), "distinct rows"),
-    (dict(weights=torch.zeros(2, 2, 40), weight_rows=[-1, 0]), "distinct rows"),
+    (dict(weights=torch.zeros(2, 2, 40), weight_rows=[-1, 0]), "negative weight_rows"),
     (dict(weights=torch.zeros(2, 2, 40), weight_rows=[0]), "1 weight_rows for 2"),
     (dict(weights=torch.zeros(1, 2, 40)), "distinct rows"),
     ({}, "no CPU fallback"),

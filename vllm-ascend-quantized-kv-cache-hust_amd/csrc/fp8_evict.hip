@@ -55,13 +55,27 @@ __device__ __forceinline__ EvictReq evict_req(int count, int unit) {
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kCachedRow = 32768;  // weights of a row that the workgroup keeps in LDS
 
-// Unsigned integers in the order of the weights.
+// Unsigned integers in the order of the weights: 0 for a place past the row's end, above
+// it -inf .. inf, NaN, and on top the rows that stay whatever they weigh.
+constexpr uint32_t kStays = 0xffffffffu;
 __device__ __forceinline__ uint32_t weight_key(uint32_t bits) {
-  if ((bits & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;  // NaN
+  if ((bits & 0x7fffffffu) > 0x7f800000u) return kStays - 1;  // NaN
   if (bits == 0x80000000u) bits = 0;
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+constexpr uint32_t kZeroKey = 0x80000000u;
+
+// x[0] + .. + x[wave - 1], in every lane.
+__device__ __forceinline__ uint32_t sum_before(const uint32_t* x, int wave, int lane) {
+  static_assert(kSelWaves == 16, "one row of lanes");
+  int v = (lane & 15) < wave ? static_cast<int>(x[lane & 15]) : 0;
+  v += __builtin_amdgcn_update_dpp(0, v, kDppQuadXor1, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, kDppQuadXor2, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, kDppHalfMirror, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, kDppRowMirror, 0xf, 0xf, false);
+  return static_cast<uint32_t>(v);
 }
 
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x, int lane) {  // inclusive
@@ -73,18 +87,78 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x, int lane) {  // inclus
   return x;
 }
 
-// A unit is one kv head of a request.
+// The row of weights as the selection reads it: wave w holds positions [w per, (w + 1)
+// per), lane l of it positions w per + 64 i + l.  HELD: all in registers, NK of them a
+// lane (every pass then runs without a load); else kBatch loads at a time.
+constexpr int kBatch = 16;
+template <int NK>
+struct WeightRow {
+  static constexpr bool kHeld = NK > 0;
+  const float* in;
+  int begin, stop, lane;  // of this wave (none: begin = stop)
+  int len, sinks, end;    // [sinks, end) is up for choice
+  uint32_t held[kHeld ? NK : 1], keys[kHeld ? NK : 1];
+  __device__ __forceinline__ uint32_t key_at(int k, uint32_t bits) const {
+    const uint32_t key = k < sinks || k >= end ? kStays : weight_key(bits);
+    return k < stop ? key : 0u;
+  }
+  __device__ __forceinline__ WeightRow(const float* row, int n, int first, int last, int wave, int l)
+      : in(row), lane(l), len(n), sinks(first), end(n - last) {
+    const int per = ((len + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
+    begin = wave * per < len ? wave * per : len;
+    stop = begin + per < len ? begin + per : len;
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        const int k = begin + 64 * i + lane;
+        held[i] = __float_as_uint(in[k < stop ? k : len - 1]);
+      }
+#pragma unroll
+      for (int i = 0; i < NK; ++i) keys[i] = key_at(begin + 64 * i + lane, held[i]);
+    }
+  }
+  // f(position, key, bits) over the wave's run in order, 64 positions at a time
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    if constexpr (kHeld) {
+      constexpr int G = NK < 4 ? NK : 4;  // places past the end come as key 0
+#pragma unroll
+      for (int i = 0; i < NK; i += G) {
+        if (begin + 64 * i >= stop) break;  // uniform
+#pragma unroll
+        for (int j = i; j < i + G; ++j) f(begin + 64 * j + lane, keys[j], held[j]);
+      }
+    } else {
+      for (int k0 = begin; k0 < stop; k0 += 64 * kBatch) {
+        uint32_t x[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int k = k0 + 64 * i + lane;
+          x[i] = __float_as_uint(in[k < stop ? k : len - 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int k = k0 + 64 * i + lane;
+          f(k, key_at(k, x[i]), x[i]);
+        }
+      }
+    }
+  }
+};
+
+// A unit is one kv head of a request.  NK: weights a lane holds (16 NK waves cover the
+// longest row that is cut), 0: the rows stay in memory.
+template <int NK>
 __global__ void __launch_bounds__(kSelThreads)
 evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const float* w_in,
-                    float* w_out, int64_t w_cols, int32_t* __restrict__ kept, int64_t kept_cols,
-                    int cached) {
-  extern __shared__ uint32_t s_row[];  // the row's bits, where it fits
+                    float* w_out, int64_t w_cols, int32_t* __restrict__ kept, int64_t kept_cols) {
   __shared__ uint32_t s_hist[kBins];
   __shared__ uint32_t s_wave[2][kSelWaves];
   __shared__ uint32_t s_found[2];
   const EvictReq r = evict_req(count, blockIdx.x);
   const int h = static_cast<int>(blockIdx.x) - r.first;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float* in = w_in + (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
   float* out = w_out + (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
   int32_t* ids = kept + (static_cast<int64_t>(r.table) * kvh + h) * kept_cols;
@@ -97,102 +171,94 @@ evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const f
     }
     return;
   }
-  if (cached) {
-    for (int k = tid; k < r.len; k += kSelThreads) s_row[k] = __float_as_uint(in[k]);
-  }
-  auto bits = [&](int k) -> uint32_t { return cached ? s_row[k] : __float_as_uint(in[k]); };
-  const int end = r.len - recent;  // the middle is [sinks, end)
-  uint32_t want = static_cast<uint32_t>(r.keep - sinks - recent);
+  if (stay == 0) return;
+  const WeightRow<NK> row(in, r.len, sinks, recent, wave, lane);
+  uint32_t want = static_cast<uint32_t>(r.keep);
   uint32_t prefix = 0, mask = 0;
   // three rounds: `want` survivors among the keys that agree with prefix on mask
-  if (want > 0) {
 #pragma unroll
-    for (int round = 0; round < 3; ++round) {
-      const int shift = round == 0 ? 21 : (round == 1 ? 10 : 0);
-      const uint32_t field = round == 2 ? 0x3ffu : 0x7ffu;
-      for (int k = tid; k < kBins; k += kSelThreads) s_hist[k] = 0;
-      __syncthreads();
-      for (int k = sinks + tid; k < end; k += kSelThreads) {
-        const uint32_t key = weight_key(bits(k));
-        if ((key & mask) == prefix) atomicAdd(&s_hist[(key >> shift) & field], 1u);
-      }
-      __syncthreads();
-      // thread t: bins 2047 - 2t and 2046 - 2t; keys in the bins above them
-      const uint32_t c0 = s_hist[kBins - 1 - 2 * tid], c1 = s_hist[kBins - 2 - 2 * tid];
-      const uint32_t upto = wave_scan(c0 + c1, lane);
-      if (lane == 63) s_wave[0][wave] = upto;
-      __syncthreads();
-      uint32_t above = upto - (c0 + c1);
-      for (int w = 0; w < wave; ++w) above += s_wave[0][w];
-      if (above < want && want <= above + c0 + c1) {  // one thread
-        const bool upper = want <= above + c0;
-        s_found[0] = static_cast<uint32_t>(kBins - 1 - 2 * tid) - (upper ? 0u : 1u);
-        s_found[1] = want - above - (upper ? 0u : c0);
-      }
-      __syncthreads();
-      prefix |= s_found[0] << shift;
-      mask |= field << shift;
-      want = s_found[1];
-      __syncthreads();  // s_found and s_wave are read before the next round writes them
+  for (int round = 0; round < 3; ++round) {
+    const int shift = round == 0 ? 21 : (round == 1 ? 10 : 0);
+    const uint32_t field = round == 2 ? 0x3ffu : 0x7ffu;
+    for (int k = tid; k < kBins; k += kSelThreads) s_hist[k] = 0;
+    __syncthreads();
+    // weights of exactly 0, of positions that nothing looked at, are many: counted by
+    // ballots, where they would queue at one counter.  (The rows that stay are known.)
+    uint32_t zeros = 0;
+    row.each([&](int, uint32_t key, uint32_t) {
+      const bool match = (key & mask) == prefix;
+      zeros += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key == kZeroKey));
+      if (match & (key != kZeroKey) & (key - 1 < kStays - 1))
+        atomicAdd(&s_hist[(key >> shift) & field], 1u);
+    });
+    if (lane == 0 && zeros && (kZeroKey & mask) == prefix)
+      atomicAdd(&s_hist[(kZeroKey >> shift) & field], zeros);
+    if (tid == 0 && (kStays & mask) == prefix) atomicAdd(&s_hist[field], sinks + recent);
+    __syncthreads();
+    // thread t: bins 2047 - 2t and 2046 - 2t; keys in the bins above them
+    const uint32_t c0 = s_hist[kBins - 1 - 2 * tid], c1 = s_hist[kBins - 2 - 2 * tid];
+    const uint32_t upto = wave_scan(c0 + c1, lane);
+    if (lane == 63) s_wave[0][wave] = upto;
+    __syncthreads();
+    const uint32_t above = upto - (c0 + c1) + sum_before(s_wave[0], wave, lane);
+    if (above < want && want <= above + c0 + c1) {  // one thread
+      const bool upper = want <= above + c0;
+      s_found[0] = static_cast<uint32_t>(kBins - 1 - 2 * tid) - (upper ? 0u : 1u);
+      s_found[1] = want - above - (upper ? 0u : c0);
     }
-  } else {
-    __syncthreads();  // the row in LDS
+    __syncthreads();
+    prefix |= s_found[0] << shift;
+    mask |= field << shift;
+    want = s_found[1];
+    __syncthreads();  // s_found and s_wave are read before the next round writes them
   }
-  const bool some = r.keep - sinks - recent > 0;
   // keys above `prefix` stay, and the first `want` that equal it
-  const int per = ((end - sinks + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
-  const int begin = sinks + wave * per;
-  const int stop = begin + per < end ? begin + per : end;
   uint32_t more = 0, same = 0;  // of this wave's run
-  if (some) {
-    for (int k = begin + lane; k - lane < stop; k += 64) {
-      const uint32_t key = k < stop ? weight_key(bits(k)) : 0u;
-      more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k < stop && key > prefix));
-      same += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k < stop && key == prefix));
-    }
-  }
+  row.each([&](int, uint32_t key, uint32_t) {
+    more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key > prefix));
+    same += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key == prefix));
+  });
   if (lane == 0) {
     s_wave[0][wave] = more;
     s_wave[1][wave] = same;
   }
-  __syncthreads();
-  uint32_t more0 = 0, same0 = 0;
-  for (int w = 0; w < wave; ++w) {
-    more0 += s_wave[0][w];
-    same0 += s_wave[1][w];
-  }
-  // `cached`: the weights move from LDS right here
-  auto put = [&](int rank, int k) {
-    ids[rank] = k;
-    if (cached) out[rank] = __uint_as_float(s_row[k]);
-  };
-  if (some) {
-    uint32_t at = sinks + more0 + (same0 < want ? same0 : want);
-    const uint64_t below = (1ull << lane) - 1;
-    for (int k = begin + lane; k - lane < stop; k += 64) {
-      const uint32_t key = k < stop ? weight_key(bits(k)) : 0u;
-      const uint64_t eq = __builtin_amdgcn_ballot_w64(k < stop && key == prefix);
-      const bool take = k < stop && (key > prefix || (key == prefix &&
-                                     same0 + __builtin_popcountll(eq & below) < want));
-      const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
-      if (take) put(static_cast<int>(at) + __builtin_popcountll(taken & below), k);
-      at += __builtin_popcountll(taken);
-      same0 += __builtin_popcountll(eq);
+  __syncthreads();  // (and every weight held has been read)
+  const uint32_t more0 = sum_before(s_wave[0], wave, lane);
+  uint32_t same0 = sum_before(s_wave[1], wave, lane);
+  uint32_t at = more0 + (same0 < want ? same0 : want);
+  const uint64_t below = (1ull << lane) - 1;
+  row.each([&](int k, uint32_t key, uint32_t bits) {
+    const uint64_t ties = __builtin_amdgcn_ballot_w64(key == prefix);
+    const uint32_t tie_rank = same0 + __builtin_popcountll(ties & below);
+    const bool take = (key > prefix) | ((key == prefix) & (tie_rank < want));
+    const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
+    if (take) {
+      const uint32_t rank = at + __builtin_popcountll(taken & below);
+      ids[rank] = k;
+      if (NK > 0) out[rank] = __uint_as_float(bits);
     }
-  }
-  for (int k = tid; k < sinks; k += kSelThreads) put(k, k);
-  for (int k = tid; k < recent; k += kSelThreads) put(r.keep - recent + k, end + k);
-  if (cached) return;
-  // long rows: through the list just written (this workgroup's), chunk by chunk;
-  // a chunk reads behind everything that the chunks before it have written
+    at += __builtin_popcountll(taken);
+    same0 += __builtin_popcountll(ties);
+  });
+  if (NK > 0) return;
+  // rows in memory: through the list just written (this workgroup's), chunk by chunk; a
+  // chunk reads behind everything that the chunks before it have written
   __syncthreads();
-  for (int k0 = 0; k0 < r.keep; k0 += kSelThreads) {
-    const int k = k0 + tid;
-    float x = 0.0f;
-    if (k < r.keep) x = in[ids[k]];
+  constexpr int kMove = 8;
+  for (int k0 = 0; k0 < r.keep; k0 += kSelThreads * kMove) {
+    float x[kMove];
+#pragma unroll
+    for (int i = 0; i < kMove; ++i) {
+      const int k = k0 + i * kSelThreads + tid;
+      x[i] = in[ids[k < r.keep ? k : r.keep - 1]];
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (k < r.keep) out[k] = x;
+#pragma unroll
+    for (int i = 0; i < kMove; ++i) {
+      const int k = k0 + i * kSelThreads + tid;
+      if (k < r.keep) out[k] = x[i];
+    }
   }
 }
 
@@ -417,18 +483,24 @@ extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_dat
                      FastDiv::make(static_cast<uint32_t>(num_kv_heads)),
                      block_index_type == KVQ_INDEX_I64, head_size};
   const FastDiv piece_div = FastDiv::make(static_cast<uint32_t>(pieces));
-  int64_t lds_max = 0;
-  const int lrc = device_lds_max(&lds_max);
-  if (lrc != KVQ_OK) return lrc;
   int rc = for_requests(
       seq_lens, keep, weight_rows, batch, [&](int64_t) { return num_kv_heads; },
       [&](const EvictArg& arg, int count, unsigned blocks, int64_t longest) -> int {
-        const int64_t row_bytes = (4 * longest + 15) / 16 * 16;
-        const int cached = longest <= kCachedRow && row_bytes + 16384 <= lds_max;
-        hipLaunchKernelGGL(evict_select_kernel, dim3(blocks), dim3(kSelThreads),
-                           cached ? static_cast<unsigned>(row_bytes) : 0u, s, arg, count,
-                           num_kv_heads, static_cast<int>(sinks), static_cast<int>(recent),
-                           weights_in, weights_out, weight_cols, kept, kept_cols, cached);
+#define KVQ_EVICT_SELECT(NK)                                                                   \
+  hipLaunchKernelGGL((evict_select_kernel<NK>), dim3(blocks), dim3(kSelThreads), 0, s, arg,    \
+                     count, num_kv_heads, static_cast<int>(sinks), static_cast<int>(recent),   \
+                     weights_in, weights_out, weight_cols, kept, kept_cols)
+        // the least a lane has to hold of the longest row that is cut
+        const int64_t held = ((longest + kSelWaves - 1) / kSelWaves + 63) / 64;
+        if (held <= 2)
+          KVQ_EVICT_SELECT(2);
+        else if (held <= 8)
+          KVQ_EVICT_SELECT(8);
+        else if (held <= 32)
+          KVQ_EVICT_SELECT(32);
+        else
+          KVQ_EVICT_SELECT(0);
+#undef KVQ_EVICT_SELECT
         KVQ_LAUNCH_CHECK();
         return KVQ_OK;
       });

@@ -19,6 +19,7 @@ launches: a call captured in a graph replays the lengths it was captured with.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 from collections.abc import Sequence
 
 import numpy as np
@@ -34,22 +35,24 @@ _EVICT = "fp8_per_token_head_evict"
 def _on_device(t: torch.Tensor):
     """Launches go to ``t``'s device, whichever is current."""
     if t.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(t.device)
 
 
-def _check_cache(k_data, k_scale, v_data, v_scale) -> None:
-    if k_data.dim() != 4 or k_data.dtype is not torch.uint8 or v_data.dtype is not torch.uint8:
+_HERE = contextlib.nullcontext()
+
+
+def _check_cache(k_data, k_scale, v_data, v_scale) -> torch.Size:
+    shape = k_data.shape
+    if len(shape) != 4 or k_data.dtype is not torch.uint8 or v_data.dtype is not torch.uint8:
         raise RuntimeError(
             "fp8_per_token_head data caches must be uint8 [NB, Bs, KVH, D], got "
-            f"{tuple(k_data.shape)} / {k_data.dtype} and {v_data.dtype}."
+            f"{tuple(shape)} / {k_data.dtype} and {v_data.dtype}."
         )
-    nb, bs, kvh, _ = k_data.shape
-    if v_data.shape != k_data.shape or k_scale.shape != (nb, bs, kvh, 1) or (
-            v_scale.shape != k_scale.shape):
+    if v_data.shape != shape or k_scale.shape != (*shape[:3], 1) or v_scale.shape != k_scale.shape:
         raise RuntimeError(
             "fp8_per_token_head cache views disagree: "
-            f"k_data {tuple(k_data.shape)}, k_scale {tuple(k_scale.shape)}, "
+            f"k_data {tuple(shape)}, k_scale {tuple(k_scale.shape)}, "
             f"v_data {tuple(v_data.shape)}, v_scale {tuple(v_scale.shape)}."
         )
     if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
@@ -57,43 +60,56 @@ def _check_cache(k_data, k_scale, v_data, v_scale) -> None:
             f"fp8_per_token_head scale caches must be float32, got {k_scale.dtype} and "
             f"{v_scale.dtype}."
         )
+    device = k_data.device
     for name, t in (("key data", k_data), ("key scale", k_scale), ("value data", v_data),
                     ("value scale", v_scale)):
-        _check_contiguous(name, t)
-        _check_same_device(name, t, k_data)
+        if not t.is_contiguous() or t.device != device:
+            _check_contiguous(name, t)
+            _check_same_device(name, t, k_data)
+    return shape
 
 
-def _lengths(what: str, values, name: str) -> np.ndarray:
-    out = np.array([int(n) for n in values], dtype=np.int64)
-    if out.size and int(out.min()) < 0:
+def _lengths(what: str, values, name: str):
+    """(int64 array for a call, the numbers)."""
+    if not isinstance(values, (list, tuple)):
+        values = [int(n) for n in values]
+    try:
+        out = (ctypes.c_int64 * len(values))(*values)
+    except TypeError:  # numpy integers
+        values = [int(n) for n in values]
+        out = (ctypes.c_int64 * len(values))(*values)
+    if values and min(values) < 0:
         raise RuntimeError(f"{what}: negative {name}.")
-    return out
+    return out, values
 
 
 def _table(block_table, host, batch: int, name: str = "block_table"):
-    """(device rows, the host's copy of them as a contiguous array)."""
+    """(device rows, the host's copy of them as a contiguous int64 array)."""
     if block_table.dim() != 2 or block_table.shape[0] < batch:
         raise RuntimeError(
             f"fp8_per_token_head {name} must be 2D with a row per request, got "
             f"{tuple(block_table.shape)} for {batch} requests."
         )
     _native.index_code(block_table.dtype)
-    table = block_table[:batch].contiguous()
-    rows = host if host is not None else table.cpu().numpy()
+    # (rows behind the batch are not read)
+    table = block_table if block_table.is_contiguous() else block_table.contiguous()
+    rows = host if host is not None else table[:batch].cpu().numpy()
     if isinstance(rows, torch.Tensor):
         rows = rows.cpu().numpy()
-    rows = np.ascontiguousarray(rows, dtype=np.int64)
-    rows = rows.reshape(rows.shape[0] if rows.ndim == 2 else -1, table.shape[1])[:batch]
-    if rows.shape[0] != batch:
+    if not (isinstance(rows, np.ndarray) and rows.dtype == np.int64 and rows.flags.c_contiguous):
+        rows = np.ascontiguousarray(rows, dtype=np.int64)
+    width = table.shape[1]
+    if rows.ndim != 2 or rows.shape[1] != width or rows.shape[0] < batch:
         raise RuntimeError(
-            f"fp8_per_token_head {name}: the host's copy has {rows.shape[0]} rows for {batch} "
-            "requests."
+            f"fp8_per_token_head {name}: the host's copy is {rows.shape}, the table "
+            f"{tuple(block_table.shape)} for {batch} requests."
         )
     return table, rows
 
 
 def _weight_rows(what: str, weights, out_weights, weight_rows, batch: int, longest: int, kvh: int,
-                 like) -> tuple[torch.Tensor, np.ndarray]:
+                 like):
+    """(where the weights go, their rows as an int64 array for a call)."""
     target = weights if out_weights is None else out_weights
     for name, t in (("weights", weights), ("out_weights", target)):
         if t.dim() != 3 or t.dtype is not torch.float32 or t.shape[1] != kvh:
@@ -103,30 +119,29 @@ def _weight_rows(what: str, weights, out_weights, weight_rows, batch: int, longe
             )
         _check_contiguous(name, t)
         _check_same_device(name, t, like)
-    if target.shape != weights.shape:
-        raise RuntimeError(
-            f"{what}: out_weights {tuple(target.shape)} does not match weights "
-            f"{tuple(weights.shape)}."
-        )
-    if target is not weights and target.data_ptr() != weights.data_ptr():
-        n = 4 * weights.numel()
-        if abs(target.data_ptr() - weights.data_ptr()) < n:
+    if target is not weights:
+        if target.shape != weights.shape:
+            raise RuntimeError(
+                f"{what}: out_weights {tuple(target.shape)} does not match weights "
+                f"{tuple(weights.shape)}."
+            )
+        apart = abs(target.data_ptr() - weights.data_ptr())
+        if 0 < apart < 4 * weights.numel():
             raise RuntimeError(f"{what}: out_weights overlaps weights.")
-    rows = np.arange(batch, dtype=np.int64) if weight_rows is None else np.array(
-        [int(r) for r in weight_rows], dtype=np.int64)
-    if rows.shape[0] != batch:
-        raise RuntimeError(f"{what}: {rows.shape[0]} weight_rows for {batch} requests.")
-    if batch and (int(rows.min()) < 0 or int(rows.max()) >= weights.shape[0]
-                  or len(set(rows.tolist())) != batch):
+    array, rows = _lengths(what, range(batch) if weight_rows is None else weight_rows,
+                           "weight_rows")
+    if len(rows) != batch:
+        raise RuntimeError(f"{what}: {len(rows)} weight_rows for {batch} requests.")
+    if batch and (max(rows) >= weights.shape[0] or len(set(rows)) != batch):
         raise RuntimeError(
             f"{what}: weight_rows must be distinct rows of the {weights.shape[0]} in weights, got "
-            f"{rows.tolist()}."
+            f"{rows}."
         )
     if longest > weights.shape[2]:
         raise RuntimeError(
             f"{what}: weights hold {weights.shape[2]} positions, the longest request has {longest}."
         )
-    return target, rows
+    return target, array
 
 
 def fp8_per_token_head_window_attention(
@@ -171,8 +186,7 @@ def fp8_per_token_head_window_attention(
     the last request's stay as they were, zeros in a fresh one.  bf16, fp16 or
     fp32 queries, any head size of the cache.
     """
-    _check_cache(k_data, k_scale, v_data, v_scale)
-    nb, bs, kvh, d = k_data.shape
+    nb, bs, kvh, d = _check_cache(k_data, k_scale, v_data, v_scale)
     if query.dim() != 3 or query.shape[2] != d:
         raise RuntimeError(
             f"{_ATTENTION}: query must be [tokens, heads, {d}], got {tuple(query.shape)}.")
@@ -186,22 +200,15 @@ def fp8_per_token_head_window_attention(
         raise RuntimeError(f"{_ATTENTION}: window must be at least 1, got {window}.")
     if sinks < 0:
         raise RuntimeError(f"{_ATTENTION}: sinks must not be negative, got {sinks}.")
-    lens = _lengths(_ATTENTION, seq_lens, "seq_lens")
-    news = _lengths(_ATTENTION, query_lens, "query_lens")
-    batch = lens.shape[0]
-    if news.shape[0] != batch:
-        raise RuntimeError(f"{_ATTENTION}: {news.shape[0]} query_lens for {batch} seq_lens.")
-    rows = int(news.sum())
+    lens, totals = _lengths(_ATTENTION, seq_lens, "seq_lens")
+    news, counts = _lengths(_ATTENTION, query_lens, "query_lens")
+    batch = len(totals)
+    if len(counts) != batch:
+        raise RuntimeError(f"{_ATTENTION}: {len(counts)} query_lens for {batch} seq_lens.")
+    rows = sum(counts)
     if rows > tokens:
         raise RuntimeError(f"{_ATTENTION}: query_lens sum to {rows}, the query has {tokens} rows.")
-    if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        if rows < tokens:
-            out[rows:].zero_()
-    elif out.shape != query.shape:
-        raise RuntimeError(
-            f"{_ATTENTION}: out {tuple(out.shape)} does not match query {tuple(query.shape)}.")
-    longest = int(lens.max()) if batch else 0
+    longest = max(totals, default=0)
     w_rows = target = None
     if weights is not None:
         target, w_rows = _weight_rows(_ATTENTION, weights, out_weights, weight_rows, batch, longest,
@@ -209,18 +216,22 @@ def fp8_per_token_head_window_attention(
     elif out_weights is not None or weight_rows is not None:
         raise RuntimeError(f"{_ATTENTION}: out_weights and weight_rows need weights.")
     _check_same_device("query", query, k_data)
-    _check_same_device("out", out, k_data)
     _check_same_device("block_table", block_table, k_data)
+    if out is not None:
+        if out.shape != query.shape:
+            raise RuntimeError(
+                f"{_ATTENTION}: out {tuple(out.shape)} does not match query {tuple(query.shape)}.")
+        _check_same_device("out", out, k_data)
     table, host = _table(block_table, block_table_host, batch)
+    width = table.shape[1]
     lib = _native.lib()
-    win = 0 if window is None else int(window)
-    bad = int(lib.kvq_fp8_pth_window_check(
-        host.ctypes.data, 1, table.shape[1], lens.ctypes.data, news.ctypes.data, batch, nb, bs, win,
-        int(sinks)))
+    win, sinks = 0 if window is None else int(window), int(sinks)
+    bad = lib.kvq_fp8_pth_window_check(host.ctypes.data, 1, width, lens, news, batch, nb, bs, win,
+                                       sinks)
     if bad == _native.KVQ_ERR_CAPACITY:
         raise RuntimeError(
             "fp8_per_token_head block_table does not cover the longest sequence: "
-            f"max_seq_len={longest}, max_blocks={table.shape[1]}, block_size={bs}."
+            f"max_seq_len={longest}, max_blocks={width}, block_size={bs}."
         )
     if bad > 0:
         raise RuntimeError(
@@ -228,36 +239,41 @@ def fp8_per_token_head_window_attention(
             f"request {bad - 1} sees."
         )
     _native.check(bad, _ATTENTION)
-    if rows == 0:
-        return out
-    _native.require_gpu_tensors(_ATTENTION, query, k_data, out)
-    q = query
-    if q.stride(2) != 1 or q.stride(1) != d or (tokens > 1 and q.stride(0) < hq * d):
-        q = q.contiguous()
     # straight into `out` unless it is laid out otherwise or is the query's own memory
-    direct = out.is_contiguous() and out.dtype == q.dtype and (
-        out.untyped_storage().data_ptr() != q.untyped_storage().data_ptr())
+    direct = out is None or (
+        out.is_contiguous() and out.dtype == query.dtype
+        and out.untyped_storage().data_ptr() != query.untyped_storage().data_ptr())
+    if rows:
+        _native.require_gpu_tensors(_ATTENTION, query, k_data)
+    q = query
+    strides = q.stride()
+    if strides[2] != 1 or strides[1] != d or (tokens > 1 and strides[0] < hq * d):
+        q = q.contiguous()
+        strides = q.stride()
+    result = torch.empty(query.shape, dtype=q.dtype, device=q.device) if (
+        out is None or not direct) else out
+    if rows < tokens and out is None:
+        result[rows:].zero_()
+    if rows == 0:
+        return result if out is None else out
     with _on_device(k_data):
-        result = out if direct else torch.empty(query.shape, dtype=q.dtype, device=q.device)
-        nbytes = int(lib.kvq_fp8_pth_window_attn_workspace_bytes(
-            lens.ctypes.data, news.ctypes.data, batch, dtype, hq, kvh, d, bs, win, int(sinks),
-            0 if target is None else 1))
+        nbytes = lib.kvq_fp8_pth_window_attn_workspace_bytes(
+            lens, news, batch, dtype, hq, kvh, d, bs, win, sinks, 0 if target is None else 1)
         _native.check(nbytes if nbytes < 0 else 0, "kvq_fp8_pth_window_attn_workspace_bytes")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib.kvq_fp8_pth_window_attn(
-            q.data_ptr(), dtype, q.stride(0) if tokens > 1 else hq * d, lens.ctypes.data,
-            news.ctypes.data, batch, hq, kvh, d, float(scale), win, int(sinks), k_data.data_ptr(),
-            k_scale.data_ptr(), v_data.data_ptr(), v_scale.data_ptr(), nb, bs, table.data_ptr(),
-            _native.index_code(table.dtype), table.shape[1],
-            None if target is None else weights.data_ptr(), _native.ptr(target),
-            None if w_rows is None else w_rows.ctypes.data,
+            q.data_ptr(), dtype, strides[0] if tokens > 1 else hq * d, lens, news, batch, hq, kvh,
+            d, scale, win, sinks, k_data.data_ptr(), k_scale.data_ptr(), v_data.data_ptr(),
+            v_scale.data_ptr(), nb, bs, table.data_ptr(), _native.index_code(table.dtype), width,
+            None if target is None else weights.data_ptr(), _native.ptr(target), w_rows,
             0 if target is None else weights.shape[2], _native.ptr(ws), nbytes, result.data_ptr(),
             _native.stream_of(k_data),
         )
     _native.check(rc, "kvq_fp8_pth_window_attn")
     if not direct:
         out[:rows].copy_(result[:rows])
-    return out
+        return out
+    return result
 
 
 def fp8_per_token_head_evict(
@@ -294,24 +310,21 @@ def fp8_per_token_head_evict(
     request only; pages shared between requests (a common prefix) can be read
     from with ``out_block_table``.
     """
-    _check_cache(k_data, k_scale, v_data, v_scale)
-    nb, bs, kvh, d = k_data.shape
+    nb, bs, kvh, d = _check_cache(k_data, k_scale, v_data, v_scale)
     if kvh == 0 or d == 0:
         raise RuntimeError(f"{_EVICT}: an empty cache {tuple(k_data.shape)}.")
     if sinks < 0 or recent < 0:
         raise RuntimeError(f"{_EVICT}: sinks and recent must not be negative.")
-    lens = _lengths(_EVICT, seq_lens, "seq_lens")
-    batch = lens.shape[0]
-    keeps = _lengths(_EVICT, [keep] * batch if isinstance(keep, (int, np.integer)) else keep, "keep")
-    if keeps.shape[0] != batch:
-        raise RuntimeError(f"{_EVICT}: {keeps.shape[0]} budgets for {batch} requests.")
-    over = lens > keeps
-    if batch and bool((over & (keeps < sinks + recent)).any()):
-        raise RuntimeError(
-            f"{_EVICT}: a budget under sinks + recent = {sinks + recent}: {keeps.tolist()}.")
-    longest = int(lens.max()) if batch else 0
-    target, rows = _weight_rows(_EVICT, weights, out_weights, weight_rows, batch, longest, kvh,
-                                k_data)
+    lens, totals = _lengths(_EVICT, seq_lens, "seq_lens")
+    batch = len(totals)
+    keeps, budgets = _lengths(
+        _EVICT, [keep] * batch if isinstance(keep, (int, np.integer)) else keep, "keep")
+    if len(budgets) != batch:
+        raise RuntimeError(f"{_EVICT}: {len(budgets)} budgets for {batch} requests.")
+    if any(k < sinks + recent and n > k for n, k in zip(totals, budgets)):
+        raise RuntimeError(f"{_EVICT}: a budget under sinks + recent = {sinks + recent}: {budgets}.")
+    target, rows = _weight_rows(_EVICT, weights, out_weights, weight_rows, batch,
+                                max(totals, default=0), kvh, k_data)
     _check_same_device("block_table", block_table, k_data)
     table, host = _table(block_table, block_table_host, batch)
     out_table = out_host = None
@@ -325,32 +338,32 @@ def fp8_per_token_head_evict(
         out_table, out_host = _table(out_block_table, out_block_table_host, batch,
                                      "out_block_table")
     lib = _native.lib()
-    bad = int(lib.kvq_fp8_pth_evict_check(
-        host.ctypes.data, None if out_host is None else out_host.ctypes.data, 1, table.shape[1],
-        0 if out_table is None else out_table.shape[1], lens.ctypes.data, keeps.ctypes.data, batch,
-        nb, bs)) if batch else 0
+    width, out_width = table.shape[1], 0 if out_table is None else out_table.shape[1]
+    bad = lib.kvq_fp8_pth_evict_check(
+        host.ctypes.data, None if out_host is None else out_host.ctypes.data, 1, width, out_width,
+        lens, keeps, batch, nb, bs) if batch else 0
     if bad == _native.KVQ_ERR_CAPACITY:
         raise RuntimeError(
-            f"{_EVICT}: a block table does not cover its rows (block_size={bs}, longest={longest}).")
+            f"{_EVICT}: a block table does not cover its rows (block_size={bs}, "
+            f"longest={max(totals)}).")
     if bad > 0:
         why = "outside the cache" if bad % 2 else "in use twice"
         raise RuntimeError(f"{_EVICT}: request {(bad - 1) // 2} has a page {why}.")
     _native.check(bad, _EVICT)
-    new_lens = np.minimum(lens, keeps)
-    width = int(new_lens.max()) if batch else 0
-    _native.require_gpu_tensors(_EVICT, k_data, weights)
+    new_lens = [min(n, k) for n, k in zip(totals, budgets)]
+    most = max(new_lens, default=0)
+    _native.require_gpu_tensors(_EVICT, k_data)
     with _on_device(k_data):
-        kept = torch.empty((batch, kvh, width), dtype=torch.int32, device=k_data.device)
+        kept = torch.empty((batch, kvh, most), dtype=torch.int32, device=k_data.device)
         rc = lib.kvq_fp8_pth_evict(
             k_data.data_ptr(), k_scale.data_ptr(), v_data.data_ptr(), v_scale.data_ptr(), nb, bs,
             kvh, d, table.data_ptr(), _native.ptr(out_table), _native.index_code(table.dtype),
-            table.shape[1], 0 if out_table is None else out_table.shape[1], lens.ctypes.data,
-            keeps.ctypes.data, batch, int(sinks), int(recent), weights.data_ptr(),
-            target.data_ptr(), rows.ctypes.data, weights.shape[2], kept.data_ptr(), width,
+            width, out_width, lens, keeps, batch, sinks, recent, weights.data_ptr(),
+            target.data_ptr(), rows, weights.shape[2], kept.data_ptr(), most,
             _native.stream_of(k_data),
-        ) if width else 0
+        ) if most else 0
     _native.check(rc, "kvq_fp8_pth_evict")
-    return new_lens.tolist(), kept
+    return new_lens, kept
 
 
 __all__ = ["fp8_per_token_head_evict", "fp8_per_token_head_window_attention"]
