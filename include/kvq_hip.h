@@ -521,13 +521,16 @@ int64_t kvq_fp8_pth_window_check(const void* block_table, int block_index_type, 
  * [batch, KVH, kept_cols], -1 behind a request's rows.  What lies behind the rows
  * kept stays as it was.  Pages are checked on the host (kvq_fp8_pth_evict_check).
  * D % 4 == 0, D <= 512, codes on 4-byte bounds.  No counterpart in the reference. */
+int64_t kvq_fp8_pth_evict_workspace_bytes(const int64_t* seq_lens, const int64_t* keep,
+                                          int64_t batch, int num_kv_heads);
 int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_data, float* v_scale,
                       int64_t num_blocks, int block_size, int num_kv_heads, int head_size,
                       const void* block_table, const void* out_block_table, int block_index_type,
                       int64_t max_blocks, int64_t out_max_blocks, const int64_t* seq_lens,
                       const int64_t* keep, int64_t batch, int64_t sinks, int64_t recent,
                       const float* weights_in, float* weights_out, const int64_t* weight_rows,
-                      int64_t weight_cols, int32_t* kept, int64_t kept_cols, void* stream);
+                      int64_t weight_cols, int32_t* kept, int64_t kept_cols, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 
 /* Host-side (no GPU call), over the host's copies of the tables: 0 when every live
  * page lies in [0, num_blocks) and no page whose rows move (in place), or that rows

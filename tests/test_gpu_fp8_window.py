@@ -328,6 +328,22 @@ def test_eviction_of_long_rows(gpu_device, keep, fresh):
                      fresh=fresh)
 
 
+@pytest.mark.parametrize("fresh", [False, True])
+@pytest.mark.parametrize("kind", ["ties", "special", "equal"])
+def test_eviction_of_long_rows_with_ties(gpu_device, kind, fresh):
+    """Thresholds among equal weights and NaN, across the chunks of a long row."""
+    _evict_and_check(gpu_device, [50001, 100, 33000], [20000, 100, 32000], 3, 7, 2, 16, 64, kind,
+                     fresh=fresh)
+
+
+@pytest.mark.parametrize("fresh", [False, True])
+@pytest.mark.parametrize("keep,sinks,recent", [(300, 100, 200), (1, 0, 0), (40000, 39990, 10),
+                                               (40000, 0, 40000), (17000, 16500, 0)])
+def test_eviction_budgets_of_long_rows(gpu_device, keep, sinks, recent, fresh):
+    """Nothing to choose, one row, and rows that stay across chunks."""
+    _evict_and_check(gpu_device, [50001], keep, sinks, recent, 1, 16, 64, "special", fresh=fresh)
+
+
 def test_eviction_of_many_requests(gpu_device):
     rng = np.random.default_rng(3)
     lens = [int(n) for n in rng.integers(0, 60, 400)]

@@ -14,12 +14,16 @@
 //   float, its sign, exponent and two bits of fraction, spread weights of similar
 //   size over many more counters than its top byte would), then each wave counts,
 //   and after one barrier writes, the survivors of a run of positions of its own.
+// Rows past kHeldRow positions are cut into chunks, a workgroup each, and the same
+//   rounds run as launches (evict_count_kernel, evict_emit_kernel), the counts passing
+//   through the workspace: integers, so their order changes nothing.
 // evict_move_kernel: a workgroup copies kMoveRows ranks of a request, all kv
 //   heads: their rows lie side by side in the destination pages.
 // evict_compact_kernel: in place.  kept[r] >= r and kept is increasing, so what a
 //   chunk of ranks reads is nothing that an earlier chunk has written; one
 //   workgroup per (request, kv head, side) walks its chunks in order, and within
 //   a chunk every load has returned before the first store.
+#include <algorithm>
 #include <vector>
 
 #include "fp8_window.h"
@@ -33,8 +37,11 @@ struct EvictReq {
   int32_t table;  // row of both block tables and of kept
   int32_t wrow;   // row of the running weights
   int32_t first;  // units of the requests before it
+  int32_t row0;   // rows (kv heads) of the requests before it, in the workspace
+  int32_t chunk0; // their chunks
+  int32_t unused;
 };
-constexpr int kEvictReqs = 160;
+constexpr int kEvictReqs = 112;
 struct EvictArg {
   EvictReq r[kEvictReqs];
 };
@@ -44,11 +51,11 @@ __device__ __forceinline__ EvictReq evict_req(int count, int unit) {
   const int lane = threadIdx.x & 63;
   int at = 0;
   for (int c = 0; c < count; c += 64) {
-    const bool on = c + lane < count && a[5 * (c + lane) + 4] <= unit;
+    const bool on = c + lane < count && a[8 * (c + lane) + 4] <= unit;
     at += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on));
   }
-  win_cint* r = a + 5 * __builtin_amdgcn_readfirstlane(at - 1);
-  return EvictReq{r[0], r[1], r[2], r[3], r[4]};
+  win_cint* r = a + 8 * __builtin_amdgcn_readfirstlane(at - 1);
+  return EvictReq{r[0], r[1], r[2], r[3], r[4], r[5], r[6], 0};
 }
 
 // ---- selection ------------------------------------------------------------------
@@ -87,67 +94,136 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x, int lane) {  // inclus
   return x;
 }
 
-// The row of weights as the selection reads it: wave w holds positions [w per, (w + 1)
-// per), lane l of it positions w per + 64 i + l.  HELD: all in registers, NK of them a
-// lane (every pass then runs without a load); else kBatch loads at a time.
-constexpr int kBatch = 16;
+// The weights of a row, or of a chunk of it, in registers: wave w holds a run of
+// positions, lane l of it its positions 64 i + l, NK of them; every pass then runs
+// without a load.
 template <int NK>
 struct WeightRow {
-  static constexpr bool kHeld = NK > 0;
   const float* in;
   int begin, stop, lane;  // of this wave (none: begin = stop)
   int len, sinks, end;    // [sinks, end) is up for choice
-  uint32_t held[kHeld ? NK : 1], keys[kHeld ? NK : 1];
+  uint32_t held[NK], keys[NK];
   __device__ __forceinline__ uint32_t key_at(int k, uint32_t bits) const {
     const uint32_t key = k < sinks || k >= end ? kStays : weight_key(bits);
     return k < stop ? key : 0u;
   }
-  __device__ __forceinline__ WeightRow(const float* row, int n, int first, int last, int wave, int l)
+  // of the row's positions, those from `from` to `to` (the whole row: 0, n)
+  __device__ __forceinline__ WeightRow(const float* row, int n, int first, int last, int from, int to,
+                                       int wave, int l)
       : in(row), lane(l), len(n), sinks(first), end(n - last) {
-    const int per = ((len + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
-    begin = wave * per < len ? wave * per : len;
-    stop = begin + per < len ? begin + per : len;
-    if constexpr (kHeld) {
+    const int per = ((to - from + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
+    begin = from + wave * per < to ? from + wave * per : to;
+    stop = begin + per < to ? begin + per : to;
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const int k = begin + 64 * i + lane;
-        held[i] = __float_as_uint(in[k < stop ? k : len - 1]);
-      }
-#pragma unroll
-      for (int i = 0; i < NK; ++i) keys[i] = key_at(begin + 64 * i + lane, held[i]);
+    for (int i = 0; i < NK; ++i) {
+      const int k = begin + 64 * i + lane;
+      held[i] = __float_as_uint(in[k < stop ? k : len - 1]);
     }
+#pragma unroll
+    for (int i = 0; i < NK; ++i) keys[i] = key_at(begin + 64 * i + lane, held[i]);
   }
   // f(position, key, bits) over the wave's run in order, 64 positions at a time
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
-    if constexpr (kHeld) {
-      constexpr int G = NK < 4 ? NK : 4;  // places past the end come as key 0
+    constexpr int G = NK < 4 ? NK : 4;  // places past the end come as key 0
 #pragma unroll
-      for (int i = 0; i < NK; i += G) {
-        if (begin + 64 * i >= stop) break;  // uniform
+    for (int i = 0; i < NK; i += G) {
+      if (begin + 64 * i >= stop) break;  // uniform
 #pragma unroll
-        for (int j = i; j < i + G; ++j) f(begin + 64 * j + lane, keys[j], held[j]);
-      }
-    } else {
-      for (int k0 = begin; k0 < stop; k0 += 64 * kBatch) {
-        uint32_t x[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int k = k0 + 64 * i + lane;
-          x[i] = __float_as_uint(in[k < stop ? k : len - 1]);
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int k = k0 + 64 * i + lane;
-          f(k, key_at(k, x[i]), x[i]);
-        }
-      }
+      for (int j = i; j < i + G; ++j) f(begin + 64 * j + lane, keys[j], held[j]);
     }
   }
 };
 
+// The rounds' fields of a key.
+__device__ __forceinline__ int round_shift(int round) { return round == 0 ? 21 : (round == 1 ? 10 : 0); }
+__device__ __forceinline__ uint32_t round_field(int round) { return round == 2 ? 0x3ffu : 0x7ffu; }
+
+// Adds this workgroup's keys that agree with prefix on mask to the counters in LDS
+// (zeroed here).  Weights of exactly 0, of positions that nothing looked at, are many:
+// counted by ballots, where they would queue at one counter.  The rows that stay are
+// known: `stay` of them among this workgroup's.
+template <int NK>
+__device__ __forceinline__ void count_keys(const WeightRow<NK>& row, uint32_t* hist, int round,
+                                           uint32_t prefix, uint32_t mask, uint32_t stay) {
+  const int tid = threadIdx.x, shift = round_shift(round);
+  const uint32_t field = round_field(round);
+  for (int k = tid; k < kBins; k += kSelThreads) hist[k] = 0;
+  __syncthreads();
+  uint32_t zeros = 0;
+  row.each([&](int, uint32_t key, uint32_t) {
+    const bool match = (key & mask) == prefix;
+    zeros += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key == kZeroKey));
+    if (match & (key != kZeroKey) & (key - 1 < kStays - 1))
+      atomicAdd(&hist[(key >> shift) & field], 1u);
+  });
+  if ((tid & 63) == 0 && zeros && (kZeroKey & mask) == prefix)
+    atomicAdd(&hist[(kZeroKey >> shift) & field], zeros);
+  if (tid == 0 && stay && (kStays & mask) == prefix) atomicAdd(&hist[field], stay);
+  __syncthreads();
+}
+
+// The bin in which the `want`th key from the top lies, and which of the bin's it is;
+// c0 and c1: thread t's counts of bins 2 N - 1 - 2 t and 2 N - 2 - 2 t, N threads.
+__device__ __forceinline__ void find_bin(uint32_t c0, uint32_t c1, uint32_t& bin, uint32_t& want,
+                                         uint32_t* s_wave, uint32_t* s_found) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t upto = wave_scan(c0 + c1, lane);
+  if (lane == 63) s_wave[wave] = upto;
+  __syncthreads();
+  const uint32_t above = upto - (c0 + c1) + sum_before(s_wave, wave, lane);
+  if (above < want && want <= above + c0 + c1) {  // one thread
+    const bool upper = want <= above + c0;
+    s_found[0] = static_cast<uint32_t>(2 * kSelThreads - 1 - 2 * tid) - (upper ? 0u : 1u);
+    s_found[1] = want - above - (upper ? 0u : c0);
+  }
+  __syncthreads();
+  bin = s_found[0];
+  want = s_found[1];
+  __syncthreads();  // read before the next call writes them
+}
+
+// Writes the survivors of this workgroup's run: the keys above `prefix`, and those equal
+// to it that are among the first `want` of the row.  more0 / same0: such keys in the
+// chunks before this one.
+template <int NK>
+__device__ __forceinline__ void emit_rows(const WeightRow<NK>& row, uint32_t prefix, uint32_t want,
+                                          uint32_t more0, uint32_t same0, uint32_t (*s_wave)[kSelWaves],
+                                          int32_t* ids, float* out) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t more = 0, same = 0;  // of this wave's run
+  row.each([&](int, uint32_t key, uint32_t) {
+    more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key > prefix));
+    same += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key == prefix));
+  });
+  if (lane == 0) {
+    s_wave[0][wave] = more;
+    s_wave[1][wave] = same;
+  }
+  __syncthreads();  // (and every weight held has been read)
+  more0 += sum_before(s_wave[0], wave, lane);
+  same0 += sum_before(s_wave[1], wave, lane);
+  uint32_t at = more0 + (same0 < want ? same0 : want);
+  const uint64_t below = (1ull << lane) - 1;
+  row.each([&](int k, uint32_t key, uint32_t bits) {
+    const uint64_t ties = __builtin_amdgcn_ballot_w64(key == prefix);
+    const uint32_t tie_rank = same0 + __builtin_popcountll(ties & below);
+    const bool take = (key > prefix) | ((key == prefix) & (tie_rank < want));
+    const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
+    if (take) {
+      const uint32_t rank = at + __builtin_popcountll(taken & below);
+      ids[rank] = k;
+      out[rank] = __uint_as_float(bits);
+    }
+    at += __builtin_popcountll(taken);
+    same0 += __builtin_popcountll(ties);
+  });
+}
+
 // A unit is one kv head of a request.  NK: weights a lane holds (16 NK waves cover the
-// longest row that is cut), 0: the rows stay in memory.
+// longest row that is cut).
 template <int NK>
 __global__ void __launch_bounds__(kSelThreads)
 evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const float* w_in,
@@ -172,94 +248,162 @@ evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const f
     return;
   }
   if (stay == 0) return;
-  const WeightRow<NK> row(in, r.len, sinks, recent, wave, lane);
-  uint32_t want = static_cast<uint32_t>(r.keep);
-  uint32_t prefix = 0, mask = 0;
+  const WeightRow<NK> row(in, r.len, sinks, recent, 0, r.len, wave, lane);
+  uint32_t want = static_cast<uint32_t>(r.keep), prefix = 0, mask = 0;
   // three rounds: `want` survivors among the keys that agree with prefix on mask
 #pragma unroll
   for (int round = 0; round < 3; ++round) {
-    const int shift = round == 0 ? 21 : (round == 1 ? 10 : 0);
-    const uint32_t field = round == 2 ? 0x3ffu : 0x7ffu;
-    for (int k = tid; k < kBins; k += kSelThreads) s_hist[k] = 0;
-    __syncthreads();
-    // weights of exactly 0, of positions that nothing looked at, are many: counted by
-    // ballots, where they would queue at one counter.  (The rows that stay are known.)
-    uint32_t zeros = 0;
+    count_keys(row, s_hist, round, prefix, mask, static_cast<uint32_t>(sinks + recent));
+    uint32_t bin;
+    find_bin(s_hist[kBins - 1 - 2 * tid], s_hist[kBins - 2 - 2 * tid], bin, want, s_wave[0], s_found);
+    prefix |= bin << round_shift(round);
+    mask |= round_field(round) << round_shift(round);
+  }
+  emit_rows(row, prefix, want, 0, 0, s_wave, ids, out);
+}
+
+// ---- rows of many chunks ---------------------------------------------------------------
+
+constexpr int kChunkNk = 16, kChunk = kSelThreads * kChunkNk;  // positions of a chunk
+constexpr int kHeldRow = 32 * kSelThreads;  // the longest row of one workgroup
+constexpr int kLowBins = 1024;              // of the last round
+
+// counts: [row][2][kBins] of the first two rounds; low: [chunk of a row][kLowBins] of the
+// last; above: per such chunk, its keys past what the first two rounds found; tmp: the
+// weights kept, [row][tmp_cols].
+struct EvictWs {
+  uint32_t *counts, *low, *above;
+  float* tmp;
+  int64_t tmp_cols;
+};
+
+__global__ void __launch_bounds__(256) evict_zero_kernel(uint4* p, int64_t n) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) p[i] = make_uint4(0, 0, 0, 0);
+}
+
+// What the first ROUNDS rounds found: the prefix and which of its keys is wanted.
+template <int ROUNDS>
+__device__ __forceinline__ void found_so_far(const uint32_t* counts, uint32_t& prefix,
+                                             uint32_t& mask, uint32_t& want, uint32_t* s_wave,
+                                             uint32_t* s_found) {
+#pragma unroll
+  for (int round = 0; round < ROUNDS; ++round) {
+    const uint32_t* c = counts + round * kBins + kBins - 2 - 2 * threadIdx.x;
+    uint32_t bin;
+    find_bin(c[1], c[0], bin, want, s_wave, s_found);
+    prefix |= bin << round_shift(round);
+    mask |= round_field(round) << round_shift(round);
+  }
+}
+
+// Round ROUND over a chunk.  A unit is a chunk of one kv head.
+template <int ROUND>
+__global__ void __launch_bounds__(kSelThreads)
+evict_count_kernel(EvictArg, int count, int kvh, int sinks, int recent, const float* w_in,
+                   int64_t w_cols, EvictWs ws) {
+  __shared__ uint32_t s_hist[kBins];
+  __shared__ uint32_t s_wave[2][kSelWaves];
+  __shared__ uint32_t s_found[2];
+  const EvictReq r = evict_req(count, blockIdx.x);
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int h = u % kvh, chunk = u / kvh, chunks = (r.len + kChunk - 1) / kChunk;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float* in = w_in + (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
+  const int from = chunk * kChunk, to = r.len - from < kChunk ? r.len : from + kChunk;
+  const WeightRow<kChunkNk> row(in, r.len, sinks, recent, from, to, wave, lane);
+  uint32_t* counts = ws.counts + static_cast<int64_t>(r.row0 + h) * 2 * kBins;
+  uint32_t want = static_cast<uint32_t>(r.keep), prefix = 0, mask = 0;
+  found_so_far<ROUND>(counts, prefix, mask, want, s_wave[0], s_found);
+  // of the rows that stay, those of this chunk
+  const int stay = max(0, min(to, sinks) - from) + max(0, to - max(from, r.len - recent));
+  count_keys(row, s_hist, ROUND, prefix, mask, static_cast<uint32_t>(stay));
+  if constexpr (ROUND < 2) {
+    for (int k = tid; k < kBins; k += kSelThreads)
+      if (s_hist[k]) atomicAdd(&counts[ROUND * kBins + k], s_hist[k]);
+  } else {
+    const int64_t at = r.chunk0 + static_cast<int64_t>(h) * chunks + chunk;
+    for (int k = tid; k < kLowBins; k += kSelThreads) ws.low[at * kLowBins + k] = s_hist[k];
+    uint32_t more = 0;
     row.each([&](int, uint32_t key, uint32_t) {
-      const bool match = (key & mask) == prefix;
-      zeros += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key == kZeroKey));
-      if (match & (key != kZeroKey) & (key - 1 < kStays - 1))
-        atomicAdd(&s_hist[(key >> shift) & field], 1u);
+      more += __builtin_popcountll(__builtin_amdgcn_ballot_w64((key & mask) > prefix));
     });
-    if (lane == 0 && zeros && (kZeroKey & mask) == prefix)
-      atomicAdd(&s_hist[(kZeroKey >> shift) & field], zeros);
-    if (tid == 0 && (kStays & mask) == prefix) atomicAdd(&s_hist[field], sinks + recent);
+    if (lane == 0) s_wave[0][wave] = more;
     __syncthreads();
-    // thread t: bins 2047 - 2t and 2046 - 2t; keys in the bins above them
-    const uint32_t c0 = s_hist[kBins - 1 - 2 * tid], c1 = s_hist[kBins - 2 - 2 * tid];
-    const uint32_t upto = wave_scan(c0 + c1, lane);
-    if (lane == 63) s_wave[0][wave] = upto;
-    __syncthreads();
-    const uint32_t above = upto - (c0 + c1) + sum_before(s_wave[0], wave, lane);
-    if (above < want && want <= above + c0 + c1) {  // one thread
-      const bool upper = want <= above + c0;
-      s_found[0] = static_cast<uint32_t>(kBins - 1 - 2 * tid) - (upper ? 0u : 1u);
-      s_found[1] = want - above - (upper ? 0u : c0);
+    if (tid == 0) {
+      uint32_t sum = 0;
+      for (int w = 0; w < kSelWaves; ++w) sum += s_wave[0][w];
+      ws.above[at] = sum;
     }
-    __syncthreads();
-    prefix |= s_found[0] << shift;
-    mask |= field << shift;
-    want = s_found[1];
-    __syncthreads();  // s_found and s_wave are read before the next round writes them
   }
-  // keys above `prefix` stay, and the first `want` that equal it
-  uint32_t more = 0, same = 0;  // of this wave's run
-  row.each([&](int, uint32_t key, uint32_t) {
-    more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key > prefix));
-    same += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key == prefix));
-  });
-  if (lane == 0) {
-    s_wave[0][wave] = more;
-    s_wave[1][wave] = same;
+}
+
+// The survivors of a chunk.  Where the weights move in place they go by ws.tmp.
+__global__ void __launch_bounds__(kSelThreads)
+evict_emit_kernel(EvictArg, int count, int kvh, int sinks, int recent, const float* w_in,
+                  float* w_out, int64_t w_cols, int32_t* __restrict__ kept, int64_t kept_cols,
+                  EvictWs ws) {
+  __shared__ uint32_t s_wave[2][kSelWaves];
+  __shared__ uint32_t s_found[2];
+  const EvictReq r = evict_req(count, blockIdx.x);
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int h = u % kvh, chunk = u / kvh, chunks = (r.len + kChunk - 1) / kChunk;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float* in = w_in + (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
+  const int from = chunk * kChunk, to = r.len - from < kChunk ? r.len : from + kChunk;
+  const WeightRow<kChunkNk> row(in, r.len, sinks, recent, from, to, wave, lane);
+  uint32_t want = static_cast<uint32_t>(r.keep), prefix = 0, mask = 0;
+  found_so_far<2>(ws.counts + static_cast<int64_t>(r.row0 + h) * 2 * kBins, prefix, mask, want,
+                  s_wave[0], s_found);
+  // thread t: the last round's bin t, in the whole row and in the chunks before this one
+  const int64_t at = r.chunk0 + static_cast<int64_t>(h) * chunks;
+  uint32_t all = 0, before = 0, more0 = 0;
+  for (int x = 0; x < chunks; ++x) {
+    const uint32_t n = ws.low[(at + x) * kLowBins + tid];
+    all += n;
+    before += x < chunk ? n : 0;
+    more0 += x < chunk ? ws.above[at + x] : 0;
   }
-  __syncthreads();  // (and every weight held has been read)
-  const uint32_t more0 = sum_before(s_wave[0], wave, lane);
-  uint32_t same0 = sum_before(s_wave[1], wave, lane);
-  uint32_t at = more0 + (same0 < want ? same0 : want);
-  const uint64_t below = (1ull << lane) - 1;
-  row.each([&](int k, uint32_t key, uint32_t bits) {
-    const uint64_t ties = __builtin_amdgcn_ballot_w64(key == prefix);
-    const uint32_t tie_rank = same0 + __builtin_popcountll(ties & below);
-    const bool take = (key > prefix) | ((key == prefix) & (tie_rank < want));
-    const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
-    if (take) {
-      const uint32_t rank = at + __builtin_popcountll(taken & below);
-      ids[rank] = k;
-      if (NK > 0) out[rank] = __uint_as_float(bits);
-    }
-    at += __builtin_popcountll(taken);
-    same0 += __builtin_popcountll(ties);
-  });
-  if (NK > 0) return;
-  // rows in memory: through the list just written (this workgroup's), chunk by chunk; a
-  // chunk reads behind everything that the chunks before it have written
+  static_assert(kLowBins == kSelThreads, "a thread a bin");
+  // as bins of find_bin: thread t's are 2047 - 2 t and 2046 - 2 t, of which those under
+  // 1024 belong to threads 512 .. 1023
+  __shared__ uint32_t s_all[kLowBins], s_before[kLowBins];
+  s_all[tid] = all;
+  s_before[tid] = before;
   __syncthreads();
-  constexpr int kMove = 8;
-  for (int k0 = 0; k0 < r.keep; k0 += kSelThreads * kMove) {
-    float x[kMove];
+  const int top = kBins - 1 - 2 * tid;
+  uint32_t bin;
+  find_bin(top < kLowBins ? s_all[top] : 0, top < kLowBins ? s_all[top - 1] : 0, bin, want,
+           s_wave[0], s_found);
+  prefix |= bin;
+  // keys of the chunks before this one past `bin`, and in it
+  uint32_t past = tid > static_cast<int>(bin) ? before : 0;
 #pragma unroll
-    for (int i = 0; i < kMove; ++i) {
-      const int k = k0 + i * kSelThreads + tid;
-      x[i] = in[ids[k < r.keep ? k : r.keep - 1]];
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kMove; ++i) {
-      const int k = k0 + i * kSelThreads + tid;
-      if (k < r.keep) out[k] = x[i];
-    }
-  }
+  for (int d = 1; d < 64; d *= 2) past += __shfl_xor(past, d, 64);
+  if (lane == 0) s_wave[0][wave] = past;
+  __syncthreads();
+  more0 += sum_before(s_wave[0], kSelWaves, lane);
+  const uint32_t same0 = s_before[bin];
+  __syncthreads();  // s_wave is read before emit_rows writes it
+  int32_t* ids = kept + (static_cast<int64_t>(r.table) * kvh + h) * kept_cols;
+  if (chunk == 0)
+    for (int64_t k = r.keep + tid; k < kept_cols; k += kSelThreads) ids[k] = -1;
+  float* out = w_in == w_out ? ws.tmp + (static_cast<int64_t>(r.row0) + h) * ws.tmp_cols
+                             : w_out + (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
+  emit_rows(row, prefix, want, more0, same0, s_wave, ids, out);
+}
+
+// ws.tmp into the weights.  A unit is a chunk of one kv head.
+__global__ void __launch_bounds__(kSelThreads)
+evict_weights_kernel(EvictArg, int count, int kvh, float* w_out, int64_t w_cols, EvictWs ws) {
+  const EvictReq r = evict_req(count, blockIdx.x);
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int h = u % kvh, from = u / kvh * kChunk;
+  const float* src = ws.tmp + (static_cast<int64_t>(r.row0) + h) * ws.tmp_cols;
+  float* dst = w_out + (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
+  for (int k = from + threadIdx.x; k < from + kChunk && k < r.keep; k += kSelThreads) dst[k] = src[k];
 }
 
 // ---- moving the rows ----------------------------------------------------------------
@@ -375,28 +519,66 @@ evict_compact_kernel(EvictArg, int count, EvictCache c, const int32_t* __restric
 
 template <typename U, typename G>
 int for_requests(const int64_t* lens, const int64_t* keeps, const int64_t* rows, int64_t batch,
-                 U&& units, G&& go) {
+                 int kvh, U&& units, G&& go) {
   EvictArg arg;
   int count = 0;
-  int64_t total = 0, longest = 0;
+  int64_t total = 0, longest = 0, row0 = 0, chunk0 = 0;
   for (int64_t b = 0; b <= batch; ++b) {
     if (count == kEvictReqs || (b == batch && count)) {
-      const int rc = go(arg, count, static_cast<unsigned>(total), longest);
+      const int rc = go(arg, count, static_cast<unsigned>(total), longest, row0, chunk0);
       if (rc != KVQ_OK) return rc;
       count = 0;
-      total = longest = 0;
+      total = longest = row0 = chunk0 = 0;
     }
     if (b == batch) break;
     const int64_t u = units(b);
     if (u <= 0) continue;
     if (total + u > 0x7fffffff) return KVQ_ERR_INVALID;
     arg.r[count++] = EvictReq{static_cast<int32_t>(lens[b]), static_cast<int32_t>(keeps[b]),
-                              static_cast<int32_t>(b), static_cast<int32_t>(rows[b]),
-                              static_cast<int32_t>(total)};
+                              static_cast<int32_t>(b), static_cast<int32_t>(rows ? rows[b] : 0),
+                              static_cast<int32_t>(total), static_cast<int32_t>(row0),
+                              static_cast<int32_t>(chunk0), 0};
     total += u;
+    row0 += kvh;
+    chunk0 += (lens[b] + kChunk - 1) / kChunk * kvh;
+    if (chunk0 > 0x7fffffff) return KVQ_ERR_INVALID;
     longest = lens[b] > keeps[b] && lens[b] > longest ? lens[b] : longest;
   }
   return KVQ_OK;
+}
+
+// Rows cut into chunks, and their workgroups.
+int64_t chunk_units(const int64_t* lens, const int64_t* keeps, int64_t b, int kvh) {
+  return keeps[b] > 0 && lens[b] > keeps[b] && lens[b] > kHeldRow
+             ? (lens[b] + kChunk - 1) / kChunk * kvh
+             : 0;
+}
+
+// Bytes of a launch's EvictWs, whose arrays lie one behind the other.
+int64_t evict_ws_bytes(int64_t rows, int64_t chunks, int64_t tmp_cols) {
+  return 4 * (rows * 2 * kBins + chunks * kLowBins + (chunks + 3) / 4 * 4 + rows * tmp_cols);
+}
+
+// The most rows that a request cut into chunks keeps.
+int64_t evict_tmp_cols(const int64_t* lens, const int64_t* keeps, int64_t batch) {
+  int64_t cols = 0;
+  for (int64_t b = 0; b < batch; ++b)
+    if (chunk_units(lens, keeps, b, 1) > 0) cols = std::max(cols, keeps[b]);
+  return (cols + 3) / 4 * 4;
+}
+
+int64_t evict_bytes(const int64_t* lens, const int64_t* keeps, int64_t batch, int kvh, int* rc) {
+  const int64_t cols = evict_tmp_cols(lens, keeps, batch);
+  int64_t most = 0;
+  *rc = cols == 0 ? KVQ_OK
+                  : for_requests(
+                        lens, keeps, nullptr, batch, kvh,
+                        [&](int64_t b) { return chunk_units(lens, keeps, b, kvh); },
+                        [&](const EvictArg&, int, unsigned, int64_t, int64_t rows, int64_t chunks) -> int {
+                          most = std::max(most, evict_ws_bytes(rows, chunks, cols));
+                          return KVQ_OK;
+                        });
+  return most;
 }
 
 int64_t table_id(const void* table, int type, int64_t at) {
@@ -443,6 +625,18 @@ extern "C" int64_t kvq_fp8_pth_evict_check(const void* block_table, const void* 
   return KVQ_OK;
 }
 
+extern "C" int64_t kvq_fp8_pth_evict_workspace_bytes(const int64_t* seq_lens, const int64_t* keep,
+                                                     int64_t batch, int num_kv_heads) {
+  if (batch < 0 || (batch > 0 && (!seq_lens || !keep)) || num_kv_heads <= 0)
+    return KVQ_ERR_INVALID;
+  for (int64_t b = 0; b < batch; ++b)
+    if (seq_lens[b] < 0 || seq_lens[b] > kMaxPositions || keep[b] < 0 || keep[b] > kMaxPositions)
+      return KVQ_ERR_INVALID;
+  int rc = KVQ_OK;
+  const int64_t bytes = evict_bytes(seq_lens, keep, batch, num_kv_heads, &rc);
+  return rc != KVQ_OK ? KVQ_ERR_INVALID : bytes;
+}
+
 extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_data, float* v_scale,
                                  int64_t num_blocks, int block_size, int num_kv_heads,
                                  int head_size, const void* block_table,
@@ -452,7 +646,7 @@ extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_dat
                                  int64_t sinks, int64_t recent, const float* weights_in,
                                  float* weights_out, const int64_t* weight_rows,
                                  int64_t weight_cols, int32_t* kept, int64_t kept_cols,
-                                 void* stream) {
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
   if (batch == 0) return KVQ_OK;
   if (!k_data || !k_scale || !v_data || !v_scale || !block_table || !seq_lens || !keep ||
       !weights_in || !weights_out || !weight_rows || !kept || batch < 0 || num_blocks <= 0 ||
@@ -483,35 +677,75 @@ extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_dat
                      FastDiv::make(static_cast<uint32_t>(num_kv_heads)),
                      block_index_type == KVQ_INDEX_I64, head_size};
   const FastDiv piece_div = FastDiv::make(static_cast<uint32_t>(pieces));
-  int rc = for_requests(
-      seq_lens, keep, weight_rows, batch, [&](int64_t) { return num_kv_heads; },
-      [&](const EvictArg& arg, int count, unsigned blocks, int64_t longest) -> int {
-#define KVQ_EVICT_SELECT(NK)                                                                   \
-  hipLaunchKernelGGL((evict_select_kernel<NK>), dim3(blocks), dim3(kSelThreads), 0, s, arg,    \
-                     count, num_kv_heads, static_cast<int>(sinks), static_cast<int>(recent),   \
-                     weights_in, weights_out, weight_cols, kept, kept_cols)
-        // the least a lane has to hold of the longest row that is cut
+  const int kvh = num_kv_heads, snk = static_cast<int>(sinks), rec = static_cast<int>(recent);
+  int rc = KVQ_OK;
+  const int64_t need = evict_bytes(seq_lens, keep, batch, kvh, &rc);
+  if (rc != KVQ_OK) return rc;
+  if (need > 0 && (!workspace || !aligned16(workspace, nullptr) || workspace_bytes < need))
+    return KVQ_ERR_INVALID;
+  rc = for_requests(
+      seq_lens, keep, weight_rows, batch, kvh,
+      [&](int64_t b) { return chunk_units(seq_lens, keep, b, kvh) > 0 ? 0 : kvh; },
+      [&](const EvictArg& arg, int count, unsigned blocks, int64_t longest, int64_t, int64_t) -> int {
+#define KVQ_EVICT_SELECT(NK)                                                                  \
+  hipLaunchKernelGGL((evict_select_kernel<NK>), dim3(blocks), dim3(kSelThreads), 0, s, arg,   \
+                     count, kvh, snk, rec, weights_in, weights_out, weight_cols, kept, kept_cols)
+        // what a lane has to hold of the longest row that is cut
         const int64_t held = ((longest + kSelWaves - 1) / kSelWaves + 63) / 64;
         if (held <= 2)
           KVQ_EVICT_SELECT(2);
         else if (held <= 8)
           KVQ_EVICT_SELECT(8);
-        else if (held <= 32)
-          KVQ_EVICT_SELECT(32);
         else
-          KVQ_EVICT_SELECT(0);
+          KVQ_EVICT_SELECT(32);
 #undef KVQ_EVICT_SELECT
         KVQ_LAUNCH_CHECK();
         return KVQ_OK;
       });
   if (rc != KVQ_OK) return rc;
+  const int64_t tmp_cols = need > 0 ? evict_tmp_cols(seq_lens, keep, batch) : 0;
+  if (need > 0)
+    rc = for_requests(
+        seq_lens, keep, weight_rows, batch, kvh,
+        [&](int64_t b) { return chunk_units(seq_lens, keep, b, kvh); },
+        [&](const EvictArg& arg, int count, unsigned blocks, int64_t, int64_t rows,
+            int64_t chunks) -> int {
+          EvictWs ws;
+          ws.counts = static_cast<uint32_t*>(workspace);
+          ws.low = ws.counts + rows * 2 * kBins;
+          ws.above = ws.low + chunks * kLowBins;
+          ws.tmp = reinterpret_cast<float*>(ws.above + (chunks + 3) / 4 * 4);
+          ws.tmp_cols = tmp_cols;
+          const int64_t words = rows * 2 * kBins / 4;
+          hipLaunchKernelGGL(evict_zero_kernel, dim3(static_cast<unsigned>((words + 255) / 256)),
+                             dim3(256), 0, s, reinterpret_cast<uint4*>(ws.counts), words);
+          KVQ_LAUNCH_CHECK();
+          const dim3 grid(blocks), block(kSelThreads);
+          hipLaunchKernelGGL((evict_count_kernel<0>), grid, block, 0, s, arg, count, kvh, snk, rec,
+                             weights_in, weight_cols, ws);
+          hipLaunchKernelGGL((evict_count_kernel<1>), grid, block, 0, s, arg, count, kvh, snk, rec,
+                             weights_in, weight_cols, ws);
+          hipLaunchKernelGGL((evict_count_kernel<2>), grid, block, 0, s, arg, count, kvh, snk, rec,
+                             weights_in, weight_cols, ws);
+          KVQ_LAUNCH_CHECK();
+          hipLaunchKernelGGL(evict_emit_kernel, grid, block, 0, s, arg, count, kvh, snk, rec,
+                             weights_in, weights_out, weight_cols, kept, kept_cols, ws);
+          KVQ_LAUNCH_CHECK();
+          if (weights_in == weights_out) {
+            hipLaunchKernelGGL(evict_weights_kernel, grid, block, 0, s, arg, count, kvh,
+                               weights_out, weight_cols, ws);
+            KVQ_LAUNCH_CHECK();
+          }
+          return KVQ_OK;
+        });
+  if (rc != KVQ_OK) return rc;
   if (out_block_table) {
     return for_requests(
-        seq_lens, keep, weight_rows, batch,
+        seq_lens, keep, weight_rows, batch, kvh,
         [&](int64_t b) {
           return ((seq_lens[b] < keep[b] ? seq_lens[b] : keep[b]) + kMoveRows - 1) / kMoveRows;
         },
-        [&](const EvictArg& arg, int count, unsigned blocks, int64_t) -> int {
+        [&](const EvictArg& arg, int count, unsigned blocks, int64_t, int64_t, int64_t) -> int {
           if (wide)
             hipLaunchKernelGGL((evict_move_kernel<uint4>), dim3(blocks), dim3(256), 0, s, arg,
                                count, c, kept, kept_cols, piece_div);
@@ -523,9 +757,9 @@ extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_dat
         });
   }
   return for_requests(
-      seq_lens, keep, weight_rows, batch,
+      seq_lens, keep, weight_rows, batch, kvh,
       [&](int64_t b) { return seq_lens[b] > keep[b] ? 2 * static_cast<int64_t>(num_kv_heads) : 0; },
-      [&](const EvictArg& arg, int count, unsigned blocks, int64_t) -> int {
+      [&](const EvictArg& arg, int count, unsigned blocks, int64_t, int64_t, int64_t) -> int {
         if (wide)
           hipLaunchKernelGGL((evict_compact_kernel<uint4>), dim3(blocks), dim3(kCompactThreads), 0,
                              s, arg, count, c, kept, kept_cols, piece_div,

@@ -131,10 +131,11 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
          _I64, _P, _P, _P, _I64, _P, _I64, _P, _P],
     ),
     "kvq_fp8_pth_window_check": (_I64, [_P, _I, _I64, _P, _P, _I64, _I64, _I, _I64, _I64]),
+    "kvq_fp8_pth_evict_workspace_bytes": (_I64, [_P, _P, _I64, _I]),
     "kvq_fp8_pth_evict": (
         _I,
         [_P, _P, _P, _P, _I64, _I, _I, _I, _P, _P, _I, _I64, _I64, _P, _P, _I64, _I64, _I64, _P,
-         _P, _P, _I64, _P, _I64, _P],
+         _P, _P, _I64, _P, _I64, _P, _I64, _P],
     ),
     "kvq_fp8_pth_evict_check": (_I64, [_P, _P, _I, _I64, _I64, _P, _P, _I64, _I64, _I]),
 }

@@ -355,12 +355,15 @@ def fp8_per_token_head_evict(
     _native.require_gpu_tensors(_EVICT, k_data)
     with _on_device(k_data):
         kept = torch.empty((batch, kvh, most), dtype=torch.int32, device=k_data.device)
+        nbytes = lib.kvq_fp8_pth_evict_workspace_bytes(lens, keeps, batch, kvh)
+        _native.check(nbytes if nbytes < 0 else 0, "kvq_fp8_pth_evict_workspace_bytes")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=k_data.device) if nbytes else None
         rc = lib.kvq_fp8_pth_evict(
             k_data.data_ptr(), k_scale.data_ptr(), v_data.data_ptr(), v_scale.data_ptr(), nb, bs,
             kvh, d, table.data_ptr(), _native.ptr(out_table), _native.index_code(table.dtype),
             width, out_width, lens, keeps, batch, sinks, recent, weights.data_ptr(),
-            target.data_ptr(), rows, weights.shape[2], kept.data_ptr(), most,
-            _native.stream_of(k_data),
+            target.data_ptr(), rows, weights.shape[2], kept.data_ptr(), most, _native.ptr(ws),
+            nbytes, _native.stream_of(k_data),
         ) if most else 0
     _native.check(rc, "kvq_fp8_pth_evict")
     return new_lens, kept
