@@ -17,8 +17,8 @@
 // Rows past kHeldRow positions are cut into chunks, a workgroup each, and the same
 //   rounds run as launches (evict_count_kernel, evict_emit_kernel), the counts passing
 //   through the workspace: integers, so their order changes nothing.
-// evict_move_kernel: a workgroup copies kMoveRows ranks of a request, all kv
-//   heads: their rows lie side by side in the destination pages.
+// evict_move_kernel: a workgroup copies some ranks of a request, all kv heads: their
+//   rows lie side by side in the destination pages.
 // evict_compact_kernel: in place.  kept[r] >= r and kept is increasing, so what a
 //   chunk of ranks reads is nothing that an earlier chunk has written; one
 //   workgroup per (request, kv head, side) walks its chunks in order, and within
@@ -425,41 +425,62 @@ struct EvictCache {
   }
 };
 
-constexpr int kMoveRows = 32;  // ranks of a workgroup
+constexpr int kMoveThreads = 256;
 
-// W: the words a row moves in.  A unit is kMoveRows ranks.
+// Ranks of a workgroup: a thread finds one row's places, then all copy.
+__host__ __device__ __forceinline__ int move_ranks(int kvh) {
+  return kvh < kMoveThreads ? kMoveThreads / kvh : 1;
+}
+
+// W: the words a row moves in.  A unit is move_ranks ranks.
 template <typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kMoveThreads)
 evict_move_kernel(EvictArg, int count, EvictCache c, const int32_t* __restrict__ kept,
                   int64_t kept_cols, FastDiv pieces) {
+  constexpr int DEPTH = 4;  // words of each side in flight per thread
+  __shared__ int64_t s_from[kMoveThreads], s_to[kMoveThreads];
   const EvictReq r = evict_req(count, blockIdx.x);
-  const int rank0 = (static_cast<int>(blockIdx.x) - r.first) * kMoveRows;
+  const int kvh = static_cast<int>(c.kvh.d), most = move_ranks(kvh), tid = threadIdx.x;
+  const int rank0 = (static_cast<int>(blockIdx.x) - r.first) * most;
   const int stay = r.len < r.keep ? r.len : r.keep;
-  const int ranks = stay - rank0 < kMoveRows ? stay - rank0 : kMoveRows;
-  const int kvh = static_cast<int>(c.kvh.d), rows = ranks * kvh;
-  // row x of this unit: rank rank0 + x / kvh, head x % kvh
-  auto source = [&](int x, int& rank, int& h) -> int64_t {
-    const int k = static_cast<int>(c.kvh.div(static_cast<uint32_t>(x)));
-    h = x - k * kvh;
-    rank = rank0 + k;
-    const int p = kept[(static_cast<int64_t>(r.table) * kvh + h) * kept_cols + rank];
-    return c.slot(c.src, c.src_cols, r.table, p) * kvh + h;
-  };
-  const int total = rows * static_cast<int>(pieces.d);
-  for (int e = threadIdx.x; e < total; e += 256) {
-    const int x = static_cast<int>(pieces.div(static_cast<uint32_t>(e)));
-    const int w = e - x * static_cast<int>(pieces.d);
-    int rank, h;
-    const int64_t from = source(x, rank, h);
-    const int64_t to = c.slot(c.dst, c.dst_cols, r.table, rank) * kvh + h;
-    const W a = reinterpret_cast<const W*>(c.kd + from * c.d)[w];
-    const W b = reinterpret_cast<const W*>(c.vd + from * c.d)[w];
-    reinterpret_cast<W*>(c.kd + to * c.d)[w] = a;
-    reinterpret_cast<W*>(c.vd + to * c.d)[w] = b;
-    if (w == 0) {
+  const int rows = (stay - rank0 < most ? stay - rank0 : most) * kvh;
+  for (int x0 = 0; x0 < rows; x0 += kMoveThreads) {  // once, up to kMoveThreads kv heads
+    const int n = rows - x0 < kMoveThreads ? rows - x0 : kMoveThreads;
+    __syncthreads();  // the last round's places are read
+    if (tid < n) {
+      // row x: rank rank0 + x / kvh, head x % kvh (rows side by side in the new pages)
+      const int x = x0 + tid, k = static_cast<int>(c.kvh.div(static_cast<uint32_t>(x)));
+      const int h = x - k * kvh, rank = rank0 + k;
+      const int p = kept[(static_cast<int64_t>(r.table) * kvh + h) * kept_cols + rank];
+      const int64_t from = c.slot(c.src, c.src_cols, r.table, p) * kvh + h;
+      const int64_t to = c.slot(c.dst, c.dst_cols, r.table, rank) * kvh + h;
+      s_from[tid] = from * c.d;
+      s_to[tid] = to * c.d;
       const float s = c.ks[from], t = c.vs[from];
       c.ks[to] = s;
       c.vs[to] = t;
+    }
+    __syncthreads();
+    const int total = n * static_cast<int>(pieces.d);
+    for (int e0 = tid; e0 < total; e0 += DEPTH * kMoveThreads) {
+      W a[DEPTH], b[DEPTH];
+      int64_t to[DEPTH];
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) {
+        const int e = e0 + i * kMoveThreads < total ? e0 + i * kMoveThreads : total - 1;
+        const int x = static_cast<int>(pieces.div(static_cast<uint32_t>(e)));
+        const int64_t off = static_cast<int64_t>(e - x * static_cast<int>(pieces.d)) * sizeof(W);
+        a[i] = *reinterpret_cast<const W*>(c.kd + s_from[x] + off);
+        b[i] = *reinterpret_cast<const W*>(c.vd + s_from[x] + off);
+        to[i] = s_to[x] + off;
+      }
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) {
+        if (e0 + i * kMoveThreads < total) {
+          *reinterpret_cast<W*>(c.kd + to[i]) = a[i];
+          *reinterpret_cast<W*>(c.vd + to[i]) = b[i];
+        }
+      }
     }
   }
 }
@@ -740,17 +761,18 @@ extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_dat
         });
   if (rc != KVQ_OK) return rc;
   if (out_block_table) {
+    const int ranks = move_ranks(kvh);
     return for_requests(
         seq_lens, keep, weight_rows, batch, kvh,
         [&](int64_t b) {
-          return ((seq_lens[b] < keep[b] ? seq_lens[b] : keep[b]) + kMoveRows - 1) / kMoveRows;
+          return ((seq_lens[b] < keep[b] ? seq_lens[b] : keep[b]) + ranks - 1) / ranks;
         },
         [&](const EvictArg& arg, int count, unsigned blocks, int64_t, int64_t, int64_t) -> int {
           if (wide)
-            hipLaunchKernelGGL((evict_move_kernel<uint4>), dim3(blocks), dim3(256), 0, s, arg,
+            hipLaunchKernelGGL((evict_move_kernel<w_u4>), dim3(blocks), dim3(kMoveThreads), 0, s, arg,
                                count, c, kept, kept_cols, piece_div);
           else
-            hipLaunchKernelGGL((evict_move_kernel<uint32_t>), dim3(blocks), dim3(256), 0, s, arg,
+            hipLaunchKernelGGL((evict_move_kernel<uint32_t>), dim3(blocks), dim3(kMoveThreads), 0, s, arg,
                                count, c, kept, kept_cols, piece_div);
           KVQ_LAUNCH_CHECK();
           return KVQ_OK;
@@ -761,7 +783,7 @@ extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_dat
       [&](int64_t b) { return seq_lens[b] > keep[b] ? 2 * static_cast<int64_t>(num_kv_heads) : 0; },
       [&](const EvictArg& arg, int count, unsigned blocks, int64_t, int64_t, int64_t) -> int {
         if (wide)
-          hipLaunchKernelGGL((evict_compact_kernel<uint4>), dim3(blocks), dim3(kCompactThreads), 0,
+          hipLaunchKernelGGL((evict_compact_kernel<w_u4>), dim3(blocks), dim3(kCompactThreads), 0,
                              s, arg, count, c, kept, kept_cols, piece_div,
                              static_cast<int>(sinks));
         else
