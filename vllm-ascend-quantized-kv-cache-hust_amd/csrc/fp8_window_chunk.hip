@@ -69,6 +69,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
   constexpr int KS = D / 32, DB = D / 16, PPR = D / 8, CH = D / 16;
   constexpr int INS = kBlock * CH / (64 * WAVES);  // 16-byte loads of a lane, block and side
   constexpr int RPI = 64 / CH;                     // rows of a wave's load
+  constexpr bool AHEAD = D < 256;
   static_assert(INS >= 1 && RPI <= 16, "a wave's load stays inside a 16-position group");
   auto vswz = [](int r) { return 2 * (r % 4) + (PPR >= 16 ? 8 * ((r / 4) % 2) : 0); };
   extern __shared__ __align__(16) char lds[];
@@ -102,16 +103,22 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
   const int nblk = static_cast<int>(static_cast<int64_t>(span.groups) * (seg + 1) / r.parts);
   auto at_block = [&](int i) { return span.pos(i, kBlock); };
 
-  int row_of[NG], pos[NG], head_of[NG];
-  bool live[NG];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    const int row = wrow0 + 16 * g + n;
-    live[g] = row < rows;
-    row_of[g] = query_of(live[g] ? row : 0);
-    head_of[g] = h * rep + (live[g] ? row : 0) - row_of[g] * rep;
-    pos[g] = live[g] ? base + row_of[g] : -1;
-  }
+  // the lane's row of column group g, found where it is needed (held, these would cost
+  // registers that the blocks lack); a row past the last sees nothing
+  struct Row {
+    bool live;
+    int i, head, pos;
+  };
+  auto row_at = [&](int g) {
+    int row = wrow0 + 16 * g + n;
+    asm volatile("" : "+v"(row));  // found anew
+    Row x;
+    x.live = row < rows;
+    x.i = query_of(x.live ? row : 0);
+    x.head = h * rep + (x.live ? row : 0) - x.i * rep;
+    x.pos = x.live ? base + x.i : -1;
+    return x;
+  };
 
   // ---- staging ----
   // slot of 16-position group `grp` of block i, from the table by scalar loads
@@ -195,11 +202,11 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
   if (blk0 >= nblk) {  // uniform
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      if (!live[g]) continue;
-      const int64_t at = (static_cast<int64_t>(r.q0) + row_of[g]) * c.hq + head_of[g];
+      const Row y = row_at(g);
+      if (!y.live) continue;
+      const int64_t at = (static_cast<int64_t>(r.q0) + y.i) * c.hq + y.head;
       if (r.parts > 1) {
-        const int64_t part =
-            r.part0 + (static_cast<int64_t>(seg) * r.n + row_of[g]) * c.hq + head_of[g];
+        const int64_t part = r.part0 + (static_cast<int64_t>(seg) * r.n + y.i) * c.hq + y.head;
         if (kg == 0) *reinterpret_cast<w_f2*>(parts.ml + 2 * part) = w_f2{-INFINITY, 0.0f};
       } else {
         for (int k = kg; k < D; k += 4) out[at * D + k] = from_f32<T>(0.0f);
@@ -209,13 +216,13 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     return;
   }
 
-  float m[NG], off[NG], thr[NG], l[NG];
+  // m of a row that has seen nothing: finite, so that 2^(t - m) needs no test for it
+  constexpr float kNone = -0x1p127f;
+  float m[NG], l[NG];
   w_f4 o[DB][NG];
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    m[g] = -INFINITY;
-    off[g] = 0.0f;
-    thr[g] = -INFINITY;
+    m[g] = kNone;
     l[g] = 0.0f;
 #pragma unroll
     for (int j = 0; j < DB; ++j) o[j][g] = w_f4{0.f, 0.f, 0.f, 0.f};
@@ -266,13 +273,14 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
   Codes next = load(blk0);
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    const T* qrow = query + (static_cast<int64_t>(r.q0) + row_of[g]) * q_stride +
-                    static_cast<int64_t>(head_of[g]) * D;
+    const Row y = row_at(g);
+    const T* qrow = query + (static_cast<int64_t>(r.q0) + y.i) * q_stride +
+                    static_cast<int64_t>(y.head) * D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) q[g][s] = load_op8(qrow + 32 * s + 8 * kg, wide & 1);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
-      if (!live[g]) q[g][s] = w_u4{0, 0, 0, 0};
+      if (!y.live) q[g][s] = w_u4{0, 0, 0, 0};
   }
   put(kbuf0, vbuf0, 0, blk0, next);
   if (blk0 + 1 < nblk) next = load(blk0 + 1);
@@ -285,15 +293,18 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     if (!active(i)) return;
     const int kb = at_block(i);
     const float* sc = reinterpret_cast<const float*>(lds + L::SCALES) + par * 192 + 4 * kg;
+    // operands are read a group ahead of their products where registers allow
     w_f4 s[4][NG];
+    w_u4 a[AHEAD ? 2 : 1][KS];
+    if (AHEAD) k_reads(kc, 0, a[0]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      w_u4 a[KS];
-      k_reads(kc, k, a);
+      if (!AHEAD) k_reads(kc, k, a[0]);
+      if (AHEAD && k < 3) k_reads(kc, k + 1, a[(k + 1) % 2]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < NG; ++g) s[k][g] = w_f4{0.f, 0.f, 0.f, 0.f};
-      k_mfmas(a, s[k]);
-      __builtin_amdgcn_sched_barrier(0);
+      k_mfmas(a[AHEAD ? k % 2 : 0], s[k]);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -307,11 +318,13 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     const bool full = kb + kBlock - 1 <= wave_first_pos &&
                       (kb > wave_last_pos - c.window || kb + kBlock - 1 < c.sinks);  // uniform
     if (!full) {
+      asm volatile("");  // a branch, or every block pays the compares
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         // position kb + 16 k + 4 kg + e is seen when 16 k + e <= rel and (> old or < snk)
-        const int rel = pos[g] - kb - 4 * kg;
-        const int old = max(pos[g], 0) - c.window - kb - 4 * kg, snk = c.sinks - kb - 4 * kg;
+        const int pos = row_at(g).pos;
+        const int rel = pos - kb - 4 * kg;
+        const int old = max(pos, 0) - c.window - kb - 4 * kg, snk = c.sinks - kb - 4 * kg;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int x = 16 * (e / 4) + e % 4;
@@ -339,25 +352,23 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     } else {
       tmax[0] = max_rows4(tmax[0]);
     }
+    // the offset moves only when a row's maximum outgrows it by 8
     bool rescale = false;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) rescale = rescale || tmax[g] > thr[g];
+    for (int g = 0; g < NG; ++g) rescale = rescale || tmax[g] - 8.0f > m[g];
     if (__any(rescale)) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const bool grow = tmax[g] > thr[g];
-        const float mn = grow ? tmax[g] : m[g];
-        const float alpha =
-            !grow ? 1.0f : (m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[g] - mn));
+        const float mn = tmax[g] - 8.0f > m[g] ? tmax[g] : m[g];
+        const float alpha = __builtin_amdgcn_exp2f(m[g] - mn);
         l[g] *= alpha;
 #pragma unroll
         for (int j = 0; j < DB; ++j) o[j][g] *= alpha;
         m[g] = mn;
-        off[g] = mn == -INFINITY ? 0.0f : mn;
-        thr[g] = mn + 8.0f;
       }
     }
-    w_u4 p[NG][2];
+    w_u4 p[NG][2], v[AHEAD ? 2 : 1][DB / 2];
+    if (AHEAD) v_reads(vc, 0, 0, v[0]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const w_f4 iv = *reinterpret_cast<const w_f4*>(sc + 128 + 16 * k);
@@ -365,28 +376,26 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(s[k][g][e] - off[g]);
-          const float p1 = __builtin_amdgcn_exp2f(s[k][g][e + 1] - off[g]);
+          const float p0 = __builtin_amdgcn_exp2f(s[k][g][e] - m[g]);
+          const float p1 = __builtin_amdgcn_exp2f(s[k][g][e + 1] - m[g]);
           l[g] = __builtin_fmaf(p0, iv[e], l[g]);
           l[g] = __builtin_fmaf(p1, iv[e + 1], l[g]);
           p[g][k / 2][2 * (k % 2) + e / 2] = pack_pair(p0, p1, f16{});
         }
     }
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    for (int x = 0; x < 4; ++x) {  // k-step x / 2, half x % 2 of the dims
+      if (!AHEAD) v_reads(vc, x / 2, x % 2, v[0]);
+      if (AHEAD && x < 3) v_reads(vc, (x + 1) / 2, (x + 1) % 2, v[(x + 1) % 2]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int jh = 0; jh < 2; ++jh) {
-        w_u4 a[DB / 2];
-        v_reads(vc, ks, jh, a);
-        __builtin_amdgcn_sched_barrier(0);  // the reads ahead of the products
+      for (int jj = 0; jj < DB / 2; ++jj)
 #pragma unroll
-        for (int jj = 0; jj < DB / 2; ++jj)
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            w_f4& acc = o[jh * (DB / 2) + jj][g];
-            acc = mfma_op(a[jj], p[g][ks], acc, f16{});
-          }
-      }
+        for (int g = 0; g < NG; ++g) {
+          w_f4& acc = o[x % 2 * (DB / 2) + jj][g];
+          acc = mfma_op(v[AHEAD ? x % 2 : 0][jj], p[g][x / 2], acc, f16{});
+        }
+    }
   };
   int i = blk0;
   for (; i + 1 < nblk; i += 2) {
@@ -405,7 +414,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
       for (int x = 0; x < kBlock && kb + x <= tile_last; ++x) {
         bool any = false;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) any = any || c.sees(pos[g], kb + x);
+        for (int g = 0; g < NG; ++g) any = any || c.sees(row_at(g).pos, kb + x);
         if (!__any(any)) continue;
         const int64_t row = (slot(i, x / 16) + x % 16) * kvh + h;
         const float vs = c.vs[row];
@@ -418,7 +427,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
           for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (c.sees(pos[g], kb + x) && (odd >> (8 * e + 7)) & 1) o[j][g][e] = NAN;
+              if (c.sees(row_at(g).pos, kb + x) && (odd >> (8 * e + 7)) & 1) o[j][g][e] = NAN;
         }
       }
     }
@@ -428,17 +437,20 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     const float sum = sum_rows4(l[g]);
-    const int64_t at = (static_cast<int64_t>(r.q0) + row_of[g]) * c.hq + head_of[g];
+    const Row y = row_at(g);
+    const int64_t at = (static_cast<int64_t>(r.q0) + y.i) * c.hq + y.head;
     if (r.parts > 1) {
-      if (!live[g]) continue;
-      const int64_t part =
-          r.part0 + (static_cast<int64_t>(seg) * r.n + row_of[g]) * c.hq + head_of[g];
+      if (!y.live) continue;
+      const int64_t part = r.part0 + (static_cast<int64_t>(seg) * r.n + y.i) * c.hq + y.head;
 #pragma unroll
       for (int j = 0; j < DB; ++j)
         *reinterpret_cast<w_f4*>(parts.o + part * D + 16 * j + 4 * kg) = o[j][g];
       // a NaN score reaches the sum but not the maximum
       if (kg == 0)
-        *reinterpret_cast<w_f2*>(parts.ml + 2 * part) = w_f2{sum != sum ? INFINITY : m[g], sum};
+        *reinterpret_cast<w_f2*>(parts.ml + 2 * part) = w_f2{sum != sum    ? INFINITY
+                                                                : sum == 0.0f ? -INFINITY
+                                                                              : m[g],
+                                                              sum};
       continue;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -456,7 +468,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
         w[1][e] = x[1];
       }
       T* d8 = dst + 16 * (j + kg % 2) + 8 * (kg / 2);
-      if (!live[g]) continue;
+      if (!y.live) continue;
       if (wide & 2) {
         *reinterpret_cast<uint4*>(d8) = make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
       } else {
@@ -469,7 +481,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
         }
       }
     }
-    if (lse && kg == 0 && live[g])
+    if (lse && kg == 0 && y.live)
       lse[at] = sum == 0.0f ? INFINITY : m[g] + __builtin_amdgcn_logf(sum);
   }
 }
