@@ -41,12 +41,9 @@ typedef short c_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) c_s4* c_lds4;
 
 constexpr int kBlock = 64;      // positions
-constexpr int kTileRows = 128;  // rows of a workgroup
 
 template <int D>
 constexpr int chk_ng() { return D == 256 ? 1 : 2; }  // 16-row column groups of a wave
-template <int D>
-constexpr int chk_waves() { return 8 / chk_ng<D>(); }
 template <int D>
 struct ChkLds {
   static constexpr int SIDE = kBlock * D * 2;
@@ -58,14 +55,14 @@ struct ChkLds {
 typedef const __attribute__((address_space(4))) int32_t chk_ci32;
 typedef const __attribute__((address_space(4))) int64_t chk_ci64;
 
-template <typename T, int D>
-__global__ void __launch_bounds__(64 * chk_waves<D>())
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
 __attribute__((amdgpu_waves_per_eu(2, 2)))
 win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int64_t q_stride,
                  int wide, float qscale, T* __restrict__ out, WinParts parts,
                  float* __restrict__ lse) {
   using L = ChkLds<D>;
-  constexpr int NG = chk_ng<D>(), WAVES = chk_waves<D>(), ROWS = 16 * NG;
+  constexpr int NG = chk_ng<D>(), ROWS = 16 * NG, kTileRows = ROWS * WAVES;
   constexpr int KS = D / 32, DB = D / 16, PPR = D / 8, CH = D / 16;
   constexpr int INS = kBlock * CH / (64 * WAVES);  // 16-byte loads of a lane, block and side
   constexpr int RPI = 64 / CH;                     // rows of a wave's load
@@ -184,9 +181,15 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
           for (int k = 0; k < 4; ++k) v[k] &= ~((nan_codes(v[k]) >> 7) * 0xffu);
         }
       }
+      // odd rows store their second column first: the even columns of two rows would
+      // share their banks
       p = vb + row * (2 * D);
-      *reinterpret_cast<w_u4*>(p + 16 * ((2 * lch) ^ vswz(row))) = code_op8<f16>(v[0], v[1]);
-      *reinterpret_cast<w_u4*>(p + 16 * ((2 * lch + 1) ^ vswz(row))) = code_op8<f16>(v[2], v[3]);
+      const int swap = row & 1;
+      const uint32_t y[4] = {swap ? v[2] : v[0], swap ? v[3] : v[1], swap ? v[0] : v[2],
+                             swap ? v[1] : v[3]};
+      *reinterpret_cast<w_u4*>(p + 16 * ((2 * lch + swap) ^ vswz(row))) = code_op8<f16>(y[0], y[1]);
+      *reinterpret_cast<w_u4*>(p + 16 * ((2 * lch + 1 - swap) ^ vswz(row))) =
+          code_op8<f16>(y[2], y[3]);
       // [0][j] ks', [1][j] lv, [2][j] 1 / v_scale; a scale of 0 stands in as 2^-100
       if (lch == 0) {
         float* d = reinterpret_cast<float*>(lds + L::SCALES) + which * 192 + row;
@@ -498,49 +501,65 @@ bool win_chunk_takes(const WinCall& call, int64_t b) {
 
 namespace {
 
-int64_t chk_tiles(const WinCall& call, int64_t b) {
+// How a call runs: waves of a workgroup, rows of a tile.
+struct ChkShape {
+  int waves, rows;
+};
+
+int64_t chk_tiles(const WinCall& call, int64_t b, int rows) {
   if (call.qlens[b] <= 0 || !win_chunk_takes(call, b)) return 0;
-  return (call.qlens[b] * call.cache.rep.d + kTileRows - 1) / kTileRows;
+  return (call.qlens[b] * call.cache.rep.d + rows - 1) / rows;
+}
+
+ChkShape chk_shape(const WinCall& call, int cus) {
+  if (call.cache.d == 256) return {8, 128};
+  if (call.cache.d == 64) return {4, 128};
+  int64_t tiles = 0;
+  for (int64_t b = 0; b < call.batch; ++b) tiles += chk_tiles(call, b, 256);
+  return tiles * call.cache.kvh >= cus ? ChkShape{8, 256} : ChkShape{4, 128};
 }
 
 // The most blocks that a tile of request b has.
-int64_t chk_blocks(const WinCall& call, int64_t b) {
+int64_t chk_blocks(const WinCall& call, int64_t b, int tile_rows) {
   const int rows = static_cast<int>(
-      std::min<int64_t>(call.qlens[b], (kTileRows + call.cache.rep.d - 2) / call.cache.rep.d + 1));
+      std::min<int64_t>(call.qlens[b], (tile_rows + call.cache.rep.d - 2) / call.cache.rep.d + 1));
   return WinSpan::of(static_cast<int>(call.lens[b]), rows, call.cache.window, call.cache.sinks,
                      kBlock)
       .groups;
 }
 
-// Segments of a tile's blocks: as many as the chip has slots for (two workgroups a
-// CU, one at head size 256), of at least 4 blocks each.
+// Segments of a tile's blocks: as many as the chip has slots for (eight waves a CU),
+// of at least 4 blocks each.
 template <typename G>
 int chk_launches(const WinCall& call, G&& go) {
   int cus = 0;
   const int rc = device_cu_count(&cus);
   if (rc != KVQ_OK) return rc;
   if (cus <= 0) cus = 256;
-  const int64_t slots = static_cast<int64_t>(cus) * (call.cache.d == 256 ? 1 : 2);
+  const ChkShape shape = chk_shape(call, cus);
+  const int64_t slots = static_cast<int64_t>(cus) * 8 / shape.waves;
   int64_t tiles = 0;
-  for (int64_t b = 0; b < call.batch; ++b) tiles += chk_tiles(call, b);
+  for (int64_t b = 0; b < call.batch; ++b) tiles += chk_tiles(call, b, shape.rows);
   const int64_t spare = tiles > 0 ? slots / (tiles * call.cache.kvh) : 1;
   return win_launches(
       call,
       [&](int64_t b, int64_t& units, int64_t& parts) {
-        const int64_t t = chk_tiles(call, b);
+        const int64_t t = chk_tiles(call, b, shape.rows);
         if (t == 0) return false;
-        parts = std::max<int64_t>(1, std::min<int64_t>(spare, chk_blocks(call, b) / 4));
+        parts = std::max<int64_t>(1, std::min<int64_t>(spare, chk_blocks(call, b, shape.rows) / 4));
         units = t * parts * call.cache.kvh;
         return true;
       },
-      go);
+      [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
+        return go(shape, arg, count, units, rows);
+      });
 }
 
 }  // namespace
 
 int64_t win_chunk_bytes(const WinCall& call, int* rc) {
   int64_t most = 0;
-  *rc = chk_launches(call, [&](const WinArg&, int, int64_t, int64_t rows) -> int {
+  *rc = chk_launches(call, [&](const ChkShape&, const WinArg&, int, int64_t, int64_t rows) -> int {
     most = std::max(most, win_parts_bytes(rows, call.cache.d));
     return KVQ_OK;
   });
@@ -550,17 +569,24 @@ int64_t win_chunk_bytes(const WinCall& call, int* rc) {
 int win_chunk(const WinCall& call, void* workspace) {
   const WinCache& c = call.cache;
   const int wide = (call.q_wide() ? 1 : 0) | (aligned16(call.out, nullptr) ? 2 : 0);
-  return chk_launches(call, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
+  return chk_launches(call, [&](const ChkShape& shape, const WinArg& arg, int count, int64_t units,
+                                int64_t rows) -> int {
     const WinParts parts{static_cast<float*>(workspace),
                          static_cast<float*>(workspace) + rows * c.d};
-#define KVQ_WIN_CHUNK(T, D)                                                                   \
-  hipLaunchKernelGGL((win_chunk_kernel<T, D>), dim3(static_cast<unsigned>(units)),            \
-                     dim3(64 * chk_waves<D>()), ChkLds<D>::BYTES, call.stream, arg, count, c, \
+#define KVQ_WIN_CHUNK(T, D, W)                                                                \
+  hipLaunchKernelGGL((win_chunk_kernel<T, D, W>), dim3(static_cast<unsigned>(units)),         \
+                     dim3(64 * W), ChkLds<D>::BYTES, call.stream, arg, count, c,              \
                      static_cast<const T*>(call.query), call.q_stride, wide, call.qscale,     \
                      static_cast<T*>(call.out), parts, call.lse)
-#define KVQ_WIN_CHUNK_D(T)                                                        \
-  if (c.d == 64) KVQ_WIN_CHUNK(T, 64); else if (c.d == 128) KVQ_WIN_CHUNK(T, 128); \
-  else KVQ_WIN_CHUNK(T, 256)
+#define KVQ_WIN_CHUNK_D(T)                             \
+  if (c.d == 64)                                       \
+    KVQ_WIN_CHUNK(T, 64, 4);                           \
+  else if (c.d == 256)                                 \
+    KVQ_WIN_CHUNK(T, 256, 8);                          \
+  else if (shape.waves == 8)                           \
+    KVQ_WIN_CHUNK(T, 128, 8);                          \
+  else                                                 \
+    KVQ_WIN_CHUNK(T, 128, 4)
     if (call.dtype == KVQ_DTYPE_BF16) {
       KVQ_WIN_CHUNK_D(bf16);
     } else {
