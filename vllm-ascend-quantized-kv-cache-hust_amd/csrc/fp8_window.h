@@ -211,10 +211,11 @@ struct WinCall {
   }
 };
 
-// Launches over some requests of a call, kWinReqs at a time.  shape(b, units, parts):
-// whether request b takes part, its workgroups and its partial results per row;
-// go(arg, requests, workgroups, partial rows).  Partial rows count from 0 in every
-// launch: launches of one stream share the workspace.
+// Launches over some requests of a call, kWinReqs at a time.  shape(b, units, parts,
+// rows): whether request b takes part, its workgroups, its parts and its partial rows
+// (of whatever the kernel leaves in the workspace); go(arg, requests, workgroups,
+// partial rows).  Partial rows count from 0 in every launch: launches of one stream
+// share the workspace.
 template <typename U, typename G>
 int win_launches(const WinCall& call, U&& shape, G&& go) {
   WinArg arg;
@@ -228,8 +229,8 @@ int win_launches(const WinCall& call, U&& shape, G&& go) {
       total = part0 = 0;
     }
     if (b == call.batch) break;
-    int64_t units = 0, parts = 1;
-    if (call.qlens[b] > 0 && shape(b, units, parts) && units > 0) {
+    int64_t units = 0, parts = 1, rows = 0;
+    if (call.qlens[b] > 0 && shape(b, units, parts, rows) && units > 0) {
       if (total + units > 0x7fffffff) return KVQ_ERR_INVALID;
       arg.r[count++] = WinReq{static_cast<int32_t>(q0), static_cast<int32_t>(call.qlens[b]),
                               static_cast<int32_t>(call.lens[b]), static_cast<int32_t>(b),
@@ -237,7 +238,7 @@ int win_launches(const WinCall& call, U&& shape, G&& go) {
                               static_cast<int32_t>(part0),
                               static_cast<int32_t>(call.w_rows ? call.w_rows[b] : 0)};
       total += units;
-      if (parts > 1) part0 += parts * call.qlens[b] * call.cache.hq;
+      part0 += rows;
       if (part0 > 0x7fffffff) return KVQ_ERR_INVALID;
     }
     q0 += call.qlens[b];
@@ -245,6 +246,10 @@ int win_launches(const WinCall& call, U&& shape, G&& go) {
   return KVQ_OK;
 }
 
+// Partial rows of an attention's request.
+inline int64_t win_part_rows(const WinCall& call, int64_t b, int64_t parts) {
+  return parts > 1 ? parts * call.qlens[b] * call.cache.hq : 0;
+}
 inline int64_t win_parts_bytes(int64_t rows, int d) {
   return rows * (static_cast<int64_t>(d) + 2) * static_cast<int64_t>(sizeof(float));
 }
@@ -265,7 +270,8 @@ int win_chunk(const WinCall& call, void* workspace);
 
 // fp8_window_weights.hip: the running weights of the requests of that geometry.
 bool win_weights_takes(const WinCall& call, int64_t b);
-int win_weights(const WinCall& call);
+int64_t win_weights_bytes(const WinCall& call, int* rc);
+int win_weights(const WinCall& call, void* workspace);
 
 // 16-bit queries, head sizes 64, 128 and 256, whole groups of 16 positions a page, at
 // most 16 query heads per kv head, codes on 16-byte bounds.

@@ -242,7 +242,7 @@ int attend_general(const WinCall& call) {
   const int64_t groups = (call.cache.hq + kGenWaves - 1) / kGenWaves;
   return win_launches(
       call,
-      [&](int64_t b, int64_t& units, int64_t&) {
+      [&](int64_t b, int64_t& units, int64_t&, int64_t&) {
         units = call.qlens[b] * groups;
         return !win_decode_takes(call, b) && !win_chunk_takes(call, b);
       },
@@ -260,7 +260,7 @@ template <typename T>
 int weigh_general(const WinCall& call) {
   return win_launches(
       call,
-      [&](int64_t b, int64_t& units, int64_t&) {
+      [&](int64_t b, int64_t& units, int64_t&, int64_t&) {
         units = (call.lens[b] + 255) / 256 * call.cache.kvh;
         return !win_weights_takes(call, b);
       },
@@ -326,10 +326,13 @@ WinCall make_call(const void* query, int dtype, int64_t query_stride, const int6
 }
 
 // Bytes of the partial results: the kernels run one after another and share them.
-int64_t parts_bytes(const WinCall& call, int* rc) {
+int64_t parts_bytes(const WinCall& call, bool weigh, int* rc) {
   const int64_t few = win_decode_bytes(call, rc);
   if (*rc != KVQ_OK) return 0;
-  return align16(std::max(few, win_chunk_bytes(call, rc)));
+  const int64_t many = win_chunk_bytes(call, rc);
+  if (*rc != KVQ_OK) return 0;
+  const int64_t sums = weigh ? win_weights_bytes(call, rc) : 0;
+  return align16(std::max(std::max(few, many), sums));
 }
 
 }  // namespace
@@ -344,7 +347,7 @@ extern "C" int64_t kvq_fp8_pth_window_attn_workspace_bytes(
   // (caches off a 16-byte bound need less: the size does not know the addresses)
   const WinCall call = make_call(nullptr, dtype, 0, seq_lens, query_lens, batch, num_heads,
                                  num_kv_heads, head_size, 1.0f, window, sinks, block_size);
-  const int64_t parts = parts_bytes(call, &rc);
+  const int64_t parts = parts_bytes(call, with_weights != 0, &rc);
   return rc != KVQ_OK ? KVQ_ERR_INVALID
                       : lse_bytes(query_lens, batch, num_heads, with_weights != 0) + parts;
 }
@@ -396,7 +399,7 @@ extern "C" int kvq_fp8_pth_window_attn(
   call.out = out;
   call.stream = static_cast<hipStream_t>(stream);
   const int64_t lse = lse_bytes(query_lens, batch, num_heads, weigh);
-  const int64_t need = lse + parts_bytes(call, &rc);
+  const int64_t need = lse + parts_bytes(call, weigh, &rc);
   if (rc != KVQ_OK) return rc;
   if (need > 0 && (!aligned16(workspace, nullptr) || !workspace || workspace_bytes < need))
     return KVQ_ERR_INVALID;
@@ -410,7 +413,7 @@ extern "C" int kvq_fp8_pth_window_attn(
     if (rc != KVQ_OK) return rc;
     if (weigh) rc = weigh_general<T>(call);
     if (rc != KVQ_OK) return rc;
-    if (weigh) rc = win_weights(call);
+    if (weigh) rc = win_weights(call, static_cast<char*>(workspace) + lse);
   });
   return rc;
 }

@@ -543,10 +543,11 @@ int chk_launches(const WinCall& call, G&& go) {
   const int64_t spare = tiles > 0 ? slots / (tiles * call.cache.kvh) : 1;
   return win_launches(
       call,
-      [&](int64_t b, int64_t& units, int64_t& parts) {
+      [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
         const int64_t t = chk_tiles(call, b, shape.rows);
         if (t == 0) return false;
         parts = std::max<int64_t>(1, std::min<int64_t>(spare, chk_blocks(call, b, shape.rows) / 4));
+        rows = win_part_rows(call, b, parts);
         units = t * parts * call.cache.kvh;
         return true;
       },

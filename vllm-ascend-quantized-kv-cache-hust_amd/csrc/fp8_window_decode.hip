@@ -442,9 +442,10 @@ int dec_launches(const WinCall& call, int64_t* split_out, G&& go) {
   const int hgs = call.cache.kvh / dec_hpw(call.cache.kvh, call.cache.d);
   return win_launches(
       call,
-      [&](int64_t b, int64_t& units, int64_t& parts) {
+      [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
         const int64_t groups = dec_groups(call, b);
         parts = (groups + split - 1) / split;
+        rows = win_part_rows(call, b, parts);
         units = parts * hgs * ((call.qlens[b] * call.cache.rep.d + 15) / 16);
         return groups > 0;
       },

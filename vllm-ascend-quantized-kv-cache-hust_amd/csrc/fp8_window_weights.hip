@@ -12,7 +12,10 @@
 //
 // Few columns: a wave per run, each code read once: bound by HBM (keys only).  Many
 // (SPLIT): the four waves of a workgroup share a run and take every fourth column
-// group, joined in LDS: bound by the exponentials, one per (row, head, position).
+// group, joined in LDS: bound by the exponentials, one per (row, head, position).  The
+// first positions are seen by every row and the last by few, so long requests' columns
+// are cut into segments of kSegTiles groups, whose sums meet in win_weights_add_kernel
+// (3 prompts of 1.5K - 4.1K, 32 heads on 8: 354 us uncut).
 #include <algorithm>
 
 #include "fp8_window.h"
@@ -23,6 +26,7 @@ using namespace kvq;
 
 constexpr int kWaves = 4;
 constexpr int kSplitCols = 64;  // columns from which a workgroup's waves share a run
+constexpr int kSegTiles = 128;  // column groups of a segment
 
 template <int D>
 constexpr int run_groups() { return D == 256 ? 4 : 8; }
@@ -39,34 +43,52 @@ __device__ __forceinline__ float sum_row16(float x) {
   return x;
 }
 
-// A unit is a workgroup's run(s) of one kv head: RUN positions if SPLIT, 4 RUN if not.
+// Groups of 16 columns with rows that may see a position of [j0, j0 + run): [lo, hi).
+__device__ __forceinline__ void seeing_tiles(const WinReq& r, const WinCache& c, int j0, int run,
+                                             int& lo, int& hi) {
+  const int rep = static_cast<int>(c.rep.d), base = r.len - r.n;
+  const int j1 = min(j0 + run, r.len);
+  const int row_lo = max(j0 - base, 0);
+  int row_hi = r.n;
+  if (c.window != kNoWindow && j0 >= c.sinks) {
+    // the last position to see j1 - 1 is j1 - 2 + window
+    const int64_t last = static_cast<int64_t>(j1) - 1 + c.window - base;
+    row_hi = static_cast<int>(last < r.n ? (last < 0 ? 0 : last) : r.n);
+  }
+  lo = row_lo * rep / 16;
+  hi = j0 < r.len ? (row_hi * rep + 15) / 16 : 0;
+}
+
+// A unit is a workgroup's run(s) of one kv head (and a segment of their columns, of
+// r.parts): RUN positions if SPLIT, 4 RUN if not.
 template <typename T, int D, bool SPLIT>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
 win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int64_t q_stride,
                    int wide, float qscale, const float* __restrict__ lse, const float* w_in,
-                   float* w_out, int64_t w_cols) {
+                   float* w_out, int64_t w_cols, float* __restrict__ seg_sums) {
   constexpr int NGRP = run_groups<D>(), RUN = 16 * NGRP, KS = D / 32, W = D / 64;
   __shared__ float s_scale[kWaves][RUN];
   __shared__ float s_sum[kWaves][RUN];
   const WinReq r = win_req(count, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
-  const int u = static_cast<int>(blockIdx.x) - r.first;
+  int u = static_cast<int>(blockIdx.x) - r.first;
   const int h = u % c.kvh;
-  const int wg0 = u / c.kvh * (SPLIT ? RUN : kWaves * RUN);
+  u /= c.kvh;
+  constexpr int SPAN = SPLIT ? RUN : kWaves * RUN;
+  const int spans = (r.len + SPAN - 1) / SPAN;
+  const int seg = u / spans;
+  const int wg0 = (u - seg * spans) * SPAN;
   const int j0 = wg0 + (SPLIT ? 0 : wave * RUN);  // the wave's first position
   const int rep = static_cast<int>(c.rep.d);
   const int cols = r.n * rep, base = r.len - r.n;
-  const int j1 = min(j0 + RUN, r.len);  // past its last
-
-  // rows that may see one of them
-  int row_lo = max(j0 - base, 0), row_hi = r.n;
-  if (c.window != kNoWindow && j0 >= c.sinks) {
-    // the last position to see j1 - 1 is j1 - 2 + window
-    const int64_t last = static_cast<int64_t>(j1) - 1 + c.window - base;
-    row_hi = static_cast<int>(last < r.n ? (last < 0 ? 0 : last) : r.n);
+  int t_lo, t_hi;
+  seeing_tiles(r, c, j0, RUN, t_lo, t_hi);
+  if (SPLIT && r.parts > 1) {
+    t_lo = max(t_lo, seg * kSegTiles);
+    t_hi = min(t_hi, (seg + 1) * kSegTiles);
+    if (t_lo >= t_hi) return;  // uniform over the workgroup
   }
-  const int t_lo = row_lo * rep / 16, t_hi = j0 < r.len ? (row_hi * rep + 15) / 16 : 0;
   float* sums = s_sum[wave];
 
   w_f4 acc[NGRP];
@@ -160,6 +182,7 @@ win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, i
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[k][e] += p[e];
+        if (k % 2) __builtin_amdgcn_sched_barrier(0);  // two groups at a time: registers
       }
       now = next;
     }
@@ -180,11 +203,34 @@ win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, i
     float sum;
     if constexpr (SPLIT) {
       sum = (s_sum[0][x] + s_sum[1][x]) + (s_sum[2][x] + s_sum[3][x]);
+      if (r.parts > 1) {
+        seg_sums[r.part0 + (static_cast<int64_t>(seg) * c.kvh + h) * r.len + j] = sum;
+        continue;
+      }
     } else {
       sum = s_sum[x / RUN][x % RUN];
     }
     w_out[dst + j] = (j < base ? w_in[dst + j] : 0.0f) + sum;
   }
+}
+
+// The segments' sums of a position, in their order.  A unit is 256 positions of a head.
+template <int D>
+__global__ void __launch_bounds__(256)
+win_weights_add_kernel(WinArg, int count, WinCache c, const float* w_in, float* w_out,
+                       int64_t w_cols, const float* __restrict__ seg_sums) {
+  const WinReq r = win_req(count, blockIdx.x);
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int h = u % c.kvh, j = u / c.kvh * 256 + static_cast<int>(threadIdx.x);
+  if (j >= r.len) return;
+  constexpr int RUN = 16 * run_groups<D>();
+  int lo, hi;
+  seeing_tiles(r, c, j / RUN * RUN, RUN, lo, hi);
+  float sum = 0.0f;
+  for (int s = lo / kSegTiles; s * kSegTiles < hi; ++s)
+    sum += seg_sums[r.part0 + (static_cast<int64_t>(s) * c.kvh + h) * r.len + j];
+  const int64_t at = (static_cast<int64_t>(r.wrow) * c.kvh + h) * w_cols + j;
+  w_out[at] = (j < r.len - r.n ? w_in[at] : 0.0f) + sum;
 }
 
 }  // namespace
@@ -197,24 +243,49 @@ bool win_weights_takes(const WinCall& call, int64_t b) {
          aligned16(c.kd, c.vd) && call.lens[b] > 0;
 }
 
-int win_weights(const WinCall& call) {
+namespace {
+
+// Launches of the requests whose columns a workgroup's waves share, or of the others.
+template <typename G>
+int wgt_launches(const WinCall& call, int split, G&& go) {
+  const WinCache& c = call.cache;
+  const int64_t run = 16 * (c.d == 256 ? 4 : 8) * (split ? 1 : kWaves);
+  return win_launches(
+      call,
+      [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
+        const int64_t cols = call.qlens[b] * c.rep.d;
+        if (!win_weights_takes(call, b) || (cols >= kSplitCols) != (split != 0)) return false;
+        parts = split ? ((cols + 15) / 16 + kSegTiles - 1) / kSegTiles : 1;
+        units = (call.lens[b] + run - 1) / run * c.kvh * parts;
+        rows = parts > 1 ? parts * c.kvh * call.lens[b] : 0;
+        return true;
+      },
+      go);
+}
+
+}  // namespace
+
+int64_t win_weights_bytes(const WinCall& call, int* rc) {
+  int64_t most = 0;
+  *rc = wgt_launches(call, 1, [&](const WinArg&, int, int64_t, int64_t rows) -> int {
+    most = std::max(most, rows * static_cast<int64_t>(sizeof(float)));
+    return KVQ_OK;
+  });
+  return most;
+}
+
+int win_weights(const WinCall& call, void* workspace) {
   const WinCache& c = call.cache;
   const int wide = call.q_wide() ? 1 : 0;
+  float* sums = static_cast<float*>(workspace);
   for (int split = 0; split < 2; ++split) {
-    const int64_t run = 16 * (c.d == 256 ? 4 : 8) * (split ? 1 : kWaves);
-    const int rc = win_launches(
-        call,
-        [&](int64_t b, int64_t& units, int64_t&) {
-          units = (call.lens[b] + run - 1) / run * c.kvh;
-          return win_weights_takes(call, b) &&
-                 (call.qlens[b] * c.rep.d >= kSplitCols) == (split != 0);
-        },
-        [&](const WinArg& arg, int count, int64_t units, int64_t) -> int {
+    const int rc = wgt_launches(
+        call, split, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
 #define KVQ_WIN_WGT(T, D, S)                                                                  \
   hipLaunchKernelGGL((win_weights_kernel<T, D, S>), dim3(static_cast<unsigned>(units)),       \
                      dim3(64 * kWaves), 0, call.stream, arg, count, c,                        \
                      static_cast<const T*>(call.query), call.q_stride, wide, call.qscale,     \
-                     call.lse, call.w_in, call.w_out, call.w_cols)
+                     call.lse, call.w_in, call.w_out, call.w_cols, sums)
 #define KVQ_WIN_WGT_S(T, D) \
   if (split) KVQ_WIN_WGT(T, D, true); else KVQ_WIN_WGT(T, D, false)
 #define KVQ_WIN_WGT_D(T)                                                                  \
@@ -228,6 +299,27 @@ int win_weights(const WinCall& call) {
 #undef KVQ_WIN_WGT_D
 #undef KVQ_WIN_WGT_S
 #undef KVQ_WIN_WGT
+          KVQ_LAUNCH_CHECK();
+          if (rows == 0) return KVQ_OK;
+          // the requests with several segments, a workgroup per 256 positions and head
+          WinArg add;
+          int n = 0;
+          int64_t blocks = 0;
+          for (int i = 0; i < count; ++i) {
+            if (arg.r[i].parts == 1) continue;
+            add.r[n] = arg.r[i];
+            add.r[n++].first = static_cast<int32_t>(blocks);
+            blocks += (static_cast<int64_t>(arg.r[i].len) + 255) / 256 * c.kvh;
+          }
+          if (blocks > 0x7fffffff) return KVQ_ERR_INVALID;
+#define KVQ_WIN_ADD(D)                                                                          \
+  hipLaunchKernelGGL((win_weights_add_kernel<D>), dim3(static_cast<unsigned>(blocks)), dim3(256), \
+                     0, call.stream, add, n, c, call.w_in, call.w_out, call.w_cols, sums)
+          if (c.d == 256)
+            KVQ_WIN_ADD(256);
+          else
+            KVQ_WIN_ADD(128);
+#undef KVQ_WIN_ADD
           KVQ_LAUNCH_CHECK();
           return KVQ_OK;
         });
