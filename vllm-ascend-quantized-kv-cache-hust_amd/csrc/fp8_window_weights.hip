@@ -2,20 +2,19 @@
 // Running attention weights of paged E4M3 positions, after the attention has left
 // each (row, head)'s log-sum-exp: w_j += sum over rows and heads of 2^(t_j - lse).
 //
-// A wave holds the keys of a run of positions (128 of them, 64 at head size 256) as
-// score operands in registers, exact, and takes the columns (row, head) of the kv
-// head's group through them 16 at a time:
-//   S^T = K * Q^T (lane (g, n): bytes D/4 g .. of position n of a 16-position group,
-//   so k-step s takes dims D/4 g + 8 s ..), p = exp2(fma(S, ks', -lse)),
+// A wave holds the keys of 64 positions as score operands in registers, exact, the
+// four waves of a workgroup 256 of one kv head, and the columns (row, head) of the
+// head's group go through them 16 at a time:
+//   S^T = K * Q^T (lane (g, n): bytes 64 w + 16 g .. of position n of a 16-position
+//   group, so k-step 2 w + x takes dims 64 w + 16 g + 8 x ..), p = exp2(fma(S, ks', -lse)),
 // summing p over columns in the lane, fp32; the 16 lanes of a position are added at
-// the end.  Every position belongs to one workgroup and is summed in a fixed order.
+// the end.  Every position belongs to one wave and is summed in a fixed order.  Columns
+// arrive in LDS by DMA, some groups ahead, for all four waves.
 //
-// Few columns: a wave per run, each code read once: bound by HBM (keys only).  Many
-// (SPLIT): the four waves of a workgroup share a run and take every fourth column
-// group, joined in LDS: bound by the exponentials, one per (row, head, position).  The
-// first positions are seen by every row and the last by few, so long requests' columns
-// are cut into segments of kSegTiles groups, whose sums meet in win_weights_add_kernel
-// (3 prompts of 1.5K - 4.1K, 32 heads on 8: 354 us uncut).
+// Few columns: each code is read once, bound by HBM (keys only).  Many: bound by the
+// exponentials, one per (row, head, position).  The first positions are seen by every
+// row and the last by few, so many columns are cut into segments of kSegTiles groups,
+// whose sums meet in win_weights_add_kernel.
 #include <algorithm>
 
 #include "fp8_window.h"
@@ -25,11 +24,18 @@ namespace {
 using namespace kvq;
 
 constexpr int kWaves = 4;
-constexpr int kSplitCols = 64;  // columns from which a workgroup's waves share a run
-constexpr int kSegTiles = 128;  // column groups of a segment
-
+constexpr int kGroups = 4;                   // 16-position groups of a wave
+constexpr int kSpan = 16 * kGroups * kWaves;  // positions of a workgroup
+constexpr int kSegTiles = 32;                // column groups of a segment
+// Column groups under way or in use, and the bytes of one: 16 rows of the query (16-byte
+// column x of row c at x ^ c % 16, or % 8), then their log-sum-exps, a copy per wave.
 template <int D>
-constexpr int run_groups() { return D == 256 ? 4 : 8; }
+constexpr int wgt_bufs() { return D == 256 ? 3 : 4; }
+template <int D>
+constexpr int wgt_buf_bytes() { return 32 * D + kWaves * 256; }
+// DMA instructions of a wave and column group
+template <int D>
+constexpr int wgt_dmas() { return (D == 256 ? 2 : 1) + 1; }
 
 typedef const __attribute__((address_space(4))) int32_t wgt_ci32;
 typedef const __attribute__((address_space(4))) int64_t wgt_ci64;
@@ -43,11 +49,11 @@ __device__ __forceinline__ float sum_row16(float x) {
   return x;
 }
 
-// Groups of 16 columns with rows that may see a position of [j0, j0 + run): [lo, hi).
-__device__ __forceinline__ void seeing_tiles(const WinReq& r, const WinCache& c, int j0, int run,
-                                             int& lo, int& hi) {
+// Groups of 16 columns with rows that may see a position of [j0, j0 + kSpan): [lo, hi).
+__device__ __forceinline__ void seeing_tiles(const WinReq& r, const WinCache& c, int j0, int& lo,
+                                             int& hi) {
   const int rep = static_cast<int>(c.rep.d), base = r.len - r.n;
-  const int j1 = min(j0 + run, r.len);
+  const int j1 = min(j0 + kSpan, r.len);
   const int row_lo = max(j0 - base, 0);
   int row_hi = r.n;
   if (c.window != kNoWindow && j0 >= c.sinks) {
@@ -56,52 +62,89 @@ __device__ __forceinline__ void seeing_tiles(const WinReq& r, const WinCache& c,
     row_hi = static_cast<int>(last < r.n ? (last < 0 ? 0 : last) : r.n);
   }
   lo = row_lo * rep / 16;
-  hi = j0 < r.len ? (row_hi * rep + 15) / 16 : 0;
+  hi = (row_hi * rep + 15) / 16;
 }
 
-// A unit is a workgroup's run(s) of one kv head (and a segment of their columns, of
-// r.parts): RUN positions if SPLIT, 4 RUN if not.
-template <typename T, int D, bool SPLIT>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// A unit is a span of positions of one kv head (and a segment of their columns, of
+// r.parts).
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * kWaves)
+__attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : D == 128 ? 3 : 4, D == 256 ? 2 : D == 128 ? 3 : 4)))
 win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int64_t q_stride,
                    int wide, float qscale, const float* __restrict__ lse, const float* w_in,
                    float* w_out, int64_t w_cols, float* __restrict__ seg_sums) {
-  constexpr int NGRP = run_groups<D>(), RUN = 16 * NGRP, KS = D / 32, W = D / 64;
-  __shared__ float s_scale[kWaves][RUN];
-  __shared__ float s_sum[kWaves][RUN];
+  constexpr int KS = D / 32, W = D / 64, NB = wgt_bufs<D>(), BYTES = wgt_buf_bytes<D>();
+  constexpr int PPR = D / 8, RPI = 64 / PPR;  // 16-byte columns of a row, rows of a DMA
+  __shared__ __align__(16) char bufs[NB * BYTES];
+  __shared__ __align__(16) float s_sum[kSpan];
   const WinReq r = win_req(count, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
   int u = static_cast<int>(blockIdx.x) - r.first;
   const int h = u % c.kvh;
   u /= c.kvh;
-  constexpr int SPAN = SPLIT ? RUN : kWaves * RUN;
-  const int spans = (r.len + SPAN - 1) / SPAN;
+  const int spans = (r.len + kSpan - 1) / kSpan;
   const int seg = u / spans;
-  const int wg0 = (u - seg * spans) * SPAN;
-  const int j0 = wg0 + (SPLIT ? 0 : wave * RUN);  // the wave's first position
+  const int span0 = (u - seg * spans) * kSpan;
+  const int j0 = span0 + 16 * kGroups * wave;  // the wave's first position
   const int rep = static_cast<int>(c.rep.d);
   const int cols = r.n * rep, base = r.len - r.n;
   int t_lo, t_hi;
-  seeing_tiles(r, c, j0, RUN, t_lo, t_hi);
-  if (SPLIT && r.parts > 1) {
+  seeing_tiles(r, c, span0, t_lo, t_hi);
+  if (r.parts > 1) {
     t_lo = max(t_lo, seg * kSegTiles);
     t_hi = min(t_hi, (seg + 1) * kSegTiles);
     if (t_lo >= t_hi) return;  // uniform over the workgroup
   }
-  float* sums = s_sum[wave];
+  w_f4 acc[kGroups];
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) acc[k] = w_f4{0.f, 0.f, 0.f, 0.f};
+  if (t_lo < t_hi) {  // uniform over the workgroup
+    // ---- columns on their way ----
+    const uint32_t lds0 = win_lds(bufs);
+    auto swz = [](int col) { return col % (PPR < 16 ? PPR : 16); };
+    // offset of column `col`'s query row, and its log-sum-exp's index
+    auto column = [&](int col, int64_t& at) -> int64_t {
+      const int x = min(col, cols - 1);  // (columns past the last see nothing)
+      const int row = static_cast<int>(c.rep.div(static_cast<uint32_t>(x)));
+      const int head = h * rep + x - row * rep;
+      at = (static_cast<int64_t>(r.q0) + row) * c.hq + head;
+      return (static_cast<int64_t>(r.q0) + row) * q_stride + static_cast<int64_t>(head) * D;
+    };
+    constexpr int INSTS = 16 / RPI;  // DMAs of the rows: waves 0 and 1 have a double at D = 64
+    auto issue = [&](int t, int b) {
+      int64_t at;
+#pragma unroll
+      for (int k = 0; k < (INSTS + kWaves - 1) / kWaves; ++k) {
+        const int i = (kWaves * k + wave) % INSTS;
+        const int col = RPI * i + lane / PPR, x = (lane % PPR) ^ swz(col);
+        const T* src = query + column(16 * t + col, at) + 8 * x;
+        if (wide & 1) {
+          const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds0 + b * BYTES + 1024 * i);
+          asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                       :
+                       : "v"(src), "{m0}"(m0)
+                       : "memory");
+        } else {
+          *reinterpret_cast<w_u4*>(bufs + b * BYTES + 1024 * i + 16 * lane) = load_op8(src, false);
+        }
+      }
+      column(16 * t + n, at);
+      const uint32_t m0 =
+          __builtin_amdgcn_readfirstlane(lds0 + b * BYTES + 32 * D + 256 * wave);
+      asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off"
+                   :
+                   : "v"(lse + at), "{m0}"(m0)
+                   : "memory");
+    };
 
-  w_f4 acc[NGRP];
-#pragma unroll
-  for (int k = 0; k < NGRP; ++k) acc[k] = w_f4{0.f, 0.f, 0.f, 0.f};
-  if (t_lo < t_hi) {  // wave-uniform
     // ---- keys ----
-    w_u4 key[NGRP][KS];
+    w_u4 key[kGroups][KS];
+    w_f4 ks[kGroups];
     {
-      w_u4 raw[NGRP][W];
-      float sc[NGRP];
+      w_u4 raw[kGroups][W];
 #pragma unroll
-      for (int k = 0; k < NGRP; ++k) {
+      for (int k = 0; k < kGroups; ++k) {
         // groups past the end read the last one (masked)
         const int p = min(j0 + 16 * k, (r.len - 1) & ~15);
         const uint32_t pg = c.bs.div(static_cast<uint32_t>(p));
@@ -116,116 +159,117 @@ win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, i
         const uint32_t lane_row = static_cast<uint32_t>(n * c.kvh);
 #pragma unroll
         for (int w = 0; w < W; ++w)
-          raw[k][w] = *reinterpret_cast<const w_u4*>(c.kd + row * D + lane_row * D + (D / 4) * kg +
-                                                     16 * w);
-        sc[k] = (c.ks + row)[lane_row];
+          raw[k][w] = *reinterpret_cast<const w_u4*>(c.kd + row * D + lane_row * D + 64 * w +
+                                                     16 * kg);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          ks[k][i] = (c.ks + row)[static_cast<uint32_t>((4 * kg + i) * c.kvh)];
       }
 #pragma unroll
-      for (int k = 0; k < NGRP; ++k) {
+      for (int k = 0; k < kGroups; ++k) {
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           key[k][2 * w] = code_op8<T>(raw[k][w][0], raw[k][w][1]);
           key[k][2 * w + 1] = code_op8<T>(raw[k][w][2], raw[k][w][3]);
         }
-        if (kg == 0) s_scale[wave][16 * k + n] = sc[k] * qscale;
+        ks[k] *= qscale;
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    // ---- columns ----
-    struct Cols {
-      w_u4 q[KS];
-      float lse;
-      int pos;
-    };
-    auto load = [&](int t) {
-      Cols x;
-      const int col = 16 * t + n;
-      const bool live = col < cols;
-      const int row = static_cast<int>(c.rep.div(static_cast<uint32_t>(live ? col : 0)));
-      const int head = h * rep + (live ? col : 0) - row * rep;
-      const int64_t at = static_cast<int64_t>(r.q0) + row;
-      const T* qrow = query + at * q_stride + static_cast<int64_t>(head) * D + (D / 4) * kg;
+    // landed: from here on only the DMAs are outstanding
 #pragma unroll
-      for (int s = 0; s < KS; ++s) x.q[s] = load_op8(qrow + 8 * s, wide & 1);
-      x.lse = lse[at * c.hq + head];
-      x.pos = live ? base + row : -1;
-      return x;
-    };
-    constexpr int STEP = SPLIT ? kWaves : 1;
-    int t = t_lo + (SPLIT ? wave : 0);
-    Cols now{};
-    if (t < t_hi) now = load(t);
-    for (; t < t_hi; t += STEP) {
-      Cols next = now;
-      if (t + STEP < t_hi) next = load(t + STEP);
+    for (int k = 0; k < kGroups; ++k) asm volatile("" : "+v"(ks[k]));
+    wait_vmcnt<0>();
+#pragma unroll
+    for (int b = 0; b < NB - 1; ++b)
+      if (t_lo + b < t_hi) issue(t_lo + b, b);
+
+    int buf = 0;
+    for (int t = t_lo; t < t_hi; ++t) {
+      if (t + NB - 2 < t_hi && (wide & 1)) {
+        wait_vmcnt<(NB - 2) * wgt_dmas<D>()>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      // group t is in LDS, and every wave is done with group t - 1, whose place the next
+      // DMA takes
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (t + NB - 1 < t_hi) issue(t + NB - 1, buf == 0 ? NB - 1 : buf - 1);
+      const char* cb = bufs + buf * BYTES;
+      buf = buf + 1 == NB ? 0 : buf + 1;
       const int pos_lo = base + static_cast<int>(c.rep.div(static_cast<uint32_t>(16 * t)));
       const int pos_hi =
           base + static_cast<int>(c.rep.div(static_cast<uint32_t>(min(16 * t + 15, cols - 1))));
+      constexpr int RUN = 16 * kGroups;
+      if (j0 > pos_hi || (j0 + RUN - 1 <= pos_lo - c.window && j0 >= c.sinks))
+        continue;  // uniform over the wave: nothing of its positions is seen
       const bool whole = 16 * t + 15 < cols && j0 + RUN <= r.len && j0 + RUN - 1 <= pos_lo &&
-                         (j0 > pos_hi - c.window || j0 + RUN - 1 < c.sinks);  // uniform
+                         (j0 > pos_hi - c.window || j0 + RUN - 1 < c.sinks);
+      w_u4 q[KS];
 #pragma unroll
-      for (int k = 0; k < NGRP; ++k) {
-        w_f4 s = w_f4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < KS; ++i)
+        q[i] = *reinterpret_cast<const w_u4*>(
+            cb + n * (2 * D) + 16 * ((8 * (i / 2) + 2 * kg + i % 2) ^ swz(n)));
+      const float off = *reinterpret_cast<const float*>(cb + 32 * D + 256 * wave + 4 * n);
+      w_f4 s[kGroups];
 #pragma unroll
-        for (int i = 0; i < KS; ++i) s = mfma_op(key[k][i], now.q[i], s, T{});
-        const w_f4 ks = *reinterpret_cast<const w_f4*>(&s_scale[wave][16 * k + 4 * kg]);
-        float p[4];
+      for (int k = 0; k < kGroups; ++k) s[k] = w_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) s[k] = mfma_op(key[k][i], q[i], s[k], T{});
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], ks[e], -now.lse));
-        if (!whole) {
+          s[k][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][e], ks[k][e], -off));
+      if (!whole) {
+        asm volatile("");  // a branch
+        const int pos =
+            16 * t + n < cols
+                ? base + static_cast<int>(c.rep.div(static_cast<uint32_t>(16 * t + n)))
+                : -1;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            p[e] = c.sees(now.pos, j0 + 16 * k + 4 * kg + e) ? p[e] : 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[k][e] += p[e];
-        if (k % 2) __builtin_amdgcn_sched_barrier(0);  // two groups at a time: registers
+            s[k][e] = c.sees(pos, j0 + 16 * k + 4 * kg + e) ? s[k][e] : 0.0f;
       }
-      now = next;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) acc[k] += s[k];
     }
   }
   // lane 0 of each 16 leaves positions 16 k + 4 kg + e
 #pragma unroll
-  for (int k = 0; k < NGRP; ++k) {
+  for (int k = 0; k < kGroups; ++k) {
     w_f4 x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = sum_row16(acc[k][e]);
-    if (n == 0) *reinterpret_cast<w_f4*>(sums + 16 * k + 4 * kg) = x;
+    if (n == 0) *reinterpret_cast<w_f4*>(s_sum + 16 * kGroups * wave + 16 * k + 4 * kg) = x;
   }
   __syncthreads();
-  const int64_t dst = (static_cast<int64_t>(r.wrow) * c.kvh + h) * w_cols;
-  for (int x = threadIdx.x; x < (SPLIT ? RUN : kWaves * RUN); x += 64 * kWaves) {
-    const int j = wg0 + x;
-    if (j >= r.len) break;
-    float sum;
-    if constexpr (SPLIT) {
-      sum = (s_sum[0][x] + s_sum[1][x]) + (s_sum[2][x] + s_sum[3][x]);
-      if (r.parts > 1) {
-        seg_sums[r.part0 + (static_cast<int64_t>(seg) * c.kvh + h) * r.len + j] = sum;
-        continue;
-      }
-    } else {
-      sum = s_sum[x / RUN][x % RUN];
-    }
-    w_out[dst + j] = (j < base ? w_in[dst + j] : 0.0f) + sum;
+  const int j = span0 + static_cast<int>(threadIdx.x);
+  static_assert(kSpan == 64 * kWaves, "a thread a position");
+  if (j >= r.len) return;
+  const float sum = s_sum[threadIdx.x];
+  if (r.parts > 1) {
+    seg_sums[r.part0 + (static_cast<int64_t>(seg) * c.kvh + h) * r.len + j] = sum;
+  } else {
+    const int64_t at = (static_cast<int64_t>(r.wrow) * c.kvh + h) * w_cols + j;
+    w_out[at] = (j < base ? w_in[at] : 0.0f) + sum;
   }
 }
 
-// The segments' sums of a position, in their order.  A unit is 256 positions of a head.
-template <int D>
-__global__ void __launch_bounds__(256)
+// The segments' sums of a position, in their order.  A unit is a span of a head.
+__global__ void __launch_bounds__(kSpan)
 win_weights_add_kernel(WinArg, int count, WinCache c, const float* w_in, float* w_out,
                        int64_t w_cols, const float* __restrict__ seg_sums) {
   const WinReq r = win_req(count, blockIdx.x);
   const int u = static_cast<int>(blockIdx.x) - r.first;
-  const int h = u % c.kvh, j = u / c.kvh * 256 + static_cast<int>(threadIdx.x);
+  const int h = u % c.kvh, span0 = u / c.kvh * kSpan;
+  const int j = span0 + static_cast<int>(threadIdx.x);
   if (j >= r.len) return;
-  constexpr int RUN = 16 * run_groups<D>();
   int lo, hi;
-  seeing_tiles(r, c, j / RUN * RUN, RUN, lo, hi);
+  seeing_tiles(r, c, span0, lo, hi);
   float sum = 0.0f;
   for (int s = lo / kSegTiles; s * kSegTiles < hi; ++s)
     sum += seg_sums[r.part0 + (static_cast<int64_t>(s) * c.kvh + h) * r.len + j];
@@ -245,18 +289,16 @@ bool win_weights_takes(const WinCall& call, int64_t b) {
 
 namespace {
 
-// Launches of the requests whose columns a workgroup's waves share, or of the others.
 template <typename G>
-int wgt_launches(const WinCall& call, int split, G&& go) {
+int wgt_launches(const WinCall& call, G&& go) {
   const WinCache& c = call.cache;
-  const int64_t run = 16 * (c.d == 256 ? 4 : 8) * (split ? 1 : kWaves);
   return win_launches(
       call,
       [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
-        const int64_t cols = call.qlens[b] * c.rep.d;
-        if (!win_weights_takes(call, b) || (cols >= kSplitCols) != (split != 0)) return false;
-        parts = split ? ((cols + 15) / 16 + kSegTiles - 1) / kSegTiles : 1;
-        units = (call.lens[b] + run - 1) / run * c.kvh * parts;
+        if (!win_weights_takes(call, b)) return false;
+        const int64_t tiles = (call.qlens[b] * c.rep.d + 15) / 16;
+        parts = (tiles + kSegTiles - 1) / kSegTiles;
+        units = (call.lens[b] + kSpan - 1) / kSpan * c.kvh * parts;
         rows = parts > 1 ? parts * c.kvh * call.lens[b] : 0;
         return true;
       },
@@ -267,7 +309,7 @@ int wgt_launches(const WinCall& call, int split, G&& go) {
 
 int64_t win_weights_bytes(const WinCall& call, int* rc) {
   int64_t most = 0;
-  *rc = wgt_launches(call, 1, [&](const WinArg&, int, int64_t, int64_t rows) -> int {
+  *rc = wgt_launches(call, [&](const WinArg&, int, int64_t, int64_t rows) -> int {
     most = std::max(most, rows * static_cast<int64_t>(sizeof(float)));
     return KVQ_OK;
   });
@@ -278,54 +320,40 @@ int win_weights(const WinCall& call, void* workspace) {
   const WinCache& c = call.cache;
   const int wide = call.q_wide() ? 1 : 0;
   float* sums = static_cast<float*>(workspace);
-  for (int split = 0; split < 2; ++split) {
-    const int rc = wgt_launches(
-        call, split, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
-#define KVQ_WIN_WGT(T, D, S)                                                                  \
-  hipLaunchKernelGGL((win_weights_kernel<T, D, S>), dim3(static_cast<unsigned>(units)),       \
+  return wgt_launches(call, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
+#define KVQ_WIN_WGT(T, D)                                                                     \
+  hipLaunchKernelGGL((win_weights_kernel<T, D>), dim3(static_cast<unsigned>(units)),          \
                      dim3(64 * kWaves), 0, call.stream, arg, count, c,                        \
                      static_cast<const T*>(call.query), call.q_stride, wide, call.qscale,     \
                      call.lse, call.w_in, call.w_out, call.w_cols, sums)
-#define KVQ_WIN_WGT_S(T, D) \
-  if (split) KVQ_WIN_WGT(T, D, true); else KVQ_WIN_WGT(T, D, false)
-#define KVQ_WIN_WGT_D(T)                                                                  \
-  if (c.d == 64) { KVQ_WIN_WGT_S(T, 64); } else if (c.d == 128) { KVQ_WIN_WGT_S(T, 128); } \
-  else { KVQ_WIN_WGT_S(T, 256); }
-          if (call.dtype == KVQ_DTYPE_BF16) {
-            KVQ_WIN_WGT_D(bf16);
-          } else {
-            KVQ_WIN_WGT_D(f16);
-          }
+#define KVQ_WIN_WGT_D(T)                                                                   \
+  if (c.d == 64) KVQ_WIN_WGT(T, 64); else if (c.d == 128) KVQ_WIN_WGT(T, 128);             \
+  else KVQ_WIN_WGT(T, 256)
+    if (call.dtype == KVQ_DTYPE_BF16) {
+      KVQ_WIN_WGT_D(bf16);
+    } else {
+      KVQ_WIN_WGT_D(f16);
+    }
 #undef KVQ_WIN_WGT_D
-#undef KVQ_WIN_WGT_S
 #undef KVQ_WIN_WGT
-          KVQ_LAUNCH_CHECK();
-          if (rows == 0) return KVQ_OK;
-          // the requests with several segments, a workgroup per 256 positions and head
-          WinArg add;
-          int n = 0;
-          int64_t blocks = 0;
-          for (int i = 0; i < count; ++i) {
-            if (arg.r[i].parts == 1) continue;
-            add.r[n] = arg.r[i];
-            add.r[n++].first = static_cast<int32_t>(blocks);
-            blocks += (static_cast<int64_t>(arg.r[i].len) + 255) / 256 * c.kvh;
-          }
-          if (blocks > 0x7fffffff) return KVQ_ERR_INVALID;
-#define KVQ_WIN_ADD(D)                                                                          \
-  hipLaunchKernelGGL((win_weights_add_kernel<D>), dim3(static_cast<unsigned>(blocks)), dim3(256), \
-                     0, call.stream, add, n, c, call.w_in, call.w_out, call.w_cols, sums)
-          if (c.d == 256)
-            KVQ_WIN_ADD(256);
-          else
-            KVQ_WIN_ADD(128);
-#undef KVQ_WIN_ADD
-          KVQ_LAUNCH_CHECK();
-          return KVQ_OK;
-        });
-    if (rc != KVQ_OK) return rc;
-  }
-  return KVQ_OK;
+    KVQ_LAUNCH_CHECK();
+    if (rows == 0) return KVQ_OK;
+    // the requests with several segments, a workgroup per span and head
+    WinArg add;
+    int n = 0;
+    int64_t blocks = 0;
+    for (int i = 0; i < count; ++i) {
+      if (arg.r[i].parts == 1) continue;
+      add.r[n] = arg.r[i];
+      add.r[n++].first = static_cast<int32_t>(blocks);
+      blocks += (static_cast<int64_t>(arg.r[i].len) + kSpan - 1) / kSpan * c.kvh;
+    }
+    if (blocks > 0x7fffffff) return KVQ_ERR_INVALID;
+    hipLaunchKernelGGL(win_weights_add_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSpan), 0,
+                       call.stream, add, n, c, call.w_in, call.w_out, call.w_cols, sums);
+    KVQ_LAUNCH_CHECK();
+    return KVQ_OK;
+  });
 }
 
 }  // namespace kvq
