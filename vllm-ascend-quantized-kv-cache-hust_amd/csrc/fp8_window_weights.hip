@@ -49,11 +49,11 @@ __device__ __forceinline__ float sum_row16(float x) {
   return x;
 }
 
-// Groups of 16 columns with rows that may see a position of [j0, j0 + kSpan): [lo, hi).
-__device__ __forceinline__ void seeing_tiles(const WinReq& r, const WinCache& c, int j0, int& lo,
-                                             int& hi) {
+// Groups of 16 columns with rows that may see a position of [j0, j0 + run): [lo, hi).
+__device__ __forceinline__ void seeing_tiles(const WinReq& r, const WinCache& c, int j0, int run,
+                                             int& lo, int& hi) {
   const int rep = static_cast<int>(c.rep.d), base = r.len - r.n;
-  const int j1 = min(j0 + kSpan, r.len);
+  const int j1 = min(j0 + run, r.len);
   const int row_lo = max(j0 - base, 0);
   int row_hi = r.n;
   if (c.window != kNoWindow && j0 >= c.sinks) {
@@ -90,7 +90,7 @@ win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, i
   const int rep = static_cast<int>(c.rep.d);
   const int cols = r.n * rep, base = r.len - r.n;
   int t_lo, t_hi;
-  seeing_tiles(r, c, span0, t_lo, t_hi);
+  seeing_tiles(r, c, span0, kSpan, t_lo, t_hi);
   if (r.parts > 1) {
     t_lo = max(t_lo, seg * kSegTiles);
     t_hi = min(t_hi, (seg + 1) * kSegTiles);
@@ -112,10 +112,47 @@ win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, i
       return (static_cast<int64_t>(r.q0) + row) * q_stride + static_cast<int64_t>(head) * D;
     };
     constexpr int INSTS = 16 / RPI;  // DMAs of the rows: waves 0 and 1 have a double at D = 64
+    // where 16 columns are whole rows, a group's addresses are the group before's plus a
+    // constant, and a lane's offset from them stays the same
+    const bool regular = (wide & 1) && 16 % rep == 0 && q_stride < (1 << 24);  // uniform
+    constexpr int PER_WAVE = (INSTS + kWaves - 1) / kWaves;
+    uint32_t lane_off[PER_WAVE], lane_lse;
+    const char* row_base = nullptr;
+    const float* lse_base = nullptr;
+    int64_t row_step = 0, lse_step = 0;
+    if (regular) {
+#pragma unroll
+      for (int k = 0; k < PER_WAVE; ++k) {
+        const int col = RPI * ((kWaves * k + wave) % INSTS) + lane / PPR;
+        const int row = static_cast<int>(c.rep.div(static_cast<uint32_t>(col)));
+        lane_off[k] = 2u * (static_cast<uint32_t>(row) * static_cast<uint32_t>(q_stride) +
+                            static_cast<uint32_t>(col - row * rep) * D) +
+                      16u * ((lane % PPR) ^ swz(col));
+      }
+      const int row = static_cast<int>(c.rep.div(static_cast<uint32_t>(n)));
+      lane_lse = 4u * static_cast<uint32_t>(row * c.hq + n - row * rep);
+      const int64_t row0 = r.q0 + static_cast<int64_t>(t_lo) * (16 / rep);
+      row_base = reinterpret_cast<const char*>(query + row0 * q_stride +
+                                               static_cast<int64_t>(h) * rep * D);
+      lse_base = lse + row0 * c.hq + h * rep;
+      row_step = 2 * (16 / rep) * q_stride;
+      lse_step = (16 / rep) * c.hq;
+    }
+    // (called for t_lo, t_lo + 1, .. in turn)
     auto issue = [&](int t, int b) {
+      if (regular && 16 * t + 15 < cols) {  // uniform
+#pragma unroll
+        for (int k = 0; k < PER_WAVE; ++k)
+          win_dma16(row_base, lane_off[k],
+                    lds0 + b * BYTES + 1024 * ((kWaves * k + wave) % INSTS));
+        win_dma4(lse_base, lane_lse, lds0 + b * BYTES + 32 * D + 256 * wave);
+        row_base += row_step;
+        lse_base += lse_step;
+        return;
+      }
       int64_t at;
 #pragma unroll
-      for (int k = 0; k < (INSTS + kWaves - 1) / kWaves; ++k) {
+      for (int k = 0; k < PER_WAVE; ++k) {
         const int i = (kWaves * k + wave) % INSTS;
         const int col = RPI * i + lane / PPR, x = (lane % PPR) ^ swz(col);
         const T* src = query + column(16 * t + col, at) + 8 * x;
@@ -183,6 +220,20 @@ win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, i
     for (int b = 0; b < NB - 1; ++b)
       if (t_lo + b < t_hi) issue(t_lo + b, b);
 
+    // groups that see some of the wave's positions, and those that see all of them
+    constexpr int RUN = 16 * kGroups;
+    int s_lo = t_hi, s_hi = t_hi;
+    if (j0 < r.len) seeing_tiles(r, c, j0, RUN, s_lo, s_hi);
+    int w_lo = t_hi, w_hi = t_hi;
+    if (j0 + RUN <= r.len) {
+      // row(16 t) >= j0 + RUN - 1 - base, 16 t + 15 < cols, row(16 t + 15) < j0 + window - base
+      w_lo = (max(j0 + RUN - 1 - base, 0) * rep + 15) / 16;
+      w_hi = cols / 16;
+      if (c.window != kNoWindow && j0 + RUN - 1 >= c.sinks) {
+        const int64_t last = static_cast<int64_t>(j0) + c.window - base;  // rows before it
+        w_hi = static_cast<int>(min(static_cast<int64_t>(w_hi), last <= 0 ? 0 : last * rep / 16));
+      }
+    }
     int buf = 0;
     for (int t = t_lo; t < t_hi; ++t) {
       if (t + NB - 2 < t_hi && (wide & 1)) {
@@ -196,14 +247,8 @@ win_weights_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, i
       if (t + NB - 1 < t_hi) issue(t + NB - 1, buf == 0 ? NB - 1 : buf - 1);
       const char* cb = bufs + buf * BYTES;
       buf = buf + 1 == NB ? 0 : buf + 1;
-      const int pos_lo = base + static_cast<int>(c.rep.div(static_cast<uint32_t>(16 * t)));
-      const int pos_hi =
-          base + static_cast<int>(c.rep.div(static_cast<uint32_t>(min(16 * t + 15, cols - 1))));
-      constexpr int RUN = 16 * kGroups;
-      if (j0 > pos_hi || (j0 + RUN - 1 <= pos_lo - c.window && j0 >= c.sinks))
-        continue;  // uniform over the wave: nothing of its positions is seen
-      const bool whole = 16 * t + 15 < cols && j0 + RUN <= r.len && j0 + RUN - 1 <= pos_lo &&
-                         (j0 > pos_hi - c.window || j0 + RUN - 1 < c.sinks);
+      if (t < s_lo || t >= s_hi) continue;  // uniform over the wave
+      const bool whole = t >= w_lo && t < w_hi;
       w_u4 q[KS];
 #pragma unroll
       for (int i = 0; i < KS; ++i)
@@ -269,7 +314,7 @@ win_weights_add_kernel(WinArg, int count, WinCache c, const float* w_in, float* 
   const int j = span0 + static_cast<int>(threadIdx.x);
   if (j >= r.len) return;
   int lo, hi;
-  seeing_tiles(r, c, span0, lo, hi);
+  seeing_tiles(r, c, span0, kSpan, lo, hi);
   float sum = 0.0f;
   for (int s = lo / kSegTiles; s * kSegTiles < hi; ++s)
     sum += seg_sums[r.part0 + (static_cast<int64_t>(s) * c.kvh + h) * r.len + j];
