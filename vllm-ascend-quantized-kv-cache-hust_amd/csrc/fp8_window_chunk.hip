@@ -57,7 +57,7 @@ typedef const __attribute__((address_space(4))) int64_t chk_ci64;
 
 template <typename T, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES)
-__attribute__((amdgpu_waves_per_eu(2, 2)))
+__attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
 win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int64_t q_stride,
                  int wide, float qscale, T* __restrict__ out, WinParts parts,
                  float* __restrict__ lse) {
@@ -528,8 +528,25 @@ int64_t chk_blocks(const WinCall& call, int64_t b, int tile_rows) {
       .groups;
 }
 
-// Segments of a tile's blocks: as many as the chip has slots for (eight waves a CU),
-// of at least 4 blocks each.
+// Segments of a tile's blocks: what ends soonest, in blocks of one workgroup (about 1.2
+// us), when `groups` workgroups of `blocks` blocks go over the chip's slots in rounds,
+// each a `segs`th as long, and the partial results (`bytes` of them a segment) go
+// through memory and back: 5 blocks and one per 6 MB.  (3 whole prompts of 1.5K - 4.1K,
+// 32 heads on 8, 1072 workgroups on 256 slots: 290 us uncut, 784 in 8 segments, their
+// joining being half of it; 2 chunks of 70 rows over 9000, 8 workgroups: 8 segments.)
+int64_t chk_segs(int64_t groups, int64_t blocks, int64_t slots, int64_t bytes) {
+  int64_t best = 1, cost = (groups + slots - 1) / slots * blocks;
+  for (int64_t segs = 2; segs <= 64 && segs * 4 <= blocks; ++segs) {
+    const int64_t rounds = (groups * segs + slots - 1) / slots;
+    const int64_t c = rounds * ((blocks + segs - 1) / segs) + 5 + segs * bytes / 6000000;
+    if (c < cost) {
+      best = segs;
+      cost = c;
+    }
+  }
+  return best;
+}
+
 template <typename G>
 int chk_launches(const WinCall& call, G&& go) {
   int cus = 0;
@@ -537,16 +554,22 @@ int chk_launches(const WinCall& call, G&& go) {
   if (rc != KVQ_OK) return rc;
   if (cus <= 0) cus = 256;
   const ChkShape shape = chk_shape(call, cus);
-  const int64_t slots = static_cast<int64_t>(cus) * 8 / shape.waves;
-  int64_t tiles = 0;
-  for (int64_t b = 0; b < call.batch; ++b) tiles += chk_tiles(call, b, shape.rows);
-  const int64_t spare = tiles > 0 ? slots / (tiles * call.cache.kvh) : 1;
+  const int64_t slots = static_cast<int64_t>(cus) * (call.cache.d == 64 ? 12 : 8) / shape.waves;
+  int64_t tiles = 0, blocks = 0;
+  for (int64_t b = 0; b < call.batch; ++b) {
+    const int64_t t = chk_tiles(call, b, shape.rows);
+    tiles += t;
+    if (t > 0) blocks = std::max(blocks, chk_blocks(call, b, shape.rows));
+  }
+  const int64_t groups = tiles * call.cache.kvh;
+  const int64_t segs =
+      chk_segs(groups, blocks, slots, groups * shape.rows * call.cache.d * 8);
   return win_launches(
       call,
       [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
         const int64_t t = chk_tiles(call, b, shape.rows);
         if (t == 0) return false;
-        parts = std::max<int64_t>(1, std::min<int64_t>(spare, chk_blocks(call, b, shape.rows) / 4));
+        parts = std::max<int64_t>(1, std::min(segs, chk_blocks(call, b, shape.rows) / 4));
         rows = win_part_rows(call, b, parts);
         units = t * parts * call.cache.kvh;
         return true;
