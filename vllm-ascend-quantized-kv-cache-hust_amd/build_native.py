@@ -57,6 +57,8 @@ EXTRA_FLAGS = {
     # registers: the 256-dim decode otherwise copies its 64 running sums between
     # the two files on every tile
     "decode_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    # likewise
+    "fp8_window_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -26,7 +26,7 @@ struct WinReq {
   int32_t first;  // units (workgroups, items) of the requests before it
   int32_t parts;  // partial results per row
   int32_t part0;  // its first partial row
-  int32_t wrow;   // its row of the running weights
+  int32_t wrow;   // its row of the running weights; where the decode leaves scores, theirs
 };
 constexpr int kWinReqs = 112;
 struct WinArg {
@@ -205,6 +205,7 @@ struct WinCall {
   int64_t w_cols;
   void* out;
   float* lse;  // per (row, head), where running weights are kept
+  float* scores;  // of the requests whose weights are summed from them (win_scores_at)
   hipStream_t stream;
   bool q_wide() const {
     return (reinterpret_cast<uintptr_t>(query) & 15) == 0 && q_stride % 8 == 0;
@@ -250,6 +251,20 @@ int win_launches(const WinCall& call, U&& shape, G&& go) {
 inline int64_t win_part_rows(const WinCall& call, int64_t b, int64_t parts) {
   return parts > 1 ? parts * call.qlens[b] * call.cache.hq : 0;
 }
+// Requests whose decode leaves its scores in the workspace, [kv head][column][positions,
+// a multiple of 16] in the log2 domain, for the weights to be summed from: writing and
+// reading 4 bytes a column and position is less than the keys once more (D + 4 bytes)
+// below this many columns, while all of them stay a small workspace.
+constexpr int kScoreCols = 16;
+constexpr int64_t kScoreBytes = 256ll << 20;
+struct WinScores {
+  bool on;
+  int64_t units;  // of 16 floats
+};
+inline int64_t win_score_units(const WinCall& call, int64_t b) {
+  return call.qlens[b] * call.cache.hq * ((call.lens[b] + 15) / 16);
+}
+
 inline int64_t win_parts_bytes(int64_t rows, int d) {
   return rows * (static_cast<int64_t>(d) + 2) * static_cast<int64_t>(sizeof(float));
 }
@@ -260,6 +275,8 @@ int launch_win_join(const WinCall& call, const WinArg& arg, int count, WinParts 
 // fp8_window_decode.hip: requests of few rows.  _takes: request b is one of them
 // (the geometry is one of the matrix kernels'); _bytes: the partial results.
 bool win_decode_takes(const WinCall& call, int64_t b);
+bool win_decode_scores(const WinCall& call, int64_t b);
+WinScores win_scores(const WinCall& call);
 int64_t win_decode_bytes(const WinCall& call, int* rc);
 int win_decode(const WinCall& call, void* workspace);
 
@@ -268,10 +285,11 @@ bool win_chunk_takes(const WinCall& call, int64_t b);
 int64_t win_chunk_bytes(const WinCall& call, int* rc);
 int win_chunk(const WinCall& call, void* workspace);
 
-// fp8_window_weights.hip: the running weights of the requests of that geometry.
+// fp8_window_weights.hip: the running weights of the requests of that geometry; `scores`:
+// those of win_decode_scores from their scores.
 bool win_weights_takes(const WinCall& call, int64_t b);
-int64_t win_weights_bytes(const WinCall& call, int* rc);
-int win_weights(const WinCall& call, void* workspace);
+int64_t win_weights_bytes(const WinCall& call, const WinScores& scores, int* rc);
+int win_weights(const WinCall& call, const WinScores& scores, void* workspace);
 
 // 16-bit queries, head sizes 64, 128 and 256, whole groups of 16 positions a page, at
 // most 16 query heads per kv head, codes on 16-byte bounds.

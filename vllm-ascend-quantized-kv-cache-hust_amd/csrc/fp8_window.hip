@@ -325,14 +325,25 @@ WinCall make_call(const void* query, int dtype, int64_t query_stride, const int6
   return call;
 }
 
-// Bytes of the partial results: the kernels run one after another and share them.
-int64_t parts_bytes(const WinCall& call, bool weigh, int* rc) {
+// A call's workspace: log-sum-exps, the decode's scores, partial results (the kernels run
+// one after another and share these).
+struct Layout {
+  int64_t lse, scores, parts;
+  WinScores scored;
+  int64_t total() const { return lse + scores + parts; }
+};
+Layout layout_of(const WinCall& call, bool weigh, int* rc) {
+  Layout x{};
+  x.lse = lse_bytes(call.qlens, call.batch, call.cache.hq, weigh);
+  if (weigh) x.scored = win_scores(call);
+  x.scores = 64 * x.scored.units;
   const int64_t few = win_decode_bytes(call, rc);
-  if (*rc != KVQ_OK) return 0;
+  if (*rc != KVQ_OK) return x;
   const int64_t many = win_chunk_bytes(call, rc);
-  if (*rc != KVQ_OK) return 0;
-  const int64_t sums = weigh ? win_weights_bytes(call, rc) : 0;
-  return align16(std::max(std::max(few, many), sums));
+  if (*rc != KVQ_OK) return x;
+  const int64_t sums = weigh ? win_weights_bytes(call, x.scored, rc) : 0;
+  x.parts = align16(std::max(std::max(few, many), sums));
+  return x;
 }
 
 }  // namespace
@@ -347,9 +358,8 @@ extern "C" int64_t kvq_fp8_pth_window_attn_workspace_bytes(
   // (caches off a 16-byte bound need less: the size does not know the addresses)
   const WinCall call = make_call(nullptr, dtype, 0, seq_lens, query_lens, batch, num_heads,
                                  num_kv_heads, head_size, 1.0f, window, sinks, block_size);
-  const int64_t parts = parts_bytes(call, with_weights != 0, &rc);
-  return rc != KVQ_OK ? KVQ_ERR_INVALID
-                      : lse_bytes(query_lens, batch, num_heads, with_weights != 0) + parts;
+  const Layout layout = layout_of(call, with_weights != 0, &rc);
+  return rc != KVQ_OK ? KVQ_ERR_INVALID : layout.total();
 }
 
 extern "C" int kvq_fp8_pth_window_attn(
@@ -398,22 +408,25 @@ extern "C" int kvq_fp8_pth_window_attn(
   call.w_cols = weight_cols;
   call.out = out;
   call.stream = static_cast<hipStream_t>(stream);
-  const int64_t lse = lse_bytes(query_lens, batch, num_heads, weigh);
-  const int64_t need = lse + parts_bytes(call, weigh, &rc);
+  const Layout layout = layout_of(call, weigh, &rc);
   if (rc != KVQ_OK) return rc;
-  if (need > 0 && (!aligned16(workspace, nullptr) || !workspace || workspace_bytes < need))
+  if (layout.total() > 0 &&
+      (!workspace || !aligned16(workspace, nullptr) || workspace_bytes < layout.total()))
     return KVQ_ERR_INVALID;
+  char* ws = static_cast<char*>(workspace);
   call.lse = weigh ? static_cast<float*>(workspace) : nullptr;
-  rc = win_decode(call, static_cast<char*>(workspace) + lse);
+  call.scores = layout.scored.on ? reinterpret_cast<float*>(ws + layout.lse) : nullptr;
+  void* parts = ws + layout.lse + layout.scores;
+  rc = win_decode(call, parts);
   if (rc != KVQ_OK) return rc;
-  rc = win_chunk(call, static_cast<char*>(workspace) + lse);
+  rc = win_chunk(call, parts);
   if (rc != KVQ_OK) return rc;
   KVQ_DISPATCH_FLOAT(dtype, T, {
     rc = attend_general<T>(call);
     if (rc != KVQ_OK) return rc;
     if (weigh) rc = weigh_general<T>(call);
     if (rc != KVQ_OK) return rc;
-    if (weigh) rc = win_weights(call, static_cast<char*>(workspace) + lse);
+    if (weigh) rc = win_weights(call, layout.scored, parts);
   });
   return rc;
 }

@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(64 * dec_waves<D>())
 __attribute__((amdgpu_waves_per_eu(dec_waves<D>() / 4, dec_waves<D>() / 4)))
 win_decode_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int64_t q_stride,
                   int wide, float qscale, int split, int hpw, T* __restrict__ out,
-                  WinParts parts, float* __restrict__ lse) {
+                  WinParts parts, float* __restrict__ lse, float* __restrict__ scores) {
   constexpr int CH = D / 16;    // 16-byte chunks of a row
   constexpr int RPI = 64 / CH;  // rows a DMA instruction brings
   constexpr int KS = D / 32;    // k-steps of a score
@@ -202,6 +202,13 @@ win_decode_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, in
           seen |= on ? 1u << (4 * j + e) : 0u;
           s[j][e] = on ? s[j][e] : -INFINITY;
         }
+    }
+    if (scores && live && cols < kScoreCols) {
+      // (one pass; the positions past the end have their places)
+      float* dst = scores + 16 * static_cast<int64_t>(r.wrow) +
+                   (static_cast<int64_t>(h) * cols + col) * ((r.len + 15) & ~15) + 4 * g;
+      *reinterpret_cast<w_f4*>(dst + p0) = s[0];
+      if (p1 != 0x7ffffff0) *reinterpret_cast<w_f4*>(dst + p1) = s[1];
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -422,6 +429,20 @@ bool win_decode_takes(const WinCall& call, int64_t b) {
          call.qlens[b] * c.rep.d <= kDecodeCols;
 }
 
+bool win_decode_scores(const WinCall& call, int64_t b) {
+  return call.qlens[b] > 0 && call.qlens[b] * call.cache.rep.d < kScoreCols &&
+         win_decode_takes(call, b);
+}
+
+WinScores win_scores(const WinCall& call) {
+  WinScores s{false, 0};
+  for (int64_t b = 0; b < call.batch; ++b)
+    if (win_decode_scores(call, b)) s.units += win_score_units(call, b);
+  s.on = s.units > 0 && 64 * s.units <= kScoreBytes;
+  if (!s.on) s.units = 0;
+  return s;
+}
+
 namespace {
 
 int64_t dec_groups(const WinCall& call, int64_t b) {
@@ -468,15 +489,23 @@ int win_decode(const WinCall& call, void* workspace) {
   const WinCache& c = call.cache;
   const int hpw = dec_hpw(c.kvh, c.d);
   const int wide = (call.q_wide() ? 1 : 0) | (aligned16(call.out, nullptr) ? 2 : 0);
-  int64_t split = 0;
-  return dec_launches(call, &split, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
+  int64_t split = 0, scored = 0;
+  return dec_launches(call, &split, [&](const WinArg& plan, int count, int64_t units, int64_t rows) -> int {
+    WinArg arg = plan;
+    if (call.scores)
+      for (int i = 0; i < count; ++i)
+        if (win_decode_scores(call, arg.r[i].table)) {
+          arg.r[i].wrow = static_cast<int32_t>(scored);
+          scored += win_score_units(call, arg.r[i].table);
+        }
     const WinParts parts{static_cast<float*>(workspace),
                          static_cast<float*>(workspace) + rows * c.d};
 #define KVQ_WIN_DECODE(T, D)                                                                  \
   hipLaunchKernelGGL((win_decode_kernel<T, D>), dim3(static_cast<unsigned>(units)),           \
                      dim3(64 * hpw), hpw * 2 * dec_tile_bytes<D>(), call.stream, arg, count, c, \
                      static_cast<const T*>(call.query), call.q_stride, wide, call.qscale,     \
-                     static_cast<int>(split), hpw, static_cast<T*>(call.out), parts, call.lse)
+                     static_cast<int>(split), hpw, static_cast<T*>(call.out), parts, call.lse, \
+                     call.scores)
 #define KVQ_WIN_DECODE_D(T)                                                     \
   if (c.d == 64) KVQ_WIN_DECODE(T, 64); else if (c.d == 128) KVQ_WIN_DECODE(T, 128); \
   else KVQ_WIN_DECODE(T, 256)

@@ -15,6 +15,9 @@
 // exponentials, one per (row, head, position).  The first positions are seen by every
 // row and the last by few, so many columns are cut into segments of kSegTiles groups,
 // whose sums meet in win_weights_add_kernel.
+//
+// Requests of fewer than kScoreCols columns: from the scores their decode left
+// (win_weights_scores_kernel), 4 bytes a column and position instead of the key.
 #include <algorithm>
 
 #include "fp8_window.h"
@@ -322,6 +325,42 @@ win_weights_add_kernel(WinArg, int count, WinCache c, const float* w_in, float* 
   w_out[at] = (j < r.len - r.n ? w_in[at] : 0.0f) + sum;
 }
 
+// From the decode's scores.  A unit is 1024 positions of one kv head, four a thread.
+constexpr int kScoreSpan = 1024;
+__global__ void __launch_bounds__(256)
+win_weights_scores_kernel(WinArg, int count, WinCache c, const float* __restrict__ lse,
+                          const float* __restrict__ scores, const float* w_in, float* w_out,
+                          int64_t w_cols) {
+  const WinReq r = win_req(count, blockIdx.x);
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int h = u % c.kvh, j0 = u / c.kvh * kScoreSpan + 4 * static_cast<int>(threadIdx.x);
+  if (j0 >= r.len) return;
+  const int rep = static_cast<int>(c.rep.d), cols = r.n * rep, base = r.len - r.n;
+  const int64_t padded = (r.len + 15) & ~15;
+  // part0: where the request's scores are, in units of 16
+  const float* src = scores + 16 * static_cast<int64_t>(r.part0) + h * cols * padded + j0;
+  w_f4 sum = w_f4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < r.n; ++i) {
+    const float* off = lse + (static_cast<int64_t>(r.q0) + i) * c.hq + h * rep;
+    bool on[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) on[e] = c.sees(base + i, j0 + e);
+    if (!(on[0] || on[1] || on[2] || on[3])) continue;  // (their scores may be unwritten)
+    for (int k = 0; k < rep; ++k) {
+      const w_f4 t = *reinterpret_cast<const w_f4*>(src + (i * rep + k) * padded);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(t[e] - off[k]);
+        sum[e] += on[e] ? p : 0.0f;
+      }
+    }
+  }
+  const int64_t at = (static_cast<int64_t>(r.wrow) * c.kvh + h) * w_cols + j0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j0 + e < r.len) w_out[at + e] = (j0 + e < base ? w_in[at + e] : 0.0f) + sum[e];
+}
+
 }  // namespace
 
 namespace kvq {
@@ -335,12 +374,12 @@ bool win_weights_takes(const WinCall& call, int64_t b) {
 namespace {
 
 template <typename G>
-int wgt_launches(const WinCall& call, G&& go) {
+int wgt_launches(const WinCall& call, const WinScores& scores, G&& go) {
   const WinCache& c = call.cache;
   return win_launches(
       call,
       [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
-        if (!win_weights_takes(call, b)) return false;
+        if (!win_weights_takes(call, b) || (scores.on && win_decode_scores(call, b))) return false;
         const int64_t tiles = (call.qlens[b] * c.rep.d + 15) / 16;
         parts = (tiles + kSegTiles - 1) / kSegTiles;
         units = (call.lens[b] + kSpan - 1) / kSpan * c.kvh * parts;
@@ -352,20 +391,42 @@ int wgt_launches(const WinCall& call, G&& go) {
 
 }  // namespace
 
-int64_t win_weights_bytes(const WinCall& call, int* rc) {
+int64_t win_weights_bytes(const WinCall& call, const WinScores& scores, int* rc) {
   int64_t most = 0;
-  *rc = wgt_launches(call, [&](const WinArg&, int, int64_t, int64_t rows) -> int {
+  *rc = wgt_launches(call, scores, [&](const WinArg&, int, int64_t, int64_t rows) -> int {
     most = std::max(most, rows * static_cast<int64_t>(sizeof(float)));
     return KVQ_OK;
   });
   return most;
 }
 
-int win_weights(const WinCall& call, void* workspace) {
+int win_weights(const WinCall& call, const WinScores& scores, void* workspace) {
   const WinCache& c = call.cache;
   const int wide = call.q_wide() ? 1 : 0;
   float* sums = static_cast<float*>(workspace);
-  return wgt_launches(call, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
+  if (scores.on) {
+    int64_t scored = 0;
+    const int rc = win_launches(
+        call,
+        [&](int64_t b, int64_t& units, int64_t&, int64_t&) {
+          units = (call.lens[b] + kScoreSpan - 1) / kScoreSpan * c.kvh;
+          return win_decode_scores(call, b);
+        },
+        [&](const WinArg& plan, int count, int64_t units, int64_t) -> int {
+          WinArg arg = plan;
+          for (int i = 0; i < count; ++i) {
+            arg.r[i].part0 = static_cast<int32_t>(scored);
+            scored += win_score_units(call, arg.r[i].table);
+          }
+          hipLaunchKernelGGL(win_weights_scores_kernel, dim3(static_cast<unsigned>(units)),
+                             dim3(256), 0, call.stream, arg, count, c, call.lse, call.scores,
+                             call.w_in, call.w_out, call.w_cols);
+          KVQ_LAUNCH_CHECK();
+          return KVQ_OK;
+        });
+    if (rc != KVQ_OK) return rc;
+  }
+  return wgt_launches(call, scores, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
 #define KVQ_WIN_WGT(T, D)                                                                     \
   hipLaunchKernelGGL((win_weights_kernel<T, D>), dim3(static_cast<unsigned>(units)),          \
                      dim3(64 * kWaves), 0, call.stream, arg, count, c,                        \
