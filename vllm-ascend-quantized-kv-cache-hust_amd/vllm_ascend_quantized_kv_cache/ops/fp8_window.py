@@ -128,14 +128,18 @@ def _weight_rows(what: str, weights, out_weights, weight_rows, batch: int, longe
         apart = abs(target.data_ptr() - weights.data_ptr())
         if 0 < apart < 4 * weights.numel():
             raise RuntimeError(f"{what}: out_weights overlaps weights.")
-    array, rows = _lengths(what, range(batch) if weight_rows is None else weight_rows,
-                           "weight_rows")
-    if len(rows) != batch:
-        raise RuntimeError(f"{what}: {len(rows)} weight_rows for {batch} requests.")
-    if batch and (max(rows) >= weights.shape[0] or len(set(rows)) != batch):
+    if weight_rows is None:
+        rows = range(batch)
+        array = (ctypes.c_int64 * batch)(*rows)
+    else:
+        array, rows = _lengths(what, weight_rows, "weight_rows")
+        if len(rows) != batch:
+            raise RuntimeError(f"{what}: {len(rows)} weight_rows for {batch} requests.")
+    if batch and (max(rows) >= weights.shape[0]
+                  or (weight_rows is not None and len(set(rows)) != batch)):
         raise RuntimeError(
             f"{what}: weight_rows must be distinct rows of the {weights.shape[0]} in weights, got "
-            f"{rows}."
+            f"{list(rows)}."
         )
     if longest > weights.shape[2]:
         raise RuntimeError(
@@ -317,14 +321,24 @@ def fp8_per_token_head_evict(
         raise RuntimeError(f"{_EVICT}: sinks and recent must not be negative.")
     lens, totals = _lengths(_EVICT, seq_lens, "seq_lens")
     batch = len(totals)
-    keeps, budgets = _lengths(
-        _EVICT, [keep] * batch if isinstance(keep, (int, np.integer)) else keep, "keep")
-    if len(budgets) != batch:
-        raise RuntimeError(f"{_EVICT}: {len(budgets)} budgets for {batch} requests.")
-    if any(k < sinks + recent and n > k for n, k in zip(totals, budgets)):
-        raise RuntimeError(f"{_EVICT}: a budget under sinks + recent = {sinks + recent}: {budgets}.")
-    target, rows = _weight_rows(_EVICT, weights, out_weights, weight_rows, batch,
-                                max(totals, default=0), kvh, k_data)
+    longest = max(totals, default=0)
+    stay = sinks + recent
+    if isinstance(keep, int):
+        if keep < 0:
+            raise RuntimeError(f"{_EVICT}: negative keep.")
+        keeps = (ctypes.c_int64 * batch)(*[keep] * batch)
+        new_lens = [n if n < keep else keep for n in totals]
+        short = keep < stay and longest > keep
+    else:
+        keeps, budgets = _lengths(_EVICT, keep, "keep")
+        if len(budgets) != batch:
+            raise RuntimeError(f"{_EVICT}: {len(budgets)} budgets for {batch} requests.")
+        new_lens = [n if n < k else k for n, k in zip(totals, budgets)]
+        short = any(k < stay and n > k for n, k in zip(totals, budgets))
+    if short:
+        raise RuntimeError(f"{_EVICT}: a budget under sinks + recent = {stay}: {keep}.")
+    target, rows = _weight_rows(_EVICT, weights, out_weights, weight_rows, batch, longest, kvh,
+                                k_data)
     _check_same_device("block_table", block_table, k_data)
     table, host = _table(block_table, block_table_host, batch)
     out_table = out_host = None
@@ -344,13 +358,11 @@ def fp8_per_token_head_evict(
         lens, keeps, batch, nb, bs) if batch else 0
     if bad == _native.KVQ_ERR_CAPACITY:
         raise RuntimeError(
-            f"{_EVICT}: a block table does not cover its rows (block_size={bs}, "
-            f"longest={max(totals)}).")
+            f"{_EVICT}: a block table does not cover its rows (block_size={bs}, longest={longest}).")
     if bad > 0:
         why = "outside the cache" if bad % 2 else "in use twice"
         raise RuntimeError(f"{_EVICT}: request {(bad - 1) // 2} has a page {why}.")
     _native.check(bad, _EVICT)
-    new_lens = [min(n, k) for n, k in zip(totals, budgets)]
     most = max(new_lens, default=0)
     _native.require_gpu_tensors(_EVICT, k_data)
     with _on_device(k_data):
