@@ -205,6 +205,7 @@ struct WinCall {
   int64_t w_cols;
   void* out;
   float* lse;  // per (row, head), where running weights are kept
+  bool tiles_only;  // requests of few rows go with the chunks' tiles (win_tiles_only)
   float* scores;  // of the requests whose weights are summed from them (win_scores_at)
   hipStream_t stream;
   bool q_wide() const {
@@ -275,6 +276,7 @@ int launch_win_join(const WinCall& call, const WinArg& arg, int count, WinParts 
 // fp8_window_decode.hip: requests of few rows.  _takes: request b is one of them
 // (the geometry is one of the matrix kernels'); _bytes: the partial results.
 bool win_decode_takes(const WinCall& call, int64_t b);
+bool win_tiles_only(const WinCall& call);
 bool win_decode_scores(const WinCall& call, int64_t b);
 WinScores win_scores(const WinCall& call);
 int64_t win_decode_bytes(const WinCall& call, int* rc);

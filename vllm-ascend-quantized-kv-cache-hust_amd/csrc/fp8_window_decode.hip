@@ -422,11 +422,42 @@ int64_t dec_split(const WinCall& call, int cus, F&& groups) {
 
 namespace kvq {
 
-bool win_decode_takes(const WinCall& call, int64_t b) {
+namespace {
+
+bool dec_few(const WinCall& call, int64_t b) {
+  return call.lens[b] > 0 && call.qlens[b] > 0 && call.qlens[b] * call.cache.rep.d <= kDecodeCols;
+}
+
+bool dec_geometry(const WinCall& call) {
   const WinCache& c = call.cache;
   return win_matrix_geometry(call.dtype, c.hq, c.kvh, c.d, static_cast<int>(c.bs.d)) &&
-         aligned16(c.kd, c.vd) && call.lens[b] > 0 &&
-         call.qlens[b] * c.rep.d <= kDecodeCols;
+         aligned16(c.kd, c.vd);
+}
+
+}  // namespace
+
+bool win_decode_takes(const WinCall& call, int64_t b) {
+  return !call.tiles_only && dec_few(call, b) && dec_geometry(call);
+}
+
+// In a batch with chunks, requests of few rows ride with their tiles where they see no
+// more than the chunks do and all tiles run at once: a launch less (19 requests of up to
+// 26 positions with 3 - 11 rows each, head size 256, with weights: 43 and 37 us a call).
+bool win_tiles_only(const WinCall& call) {
+  if (!dec_geometry(call)) return false;
+  const WinCache& c = call.cache;
+  int64_t few = 0, many = 0, tiles = 0;  // most positions seen by either kind
+  for (int64_t b = 0; b < call.batch; ++b) {
+    if (call.lens[b] <= 0 || call.qlens[b] <= 0) continue;
+    const int64_t seen = WinSpan::of(static_cast<int>(call.lens[b]), static_cast<int>(call.qlens[b]),
+                                     c.window, c.sinks, kGroup).groups;
+    int64_t& most = dec_few(call, b) ? few : many;
+    most = std::max(most, seen);
+    tiles += (call.qlens[b] * c.rep.d + 127) / 128;
+  }
+  int cus = 0;
+  if (device_cu_count(&cus) != KVQ_OK || cus <= 0) cus = 256;
+  return few > 0 && few <= many && tiles * c.kvh <= cus;
 }
 
 bool win_decode_scores(const WinCall& call, int64_t b) {
@@ -436,9 +467,20 @@ bool win_decode_scores(const WinCall& call, int64_t b) {
 
 WinScores win_scores(const WinCall& call) {
   WinScores s{false, 0};
-  for (int64_t b = 0; b < call.batch; ++b)
-    if (win_decode_scores(call, b)) s.units += win_score_units(call, b);
-  s.on = s.units > 0 && 64 * s.units <= kScoreBytes;
+  int64_t keys = 0;  // (position, kv head)s that the scores spare
+  bool rest = false;
+  for (int64_t b = 0; b < call.batch; ++b) {
+    if (win_decode_scores(call, b)) {
+      s.units += win_score_units(call, b);
+      keys += call.lens[b] * call.cache.kvh;
+    } else {
+      rest = rest || (call.qlens[b] > 0 && call.lens[b] > 0);
+    }
+  }
+  // beside other requests, whose keys are read anyway, only where it is worth a launch
+  // (5 us, or 25 MB of keys)
+  s.on = s.units > 0 && 64 * s.units <= kScoreBytes &&
+         (!rest || keys * call.cache.d >= (25 << 20));
   if (!s.on) s.units = 0;
   return s;
 }
