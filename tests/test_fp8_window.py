@@ -40,6 +40,7 @@ def _attend(lens=(40, 17), news=(1, 3), hq=4, kvh=2, d=64, edit=None, **kw):
     (dict(query=torch.zeros(3, 4, 64, dtype=torch.bfloat16)), "sum to 4"),
     (dict(scale=0.0), "scale must be positive"),
     (dict(scale=float("nan")), "scale must be positive"),
+    (dict(scale=float("inf")), "scale must be positive"),
     (dict(window=0), "window must be at least 1"),
     (dict(sinks=-1), "sinks must not be negative"),
     (dict(seq_lens=[40, -1]), "negative seq_lens"),
@@ -94,6 +95,15 @@ def test_a_call_without_rows_needs_no_gpu():
     q = torch.ones(2, 1, 16, dtype=torch.bfloat16)
     assert not attend(q, *c.args(), [5], [0], 0.1).any()
     assert attend(q[:0], *c.args(), [], [], 0.1).shape == (0, 1, 16)
+
+
+def test_numpy_lengths_and_tensors_are_lengths():
+    c = ref.Cache([5, 7], 1, 16, 16)
+    q = torch.ones(0, 1, 16, dtype=torch.bfloat16)
+    for lens in (np.array([5, 7]), torch.tensor([5, 7]), (5, 7), [np.int32(5), 7]):
+        assert attend(q, *c.args(), lens, [0, 0], 0.1).shape == (0, 1, 16)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        evict(*c.args(), np.array([5, 7]), torch.zeros(2, 1, 7), np.int64(5))
 
 
 @pytest.mark.parametrize("window,sinks,bad,ok", [

@@ -89,6 +89,19 @@ def test_long_histories(gpu_device, news, window, sinks):
     _attend_and_check(gpu_device, [9000, 5003, 2048], news, 16, 4, 128, 128, BF16, window, sinks)
 
 
+@pytest.mark.parametrize("news", [[12000], [3000], [700, 12000]])
+def test_long_prompts(gpu_device, news):
+    """Whole prompts: many tiles, columns in segments, few and many of them."""
+    _attend_and_check(gpu_device, [12000] * len(news), news, 2, 1, 64, 64, BF16, None, 0)
+
+
+@pytest.mark.parametrize("kvh,hq", [(1, 2), (1, 15), (1, 16)])
+def test_one_request_over_many_positions(gpu_device, kvh, hq):
+    """Hundreds of parts of a row; scores from the decode, and keys read again."""
+    _attend_and_check(gpu_device, [150000], [1], hq, kvh, 64, 64, FP16, None, 0)
+    _attend_and_check(gpu_device, [150000], [1], hq, kvh, 64, 64, BF16, 100000, 3000)
+
+
 @pytest.mark.parametrize("d,hq,kvh", [(64, 4, 2), (256, 8, 1)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_long_chunks_other_heads(gpu_device, d, hq, kvh, dtype):
@@ -349,6 +362,41 @@ def test_eviction_of_many_requests(gpu_device):
     lens = [int(n) for n in rng.integers(0, 60, 400)]
     _evict_and_check(gpu_device, lens, 20, 2, 3, 1, 16, 16, "ties", fresh=False)
     _evict_and_check(gpu_device, lens, 20, 2, 3, 1, 16, 16, "ties", fresh=True)
+
+
+def test_captured_evictions(gpu_device):
+    """Into fresh pages, short and long rows; replays follow the weights."""
+    lens, keep = [40000, 900], 500
+    c = ref.Cache(lens, 2, 64, 64, device=gpu_device, seed=6, spare=40)
+    used = set(c.host.reshape(-1).tolist())
+    free = [i for i in range(c.nb) if i not in used][:16]
+    dst = torch.tensor(free, dtype=torch.int32, device=gpu_device).view(2, 8)
+    w = torch.rand(2, 2, 40000, device=gpu_device)
+    out_w = torch.zeros_like(w)
+    kw = dict(sinks=4, recent=50, out_block_table=dst, out_weights=out_w, block_table_host=c.host,
+              out_block_table_host=dst.cpu().numpy().astype(np.int64))
+    evict(*c.args(), lens, w, keep, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, kept = evict(*c.args(), lens, w, keep, **kw)
+    for seed in range(3):
+        w.copy_(torch.rand(w.shape, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (kept, c.k, c.ks, c.v, c.vs, out_w)]
+        _, again = evict(*c.args(), lens, w, keep, **kw)
+        torch.cuda.synchronize()
+        for a, b in zip(got, (again, c.k, c.ks, c.v, c.vs, out_w)):
+            assert torch.equal(a, b)
+        ids = ref.kept_rows(w[0, 1].cpu().numpy(), lens[0], keep, 4, 50)
+        np.testing.assert_array_equal(again[0, 1].cpu().numpy(), ids)
+
+
+def test_no_requests(gpu_device):
+    c = ref.Cache([10], 1, 16, 16, device=gpu_device)
+    new_lens, kept = evict(*c.args(), [], torch.ones(1, 1, 10, device=gpu_device), 4)
+    assert new_lens == [] and kept.shape == (0, 1, 0)
 
 
 def test_nothing_to_keep(gpu_device):

@@ -24,7 +24,8 @@
 //   workgroup per (request, kv head, side) walks its chunks in order, and within
 //   a chunk every load has returned before the first store.
 #include <algorithm>
-#include <vector>
+#include <memory>
+#include <new>
 
 #include "fp8_window.h"
 
@@ -620,7 +621,8 @@ extern "C" int64_t kvq_fp8_pth_evict_check(const void* block_table, const void* 
     return KVQ_ERR_INVALID;
   // 1: a page of some request's rows, 2: of one whose rows move within it (or a
   // page that rows move to)
-  std::vector<uint8_t> seen(static_cast<size_t>(num_blocks), 0);
+  const std::unique_ptr<uint8_t[]> seen(new (std::nothrow) uint8_t[num_blocks]());
+  if (!seen) return KVQ_ERR_INVALID;
   for (int64_t b = 0; b < batch; ++b) {
     if (seq_lens[b] < 0 || keep[b] < 0) return KVQ_ERR_INVALID;
     if (seq_lens[b] > max_blocks * block_size) return KVQ_ERR_CAPACITY;

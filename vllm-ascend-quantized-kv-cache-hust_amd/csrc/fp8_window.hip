@@ -184,11 +184,22 @@ win_join_kernel(WinArg, int hq, WinParts parts, T* __restrict__ out, float* __re
   l = sum_wave64(l);
   const int slice = tid / LANES, k = tid % LANES;
   w_f4 acc = w_f4{0.f, 0.f, 0.f, 0.f};
-  for (int s = slice; s < count; s += SLICES) {
-    const float ms = ml[s * stride][0];
-    if (ms == -INFINITY) continue;  // sees nothing
-    const w_f4 y = *reinterpret_cast<const w_f4*>(parts.o + (part0 + s * stride + x) * D + 4 * k);
-    acc += __builtin_amdgcn_exp2f(ms - m) * y;
+  constexpr int DEPTH = 4;  // loads in flight
+  for (int s0 = slice; s0 < count; s0 += DEPTH * SLICES) {
+    float ms[DEPTH];
+    w_f4 y[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      const int64_t s = min(s0 + i * SLICES, count - 1);
+      ms[i] = s0 + i * SLICES < count ? ml[s * stride][0] : -INFINITY;
+      y[i] = *reinterpret_cast<const w_f4*>(parts.o + (part0 + s * stride + x) * D + 4 * k);
+    }
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      const float w = ms[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[i] - m);
+      // one that sees nothing may be unwritten
+      acc += ms[i] == -INFINITY ? w_f4{0.f, 0.f, 0.f, 0.f} : w * y[i];
+    }
   }
   s_o[slice][k] = acc;
   __syncthreads();
@@ -378,7 +389,7 @@ extern "C" int kvq_fp8_pth_window_attn(
   for (int64_t b = 0; b < batch; ++b) rows += query_lens[b];
   if (rows == 0) return KVQ_OK;
   if (!query || !k_data || !k_scale || !v_data || !v_scale || !block_table || !out ||
-      num_blocks <= 0 || max_blocks < 0 || !(scale > 0.0f) ||
+      num_blocks <= 0 || max_blocks < 0 || !(scale > 0.0f && scale < INFINITY) ||
       query_stride < static_cast<int64_t>(num_heads) * head_size)
     return KVQ_ERR_INVALID;
   if (block_index_type != KVQ_INDEX_I32 && block_index_type != KVQ_INDEX_I64)

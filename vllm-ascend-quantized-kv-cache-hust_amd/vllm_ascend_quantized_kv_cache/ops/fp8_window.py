@@ -198,7 +198,7 @@ def fp8_per_token_head_window_attention(
     dtype = _native.dtype_code(query.dtype)
     if kvh == 0 or hq == 0 or hq % kvh:
         raise RuntimeError(f"{_ATTENTION}: {hq} query heads over {kvh} kv heads.")
-    if not scale > 0:
+    if not 0 < scale < float("inf"):
         raise RuntimeError(f"{_ATTENTION}: scale must be positive, got {scale}.")
     if window is not None and window < 1:
         raise RuntimeError(f"{_ATTENTION}: window must be at least 1, got {window}.")
@@ -323,7 +323,8 @@ def fp8_per_token_head_evict(
     batch = len(totals)
     longest = max(totals, default=0)
     stay = sinks + recent
-    if isinstance(keep, int):
+    if isinstance(keep, (int, np.integer)):
+        keep = int(keep)
         if keep < 0:
             raise RuntimeError(f"{_EVICT}: negative keep.")
         keeps = (ctypes.c_int64 * batch)(*[keep] * batch)
