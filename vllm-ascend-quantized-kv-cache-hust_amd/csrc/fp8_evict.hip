@@ -166,7 +166,8 @@ __device__ __forceinline__ void count_keys(const WeightRow<NK>& row, uint32_t* h
 
 // The bin in which the `want`th key from the top lies, and which of the bin's it is;
 // c0 and c1: thread t's counts of bins 2 N - 1 - 2 t and 2 N - 2 - 2 t, N threads.
-__device__ __forceinline__ void find_bin(uint32_t c0, uint32_t c1, uint32_t& bin, uint32_t& want,
+// Returns whether it is the bin's last.
+__device__ __forceinline__ bool find_bin(uint32_t c0, uint32_t c1, uint32_t& bin, uint32_t& want,
                                          uint32_t* s_wave, uint32_t* s_found) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -177,12 +178,16 @@ __device__ __forceinline__ void find_bin(uint32_t c0, uint32_t c1, uint32_t& bin
   if (above < want && want <= above + c0 + c1) {  // one thread
     const bool upper = want <= above + c0;
     s_found[0] = static_cast<uint32_t>(2 * kSelThreads - 1 - 2 * tid) - (upper ? 0u : 1u);
-    s_found[1] = want - above - (upper ? 0u : c0);
+    const uint32_t nth = want - above - (upper ? 0u : c0);
+    s_found[1] = nth;
+    s_found[2] = nth == (upper ? c0 : c1);
   }
   __syncthreads();
   bin = s_found[0];
   want = s_found[1];
+  const bool last = s_found[2] != 0;
   __syncthreads();  // read before the next call writes them
+  return last;
 }
 
 // Writes the survivors of this workgroup's run: the keys above `prefix`, and those equal
@@ -231,7 +236,7 @@ evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const f
                     float* w_out, int64_t w_cols, int32_t* __restrict__ kept, int64_t kept_cols) {
   __shared__ uint32_t s_hist[kBins];
   __shared__ uint32_t s_wave[2][kSelWaves];
-  __shared__ uint32_t s_found[2];
+  __shared__ uint32_t s_found[3];
   const EvictReq r = evict_req(count, blockIdx.x);
   const int h = static_cast<int>(blockIdx.x) - r.first;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -256,9 +261,15 @@ evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const f
   for (int round = 0; round < 3; ++round) {
     count_keys(row, s_hist, round, prefix, mask, static_cast<uint32_t>(sinks + recent));
     uint32_t bin;
-    find_bin(s_hist[kBins - 1 - 2 * tid], s_hist[kBins - 2 - 2 * tid], bin, want, s_wave[0], s_found);
+    const bool all = find_bin(s_hist[kBins - 1 - 2 * tid], s_hist[kBins - 2 - 2 * tid], bin, want,
+                              s_wave[0], s_found);
     prefix |= bin << round_shift(round);
     mask |= round_field(round) << round_shift(round);
+    if (all && round < 2) {  // uniform: every key of the bin stays, whatever its other bits
+      prefix = prefix ? prefix - 1 : 0;  // (0 is no weight's key)
+      want = 0;
+      break;
+    }
   }
   emit_rows(row, prefix, want, 0, 0, s_wave, ids, out);
 }
@@ -305,7 +316,7 @@ evict_count_kernel(EvictArg, int count, int kvh, int sinks, int recent, const fl
                    int64_t w_cols, EvictWs ws) {
   __shared__ uint32_t s_hist[kBins];
   __shared__ uint32_t s_wave[2][kSelWaves];
-  __shared__ uint32_t s_found[2];
+  __shared__ uint32_t s_found[3];
   const EvictReq r = evict_req(count, blockIdx.x);
   const int u = static_cast<int>(blockIdx.x) - r.first;
   const int h = u % kvh, chunk = u / kvh, chunks = (r.len + kChunk - 1) / kChunk;
@@ -346,7 +357,7 @@ evict_emit_kernel(EvictArg, int count, int kvh, int sinks, int recent, const flo
                   float* w_out, int64_t w_cols, int32_t* __restrict__ kept, int64_t kept_cols,
                   EvictWs ws) {
   __shared__ uint32_t s_wave[2][kSelWaves];
-  __shared__ uint32_t s_found[2];
+  __shared__ uint32_t s_found[3];
   const EvictReq r = evict_req(count, blockIdx.x);
   const int u = static_cast<int>(blockIdx.x) - r.first;
   const int h = u % kvh, chunk = u / kvh, chunks = (r.len + kChunk - 1) / kChunk;
