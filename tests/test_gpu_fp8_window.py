@@ -108,6 +108,27 @@ def test_long_chunks_other_heads(gpu_device, d, hq, kvh, dtype):
     _attend_and_check(gpu_device, [3000, 2999], [600, 1], hq, kvh, d, 64, dtype, 777, 33)
 
 
+@pytest.mark.parametrize("window,sinks", [(None, 0), (3500, 20)])
+@pytest.mark.parametrize("batch,n,hq,kvh,d", [(16, 8, 32, 8, 128), (64, 5, 20, 4, 64),
+                                              (32, 4, 16, 2, 256)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_a_few_rows_of_a_large_batch(gpu_device, batch, n, hq, kvh, d, dtype, window, sinks):
+    """25 or 32 rows and heads to a kv head, over enough positions for one pass over
+    the codes, beside single tokens, a longer chunk and a request without history.
+    The requests share pages, and values that are NaN: seen by all rows of some
+    requests, by some rows of others, by none of others."""
+    lens = [4000 - 9 * b for b in range(batch)] + [4000, 0, 37, 300]
+    news = [n - (b % 3 == 1) for b in range(batch)] + [1, 0, 1, 50]
+    c = ref.Cache([4000], kvh, d, 16, device=gpu_device, seed=5, spare=60)
+    rng = np.random.default_rng(5)
+    c.host = np.stack([rng.permutation(c.nb)[:250] for _ in lens]).astype(np.int64)
+    c.table = torch.from_numpy(c.host).to(gpu_device, torch.int32)
+    c.lens = lens
+    for b, back, dim in ((0, 2, 3), (1, 1, d - 1), (2, 60, 17)):
+        c.v.view(-1, kvh, d)[int(c.slots(b, lens[b] - back)), 0, dim] = 0xff
+    _attend_and_check(gpu_device, lens, news, hq, kvh, d, 16, dtype, window, sinks, cache=c)
+
+
 def test_many_requests(gpu_device):
     """More requests than one launch's argument holds, some without rows."""
     rng = np.random.default_rng(5)

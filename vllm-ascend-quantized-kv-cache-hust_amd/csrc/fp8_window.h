@@ -205,6 +205,7 @@ struct WinCall {
   int64_t w_cols;
   void* out;
   float* lse;  // per (row, head), where running weights are kept
+  int few_cols;     // columns (row, head) up to which a request is one of few rows (win_few_cols)
   bool tiles_only;  // requests of few rows go with the chunks' tiles (win_tiles_only)
   float* scores;  // of the requests whose weights are summed from them (win_scores_at)
   hipStream_t stream;
@@ -276,6 +277,7 @@ int launch_win_join(const WinCall& call, const WinArg& arg, int count, WinParts 
 // fp8_window_decode.hip: requests of few rows.  _takes: request b is one of them
 // (the geometry is one of the matrix kernels'); _bytes: the partial results.
 bool win_decode_takes(const WinCall& call, int64_t b);
+int win_few_cols(const WinCall& call);
 bool win_tiles_only(const WinCall& call);
 bool win_decode_scores(const WinCall& call, int64_t b);
 WinScores win_scores(const WinCall& call);

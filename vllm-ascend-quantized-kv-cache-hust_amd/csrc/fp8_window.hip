@@ -333,6 +333,7 @@ WinCall make_call(const void* query, int dtype, int64_t query_stride, const int6
   call.cache.sinks =
       static_cast<int>(window > 0 ? std::min<int64_t>(sinks, kMaxPositions) : 0);
   call.qscale = scale * 1.4426950408889634f;
+  call.few_cols = win_few_cols(call);
   call.tiles_only = win_tiles_only(call);
   return call;
 }

@@ -2,10 +2,10 @@
 // Windowed attention over paged E4M3 rows for requests of few rows (decode): the
 // codes stream through once, bound by HBM.
 //
-// A unit is an item (a run of a request's visible 16-position groups), a pass of 16
-// columns (row, head) and some kv heads, one wave per kv head; the waves of a
-// workgroup step through the item together, so that the rows of one token, which
-// its heads' codes share DRAM pages for, are requested together.
+// A unit is an item (a run of a request's visible 16-position groups) and some kv heads,
+// one wave per kv head, which takes all of the request's columns (row, head): at most 16
+// or 32.  The waves of a workgroup step through the item together, so that the rows of
+// one token, which its heads' codes share DRAM pages for, are requested together.
 //
 // A wave's tile is two groups of 16 positions, double-buffered in its own LDS by
 // DMA (16 bytes a lane, whole rows; 16-byte chunk c of row t sits at c ^ t % (D/16),
@@ -46,7 +46,8 @@ constexpr int dec_dmas() { return D / 16 + 1; }
 typedef const __attribute__((address_space(4))) int32_t dec_ci32;
 typedef const __attribute__((address_space(4))) int64_t dec_ci64;
 
-template <typename T, int D>
+// NG: groups of 16 columns, sharing the loads and conversions.
+template <typename T, int D, int NG>
 __global__ void __launch_bounds__(64 * dec_waves<D>())
 __attribute__((amdgpu_waves_per_eu(dec_waves<D>() / 4, dec_waves<D>() / 4)))
 win_decode_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int64_t q_stride,
@@ -64,23 +65,24 @@ win_decode_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, in
   const int n = lane & 15, g = lane >> 4;
   const int rep = static_cast<int>(c.rep.d);
   const int cols = r.n * rep;
-  const int passes = (cols + 15) / 16, hgs = c.kvh / hpw;
-  int u = static_cast<int>(blockIdx.x) - r.first;
-  const int hg = u % hgs;
-  u /= hgs;
-  const int pass = u % passes, item = u / passes;
+  const int hgs = c.kvh / hpw;
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int hg = u % hgs, item = u / hgs;
   const int h = hg * hpw + wave;
   const WinSpan span = WinSpan::of(r.len, r.n, c.window, c.sinks, kGroup);
   const int g0 = item * split, g1 = min(span.groups, g0 + split);
-  // the column's row, head and position; -1 sees nothing
-  const int col = 16 * pass + n;
-  const bool live = col < cols;
-  const int row = static_cast<int>(c.rep.div(static_cast<uint32_t>(live ? col : 0)));
-  const int head = h * rep + (live ? col : 0) - row * rep;
-  const int pos = live ? r.len - r.n + row : -1;
-  const int pos_lo = r.len - r.n + static_cast<int>(c.rep.div(static_cast<uint32_t>(16 * pass)));
-  const int pos_hi = r.len - r.n + static_cast<int>(c.rep.div(
-                                       static_cast<uint32_t>(min(16 * pass + 15, cols - 1))));
+  // the columns' rows, heads and positions; -1 sees nothing
+  bool live[NG];
+  int row[NG], head[NG], pos[NG];
+#pragma unroll
+  for (int x = 0; x < NG; ++x) {
+    const int col = 16 * x + n;
+    live[x] = col < cols;
+    row[x] = static_cast<int>(c.rep.div(static_cast<uint32_t>(live[x] ? col : 0)));
+    head[x] = h * rep + (live[x] ? col : 0) - row[x] * rep;
+    pos[x] = live[x] ? r.len - r.n + row[x] : -1;
+  }
+  const int pos_lo = r.len - r.n, pos_hi = r.len - 1;
 
   // ---- tiles ----
   char* const buf = dec_lds + wave * 2 * dec_tile_bytes<D>();
@@ -133,25 +135,31 @@ win_decode_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, in
 
   int64_t s0 = slot(g0), s1 = slot(g0 + 1);
   issue(0, s0, s1);
-  w_u4 q[KS];
-  {
-    const T* qrow = query + (static_cast<int64_t>(r.q0) + row) * q_stride +
-                    static_cast<int64_t>(head) * D + (D / 4) * g;
+  w_u4 q[NG][KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) q[s] = load_op8(qrow + 8 * s, wide & 1);
+  for (int x = 0; x < NG; ++x) {
+    const T* qrow = query + (static_cast<int64_t>(r.q0) + row[x]) * q_stride +
+                    static_cast<int64_t>(head[x]) * D + (D / 4) * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[x][s] = load_op8(qrow + 8 * s, wide & 1);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
-      if (!live) q[s] = w_u4{0, 0, 0, 0};
+      if (!live[x]) q[x][s] = w_u4{0, 0, 0, 0};
     // landed before the loop: a wait for them inside it would be one for the DMA too
 #pragma unroll
-    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[s]));
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[x][s]));
   }
   s0 = slot(g0 + 2);
   s1 = slot(g0 + 3);
-  float m = -INFINITY, l = 0.0f;
-  w_f4 o[DB];
+  float m[NG], l[NG];
+  w_f4 o[DB][NG];
 #pragma unroll
-  for (int t = 0; t < DB; ++t) o[t] = w_f4{0.f, 0.f, 0.f, 0.f};
+  for (int x = 0; x < NG; ++x) {
+    m[x] = -INFINITY;
+    l[x] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DB; ++t) o[t][x] = w_f4{0.f, 0.f, 0.f, 0.f};
+  }
 
   int which = 0;
   for (int gr = g0; gr < g1; gr += kTileGroups, which ^= 1) {
@@ -174,79 +182,94 @@ win_decode_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, in
     const bool whole = p1 != 0x7ffffff0 && all_see(p0) && all_see(p1);  // uniform
 
     // ---- scores ----
-    w_f4 s[2];
-    float mx = -INFINITY;
+    w_f4 s[2][NG];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const char* kr = b + (16 * j + n) * D;
-      w_f4 acc = w_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < NG; ++x) s[j][x] = w_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         const w_u4 k = *reinterpret_cast<const w_u4*>(kr + 16 * ((W * g + w) ^ (n % CH)));
-        acc = mfma_op(code_op8<T>(k[0], k[1]), q[2 * w], acc, T{});
-        acc = mfma_op(code_op8<T>(k[2], k[3]), q[2 * w + 1], acc, T{});
+        const w_u4 k0 = code_op8<T>(k[0], k[1]), k1 = code_op8<T>(k[2], k[3]);
+#pragma unroll
+        for (int x = 0; x < NG; ++x) {
+          s[j][x] = mfma_op(k0, q[x][2 * w], s[j][x], T{});
+          s[j][x] = mfma_op(k1, q[x][2 * w + 1], s[j][x], T{});
+        }
       }
       const w_f4 ks = *reinterpret_cast<const w_f4*>(sc + 16 * j + 4 * g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[j][e] = acc[e] * (ks[e] * qscale);
+      for (int x = 0; x < NG; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][x][e] *= ks[e] * qscale;
     }
-    uint32_t seen = 0xff;
+    uint32_t seen[NG];
+#pragma unroll
+    for (int x = 0; x < NG; ++x) seen[x] = 0xff;
     if (!whole) {
-      seen = 0;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        seen[x] = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int p = (j ? p1 : p0) + 4 * g + e;
+            const bool on = c.sees(pos[x], p);
+            seen[x] |= on ? 1u << (4 * j + e) : 0u;
+            s[j][x][e] = on ? s[j][x][e] : -INFINITY;
+          }
+      }
+    }
+    if (scores && live[0] && cols < kScoreCols) {
+      // (one group of columns; the positions past the end have their places)
+      float* dst = scores + 16 * static_cast<int64_t>(r.wrow) +
+                   (static_cast<int64_t>(h) * cols + n) * ((r.len + 15) & ~15) + 4 * g;
+      *reinterpret_cast<w_f4*>(dst + p0) = s[0][0];
+      if (p1 != 0x7ffffff0) *reinterpret_cast<w_f4*>(dst + p1) = s[1][0];
+    }
+    const w_f4 vs[2] = {*reinterpret_cast<const w_f4*>(sc + 32 + 4 * g),
+                        *reinterpret_cast<const w_f4*>(sc + 48 + 4 * g)};
+    w_u4 bh[NG], bl[NG];  // p * value scale, hi and lo parts
+#pragma unroll
+    for (int x = 0; x < NG; ++x) {
+      float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[j][x][e]);
+      mx = max_rows4(mx);
+      const float m_new = fmaxf(m[x], mx);
+      const float base = m_new == -INFINITY ? 0.0f : m_new;
+      const float alpha = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - base);
+      m[x] = m_new;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float pv[4];
+#pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int p = (j ? p1 : p0) + 4 * g + e;
-          const bool on = c.sees(pos, p);
-          seen |= on ? 1u << (4 * j + e) : 0u;
-          s[j][e] = on ? s[j][e] : -INFINITY;
+          const float p = __builtin_amdgcn_exp2f(s[j][x][e] - base);
+          sum += p;
+          pv[e] = whole || (seen[x] >> (4 * j + e)) & 1 ? p * vs[j][e] : 0.0f;
         }
-    }
-    if (scores && live && cols < kScoreCols) {
-      // (one pass; the positions past the end have their places)
-      float* dst = scores + 16 * static_cast<int64_t>(r.wrow) +
-                   (static_cast<int64_t>(h) * cols + col) * ((r.len + 15) & ~15) + 4 * g;
-      *reinterpret_cast<w_f4*>(dst + p0) = s[0];
-      if (p1 != 0x7ffffff0) *reinterpret_cast<w_f4*>(dst + p1) = s[1];
-    }
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[j][e]);
-    mx = max_rows4(mx);
-    const float m_new = fmaxf(m, mx);
-    const float base = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - base);
-    m = m_new;
-    float sum = 0.0f;
-    uint32_t ph[4], pl[4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const w_f4 vs = *reinterpret_cast<const w_f4*>(sc + 32 + 16 * j + 4 * g);
-      float pv[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = __builtin_amdgcn_exp2f(s[j][e] - base);
-        sum += p;
-        pv[e] = whole || (seen >> (4 * j + e)) & 1 ? p * vs[e] : 0.0f;
+        for (int e = 0; e < 4; e += 2) {
+          const uint32_t hi = pack_pair(pv[e], pv[e + 1], bf16{});
+          bh[x][2 * j + e / 2] = hi;
+          bl[x][2 * j + e / 2] = pack_pair(pv[e] - __uint_as_float(hi << 16),
+                                           pv[e + 1] - __uint_as_float(hi & 0xffff0000u), bf16{});
+        }
       }
+      l[x] = l[x] * alpha + sum;
+      if (__any(alpha != 1.0f)) {
 #pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const uint32_t hi = pack_pair(pv[e], pv[e + 1], bf16{});
-        ph[2 * j + e / 2] = hi;
-        pl[2 * j + e / 2] = pack_pair(pv[e] - __uint_as_float(hi << 16),
-                                      pv[e + 1] - __uint_as_float(hi & 0xffff0000u), bf16{});
+        for (int t = 0; t < DB; ++t) o[t][x] *= alpha;
       }
-    }
-    l = l * alpha + sum;
-    if (__any(alpha != 1.0f)) {
-#pragma unroll
-      for (int t = 0; t < DB; ++t) o[t] *= alpha;
     }
 
     // ---- values ----
-    const w_u4 bh = {ph[0], ph[1], ph[2], ph[3]}, bl = {pl[0], pl[1], pl[2], pl[3]};
     uint32_t v[2][4][W];  // [group][position 4 g + e][word]
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -287,48 +310,55 @@ win_decode_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, in
           for (int w = 0; w < W; ++w) odd |= nan_codes(v[j][e][w]);
     }
     if (__any(odd != 0)) {  // an edge tile with NaN codes
-      w_u4 ones;            // the columns' masks as operand
+      w_u4 ones[NG];        // the columns' masks as operands
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        ones[k] = ((seen >> (2 * k)) & 1 ? 0x3f80u : 0u) |
-                  ((seen >> (2 * k + 1)) & 1 ? 0x3f800000u : 0u);
+      for (int x = 0; x < NG; ++x)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          ones[x][k] = ((seen[x] >> (2 * k)) & 1 ? 0x3f80u : 0u) |
+                       ((seen[x] >> (2 * k + 1)) & 1 ? 0x3f800000u : 0u);
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         uint32_t tr[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint32_t x[4] = {v[j][0][w], v[j][1][w], v[j][2][w], v[j][3][w]};
+          uint32_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = nan_codes(v[j][e][w]) >> 7;
+            v[j][e][w] &= ~(x[e] * 0xffu);
+            x[e] *= 0x38u;  // the code of 1
+          }
           transpose(x, tr[j]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t n0 = nan_codes(tr[0][k]) >> 7, n1 = nan_codes(tr[1][k]) >> 7;
-          const w_u4 a = code_op8<bf16>(tr[0][k] & ~(n0 * 0xffu), tr[1][k] & ~(n1 * 0xffu));
-          w_f4& acc = o[4 * w + k];
-          acc = mfma_op(a, bh, acc, bf16{});
-          acc = mfma_op(a, bl, acc, bf16{});
-          // 0x38: the code of 1
-          const w_f4 hit = mfma_op(code_op8<bf16>(n0 * 0x38u, n1 * 0x38u), ones,
-                                   w_f4{0.f, 0.f, 0.f, 0.f}, bf16{});
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = hit[e] > 0.0f ? NAN : acc[e];
-        }
+          for (int x = 0; x < NG; ++x) {
+            const w_f4 hit = mfma_op(code_op8<bf16>(tr[0][k], tr[1][k]), ones[x],
+                                     w_f4{0.f, 0.f, 0.f, 0.f}, bf16{});
+            w_f4& acc = o[4 * w + k][x];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = hit[e] > 0.0f ? NAN : acc[e];
+          }
       }
-    } else {
+    }
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        uint32_t tr[2][4];
+    for (int w = 0; w < W; ++w) {
+      uint32_t tr[2][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t x[4] = {v[j][0][w], v[j][1][w], v[j][2][w], v[j][3][w]};
-          transpose(x, tr[j]);
-        }
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t x[4] = {v[j][0][w], v[j][1][w], v[j][2][w], v[j][3][w]};
+        transpose(x, tr[j]);
+      }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const w_u4 a = code_op8<bf16>(tr[0][k], tr[1][k]);
-          w_f4& acc = o[4 * w + k];
-          acc = mfma_op(a, bh, acc, bf16{});
-          acc = mfma_op(a, bl, acc, bf16{});
+      for (int k = 0; k < 4; ++k) {
+        const w_u4 a = code_op8<bf16>(tr[0][k], tr[1][k]);
+#pragma unroll
+        for (int x = 0; x < NG; ++x) {
+          w_f4& acc = o[4 * w + k][x];
+          acc = mfma_op(a, bh[x], acc, bf16{});
+          acc = mfma_op(a, bl[x], acc, bf16{});
         }
       }
     }
@@ -337,55 +367,56 @@ win_decode_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, in
     if (hpw > 1) __builtin_amdgcn_s_barrier();  // the workgroup's heads share the item
   }
 
-  // ---- results: o[t][e] is dim DB * (4 g + e) + t of the column ----
-  l = sum_rows4(l);
-  if (!live) return;
-  const int64_t at = (static_cast<int64_t>(r.q0) + row) * c.hq + head;
-  if (r.parts == 1) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  // ---- results: o[t][x][e] is dim DB * (4 g + e) + t of the column ----
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      T* dst = out + at * D + DB * (4 * g + e);
-      uint32_t w[DB / 2];
+  for (int x = 0; x < NG; ++x) {
+    const float sum = sum_rows4(l[x]);
+    if (!live[x]) continue;
+    const int64_t at = (static_cast<int64_t>(r.q0) + row[x]) * c.hq + head[x];
+    if (r.parts == 1) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-      for (int t = 0; t < DB; t += 2)
-        w[t / 2] = pack_pair(o[t][e] * inv, o[t + 1][e] * inv, T{});
-      if (wide & 2) {
-        if constexpr (DB == 4)
-          *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-        else
+      for (int e = 0; e < 4; ++e) {
+        T* dst = out + at * D + DB * (4 * g + e);
+        uint32_t w[DB / 2];
 #pragma unroll
-          for (int t = 0; t < DB / 8; ++t)
-            reinterpret_cast<uint4*>(dst)[t] =
-                make_uint4(w[4 * t], w[4 * t + 1], w[4 * t + 2], w[4 * t + 3]);
-      } else {
-        uint16_t* d16 = reinterpret_cast<uint16_t*>(dst);
+        for (int t = 0; t < DB; t += 2)
+          w[t / 2] = pack_pair(o[t][x][e] * inv, o[t + 1][x][e] * inv, T{});
+        if (wide & 2) {
+          if constexpr (DB == 4)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+          else
 #pragma unroll
-        for (int t = 0; t < DB / 2; ++t) {
-          d16[2 * t] = static_cast<uint16_t>(w[t]);
-          d16[2 * t + 1] = static_cast<uint16_t>(w[t] >> 16);
+            for (int t = 0; t < DB / 8; ++t)
+              reinterpret_cast<uint4*>(dst)[t] =
+                  make_uint4(w[4 * t], w[4 * t + 1], w[4 * t + 2], w[4 * t + 3]);
+        } else {
+          uint16_t* d16 = reinterpret_cast<uint16_t*>(dst);
+#pragma unroll
+          for (int t = 0; t < DB / 2; ++t) {
+            d16[2 * t] = static_cast<uint16_t>(w[t]);
+            d16[2 * t + 1] = static_cast<uint16_t>(w[t] >> 16);
+          }
         }
       }
+      if (lse && g == 0) lse[at] = sum == 0.0f ? INFINITY : m[x] + __builtin_amdgcn_logf(sum);
+      continue;
     }
-    if (lse && g == 0) lse[at] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
-    return;
-  }
-  const int64_t part = r.part0 + (static_cast<int64_t>(item) * r.n + row) * c.hq + head;
+    const int64_t part = r.part0 + (static_cast<int64_t>(item) * r.n + row[x]) * c.hq + head[x];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float* dst = parts.o + part * D + DB * (4 * g + e);
+    for (int e = 0; e < 4; ++e) {
+      float* dst = parts.o + part * D + DB * (4 * g + e);
 #pragma unroll
-    for (int t = 0; t < DB; t += 4)
-      *reinterpret_cast<w_f4*>(dst + t) = w_f4{o[t][e], o[t + 1][e], o[t + 2][e], o[t + 3][e]};
+      for (int t = 0; t < DB; t += 4)
+        *reinterpret_cast<w_f4*>(dst + t) =
+            w_f4{o[t][x][e], o[t + 1][x][e], o[t + 2][x][e], o[t + 3][x][e]};
+    }
+    if (g == 0)  // a NaN score leaves m without it, but not l
+      *reinterpret_cast<w_f2*>(parts.ml + 2 * part) = w_f2{sum != sum ? INFINITY : m[x], sum};
   }
-  if (g == 0)  // a NaN score leaves m without it, but not l
-    *reinterpret_cast<w_f2*>(parts.ml + 2 * part) = w_f2{l != l ? INFINITY : m, l};
 }
 
 // ---- host -----------------------------------------------------------------------
-
-// Rows up to which a request is one of few rows: columns of its passes.
-constexpr int kDecodeCols = 64;
 
 int dec_hpw(int kvh, int d) {
   const int most = d == 256 ? 4 : 8;
@@ -401,14 +432,19 @@ template <typename F>
 int64_t dec_split(const WinCall& call, int cus, F&& groups) {
   const WinCache& c = call.cache;
   const int64_t waves = c.d == 256 ? 4 : 8;
-  int64_t total = 0, requests = 0;
+  int64_t total = 0, requests = 0, cells = 0;  // (group, row, head)s
   for (int64_t b = 0; b < call.batch; ++b) {
     const int64_t n = groups(b);
     total += n;
+    cells += n * call.qlens[b] * c.hq;
     requests += n > 0;
   }
   const int64_t target = std::max<int64_t>(1, cus * waves / c.kvh);
-  int64_t split = std::max<int64_t>(4, ((total + target - 1) / target + 1) / 2 * 2);
+  // items of 4 groups, or of 8 where those of 4 leave 8 MB of partial results (4 requests
+  // of up to 16000 positions, 2 kv heads of 128, 16 columns: 20.5 for 23.1 us; 8 of up to
+  // 1000, 8 kv heads, 4 columns, which leave less: 17.2 for 13.3)
+  const int64_t least = cells / 4 * c.d * 4 > 8 << 20 ? 8 : 4;
+  int64_t split = std::max<int64_t>(least, ((total + target - 1) / target + 1) / 2 * 2);
   auto items = [&](int64_t s) {
     int64_t n = 0;
     for (int64_t b = 0; b < call.batch; ++b) n += (groups(b) + s - 1) / s;
@@ -425,7 +461,7 @@ namespace kvq {
 namespace {
 
 bool dec_few(const WinCall& call, int64_t b) {
-  return call.lens[b] > 0 && call.qlens[b] > 0 && call.qlens[b] * call.cache.rep.d <= kDecodeCols;
+  return call.lens[b] > 0 && call.qlens[b] > 0 && call.qlens[b] * call.cache.rep.d <= call.few_cols;
 }
 
 bool dec_geometry(const WinCall& call) {
@@ -440,9 +476,30 @@ bool win_decode_takes(const WinCall& call, int64_t b) {
   return !call.tiles_only && dec_few(call, b) && dec_geometry(call);
 }
 
+// Columns up to which a request comes here instead of to the tiles of
+// fp8_window_chunk.hip, both sides in us a call.  16: one request of 4000 positions, 8 kv
+// heads of 128, 4 and 16 columns, 14 and 17 here, 20 and 20 there; 8 of 1000, 13 and 19,
+// 22 and 23.  Past that the partial results cost more than the codes that a tile reads
+// again (4 of up to 16000, 2 kv heads, 16, 32 and 64 columns: 21, 30 and 40, 21, 22 and
+// 25), but where the requests of 17 - 32 columns have 100 MB of codes to stream (32 of up
+// to 2000: 55 and 56; of up to 16384: 171 and 391) and the others, whom the second group
+// of columns costs a fifth (122 and 147), are not most of the work.
+int win_few_cols(const WinCall& call) {
+  const WinCache& c = call.cache;
+  int64_t wide = 0, narrow = 0;  // positions seen
+  for (int64_t b = 0; b < call.batch; ++b) {
+    const int64_t cols = call.qlens[b] * c.rep.d;
+    if (call.lens[b] <= 0 || cols <= 0 || cols > 32) continue;
+    (cols > 16 ? wide : narrow) +=
+        WinSpan::of(static_cast<int>(call.lens[b]), static_cast<int>(call.qlens[b]), c.window,
+                    c.sinks, kGroup).groups * int64_t{kGroup};
+  }
+  return 2 * wide * c.kvh * c.d >= 100 << 20 && wide >= narrow / 8 ? 32 : 16;
+}
+
 // In a batch with chunks, requests of few rows ride with their tiles where they see no
 // more than the chunks do and all tiles run at once: a launch less (19 requests of up to
-// 26 positions with 3 - 11 rows each, head size 256, with weights: 43 and 37 us a call).
+// 26 positions with 3 - 11 rows each, head size 256, with weights: 43 and 39 us a call).
 bool win_tiles_only(const WinCall& call) {
   if (!dec_geometry(call)) return false;
   const WinCache& c = call.cache;
@@ -509,7 +566,7 @@ int dec_launches(const WinCall& call, int64_t* split_out, G&& go) {
         const int64_t groups = dec_groups(call, b);
         parts = (groups + split - 1) / split;
         rows = win_part_rows(call, b, parts);
-        units = parts * hgs * ((call.qlens[b] * call.cache.rep.d + 15) / 16);
+        units = parts * hgs;
         return groups > 0;
       },
       go);
@@ -542,21 +599,32 @@ int win_decode(const WinCall& call, void* workspace) {
         }
     const WinParts parts{static_cast<float*>(workspace),
                          static_cast<float*>(workspace) + rows * c.d};
-#define KVQ_WIN_DECODE(T, D)                                                                  \
-  hipLaunchKernelGGL((win_decode_kernel<T, D>), dim3(static_cast<unsigned>(units)),           \
+#define KVQ_WIN_DECODE(T, D, NG)                                                              \
+  hipLaunchKernelGGL((win_decode_kernel<T, D, NG>), dim3(static_cast<unsigned>(units)),       \
                      dim3(64 * hpw), hpw * 2 * dec_tile_bytes<D>(), call.stream, arg, count, c, \
                      static_cast<const T*>(call.query), call.q_stride, wide, call.qscale,     \
                      static_cast<int>(split), hpw, static_cast<T*>(call.out), parts, call.lse, \
                      call.scores)
-#define KVQ_WIN_DECODE_D(T)                                                     \
-  if (c.d == 64) KVQ_WIN_DECODE(T, 64); else if (c.d == 128) KVQ_WIN_DECODE(T, 128); \
-  else KVQ_WIN_DECODE(T, 256)
+#define KVQ_WIN_DECODE_N(T, D)  \
+  if (call.few_cols > 16)       \
+    KVQ_WIN_DECODE(T, D, 2);    \
+  else                          \
+    KVQ_WIN_DECODE(T, D, 1)
+#define KVQ_WIN_DECODE_D(T)     \
+  if (c.d == 256) {             \
+    KVQ_WIN_DECODE_N(T, 256);   \
+  } else if (c.d == 128) {      \
+    KVQ_WIN_DECODE_N(T, 128);   \
+  } else {                      \
+    KVQ_WIN_DECODE_N(T, 64);    \
+  }
     if (call.dtype == KVQ_DTYPE_BF16) {
-      KVQ_WIN_DECODE_D(bf16);
+      KVQ_WIN_DECODE_D(bf16)
     } else {
-      KVQ_WIN_DECODE_D(f16);
+      KVQ_WIN_DECODE_D(f16)
     }
 #undef KVQ_WIN_DECODE_D
+#undef KVQ_WIN_DECODE_N
 #undef KVQ_WIN_DECODE
     KVQ_LAUNCH_CHECK();
     return rows > 0 ? launch_win_join(call, arg, count, parts) : KVQ_OK;
