@@ -89,6 +89,18 @@ def test_long_histories(gpu_device, news, window, sinks):
     _attend_and_check(gpu_device, [9000, 5003, 2048], news, 16, 4, 128, 128, BF16, window, sinks)
 
 
+@pytest.mark.parametrize("hq,kvh,d,bs,dtype", [
+    (6, 2, 80, 16, BF16), (4, 1, 4, 16, FP16), (2, 1, 512, 32, BF16), (3, 1, 260, 16, FP16),
+    (5, 5, 12, 1, BF16), (4, 2, 160, 64, BF16), (8, 2, 128, 24, FP16), (40, 2, 128, 16, BF16),
+    (4, 2, 64, 16, FP32), (4, 2, 96, 128, FP32),
+])
+@pytest.mark.parametrize("news", [[1, 1, 1], [3, 1, 40], [300, 2, 0]])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (700, 130)])
+def test_long_histories_of_any_geometry(gpu_device, hq, kvh, d, bs, dtype, news, window, sinks):
+    """The general kernels' parts: rows that see more, fewer and none of a part's positions."""
+    _attend_and_check(gpu_device, [5003, 1, 2048], news, hq, kvh, d, bs, dtype, window, sinks)
+
+
 @pytest.mark.parametrize("news", [[12000], [3000], [700, 12000]])
 def test_long_prompts(gpu_device, news):
     """Whole prompts: many tiles, columns in segments, few and many of them."""

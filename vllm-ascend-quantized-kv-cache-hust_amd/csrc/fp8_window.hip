@@ -11,10 +11,13 @@
 // w_j = (j < len - n ? w_j : 0) + sum over the rows i and the heads of the kv
 // head's group of p_ij.
 //
-// The general kernels: one wave per (row, head), 64 positions at a time, a lane
-// a position for the scores and a word of the row for the values, all in fp32
-// with the softmax's running maximum and sum; bound by their lanes' 4-byte loads
-// and by reading each code once per query head.
+// The general kernels: one wave per (row, head) and run of the row's positions, 64
+// positions at a time, a lane a position for the scores; for the values as many
+// positions at once as a row's words leave lanes for, four of each in flight; all in
+// fp32 with the softmax's running maximum and sum.  Bound by the latency and the lanes
+// of their loads, and by reading each code once per query head: one token at 31000
+// positions, 32 heads on 8 of 96, 57 us (11050 with a wave to a row's whole history and
+// one position in flight); 32 of 2048 - 16384 positions, 513 us (7881), 0.9 TB/s.
 #include <algorithm>
 
 #include "fp8_window.h"
@@ -35,47 +38,75 @@ __device__ __forceinline__ void codes4(uint32_t w, float (&x)[4]) {
 constexpr int kGenWaves = 4;
 constexpr int kGenMaxD = 512;
 
-// fp32 dot product of the query row in LDS with a row of codes.
-__device__ __forceinline__ float dot_codes(const float* q, const uint8_t* row, int d) {
+// fp32 dot product of the query row in LDS with a row of codes, 16 bytes at a time where
+// rows are such (wide).
+__device__ __forceinline__ float dot_codes(const float* q, const uint8_t* row, int d, bool wide) {
   float s = 0.0f;
-  for (int i = 0; i < d; i += 4) {
+  auto word = [&](uint32_t w, const float* at) {
     float x[4];
-    codes4(*reinterpret_cast<const uint32_t*>(row + i), x);
+    codes4(w, x);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s = __builtin_fmaf(q[i + k], x[k], s);
+    for (int k = 0; k < 4; ++k) s = __builtin_fmaf(at[k], x[k], s);
+  };
+  if (wide) {
+#pragma unroll 4
+    for (int i = 0; i < d; i += 16) {
+      const w_u4 w = *reinterpret_cast<const w_u4*>(row + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) word(w[k], q + i + 4 * k);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < d; i += 4) word(*reinterpret_cast<const uint32_t*>(row + i), q + i);
   }
   return s;
 }
 
-// A unit is one row and kGenWaves heads.
+// What a wave wrote to its own LDS is what it reads from here on.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A unit is one row, kGenWaves heads and an item: `split` 64-position groups of what the
+// row sees.
 template <typename T>
 __global__ void __launch_bounds__(64 * kGenWaves)
 win_attn_general_kernel(WinArg, int count, WinCache c, const T* __restrict__ query,
-                        int64_t q_stride, float qscale, T* __restrict__ out,
-                        float* __restrict__ lse) {
-  __shared__ float s_q[kGenWaves][kGenMaxD];
+                        int64_t q_stride, int wide, float qscale, int split, T* __restrict__ out,
+                        WinParts parts, float* __restrict__ lse) {
+  __shared__ __align__(16) float s_q[kGenWaves][kGenMaxD];
   const WinReq r = win_req(count, blockIdx.x);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int groups = (c.hq + kGenWaves - 1) / kGenWaves;
   const int u = static_cast<int>(blockIdx.x) - r.first;
-  const int i = u / groups, head = (u - i * groups) * kGenWaves + wave;
+  const int i = u / groups / r.parts, item = u / groups - i * r.parts;
+  const int head = u % groups * kGenWaves + wave;
   if (head >= c.hq) return;  // no barrier below: a wave reads its own part of s_q
   const int h = static_cast<int>(c.rep.div(static_cast<uint32_t>(head)));
   const int pos = r.len - r.n + i;
   const int64_t row = static_cast<int64_t>(r.q0) + i;
   const T* q = query + row * q_stride + static_cast<int64_t>(head) * c.d;
   for (int k = lane; k < c.d; k += 64) s_q[wave][k] = to_f32(q[k]);
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  float m = -INFINITY, l = 0.0f, acc[2][4] = {};
+  wave_lds_fence();
+  // lane: word `word` (and 64 words on) of the positions `slice`, `slices` + `slice`, ..
+  const int words = c.d / 4, width = min(words, 64), slices = 64 / width;
+  const int slice = lane / width, word = lane - slice * width;
+  const bool mine = slice < slices;
+  float m = -INFINITY, l = 0.0f;
+  w_f4 acc[2] = {w_f4{0.f, 0.f, 0.f, 0.f}, w_f4{0.f, 0.f, 0.f, 0.f}};
   const WinSpan span = pos >= 0 ? WinSpan::of(pos + 1, 1, c.window, c.sinks, 64) : WinSpan{0, 0, 0};
-  for (int g = 0; g < span.groups; ++g) {
+  const int g1 = min(span.groups, (item + 1) * split);
+  for (int g = item * split; g < g1; ++g) {
     const int j = span.pos(g, 64) + lane;
     const bool on = c.sees(pos, j);
     const int64_t at = (on ? c.slot(r.table, j) : 0) * c.kvh + h;
-    float s = -INFINITY;
-    if (on) s = dot_codes(s_q[wave], c.kd + at * c.d, c.d) * (c.ks[at] * qscale);
+    float s = -INFINITY, vs = 0.0f;
+    if (on) {
+      s = dot_codes(s_q[wave], c.kd + at * c.d, c.d, wide) * (c.ks[at] * qscale);
+      vs = c.vs[at];
+    }
     const uint64_t mask = __builtin_amdgcn_ballot_w64(on);
     if (!mask) continue;
     const float top = fmaxf(m, max_wave64(s));
@@ -84,36 +115,66 @@ win_attn_general_kernel(WinArg, int count, WinCache c, const T* __restrict__ que
     const float p = on ? __builtin_amdgcn_exp2f(s - base) : 0.0f;
     m = top;
     l = l * alpha + sum_wave64(p);
-    const float pv = on ? p * c.vs[at] : 0.0f;
+    const float pv = on ? p * vs : 0.0f;
+    acc[0] *= alpha;
+    acc[1] *= alpha;
+    constexpr int DEPTH = 4;  // positions in flight
+    for (int t0 = 0; t0 < 64; t0 += DEPTH * slices) {
+      if (!(mask >> t0)) break;
+      uint32_t x[DEPTH][2];
+      float pt[DEPTH];
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[w][k] *= alpha;
-    for (uint64_t left = mask; left; left &= left - 1) {
-      const int t = __builtin_ctzll(left);
-      const float pt = __shfl(pv, t, 64);
-      const int64_t src = __shfl(at, t, 64);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int col = 4 * (lane + 64 * w);
-        if (col < c.d) {
-          float x[4];
-          codes4(*reinterpret_cast<const uint32_t*>(c.vd + src * c.d + col), x);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[w][k] = __builtin_fmaf(pt, x[k], acc[w][k]);
-        }
+      for (int e = 0; e < DEPTH; ++e) {
+        const int t = t0 + e * slices + slice;
+        const bool seen = mine && t < 64 && ((mask >> (t & 63)) & 1);
+        pt[e] = __shfl(pv, t & 63, 64);
+        const uint8_t* v = c.vd + __shfl(at, t & 63, 64) * c.d + 4 * word;
+        x[e][0] = seen ? *reinterpret_cast<const uint32_t*>(v) : 0u;
+        x[e][1] = seen && word + 64 < words ? *reinterpret_cast<const uint32_t*>(v + 256) : 0u;
+        pt[e] = seen ? pt[e] : 0.0f;
       }
+#pragma unroll
+      for (int e = 0; e < DEPTH; ++e)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          float y[4];
+          codes4(x[e][w], y);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[w][k] = __builtin_fmaf(pt[e], y[k], acc[w][k]);
+        }
     }
   }
-  T* o = out + (row * c.hq + head) * c.d;
+  if (slices > 1) {  // rows of at most 32 words
+    float* sum = s_q[wave];
+    wave_lds_fence();
+    if (mine) *reinterpret_cast<w_f4*>(sum + slice * c.d + 4 * word) = acc[0];
+    wave_lds_fence();
+    if (slice == 0)
+      for (int x = 1; x < slices; ++x)
+        acc[0] += *reinterpret_cast<const w_f4*>(sum + x * c.d + 4 * word);
+  }
+  if (r.parts > 1) {
+    const int64_t part = r.part0 + (static_cast<int64_t>(item) * r.n + i) * c.hq + head;
+    if (slice == 0) {
 #pragma unroll
-  for (int w = 0; w < 2; ++w)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int col = 4 * (lane + 64 * w) + k;
-      // l is 0 only where nothing is seen; a NaN goes through
-      if (col < c.d) o[col] = from_f32<T>(l == 0.0f ? 0.0f : acc[w][k] / l);
+      for (int w = 0; w < 2; ++w)
+        if (word + 64 * w < words)
+          *reinterpret_cast<w_f4*>(parts.o + part * c.d + 4 * (word + 64 * w)) = acc[w];
     }
+    if (lane == 0)  // a NaN score leaves m without it, but not l
+      *reinterpret_cast<w_f2*>(parts.ml + 2 * part) = w_f2{l != l ? INFINITY : m, l};
+    return;
+  }
+  T* o = out + (row * c.hq + head) * c.d;
+  if (slice == 0) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      if (word + 64 * w < words)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          // l is 0 only where nothing is seen; a NaN goes through
+          o[4 * (word + 64 * w) + k] = from_f32<T>(l == 0.0f ? 0.0f : acc[w][k] / l);
+  }
   // (max, sum) in one number: p = 2^(s - lse)
   if (lse && lane == 0) lse[row * c.hq + head] = l == 0.0f ? INFINITY : m + __log2f(l);
 }
@@ -159,13 +220,15 @@ win_weights_general_kernel(WinArg, int count, WinCache c, const T* __restrict__ 
 
 constexpr int kJoinThreads = 256;
 
-// blockIdx.y: the request, blockIdx.x: row * hq + head.  D / 4 threads hold a part's
-// row, the workgroup several parts at once, joined in LDS in a fixed order.
+// blockIdx.y: the request, blockIdx.x: row * hq + head.  d / 4 threads hold a part's
+// row, the workgroup several parts at once, joined in LDS in a fixed order.  D: d, or 0
+// for any.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-win_join_kernel(WinArg, int hq, WinParts parts, T* __restrict__ out, float* __restrict__ lse) {
-  constexpr int LANES = D / 4, SLICES = kJoinThreads / LANES;
-  __shared__ w_f4 s_o[SLICES][LANES];
+win_join_kernel(WinArg, int hq, int any_d, WinParts parts, T* __restrict__ out,
+                float* __restrict__ lse) {
+  const int d = D ? D : any_d, lanes = d / 4, slices = kJoinThreads / lanes;
+  __shared__ w_f4 s_o[kJoinThreads];
   win_cint* a = (win_cint*)__builtin_amdgcn_kernarg_segment_ptr() + 8 * blockIdx.y;
   const int q0 = a[0], n = a[1], count = a[5], part0 = a[6];
   const int64_t x = blockIdx.x, stride = static_cast<int64_t>(n) * hq;
@@ -175,24 +238,24 @@ win_join_kernel(WinArg, int hq, WinParts parts, T* __restrict__ out, float* __re
   float m = -INFINITY;
   for (int s = lane; s < count; s += 64) m = fmaxf(m, ml[s * stride][0]);
   m = max_wave64(m);
-  if (m > 0x1.fffffep126f) m = INFINITY;  // the maxima come no higher than FLT_MAX
+  if (m >= 0x1.fffffep127f) m = INFINITY;  // the tiles' maxima stop at FLT_MAX
   float l = 0.0f;
   for (int s = lane; s < count; s += 64) {
     const w_f2 y = ml[s * stride];
     l += y[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y[0] - m) * y[1];
   }
   l = sum_wave64(l);
-  const int slice = tid / LANES, k = tid % LANES;
+  const int slice = tid / lanes, k = tid - slice * lanes;
   w_f4 acc = w_f4{0.f, 0.f, 0.f, 0.f};
   constexpr int DEPTH = 4;  // loads in flight
-  for (int s0 = slice; s0 < count; s0 += DEPTH * SLICES) {
+  for (int s0 = slice < slices ? slice : count; s0 < count; s0 += DEPTH * slices) {
     float ms[DEPTH];
     w_f4 y[DEPTH];
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) {
-      const int64_t s = min(s0 + i * SLICES, count - 1);
-      ms[i] = s0 + i * SLICES < count ? ml[s * stride][0] : -INFINITY;
-      y[i] = *reinterpret_cast<const w_f4*>(parts.o + (part0 + s * stride + x) * D + 4 * k);
+      const int64_t s = min(s0 + i * slices, count - 1);
+      ms[i] = s0 + i * slices < count ? ml[s * stride][0] : -INFINITY;
+      y[i] = *reinterpret_cast<const w_f4*>(parts.o + (part0 + s * stride + x) * d + 4 * k);
     }
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) {
@@ -201,15 +264,15 @@ win_join_kernel(WinArg, int hq, WinParts parts, T* __restrict__ out, float* __re
       acc += ms[i] == -INFINITY ? w_f4{0.f, 0.f, 0.f, 0.f} : w * y[i];
     }
   }
-  s_o[slice][k] = acc;
+  s_o[tid] = acc;
   __syncthreads();
   if (slice) return;
-#pragma unroll
-  for (int s = 1; s < SLICES; ++s) acc += s_o[s][k];
+#pragma unroll D ? 4 : 1
+  for (int s = 1; s < slices; ++s) acc += s_o[s * lanes + k];
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t at = static_cast<int64_t>(q0) * hq + x;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[at * D + 4 * k + e] = from_f32<T>(acc[e] * inv);
+  for (int e = 0; e < 4; ++e) out[at * d + 4 * k + e] = from_f32<T>(acc[e] * inv);
   if (lse && k == 0) lse[at] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -226,14 +289,17 @@ int launch_win_join(const WinCall& call, const WinArg& arg, int count, WinParts 
   const dim3 grid(static_cast<unsigned>(rows * hq), static_cast<unsigned>(count));
 #define KVQ_WIN_JOIN(T, D)                                                                    \
   hipLaunchKernelGGL((win_join_kernel<T, D>), grid, dim3(kJoinThreads), 0, call.stream, arg, hq, \
-                     parts, static_cast<T*>(call.out), call.lse)
+                     call.cache.d, parts, static_cast<T*>(call.out), call.lse)
 #define KVQ_WIN_JOIN_D(T)                                                              \
   if (call.cache.d == 64) KVQ_WIN_JOIN(T, 64); else if (call.cache.d == 128)           \
-  KVQ_WIN_JOIN(T, 128); else KVQ_WIN_JOIN(T, 256)
+  KVQ_WIN_JOIN(T, 128); else if (call.cache.d == 256) KVQ_WIN_JOIN(T, 256); else       \
+  KVQ_WIN_JOIN(T, 0)
   if (call.dtype == KVQ_DTYPE_BF16) {
     KVQ_WIN_JOIN_D(bf16);
-  } else {
+  } else if (call.dtype == KVQ_DTYPE_F16) {
     KVQ_WIN_JOIN_D(f16);
+  } else {
+    KVQ_WIN_JOIN(float, 0);
   }
 #undef KVQ_WIN_JOIN_D
 #undef KVQ_WIN_JOIN
@@ -247,23 +313,59 @@ namespace {
 
 // ---- host -----------------------------------------------------------------------
 
+// 64-position groups of an item of the general kernel: 16 waves a CU, or items of two
+// groups.  From the lengths alone, whichever kernel takes them: the workspace's size,
+// which does not know the addresses, goes by it.
+int64_t gen_groups(const WinCall& call, int64_t b) {
+  return call.qlens[b] > 0 && call.lens[b] > 0
+             ? WinSpan::of(static_cast<int>(call.lens[b]), static_cast<int>(call.qlens[b]),
+                           call.cache.window, call.cache.sinks, 64)
+                   .groups
+             : 0;
+}
+int64_t gen_split(const WinCall& call) {
+  int cus = 0;
+  if (device_cu_count(&cus) != KVQ_OK || cus <= 0) cus = 256;
+  int64_t total = 0;
+  for (int64_t b = 0; b < call.batch; ++b)
+    total += gen_groups(call, b) * call.qlens[b] * call.cache.hq;
+  return std::min<int64_t>(std::max<int64_t>(2, total / (16 * cus)), kMaxPositions / 64);
+}
+int64_t gen_parts(const WinCall& call, int64_t b, int64_t split) {
+  return std::max<int64_t>(1, (gen_groups(call, b) + split - 1) / split);
+}
+int64_t general_bytes(const WinCall& call) {
+  const int64_t split = gen_split(call);
+  int64_t rows = 0;
+  for (int64_t b = 0; b < call.batch; ++b)
+    rows += win_part_rows(call, b, gen_parts(call, b, split));
+  return win_parts_bytes(rows, call.cache.d);
+}
+
 // Requests that no matrix kernel takes.
 template <typename T>
-int attend_general(const WinCall& call) {
-  const int64_t groups = (call.cache.hq + kGenWaves - 1) / kGenWaves;
+int attend_general(const WinCall& call, void* workspace) {
+  const WinCache& c = call.cache;
+  const int64_t groups = (c.hq + kGenWaves - 1) / kGenWaves, split = gen_split(call);
+  const int wide = c.d % 16 == 0 && aligned16(c.kd, nullptr);
   return win_launches(
       call,
-      [&](int64_t b, int64_t& units, int64_t&, int64_t&) {
-        units = call.qlens[b] * groups;
-        return !win_decode_takes(call, b) && !win_chunk_takes(call, b);
+      [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
+        if (win_decode_takes(call, b) || win_chunk_takes(call, b)) return false;
+        parts = gen_parts(call, b, split);
+        rows = win_part_rows(call, b, parts);
+        units = call.qlens[b] * parts * groups;
+        return true;
       },
-      [&](const WinArg& arg, int count, int64_t blocks, int64_t) -> int {
+      [&](const WinArg& arg, int count, int64_t blocks, int64_t rows) -> int {
+        const WinParts parts{static_cast<float*>(workspace),
+                             static_cast<float*>(workspace) + rows * c.d};
         hipLaunchKernelGGL((win_attn_general_kernel<T>), dim3(static_cast<unsigned>(blocks)),
-                           dim3(64 * kGenWaves), 0, call.stream, arg, count, call.cache,
-                           static_cast<const T*>(call.query), call.q_stride, call.qscale,
-                           static_cast<T*>(call.out), call.lse);
+                           dim3(64 * kGenWaves), 0, call.stream, arg, count, c,
+                           static_cast<const T*>(call.query), call.q_stride, wide, call.qscale,
+                           static_cast<int>(split), static_cast<T*>(call.out), parts, call.lse);
         KVQ_LAUNCH_CHECK();
-        return KVQ_OK;
+        return rows > 0 ? launch_win_join(call, arg, count, parts) : KVQ_OK;
       });
 }
 
@@ -355,7 +457,7 @@ Layout layout_of(const WinCall& call, bool weigh, int* rc) {
   const int64_t many = win_chunk_bytes(call, rc);
   if (*rc != KVQ_OK) return x;
   const int64_t sums = weigh ? win_weights_bytes(call, x.scored, rc) : 0;
-  x.parts = align16(std::max(std::max(few, many), sums));
+  x.parts = align16(std::max(std::max(few, many), std::max(sums, general_bytes(call))));
   return x;
 }
 
@@ -435,7 +537,7 @@ extern "C" int kvq_fp8_pth_window_attn(
   rc = win_chunk(call, parts);
   if (rc != KVQ_OK) return rc;
   KVQ_DISPATCH_FLOAT(dtype, T, {
-    rc = attend_general<T>(call);
+    rc = attend_general<T>(call, parts);
     if (rc != KVQ_OK) return rc;
     if (weigh) rc = weigh_general<T>(call);
     if (rc != KVQ_OK) return rc;
