@@ -23,6 +23,11 @@
 //   chunk of ranks reads is nothing that an earlier chunk has written; one
 //   workgroup per (request, kv head, side) walks its chunks in order, and within
 //   a chunk every load has returned before the first store.
+//
+// Bound by HBM where much moves, by the rounds' latencies where little does: 32 requests
+// of 4096 - 16384 rows, 8 kv heads of 128, 2048 kept, 83 us a call, of which 19 to select
+// and 52 to move (5.3 TB/s); one of 100001, 50000 kept, 87, of which 38 in the selection's
+// launches; one of 1100, 2 kv heads, 600 kept, 27, most of it the host's launches.
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -277,7 +282,9 @@ evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const f
 // ---- rows of many chunks ---------------------------------------------------------------
 
 constexpr int kChunkNk = 16, kChunk = kSelThreads * kChunkNk;  // positions of a chunk
-constexpr int kHeldRow = 32 * kSelThreads;  // the longest row of one workgroup
+// The longest row of one workgroup: what its registers hold.  Up to there it is the
+// faster way (8 rows of 32000: 35 us a call, 50 in chunks; 256 of 16000: 125, 148).
+constexpr int kHeldRow = 32 * kSelThreads;
 constexpr int kLowBins = 1024;              // of the last round
 
 // counts: [row][2][kBins] of the first two rounds; low: [chunk of a row][kLowBins] of the
@@ -500,7 +507,8 @@ evict_move_kernel(EvictArg, int count, EvictCache c, const int32_t* __restrict__
 constexpr int kCompactThreads = 1024;
 constexpr int kCompactDepth = 4;  // words in flight per thread
 
-// In place.  A unit is one side of one kv head.
+// In place.  A unit is one side of one kv head, and a slice of its rows' bytes: slices
+// move by themselves.
 template <typename W>
 __global__ void __launch_bounds__(kCompactThreads)
 evict_compact_kernel(EvictArg, int count, EvictCache c, const int32_t* __restrict__ kept,
@@ -508,8 +516,9 @@ evict_compact_kernel(EvictArg, int count, EvictCache c, const int32_t* __restric
   const EvictReq r = evict_req(count, blockIdx.x);
   const int u = static_cast<int>(blockIdx.x) - r.first;
   const int kvh = static_cast<int>(c.kvh.d);
-  const int h = u >> 1;
-  uint8_t* data = u & 1 ? c.vd : c.kd;
+  const int slice = u / (2 * kvh), h = (u - slice * 2 * kvh) >> 1;
+  const bool scales = slice == 0;
+  uint8_t* data = (u & 1 ? c.vd : c.kd) + static_cast<int64_t>(slice) * pieces.d * sizeof(W);
   float* scale = u & 1 ? c.vs : c.ks;
   const int32_t* ids = kept + (static_cast<int64_t>(r.table) * kvh + h) * kept_cols;
   const int64_t total = static_cast<int64_t>(r.keep) * pieces.d;  // words, < 2^31 (host)
@@ -531,7 +540,7 @@ evict_compact_kernel(EvictArg, int count, EvictCache c, const int32_t* __restric
           const int64_t from = c.slot(c.src, c.src_cols, r.table, p) * kvh + h;
           to[k] = c.slot(c.src, c.src_cols, r.table, rank) * kvh + h;
           word[k] = reinterpret_cast<const W*>(data + from * c.d)[part[k]];
-          if (part[k] == 0) s[k] = scale[from];
+          if (scales && part[k] == 0) s[k] = scale[from];
         }
       }
     }
@@ -542,7 +551,7 @@ evict_compact_kernel(EvictArg, int count, EvictCache c, const int32_t* __restric
     for (int k = 0; k < kCompactDepth; ++k) {
       if (to[k] >= 0) {
         reinterpret_cast<W*>(data + to[k] * c.d)[part[k]] = word[k];
-        if (part[k] == 0) scale[to[k]] = s[k];
+        if (scales && part[k] == 0) scale[to[k]] = s[k];
       }
     }
   }
@@ -791,17 +800,25 @@ extern "C" int kvq_fp8_pth_evict(uint8_t* k_data, float* k_scale, uint8_t* v_dat
           return KVQ_OK;
         });
   }
+  // slices of the rows while CUs are free (1 request, 8 kv heads of 128, 32768 of 100001
+  // rows kept: 406, 222, 166 and 144 us in 1, 2, 4 and 8; 1000 of 1100: 26 - 28)
+  int cus = 0;
+  if (device_cu_count(&cus) != KVQ_OK || cus <= 0) cus = 256;
+  int64_t moved = 0, slices = 1;
+  for (int64_t b = 0; b < batch; ++b) moved += seq_lens[b] > keep[b];
+  while (moved * 2 * num_kv_heads * slices * 2 <= cus && piece_div.d % (2 * slices) == 0) slices *= 2;
+  const FastDiv slice_div = FastDiv::make(static_cast<uint32_t>(piece_div.d / slices));
   return for_requests(
       seq_lens, keep, weight_rows, batch, kvh,
-      [&](int64_t b) { return seq_lens[b] > keep[b] ? 2 * static_cast<int64_t>(num_kv_heads) : 0; },
+      [&](int64_t b) { return seq_lens[b] > keep[b] ? 2 * slices * num_kv_heads : 0; },
       [&](const EvictArg& arg, int count, unsigned blocks, int64_t, int64_t, int64_t) -> int {
         if (wide)
           hipLaunchKernelGGL((evict_compact_kernel<w_u4>), dim3(blocks), dim3(kCompactThreads), 0,
-                             s, arg, count, c, kept, kept_cols, piece_div,
+                             s, arg, count, c, kept, kept_cols, slice_div,
                              static_cast<int>(sinks));
         else
           hipLaunchKernelGGL((evict_compact_kernel<uint32_t>), dim3(blocks), dim3(kCompactThreads),
-                             0, s, arg, count, c, kept, kept_cols, piece_div,
+                             0, s, arg, count, c, kept, kept_cols, slice_div,
                              static_cast<int>(sinks));
         KVQ_LAUNCH_CHECK();
         return KVQ_OK;
