@@ -1,10 +1,15 @@
 // SPDX-License-Identifier: Apache-2.0
-// Windowed attention over paged E4M3 rows for chunks: tiles of 128 rows (a row is
-// one query of one head of a kv head's group), 64-position blocks, bound by the
-// matrix units and the softmax beside them.
+// Windowed attention over paged E4M3 rows for chunks: tiles of 128 or 256 rows (a row
+// is one query of one head of a kv head's group), 64-position blocks, bound by the
+// matrix units and the softmax beside them: 4 chunks of 2048 queries over 10240
+// positions, 40 heads on 8 of 128, 1.65 ms, 0.94 PFLOP/s, where a plain 8192^3 product
+// reaches 1.28; 6 of 200 - 1500 over 3000 - 9000, 8 heads on 1 of 256, window 2048, 100 us,
+// the operands' LDS reads (64 KB a wave and block) being most of it.  Matrix and vector
+// work of a SIMD's waves overlap only in part: 64 products of 16 x 16 x 32 by themselves
+// take 480 ns, 256 fma 478, both, on each of two waves, 690 a wave.
 //
-// One workgroup per tile, kv head and segment of the tile's blocks; at head sizes 64
-// and 128 four waves of 32 rows, two workgroups a CU, at 256 eight waves of 16, one.
+// One workgroup of four or eight waves (chk_shape) per tile, kv head and segment of the
+// tile's blocks.
 // Codes come from their pages into registers two blocks ahead, are converted once
 // per workgroup (exact, a pair an instruction) and staged in LDS as 16-bit rows, keys
 // in the query's type, values in fp16:
@@ -66,6 +71,8 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
   constexpr int KS = D / 32, DB = D / 16, PPR = D / 8, CH = D / 16;
   constexpr int INS = kBlock * CH / (64 * WAVES);  // 16-byte loads of a lane, block and side
   constexpr int RPI = 64 / CH;                     // rows of a wave's load
+  // operands read from LDS one product ahead (D = 128: 1.73 for 1.83 ms; at 256 they
+  // would spill, 197 for 100 us)
   constexpr bool AHEAD = D < 256;
   static_assert(INS >= 1 && RPI <= 16, "a wave's load stays inside a 16-position group");
   auto vswz = [](int r) { return 2 * (r % 4) + (PPR >= 16 ? 8 * ((r / 4) % 2) : 0); };
@@ -511,12 +518,23 @@ int64_t chk_tiles(const WinCall& call, int64_t b, int rows) {
   return (call.qlens[b] * call.cache.rep.d + rows - 1) / rows;
 }
 
-ChkShape chk_shape(const WinCall& call, int cus) {
+// Head size 64: four waves of 32 rows, three workgroups a CU.  256: eight waves of 16 (four
+// of 32 spill: 265 us for 100 on 6 chunks over 3000 - 9000 positions, window 2048).  128:
+// eight waves of 32, which convert a block for 256 rows, or four, two workgroups a CU,
+// where requests have few columns (row, head) to fill tiles with: over 30000 positions, 512
+// and 8192 x 1 kv head, 96 and 302 us with eight, 104 and 330 with four; 4 of 10240
+// positions, 8192 columns, 1291 and 1416; 256 and 280 columns over 3000 and 9000, 34 and
+// 50, 32 and 46; 23 requests of 20 - 800, 191 and 175.
+ChkShape chk_shape(const WinCall& call) {
   if (call.cache.d == 256) return {8, 128};
   if (call.cache.d == 64) return {4, 128};
-  int64_t tiles = 0;
-  for (int64_t b = 0; b < call.batch; ++b) tiles += chk_tiles(call, b, 256);
-  return tiles * call.cache.kvh >= cus ? ChkShape{8, 256} : ChkShape{4, 128};
+  int64_t cols = 0, requests = 0;
+  for (int64_t b = 0; b < call.batch; ++b)
+    if (chk_tiles(call, b, 256) > 0) {
+      cols += call.qlens[b] * call.cache.rep.d;
+      ++requests;
+    }
+  return cols >= 512 * requests ? ChkShape{8, 256} : ChkShape{4, 128};
 }
 
 // The most blocks that a tile of request b has.
@@ -532,8 +550,9 @@ int64_t chk_blocks(const WinCall& call, int64_t b, int tile_rows) {
 // us), when `groups` workgroups of `blocks` blocks go over the chip's slots in rounds,
 // each a `segs`th as long, and the partial results (`bytes` of them a segment) go
 // through memory and back: 5 blocks and one per 6 MB.  (3 whole prompts of 1.5K - 4.1K,
-// 32 heads on 8, 1072 workgroups on 256 slots: 290 us uncut, 784 in 8 segments, their
-// joining being half of it; 2 chunks of 70 rows over 9000, 8 workgroups: 8 segments.)
+// 32 heads on 8, 1072 workgroups on 256 slots: 303 us uncut, 784 in 8 segments, their
+// joining being half of it.  70 rows over 9000 positions, 24 workgroups: 48 us cut, 261
+// uncut; 128 over 30000: 109 and 846; 2048 of one kv head: 347 and 845.)
 int64_t chk_segs(int64_t groups, int64_t blocks, int64_t slots, int64_t bytes) {
   int64_t best = 1, cost = (groups + slots - 1) / slots * blocks;
   for (int64_t segs = 2; segs <= 64 && segs * 4 <= blocks; ++segs) {
@@ -553,7 +572,7 @@ int chk_launches(const WinCall& call, G&& go) {
   const int rc = device_cu_count(&cus);
   if (rc != KVQ_OK) return rc;
   if (cus <= 0) cus = 256;
-  const ChkShape shape = chk_shape(call, cus);
+  const ChkShape shape = chk_shape(call);
   const int64_t slots = static_cast<int64_t>(cus) * (call.cache.d == 64 ? 12 : 8) / shape.waves;
   int64_t tiles = 0, blocks = 0;
   for (int64_t b = 0; b < call.batch; ++b) {
