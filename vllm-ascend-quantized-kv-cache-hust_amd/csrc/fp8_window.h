@@ -256,7 +256,9 @@ inline int64_t win_part_rows(const WinCall& call, int64_t b, int64_t parts) {
 // Requests whose decode leaves its scores in the workspace, [kv head][column][positions,
 // a multiple of 16] in the log2 domain, for the weights to be summed from: writing and
 // reading 4 bytes a column and position is less than the keys once more (D + 4 bytes)
-// below this many columns, while all of them stay a small workspace.
+// below this many columns, while all of them stay a small workspace (32 requests of
+// 2048 - 16384 positions, 8 kv heads of 128, 4, 12 and 16 columns: 161, 201 and 227 us a
+// call with the scores, 215, 217 and 215 without).
 constexpr int kScoreCols = 16;
 constexpr int64_t kScoreBytes = 256ll << 20;
 struct WinScores {

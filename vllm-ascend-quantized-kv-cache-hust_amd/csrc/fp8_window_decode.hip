@@ -538,10 +538,11 @@ WinScores win_scores(const WinCall& call) {
       rest = rest || (call.qlens[b] > 0 && call.lens[b] > 0);
     }
   }
-  // beside other requests, whose keys are read anyway, only where it is worth a launch
-  // (5 us, or 25 MB of keys)
+  // beside other requests, whose launch these could share, only where it is worth one
+  // (16 requests of 1000 - 2000 positions beside a chunk of 64 rows, 24 MB of keys: 65 us
+  // with the scores, 60 without; of 3000 - 6000, 74 MB: 87 and 91)
   s.on = s.units > 0 && 64 * s.units <= kScoreBytes &&
-         (!rest || keys * call.cache.d >= (25 << 20));
+         (!rest || keys * call.cache.d >= (40 << 20));
   if (!s.on) s.units = 0;
   return s;
 }
