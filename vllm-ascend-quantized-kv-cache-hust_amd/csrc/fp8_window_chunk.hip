@@ -2,7 +2,7 @@
 // Windowed attention over paged E4M3 rows for chunks: tiles of 128 or 256 rows (a row
 // is one query of one head of a kv head's group), 64-position blocks, bound by the
 // matrix units and the softmax beside them: 4 chunks of 2048 queries over 10240
-// positions, 40 heads on 8 of 128, 1.65 ms, 0.94 PFLOP/s, where a plain 8192^3 product
+// positions, 40 heads on 8 of 128, 1.60 ms, 0.97 PFLOP/s, where a plain 8192^3 product
 // reaches 1.28; 6 of 200 - 1500 over 3000 - 9000, 8 heads on 1 of 256, window 2048, 100 us,
 // the operands' LDS reads (64 KB a wave and block) being most of it.  Matrix and vector
 // work of a SIMD's waves overlap only in part: 64 products of 16 x 16 x 32 by themselves
@@ -17,9 +17,9 @@
 //     score operand reads sit in different banks;
 //   V [64][D]: column x at x ^ (2 (r % 4) + 8 ((r / 4) % 2)) (the second term from
 //     D = 128 on), likewise for the transposing reads of the value operand.
-// A step converts and stages block i + 1 (loaded a step earlier), sends for block
-// i + 2, and computes block i; the SIMD's other wave fills its matrix units while
-// this one does its softmax.
+// A step converts and stages block i + 1 (or i + 2, ChkLds; loaded a step earlier), sends
+// for the block after it, and computes block i; the SIMD's other wave fills its matrix
+// units while this one does its softmax.
 //
 // The scales stay out of the operands.  With ks' = k_scale * scale * log2(e) and
 // lv = log2(v_scale) per position,
@@ -49,11 +49,13 @@ constexpr int kBlock = 64;      // positions
 
 template <int D>
 constexpr int chk_ng() { return D == 256 ? 1 : 2; }  // 16-row column groups of a wave
-template <int D>
+template <int D, int WAVES>
 struct ChkLds {
+  // blocks; with four, two steps run between barriers (D = 128: 1.60 for 1.66 ms)
+  static constexpr int BUFS = D == 128 && WAVES == 8 ? 4 : 2;
   static constexpr int SIDE = kBlock * D * 2;
-  static constexpr int SCALES = 4 * SIDE;               // two of [3][64] floats
-  static constexpr int FLAG = SCALES + 2 * 3 * 64 * 4;  // a NaN put aside that some row sees
+  static constexpr int SCALES = 2 * BUFS * SIDE;           // BUFS of [3][64] floats
+  static constexpr int FLAG = SCALES + BUFS * 3 * 64 * 4;  // a NaN put aside that some row sees
   static constexpr int BYTES = FLAG + 16;
 };
 
@@ -66,7 +68,7 @@ __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
 win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int64_t q_stride,
                  int wide, float qscale, T* __restrict__ out, WinParts parts,
                  float* __restrict__ lse) {
-  using L = ChkLds<D>;
+  using L = ChkLds<D, WAVES>;
   constexpr int NG = chk_ng<D>(), ROWS = 16 * NG, kTileRows = ROWS * WAVES;
   constexpr int KS = D / 32, DB = D / 16, PPR = D / 8, CH = D / 16;
   constexpr int INS = kBlock * CH / (64 * WAVES);  // 16-byte loads of a lane, block and side
@@ -239,10 +241,9 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
   }
   w_u4 q[NG][KS];
 
-  char* const kbuf0 = lds;
-  char* const kbuf1 = lds + L::SIDE;
-  char* const vbuf0 = lds + 2 * L::SIDE;
-  char* const vbuf1 = lds + 3 * L::SIDE;
+  constexpr int AWAY = L::BUFS / 2;  // steps from a block's staging to its use
+  auto kbuf = [&](int b) { return lds + b % L::BUFS * L::SIDE; };
+  auto vbuf = [&](int b) { return lds + (L::BUFS + b % L::BUFS) * L::SIDE; };
   auto k_reads = [&](const char* sk, int grp, w_u4 (&a)[KS]) {
     const int row = 16 * grp + n;
 #pragma unroll
@@ -279,8 +280,9 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
 
   if (tid == 0) *reinterpret_cast<uint32_t*>(lds + L::FLAG) = 0;
   __syncthreads();
-  // prologue: the first block staged, the second's codes on their way
-  Codes next = load(blk0);
+  // prologue: the first AWAY blocks staged, the next one's codes on their way
+  Codes first = load(blk0), next = first;
+  if (AWAY > 1 && blk0 + 1 < nblk) next = load(blk0 + 1);
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     const Row y = row_at(g);
@@ -292,17 +294,19 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     for (int s = 0; s < KS; ++s)
       if (!y.live) q[g][s] = w_u4{0, 0, 0, 0};
   }
-  put(kbuf0, vbuf0, 0, blk0, next);
-  if (blk0 + 1 < nblk) next = load(blk0 + 1);
+  put(kbuf(0), vbuf(0), 0, blk0, first);
+  if (AWAY > 1 && blk0 + 1 < nblk) put(kbuf(1), vbuf(1), 1, blk0 + 1, next);
+  if (blk0 + AWAY < nblk) next = load(blk0 + AWAY);
   __syncthreads();
 
-  // Step i, block i in kc / vc (PAR = (i - blk0) % 2); kd / vd take block i + 1.
-  auto step = [&](const char* kc, const char* vc, char* kd, char* vd, int par, int i) {
-    if (i + 1 < nblk) put(kd, vd, par ^ 1, i + 1, next);
-    if (i + 2 < nblk) next = load(i + 2);
+  // Step i, block i in buffer `cur`.
+  auto step = [&](int cur, int i) {
+    const char *kc = kbuf(cur), *vc = vbuf(cur);
+    if (i + AWAY < nblk) put(kbuf(cur + AWAY), vbuf(cur + AWAY), (cur + AWAY) % L::BUFS, i + AWAY, next);
+    if (i + AWAY + 1 < nblk) next = load(i + AWAY + 1);
     if (!active(i)) return;
     const int kb = at_block(i);
-    const float* sc = reinterpret_cast<const float*>(lds + L::SCALES) + par * 192 + 4 * kg;
+    const float* sc = reinterpret_cast<const float*>(lds + L::SCALES) + cur * 192 + 4 * kg;
     // operands are read a group ahead of their products where registers allow
     w_f4 s[4][NG];
     w_u4 a[AHEAD ? 2 : 1][KS];
@@ -408,13 +412,14 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     }
   };
   int i = blk0;
-  for (; i + 1 < nblk; i += 2) {
-    step(kbuf0, vbuf0, kbuf1, vbuf1, 0, i);
-    __syncthreads();
-    step(kbuf1, vbuf1, kbuf0, vbuf0, 1, i + 1);
-    __syncthreads();
+  while (i < nblk) {
+#pragma unroll
+    for (int cur = 0; cur < L::BUFS; ++cur) {
+      step(cur, i);
+      if (++i >= nblk) break;
+      if (cur % AWAY == AWAY - 1) __syncthreads();
+    }
   }
-  if (i < nblk) step(kbuf0, vbuf0, kbuf1, vbuf1, 0, i);
 
   __syncthreads();
   if (*reinterpret_cast<const uint32_t*>(lds + L::FLAG)) {  // uniform
@@ -618,7 +623,7 @@ int win_chunk(const WinCall& call, void* workspace) {
                          static_cast<float*>(workspace) + rows * c.d};
 #define KVQ_WIN_CHUNK(T, D, W)                                                                \
   hipLaunchKernelGGL((win_chunk_kernel<T, D, W>), dim3(static_cast<unsigned>(units)),         \
-                     dim3(64 * W), ChkLds<D>::BYTES, call.stream, arg, count, c,              \
+                     dim3(64 * W), (ChkLds<D, W>::BYTES), call.stream, arg, count, c,         \
                      static_cast<const T*>(call.query), call.q_stride, wide, call.qscale,     \
                      static_cast<T*>(call.out), parts, call.lse)
 #define KVQ_WIN_CHUNK_D(T)                             \
