@@ -2,8 +2,8 @@
 // Windowed attention over paged E4M3 rows for chunks: tiles of 128 or 256 rows (a row
 // is one query of one head of a kv head's group), 64-position blocks, bound by the
 // matrix units and the softmax beside them: 4 chunks of 2048 queries over 10240
-// positions, 40 heads on 8 of 128, 1.60 ms, 0.97 PFLOP/s, where a plain 8192^3 product
-// reaches 1.28; 6 of 200 - 1500 over 3000 - 9000, 8 heads on 1 of 256, window 2048, 100 us,
+// positions, 40 heads on 8 of 128, 1.57 ms, 0.98 PFLOP/s, where a plain 8192^3 product
+// reaches 1.28; 6 of 200 - 1500 over 3000 - 9000, 8 heads on 1 of 256, window 2048, 97 us,
 // the operands' LDS reads (64 KB a wave and block) being most of it.  Matrix and vector
 // work of a SIMD's waves overlap only in part: 64 products of 16 x 16 x 32 by themselves
 // take 480 ns, 256 fma 478, both, on each of two waves, 690 a wave.
@@ -311,6 +311,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     w_f4 s[4][NG];
     w_u4 a[AHEAD ? 2 : 1][KS];
     if (AHEAD) k_reads(kc, 0, a[0]);
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (!AHEAD) k_reads(kc, k, a[0]);
@@ -320,6 +321,9 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
       for (int g = 0; g < NG; ++g) s[k][g] = w_f4{0.f, 0.f, 0.f, 0.f};
       k_mfmas(a[AHEAD ? k % 2 : 0], s[k]);
     }
+    // vector work goes before the other wave's products, which it leaves gaps for (2 - 3%
+    // at head sizes 128 and 256; the other way round, nothing)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const w_f4 ks = *reinterpret_cast<const w_f4*>(sc + 16 * k);
@@ -397,6 +401,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
           p[g][k / 2][2 * (k % 2) + e / 2] = pack_pair(p0, p1, f16{});
         }
     }
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {  // k-step x / 2, half x % 2 of the dims
       if (!AHEAD) v_reads(vc, x / 2, x % 2, v[0]);
@@ -410,6 +415,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
           acc = mfma_op(v[AHEAD ? x % 2 : 0][jj], p[g][x / 2], acc, f16{});
         }
     }
+    __builtin_amdgcn_s_setprio(1);
   };
   int i = blk0;
   while (i < nblk) {
