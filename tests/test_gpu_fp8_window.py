@@ -268,6 +268,61 @@ def test_another_stream_and_a_captured_call(gpu_device):
         assert torch.equal(out, again) and torch.equal(w3, w1)
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 96), (FP32, 128)])
+def test_more_rows_than_history_in_any_geometry(gpu_device, dtype, d):
+    _attend_and_check(gpu_device, [5, 0, 900], [9, 3, 1000], 6, 2, d, 16, dtype, None, 0)
+    _attend_and_check(gpu_device, [5, 0, 900], [9, 3, 1000], 6, 2, d, 16, dtype, 70, 66)
+
+
+def test_many_requests_of_any_geometry(gpu_device):
+    """More than a launch takes, some of them in parts."""
+    lens = [(97 * b) % 701 for b in range(250)]
+    news = [(b * 7) % 4 for b in range(250)]
+    _attend_and_check(gpu_device, lens, news, 4, 2, 80, 16, FP16, None, 0)
+    _attend_and_check(gpu_device, lens, news, 4, 2, 80, 16, FP16, 130, 70)
+
+
+@pytest.mark.parametrize("batch,lens,n,hq,kvh,d", [
+    (16, 4000, 8, 32, 8, 128),  # two groups of columns
+    (3, 900, 2, 6, 2, 96),      # the general kernels
+    (2, 3000, 300, 8, 2, 128),  # tiles of 256 rows
+])
+def test_streams_and_graphs_of_every_kernel(gpu_device, batch, lens, n, hq, kvh, d):
+    """Two calls at once on two streams, and replays of a captured one."""
+    c = ref.Cache([lens] * batch, kvh, d, 32, device=gpu_device, seed=15)
+    ls, ns = [lens] * batch, [n] * batch
+    qs = [ref.query(sum(ns), hq, d, BF16, gpu_device, seed=s) for s in (1, 2)]
+    w0 = torch.rand(batch, kvh, lens, device=gpu_device)
+
+    def call(q, w, **kw):
+        return attend(q, *c.args(), ls, ns, 0.1, weights=w0, out_weights=w,
+                      block_table_host=c.host, **kw)
+
+    wants, ws = [], [torch.zeros_like(w0) for _ in range(4)]
+    for q, w in zip(qs, ws):
+        wants.append(call(q, w))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    gots = []
+    for q, w, stream in zip(qs, ws[2:], streams):
+        with torch.cuda.stream(stream):
+            gots.append(call(q, w))
+    torch.cuda.synchronize()
+    for a, b in zip(gots + ws[2:], wants + ws[:2]):
+        assert torch.equal(a, b)
+    q, out, w3 = qs[0].clone(), torch.zeros_like(qs[0]), torch.zeros_like(w0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(q, w3, out=out)
+    for k in (1, 0, 1):
+        q.copy_(qs[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, wants[k]) and torch.equal(w3, ws[k])
+        assert torch.equal(call(qs[1 - k], ws[2]), wants[1 - k])
+        torch.cuda.synchronize()
+
+
 def test_agrees_with_the_rounded_rows_of_the_older_call(gpu_device):
     lens = [1000, 77]
     c = ref.Cache(lens, 2, 128, 32, device=gpu_device, seed=14)
