@@ -557,18 +557,23 @@ int64_t chk_blocks(const WinCall& call, int64_t b, int tile_rows) {
       .groups;
 }
 
-// Segments of a tile's blocks: what ends soonest, in blocks of one workgroup (about 1.2
-// us), when `groups` workgroups of `blocks` blocks go over the chip's slots in rounds,
-// each a `segs`th as long, and the partial results (`bytes` of them a segment) go
-// through memory and back: 5 blocks and one per 6 MB.  (3 whole prompts of 1.5K - 4.1K,
-// 32 heads on 8, 1072 workgroups on 256 slots: 303 us uncut, 784 in 8 segments, their
-// joining being half of it.  70 rows over 9000 positions, 24 workgroups: 48 us cut, 261
-// uncut; 128 over 30000: 109 and 846; 2048 of one kv head: 347 and 845.)
-int64_t chk_segs(int64_t groups, int64_t blocks, int64_t slots, int64_t bytes) {
-  int64_t best = 1, cost = (groups + slots - 1) / slots * blocks;
+// Segments of a tile's blocks: what ends soonest, in blocks of one workgroup (1.3 - 1.9
+// us), when `groups` workgroups of `blocks` blocks share the CUs (two or more on one
+// overlap to three fifths, where it has room for them), each a `segs`th as long, and the
+// partial results (`bytes` of them a segment) go through memory and back: 3 blocks and one
+// per 6 MB.  (3 whole prompts of 1.5K - 4.1K, 32 heads on 8, 1072 workgroups on 256 CUs:
+// 303 us uncut, 784 in 8 segments, their joining being half of it.  70 rows over 9000
+// positions, 24 workgroups: 48 us cut, 261 uncut; 128 over 30000: 96 and 846; 2048 of one
+// kv head: 302 and 845; 18 over 512 of one: 18.5 and 21.5; 128 times 18 over 1100, 256
+// workgroups: 69 and 61.)
+int64_t chk_segs(int64_t groups, int64_t blocks, int64_t cus, bool several, int64_t bytes) {
+  auto time = [&](int64_t segs) {
+    const int64_t each = (groups * segs + cus - 1) / cus;  // workgroups of a CU
+    return each * ((blocks + segs - 1) / segs) * (each > 1 && several ? 3 : 5);
+  };
+  int64_t best = 1, cost = time(1);  // in fifths of a block
   for (int64_t segs = 2; segs <= 64 && segs * 4 <= blocks; ++segs) {
-    const int64_t rounds = (groups * segs + slots - 1) / slots;
-    const int64_t c = rounds * ((blocks + segs - 1) / segs) + 5 + segs * bytes / 6000000;
+    const int64_t c = time(segs) + 5 * (3 + segs * bytes / 6000000);
     if (c < cost) {
       best = segs;
       cost = c;
@@ -584,7 +589,6 @@ int chk_launches(const WinCall& call, G&& go) {
   if (rc != KVQ_OK) return rc;
   if (cus <= 0) cus = 256;
   const ChkShape shape = chk_shape(call);
-  const int64_t slots = static_cast<int64_t>(cus) * (call.cache.d == 64 ? 12 : 8) / shape.waves;
   int64_t tiles = 0, blocks = 0;
   for (int64_t b = 0; b < call.batch; ++b) {
     const int64_t t = chk_tiles(call, b, shape.rows);
@@ -593,7 +597,7 @@ int chk_launches(const WinCall& call, G&& go) {
   }
   const int64_t groups = tiles * call.cache.kvh;
   const int64_t segs =
-      chk_segs(groups, blocks, slots, groups * shape.rows * call.cache.d * 8);
+      chk_segs(groups, blocks, cus, shape.waves == 4, groups * shape.rows * call.cache.d * 8);
   return win_launches(
       call,
       [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
