@@ -26,7 +26,7 @@
 //
 // Bound by HBM where much moves, by the rounds' latencies where little does: 32 requests
 // of 4096 - 16384 rows, 8 kv heads of 128, 2048 kept, 83 us a call, of which 19 to select
-// and 52 to move (5.3 TB/s); one of 100001, 50000 kept, 87, of which 38 in the selection's
+// and 52 to move (5.3 TB/s); one of 100001, 50000 kept, 80, of which 31 in the selection's
 // launches; one of 1100, 2 kv heads, 600 kept, 27, most of it the host's launches.
 #include <algorithm>
 #include <memory>
@@ -281,7 +281,9 @@ evict_select_kernel(EvictArg, int count, int kvh, int sinks, int recent, const f
 
 // ---- rows of many chunks ---------------------------------------------------------------
 
-constexpr int kChunkNk = 16, kChunk = kSelThreads * kChunkNk;  // positions of a chunk
+// (4, 8 and 16 a lane: 1 request of 100001 rows, 8 kv heads, 73, 77 and 84 us a call; 4 of
+// 60000, 70, 62 and 69; 1 of 10^6, 2 kv heads, 89, 52 and 61.)
+constexpr int kChunkNk = 8, kChunk = kSelThreads * kChunkNk;  // positions of a chunk
 // The longest row of one workgroup: what its registers hold.  Up to there it is the
 // faster way (8 rows of 32000: 35 us a call, 50 in chunks; 256 of 16000: 125, 148).
 constexpr int kHeldRow = 32 * kSelThreads;
@@ -379,6 +381,7 @@ evict_emit_kernel(EvictArg, int count, int kvh, int sinks, int recent, const flo
   // thread t: the last round's bin t, in the whole row and in the chunks before this one
   const int64_t at = r.chunk0 + static_cast<int64_t>(h) * chunks;
   uint32_t all = 0, before = 0, more0 = 0;
+#pragma unroll 8
   for (int x = 0; x < chunks; ++x) {
     const uint32_t n = ws.low[(at + x) * kLowBins + tid];
     all += n;
