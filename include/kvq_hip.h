@@ -482,8 +482,8 @@ int kvq_fp8_pth_decode_attn(const void* query, int dtype, int64_t batch, int64_t
  * every cached position j,
  *   weights_out = (j < seq_lens[b] - query_lens[b] ? weights_in : 0)
  *                 + the sum of its attention weights over the request's rows and
- *                   the heads of the kv head's group,
- * positions behind seq_lens[b] and requests without rows untouched.
+ *                   the heads of the kv head's group
+ * (a request without rows: its weights_in), positions behind seq_lens[b] untouched.
  * The lengths (host int64 [batch]) are read during the call and travel with the
  * launches.  `workspace` holds kvq_fp8_pth_window_attn_workspace_bytes for the
  * same arguments and device; a smaller one returns KVQ_ERR_INVALID before

@@ -1,0 +1,63 @@
+# SPDX-License-Identifier: Apache-2.0
+"""Windowed attention, running weights and eviction over the paged E4M3 cache, on
+the GPU: calls and values at the edges of what is allowed."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import _fp8_window as ref
+from vllm_ascend_quantized_kv_cache.ops import fp8_window
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+attend = fp8_window.fp8_per_token_head_window_attention
+
+
+# ---- requests without new rows ---------------------------------------------------
+
+
+@pytest.mark.parametrize("hq,kvh,d,bs,dtype", [(8, 2, 128, 32, BF16), (4, 2, 64, 16, FP16),
+                                               (6, 2, 96, 16, BF16), (4, 1, 64, 16, FP32)])
+@pytest.mark.parametrize("news", [[2, 0, 0, 70, 0], [0, 0, 0, 0, 1], [0] * 5])
+def test_weights_of_idle_requests_go_on(gpu_device, hq, kvh, d, bs, dtype, news):
+    """A step's ``out_weights`` hold every request's running weights: those of one
+    without rows as they were, up to its length."""
+    lens, rows, cols = [300, 1500, 0, 90, 1], [4, 0, 5, 2, 1], 1507
+    c = ref.Cache(lens, kvh, d, bs, device=gpu_device, seed=31)
+    q = ref.query(sum(news), hq, d, dtype, gpu_device)
+    scale = d ** -0.5
+    out, bound, sums, sum_bounds = ref.attention64(q, c, lens, news, scale, 200, 4)
+    before = torch.rand(7, kvh, cols, device=gpu_device)
+    start = torch.full_like(before, -3.0)
+    for b, r in enumerate(rows):  # what the step leaves of the old weights, and where
+        start[r, :, :lens[b]] = before[r, :, :lens[b]]
+    after = torch.full_like(before, -3.0)
+    got = attend(q, *c.args(), lens, news, scale, window=200, sinks=4, weights=before,
+                 out_weights=after, weight_rows=rows, block_table_host=c.host)
+    ref.check_out(got, out, bound, dtype)
+    ref.check_weights(start, after, sums, sum_bounds, rows, lens, news)
+    same = before.clone()
+    attend(q, *c.args(), lens, news, scale, window=200, sinks=4, weights=same, weight_rows=rows,
+           block_table_host=c.host)
+    for b, r in enumerate(rows):
+        assert torch.equal(same[r, :, :lens[b]], after[r, :, :lens[b]])
+        assert torch.equal(same[r, :, lens[b]:], before[r, :, lens[b]:])
+
+
+def test_weights_of_many_idle_requests(gpu_device):
+    """More than a launch's argument holds, two buffers in turn."""
+    lens = [(53 * b) % 97 for b in range(260)]
+    c = ref.Cache(lens, 1, 64, 16, device=gpu_device, seed=32)
+    w = [torch.rand(260, 1, 97, device=gpu_device), torch.full((260, 1, 97), -1.0,
+                                                               device=gpu_device)]
+    one = w[0].clone()
+    for step in range(4):
+        news = [int(b % 50 == step and lens[b] > 0) for b in range(260)]
+        q = ref.query(sum(news), 2, 64, BF16, gpu_device, seed=step)
+        attend(q, *c.args(), lens, news, 0.1, weights=w[step % 2], out_weights=w[1 - step % 2])
+        attend(q, *c.args(), lens, news, 0.1, weights=one)
+    for b, n in enumerate(lens):
+        assert torch.equal(w[0][b, :, :n], one[b, :, :n])

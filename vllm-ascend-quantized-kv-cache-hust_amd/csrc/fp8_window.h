@@ -218,9 +218,9 @@ struct WinCall {
 // rows): whether request b takes part, its workgroups, its parts and its partial rows
 // (of whatever the kernel leaves in the workspace); go(arg, requests, workgroups,
 // partial rows).  Partial rows count from 0 in every launch: launches of one stream
-// share the workspace.
+// share the workspace.  Of the requests with rows, or those without (idle).
 template <typename U, typename G>
-int win_launches(const WinCall& call, U&& shape, G&& go) {
+int win_launches(const WinCall& call, U&& shape, G&& go, bool idle = false) {
   WinArg arg;
   int count = 0;
   int64_t total = 0, q0 = 0, part0 = 0;
@@ -233,7 +233,7 @@ int win_launches(const WinCall& call, U&& shape, G&& go) {
     }
     if (b == call.batch) break;
     int64_t units = 0, parts = 1, rows = 0;
-    if (call.qlens[b] > 0 && shape(b, units, parts, rows) && units > 0) {
+    if ((call.qlens[b] == 0) == idle && shape(b, units, parts, rows) && units > 0) {
       if (total + units > 0x7fffffff) return KVQ_ERR_INVALID;
       arg.r[count++] = WinReq{static_cast<int32_t>(q0), static_cast<int32_t>(call.qlens[b]),
                               static_cast<int32_t>(call.lens[b]), static_cast<int32_t>(b),

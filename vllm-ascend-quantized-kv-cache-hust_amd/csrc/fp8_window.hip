@@ -251,6 +251,22 @@ win_weights_general_kernel(WinArg, int count, WinCache c, const T* __restrict__ 
   w_out[dst] = (j < first ? w_in[dst] : 0.0f) + sum;
 }
 
+// The running weights of a request without rows, into the other array.  A unit is
+// kIdleSpan positions of one kv head.
+constexpr int kIdleSpan = 1024;
+
+__global__ void __launch_bounds__(256)
+win_weights_idle_kernel(WinArg, int count, int kvh, const float* __restrict__ w_in,
+                        float* __restrict__ w_out, int64_t w_cols) {
+  const WinReq r = win_req(count, blockIdx.x);
+  const int u = static_cast<int>(blockIdx.x) - r.first;
+  const int h = u % kvh, j0 = u / kvh * kIdleSpan + static_cast<int>(threadIdx.x);
+  const int64_t row = (static_cast<int64_t>(r.wrow) * kvh + h) * w_cols;
+#pragma unroll
+  for (int k = 0; k < kIdleSpan; k += 256)
+    if (j0 + k < r.len) w_out[row + j0 + k] = w_in[row + j0 + k];
+}
+
 // ---- joining partial results ---------------------------------------------------------
 
 constexpr int kJoinThreads = 256;
@@ -423,6 +439,24 @@ int weigh_general(const WinCall& call) {
       });
 }
 
+// What running weights that go to another array leave of requests without rows.
+int copy_idle(const WinCall& call) {
+  return win_launches(
+      call,
+      [&](int64_t b, int64_t& units, int64_t&, int64_t&) {
+        units = (call.lens[b] + kIdleSpan - 1) / kIdleSpan * call.cache.kvh;
+        return true;
+      },
+      [&](const WinArg& arg, int count, int64_t blocks, int64_t) -> int {
+        hipLaunchKernelGGL(win_weights_idle_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256),
+                           0, call.stream, arg, count, call.cache.kvh, call.w_in, call.w_out,
+                           call.w_cols);
+        KVQ_LAUNCH_CHECK();
+        return KVQ_OK;
+      },
+      true);
+}
+
 // Lengths, window and geometry, checked alike by the sizing call and the call.
 int check_shape(const int64_t* lens, const int64_t* qlens, int64_t batch, int dtype, int hq, int kvh,
                 int d, int bs, int64_t window, int64_t sinks) {
@@ -526,20 +560,22 @@ extern "C" int kvq_fp8_pth_window_attn(
   if (rc != KVQ_OK) return rc;
   int64_t rows = 0;
   for (int64_t b = 0; b < batch; ++b) rows += query_lens[b];
-  if (rows == 0) return KVQ_OK;
-  if (!query || !k_data || !k_scale || !v_data || !v_scale || !block_table || !out ||
-      num_blocks <= 0 || max_blocks < 0 || !(scale > 0.0f && scale < INFINITY) ||
-      query_stride < static_cast<int64_t>(num_heads) * head_size)
+  // running weights that go to another array go there whole: of requests without rows too
+  const bool weigh = weights_out != nullptr, apart = weigh && weights_in && weights_in != weights_out;
+  if (rows == 0 && !apart) return KVQ_OK;
+  if (rows > 0 &&
+      (!query || !k_data || !k_scale || !v_data || !v_scale || !block_table || !out ||
+       num_blocks <= 0 || max_blocks < 0 || !(scale > 0.0f && scale < INFINITY) ||
+       query_stride < static_cast<int64_t>(num_heads) * head_size))
     return KVQ_ERR_INVALID;
   if (block_index_type != KVQ_INDEX_I32 && block_index_type != KVQ_INDEX_I64)
     return KVQ_ERR_INVALID;
   if ((reinterpret_cast<uintptr_t>(k_data) | reinterpret_cast<uintptr_t>(v_data)) & 3)
     return KVQ_ERR_GEOMETRY;  // a row's words
-  const bool weigh = weights_out != nullptr;
   if (weigh != (weights_in != nullptr) || (weigh && !weight_rows)) return KVQ_ERR_INVALID;
   for (int64_t b = 0; b < batch; ++b) {
-    if (query_lens[b] == 0) continue;
-    if (seq_lens[b] > max_blocks * block_size) return KVQ_ERR_INVALID;
+    if (query_lens[b] == 0 && !apart) continue;
+    if (query_lens[b] > 0 && seq_lens[b] > max_blocks * block_size) return KVQ_ERR_INVALID;
     if (weigh && (seq_lens[b] > weight_cols || weight_rows[b] < 0 || weight_rows[b] > kMaxPositions))
       return KVQ_ERR_INVALID;
   }
@@ -559,6 +595,8 @@ extern "C" int kvq_fp8_pth_window_attn(
   call.w_cols = weight_cols;
   call.out = out;
   call.stream = static_cast<hipStream_t>(stream);
+  if (apart) rc = copy_idle(call);
+  if (rc != KVQ_OK || rows == 0) return rc;
   const Layout layout = layout_of(call, weigh, &rc);
   if (rc != KVQ_OK) return rc;
   if (layout.total() > 0 &&

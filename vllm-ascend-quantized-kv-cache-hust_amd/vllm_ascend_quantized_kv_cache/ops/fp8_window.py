@@ -183,7 +183,9 @@ def fp8_per_token_head_window_attention(
     ``weight_rows[b]``, by default ``b``) are the running attention weights:
     every cached position gains the sum of its weights over the request's rows
     and the query heads of the kv head; the new rows' own positions start from
-    nothing.  They are updated in place, or written to ``out_weights``.
+    nothing.  They are updated in place, or written to ``out_weights``, where a
+    request without new rows has its old ones; positions past a request's length
+    and rows of other requests stay as they were there.
 
     ``query`` may have rows behind the last request's (a padded batch), and its
     rows may lie apart (a view of a fused projection); rows of ``out`` behind
@@ -247,7 +249,9 @@ def fp8_per_token_head_window_attention(
     direct = out is None or (
         out.is_contiguous() and out.dtype == query.dtype
         and out.untyped_storage().data_ptr() != query.untyped_storage().data_ptr())
-    if rows:
+    # weights that go to another tensor go there of requests without rows too
+    apart = target is not None and longest > 0 and target.data_ptr() != weights.data_ptr()
+    if rows or apart:
         _native.require_gpu_tensors(_ATTENTION, query, k_data)
     q = query
     strides = q.stride()
@@ -258,7 +262,7 @@ def fp8_per_token_head_window_attention(
         out is None or not direct) else out
     if rows < tokens and out is None:
         result[rows:].zero_()
-    if rows == 0:
+    if rows == 0 and not apart:
         return result if out is None else out
     with _on_device(k_data):
         nbytes = lib.kvq_fp8_pth_window_attn_workspace_bytes(
