@@ -4,6 +4,9 @@ the GPU: calls and values at the edges of what is allowed."""
 
 from __future__ import annotations
 
+import math
+
+import numpy as np
 import pytest
 import torch
 
@@ -61,3 +64,51 @@ def test_weights_of_many_idle_requests(gpu_device):
         attend(q, *c.args(), lens, news, 0.1, weights=one)
     for b, n in enumerate(lens):
         assert torch.equal(w[0][b, :, :n], one[b, :, :n])
+
+
+# ---- probabilities of any size -----------------------------------------------------
+
+
+def _constant_rows(device, length, d, heavy, light, every=64):
+    """One request whose keys give the scores `heavy` (every `every`th position) and
+    `light`, exact for a query of ones and a scale of 1 / D; the heavy rows' values
+    are 1 in dim 0, the light ones' 448 in dim 1, zeros elsewhere."""
+    c = ref.Cache([length], 1, d, 64, device=device, seed=33)
+    c.k.fill_(0x38)
+    at = torch.from_numpy(c.slots(0, np.arange(length))).to(device)
+    big = torch.arange(length, device=device) % every == 0
+    c.ks.view(-1)[at] = torch.where(big, heavy, light).float()
+    c.vs.fill_(1.0)
+    c.v.zero_()
+    v = c.v.view(-1, d)
+    v[at[big], 0] = 0x38
+    v[at[~big], 1] = 0x7E
+    return c
+
+
+@pytest.mark.parametrize("n,hq,d", [(1, 8, 128), (60, 8, 64), (40, 8, 128), (100, 8, 128),
+                                    (2, 64, 128), (40, 8, 256), (40, 8, 96)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("below", [16.0, 25.6, 31.0])
+def test_small_weights_count_beside_large_ones(gpu_device, n, hq, d, dtype, below):
+    """Weights of 2^-below of the largest: they alone fill dim 1 of the result.
+
+    Off by half a step of the result; by the weights' rounding to 16 bits, 2^-11 of
+    each, or 2^-32 of the largest where that is more; and by 2^-16 for the fp32
+    arithmetic (exp2 of exponents up to 32: 32 2^-24, and sums of 700 terms)."""
+    length = 700
+    heavy = float(np.float32(below * math.log(2.0)))
+    c = _constant_rows(gpu_device, length, d, heavy, 0.0)
+    q = torch.ones(n, hq, d, dtype=dtype, device=gpu_device)
+    got = attend(q, *c.args(), [length], [n], 1.0 / d, block_table_host=c.host).double()
+    pos = torch.arange(length - n, length, device=gpu_device, dtype=torch.float64)
+    big = torch.floor(pos / 64) + 1
+    w = math.exp(-heavy)
+    norm = big + (pos + 1 - big) * w
+    want = torch.zeros(n, d, dtype=torch.float64, device=gpu_device)
+    want[:, 0], want[:, 1] = big / norm, 448 * (pos + 1 - big) * w / norm
+    off = (got - want[:, None]).abs()
+    part = ref.HALF_STEP[dtype] + 2.0 ** -11 + 2.0 ** -16
+    tiny = float(torch.finfo(dtype).smallest_normal) * ref.HALF_STEP[dtype] * 2
+    limit = want * (part + torch.tensor([0, 2.0 ** -32 / w] + [0] * (d - 2), device=gpu_device))
+    assert bool((off <= limit[:, None] + tiny).all()), (off - limit[:, None]).max().item()

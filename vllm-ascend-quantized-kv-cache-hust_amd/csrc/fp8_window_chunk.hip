@@ -23,11 +23,16 @@
 //
 // The scales stay out of the operands.  With ks' = k_scale * scale * log2(e) and
 // lv = log2(v_scale) per position,
-//   t = fma(S, ks', lv),  M = running max of t per row,  p' = 2^(t - M) = p v_scale,
-//   O^T += V^T * p'^T (codes in fp16, p' rounded to fp16: 2^-11 of it at most),
+//   t = fma(S, ks', lv),  M = running max of t per row, less 7,  p' = 2^(t - M) = p v_scale,
+//   O^T += V^T * p'^T (codes in fp16, p' rounded to fp16),
 //   l += p' / v_scale in fp32.
 // Taking the maximum with the value scale in it keeps p' within fp16's range
-// whatever the scales are; M moves only when a row's maximum outgrows it by 8.
+// whatever the scales are.  M moves only when a row's maximum outgrows it by 8, so a
+// row's largest p' lies between 2^7 and 2^15 (fp16 ends at 2^16): the rounding is 2^-11
+// of p' at most, or, where fp16 is subnormal, 2^-32 of the row's largest; what is
+// smaller than that counts in l alone (2^20 positions of it: 2^-12).  M closer to the
+// maximum leaves more room below and moves more often (outgrown by 4, less 11: 1647 us
+// for 1612 on the full chunk above and the same card; at every new maximum, less 15: 1691).
 // A value scale that is no positive finite number makes its row of values NaN.
 //
 // Positions a row does not see: weights by selection; in blocks that some row does not
@@ -46,6 +51,8 @@ typedef short c_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) c_s4* c_lds4;
 
 constexpr int kBlock = 64;      // positions
+// a row's maximum lies kRaise over its offset M, and up to kOutgrow more before M moves
+constexpr float kRaise = 7.0f, kOutgrow = 8.0f;
 
 template <int D>
 constexpr int chk_ng() { return D == 256 ? 1 : 2; }  // 16-row column groups of a wave
@@ -370,14 +377,13 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     } else {
       tmax[0] = max_rows4(tmax[0]);
     }
-    // the offset moves only when a row's maximum outgrows it by 8
     bool rescale = false;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) rescale = rescale || tmax[g] - 8.0f > m[g];
+    for (int g = 0; g < NG; ++g) rescale = rescale || tmax[g] - (kRaise + kOutgrow) > m[g];
     if (__any(rescale)) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const float mn = tmax[g] - 8.0f > m[g] ? tmax[g] : m[g];
+        const float mn = tmax[g] - (kRaise + kOutgrow) > m[g] ? tmax[g] - kRaise : m[g];
         const float alpha = __builtin_amdgcn_exp2f(m[g] - mn);
         l[g] *= alpha;
 #pragma unroll
