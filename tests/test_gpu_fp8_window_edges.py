@@ -112,3 +112,47 @@ def test_small_weights_count_beside_large_ones(gpu_device, n, hq, d, dtype, belo
     tiny = float(torch.finfo(dtype).smallest_normal) * ref.HALF_STEP[dtype] * 2
     limit = want * (part + torch.tensor([0, 2.0 ** -32 / w] + [0] * (d - 2), device=gpu_device))
     assert bool((off <= limit[:, None] + tiny).all()), (off - limit[:, None]).max().item()
+
+
+# ---- value scales of any kind --------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,hq,kvh,d", [(1, 8, 2, 128), (3, 8, 2, 128), (40, 8, 2, 128),
+                                        (300, 8, 2, 128), (60, 4, 2, 64), (40, 8, 1, 256),
+                                        (40, 6, 2, 96)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (100, 7)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_value_scales_of_any_sign(gpu_device, n, hq, kvh, d, window, sinks, dtype):
+    """Negative scales, zero and tiny ones, whichever kernel the rows go to: V is
+    code * scale."""
+    lens = [500, 37]
+    news = [n, min(n, 37)]
+    c = ref.Cache(lens, kvh, d, 32, device=gpu_device, seed=34)
+    vs = c.vs.view(-1, kvh)
+    rng = np.random.default_rng(34)
+    kind = torch.from_numpy(rng.integers(0, 6, vs.shape)).to(gpu_device)
+    vs.copy_(torch.where(kind == 0, -vs, torch.where(kind == 1, torch.zeros_like(vs), vs)))
+    vs.copy_(torch.where(kind == 2, vs * 2.0 ** -60, torch.where(kind == 3, vs * -0.0, vs)))
+    # a request whose first positions have nothing but zero scales
+    first = torch.from_numpy(c.slots(1, np.arange(20))).to(gpu_device)
+    vs[first] = 0.0
+    q = ref.query(sum(news), hq, d, dtype, gpu_device, seed=35)
+    scale = d ** -0.5
+    out, bound, sums, sum_bounds = ref.attention64(q, c, lens, news, scale, window, sinks)
+    w = torch.zeros(2, kvh, 500, device=gpu_device)
+    got = attend(q, *c.args(), lens, news, scale, window=window, sinks=sinks, weights=w)
+    ref.check_out(got, out, bound, dtype)
+    ref.check_weights(torch.zeros_like(w), w, sums, sum_bounds, [0, 1], lens, news)
+
+
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_a_value_scale_that_is_no_number_reaches_who_sees_it(gpu_device, n):
+    """NaN and infinite scales: nothing finite from the rows that see one."""
+    lens = [500]
+    for value in (math.nan, math.inf, -math.inf):
+        c = ref.Cache(lens, 1, 128, 32, device=gpu_device, seed=36)
+        c.vs.view(-1)[int(c.slots(0, np.array([490]))[0])] = value
+        q = ref.query(n, 8, 128, BF16, gpu_device, seed=37)
+        got = attend(q, *c.args(), lens, [n], 0.1)
+        see = torch.arange(500 - n, 500, device=gpu_device) >= 490
+        assert not got[see].isfinite().any() and got[~see].isfinite().all()

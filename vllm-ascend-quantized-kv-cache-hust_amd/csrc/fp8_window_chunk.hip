@@ -33,7 +33,9 @@
 // smaller than that counts in l alone (2^20 positions of it: 2^-12).  M closer to the
 // maximum leaves more room below and moves more often (outgrown by 4, less 11: 1647 us
 // for 1612 on the full chunk above and the same card; at every new maximum, less 15: 1691).
-// A value scale that is no positive finite number makes its row of values NaN.
+// lv is that of the scale's magnitude: a negative scale's sign goes to its codes.  One
+// under 2^-90 counts as 0 (codes 0, and 2^-90 stands in for it in lv, which leaves p' and
+// p' / v_scale room in fp32 on either side); one that is not finite makes its row NaN.
 //
 // Positions a row does not see: weights by selection; in blocks that some row does not
 // wholly see, NaN codes of values (and rows of such a scale) are staged as zeros, and
@@ -53,6 +55,7 @@ typedef __attribute__((address_space(3))) c_s4* c_lds4;
 constexpr int kBlock = 64;      // positions
 // a row's maximum lies kRaise over its offset M, and up to kOutgrow more before M moves
 constexpr float kRaise = 7.0f, kOutgrow = 8.0f;
+constexpr float kLeastScale = 0x1p-90f;  // value scales under it count as 0
 
 template <int D>
 constexpr int chk_ng() { return D == 256 ? 1 : 2; }  // 16-row column groups of a wave
@@ -184,9 +187,19 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
           code_op8<T>(x.k[a][0], x.k[a][1]);
       *reinterpret_cast<w_u4*>(p + 16 * ((2 * lch + 1) ^ (row % PPR))) =
           code_op8<T>(x.k[a][2], x.k[a][3]);
-      const bool fine = x.vs[a] >= 0.0f && x.vs[a] < INFINITY;
       w_u4 v = x.v[a];
-      if (!fine) v = w_u4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+      float vs = x.vs[a];
+      if (__any(!(vs >= kLeastScale && vs < INFINITY))) {  // (none that the store writes)
+        const float size = fabsf(vs);
+        const bool fine = size < INFINITY, none = size < kLeastScale;
+        const uint32_t flip = vs < 0.0f ? 0x80808080u : 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t odd = (nan_codes(v[k]) >> 7) * 0xffu;  // NaN stays, times 0 too
+          v[k] = !fine ? 0x7f7f7f7fu : none ? v[k] & odd : v[k] ^ flip;
+        }
+        vs = !fine ? 1.0f : none ? kLeastScale : size;
+      }
       if (cut) {
         const uint32_t odd = nan_codes(v[0]) | nan_codes(v[1]) | nan_codes(v[2]) | nan_codes(v[3]);
         const int at = at_block(i) + row;
@@ -206,13 +219,12 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
       *reinterpret_cast<w_u4*>(p + 16 * ((2 * lch + swap) ^ vswz(row))) = code_op8<f16>(y[0], y[1]);
       *reinterpret_cast<w_u4*>(p + 16 * ((2 * lch + 1 - swap) ^ vswz(row))) =
           code_op8<f16>(y[2], y[3]);
-      // [0][j] ks', [1][j] lv, [2][j] 1 / v_scale; a scale of 0 stands in as 2^-100
+      // [0][j] ks', [1][j] lv, [2][j] 1 / v_scale
       if (lch == 0) {
         float* d = reinterpret_cast<float*>(lds + L::SCALES) + which * 192 + row;
-        const float y = x.vs[a] > 0x1p-100f ? x.vs[a] : 0x1p-100f;
         d[0] = x.ks[a] * qscale;
-        d[64] = fine ? __builtin_amdgcn_logf(y) : 0.0f;
-        d[128] = fine ? __builtin_amdgcn_rcpf(y) : 1.0f;
+        d[64] = __builtin_amdgcn_logf(vs);
+        d[128] = __builtin_amdgcn_rcpf(vs);
       }
     }
   };
@@ -444,8 +456,7 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
         for (int g = 0; g < NG; ++g) any = any || c.sees(row_at(g).pos, kb + x);
         if (!__any(any)) continue;
         const int64_t row = (slot(i, x / 16) + x % 16) * kvh + h;
-        const float vs = c.vs[row];
-        const uint32_t all = vs >= 0.0f && vs < INFINITY ? 0u : 0x80808080u;
+        const uint32_t all = fabsf(c.vs[row]) < INFINITY ? 0u : 0x80808080u;
 #pragma unroll
         for (int j = 0; j < DB; ++j) {
           const uint32_t odd =

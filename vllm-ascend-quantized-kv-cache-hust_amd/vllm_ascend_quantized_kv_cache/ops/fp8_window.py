@@ -175,8 +175,9 @@ def fp8_per_token_head_window_attention(
     ``p`` sees positions ``j <= p``; with ``window``, of those the last
     ``window`` and the first ``sinks``.  A row that sees nothing gives zeros.
     Pages that no row sees any more may be gone from the table (any id).
-    Keys and values are ``code * scale``, not rounded to the query's type, so
-    without a window the result is nearer to that definition than
+    Keys and values are ``code * scale``, whatever the scale's sign (value scales
+    under 2^-90 may count as 0; one that is not finite leaves no finite number in
+    the rows that see it), not rounded to the query's type, so without a window the result is nearer to that definition than
     ``fp8_per_token_head_attention``'s, which attends to rounded rows.
 
     ``weights`` (fp32 ``[rows, KVH, positions]``, request ``b`` in row
