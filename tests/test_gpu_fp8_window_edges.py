@@ -17,6 +17,7 @@ pytestmark = pytest.mark.gpu
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 attend = fp8_window.fp8_per_token_head_window_attention
+evict = fp8_window.fp8_per_token_head_evict
 
 
 # ---- requests without new rows ---------------------------------------------------
@@ -156,3 +157,28 @@ def test_a_value_scale_that_is_no_number_reaches_who_sees_it(gpu_device, n):
         got = attend(q, *c.args(), lens, [n], 0.1)
         see = torch.arange(500 - n, 500, device=gpu_device) >= 490
         assert not got[see].isfinite().any() and got[~see].isfinite().all()
+
+
+# ---- numbers past 64 bits --------------------------------------------------------------
+
+
+@pytest.mark.parametrize("past", [2 ** 31, 2 ** 63, 2 ** 64 + 1])
+def test_windows_and_budgets_without_an_end(gpu_device, past):
+    """A window, sinks or a budget past every length: everything is seen, or stays."""
+    lens, news = [300, 90], [1, 40]
+    c = ref.Cache(lens, 2, 64, 16, device=gpu_device, seed=38)
+    q = ref.query(sum(news), 4, 64, BF16, gpu_device)
+    want = attend(q, *c.args(), lens, news, 0.1)
+    assert torch.equal(attend(q, *c.args(), lens, news, 0.1, window=past, sinks=1), want)
+    assert torch.equal(attend(q, *c.args(), lens, news, 0.1, window=1, sinks=past), want)
+    w = torch.rand(2, 2, 300, device=gpu_device)
+    image = [t.clone() for t in (c.k, c.ks, c.v, c.vs, w)]
+    for keep in (past, [past, past]):
+        new_lens, kept = evict(*c.args(), lens, w, keep, sinks=past, recent=past)
+        assert new_lens == lens
+        for b, n in enumerate(lens):
+            assert torch.equal(kept[b, 0, :n].cpu(), torch.arange(n, dtype=torch.int32))
+            assert bool((kept[b, :, n:] == -1).all())
+    assert all(torch.equal(a, b) for a, b in zip(image, (c.k, c.ks, c.v, c.vs, w)))
+    new_lens, _ = evict(*c.args(), lens, w, [past, 50], sinks=4)
+    assert new_lens == [300, 50]

@@ -30,6 +30,9 @@ from .fp8_ops import _check_contiguous, _check_same_device
 
 _ATTENTION = "fp8_per_token_head_window_attention"
 _EVICT = "fp8_per_token_head_evict"
+#: the most cached positions of a request (the library's limit); windows, sinks and
+#: budgets past it are as good as it
+_MOST = 0x7FFF0000
 
 
 def _on_device(t: torch.Tensor):
@@ -80,6 +83,8 @@ def _lengths(what: str, values, name: str):
         out = (ctypes.c_int64 * len(values))(*values)
     if values and min(values) < 0:
         raise RuntimeError(f"{what}: negative {name}.")
+    if values and max(values) > _MOST:
+        raise RuntimeError(f"{what}: {name} past {_MOST}: {max(values)}.")
     return out, values
 
 
@@ -232,7 +237,7 @@ def fp8_per_token_head_window_attention(
     table, host = _table(block_table, block_table_host, batch)
     width = table.shape[1]
     lib = _native.lib()
-    win, sinks = 0 if window is None else int(window), int(sinks)
+    win, sinks = 0 if window is None else min(int(window), _MOST), min(int(sinks), _MOST)
     bad = lib.kvq_fp8_pth_window_check(host.ctypes.data, 1, width, lens, news, batch, nb, bs, win,
                                        sinks)
     if bad == _native.KVQ_ERR_CAPACITY:
@@ -329,14 +334,14 @@ def fp8_per_token_head_evict(
     longest = max(totals, default=0)
     stay = sinks + recent
     if isinstance(keep, (int, np.integer)):
-        keep = int(keep)
+        keep = min(int(keep), _MOST)
         if keep < 0:
             raise RuntimeError(f"{_EVICT}: negative keep.")
         keeps = (ctypes.c_int64 * batch)(*[keep] * batch)
         new_lens = [n if n < keep else keep for n in totals]
         short = keep < stay and longest > keep
     else:
-        keeps, budgets = _lengths(_EVICT, keep, "keep")
+        keeps, budgets = _lengths(_EVICT, [min(int(k), _MOST) for k in keep], "keep")
         if len(budgets) != batch:
             raise RuntimeError(f"{_EVICT}: {len(budgets)} budgets for {batch} requests.")
         new_lens = [n if n < k else k for n, k in zip(totals, budgets)]
@@ -379,7 +384,7 @@ def fp8_per_token_head_evict(
         rc = lib.kvq_fp8_pth_evict(
             k_data.data_ptr(), k_scale.data_ptr(), v_data.data_ptr(), v_scale.data_ptr(), nb, bs,
             kvh, d, table.data_ptr(), _native.ptr(out_table), _native.index_code(table.dtype),
-            width, out_width, lens, keeps, batch, sinks, recent, weights.data_ptr(),
+            width, out_width, lens, keeps, batch, min(sinks, _MOST), min(recent, _MOST), weights.data_ptr(),
             target.data_ptr(), rows, weights.shape[2], kept.data_ptr(), most, _native.ptr(ws),
             nbytes, _native.stream_of(k_data),
         ) if most else 0
