@@ -182,3 +182,148 @@ def test_windows_and_budgets_without_an_end(gpu_device, past):
     assert all(torch.equal(a, b) for a, b in zip(image, (c.k, c.ks, c.v, c.vs, w)))
     new_lens, _ = evict(*c.args(), lens, w, [past, 50], sinks=4)
     assert new_lens == [300, 50]
+
+
+# ---- pages that are gone, NaN in tall tiles, fp32, captured evictions in place --------
+
+
+@pytest.mark.parametrize("news,hq,kvh,d,bs,dtype", [
+    ([70, 9], 8, 2, 128, 32, BF16),   # keys read for many columns
+    ([1, 3], 8, 2, 128, 32, FP16),    # from the decode's scores
+    ([300, 1], 16, 2, 128, 16, BF16),  # columns in segments
+    ([3, 70], 6, 2, 96, 32, BF16),    # any geometry
+    ([3, 70], 6, 2, 64, 24, FP32),
+])
+@pytest.mark.parametrize("sinks", [0, 20])
+def test_weights_beside_vanished_pages(gpu_device, news, hq, kvh, d, bs, dtype, sinks):
+    """Pages behind the window, gone from the table or given to others that hold NaN,
+    reach neither results nor weights."""
+    lens, window = [2000, 900], 256
+    c = ref.Cache(lens, kvh, d, bs, device=gpu_device, seed=41)
+    q = ref.query(sum(news), hq, d, dtype, gpu_device)
+    scale = d ** -0.5
+    out, bound, sums, sum_bounds = ref.attention64(q, c, lens, news, scale, window, sinks)
+    host, live = c.host.copy(), set()
+    for b in range(2):
+        first = (lens[b] - news[b] - window + 1) // bs
+        for i in range(c.host.shape[1]):
+            if -(-sinks // bs) <= i < first or i >= -(-lens[b] // bs):
+                host[b, i] = (-1, 10 ** 6, 0, c.nb - 1)[i % 4]
+            else:
+                live.add(int(c.host[b, i]))
+    gone = torch.tensor([i for i in range(c.nb) if i not in live], device=gpu_device)
+    c.k[gone], c.v[gone] = 0x7F, 0xFF
+    c.ks[gone], c.vs[gone] = math.nan, math.nan
+    table = torch.from_numpy(host).to(gpu_device, torch.int64)
+    before = torch.rand(2, kvh, 2000, device=gpu_device)
+    after = before.clone()
+    got = attend(q, *c.args()[:4], table, lens, news, scale, window=window, sinks=sinks,
+                 weights=before, out_weights=after, block_table_host=host)
+    ref.check_out(got, out, bound, dtype)
+    ref.check_weights(before, after, sums, sum_bounds, [0, 1], lens, news)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (64, 5), (333, 130)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_nan_in_tall_tiles(gpu_device, window, sinks, dtype):
+    """256-row tiles at head size 128: NaN keys, values and scales at the edges of
+    what their rows see, over more blocks than LDS holds."""
+    lens, news, kvh, d = [1100, 700], [333, 290], 2, 128
+    c = ref.Cache(lens, kvh, d, 32, device=gpu_device, seed=42)
+    k, v = c.k.view(-1, kvh, d), c.v.view(-1, kvh, d)
+    ks, vs = c.ks.view(-1, kvh), c.vs.view(-1, kvh)
+    for b, length in enumerate(lens):  # stale rows behind the last position
+        stale = torch.from_numpy(c.slots(b, np.arange(length, c.host.shape[1] * 32))).to(gpu_device)
+        k[stale], v[stale] = 0x7F, 0xFF
+        ks[stale], vs[stale] = math.nan, math.inf
+
+    def at(b, p):
+        return int(c.slots(b, np.array([p]))[0])
+
+    for p, dim in ((1099, 0), (1000, 77), (868, 127), (800, 31), (3, 5)):
+        v[at(0, p), 0, dim] = 0x7F
+    vs[at(1, 650), 1] = math.nan
+    vs[at(1, 470), 0] = math.inf
+    k[at(1, 699), 0, 9] = 0xFF
+    ks[at(0, 1050), 1] = math.nan
+    q = ref.query(sum(news), 8, d, dtype, gpu_device)
+    scale = d ** -0.5
+    # (the infinite scale's row of values: none finite, as the other kind of scale)
+    out, bound, sums, sum_bounds = ref.attention64(q, c, lens, news, scale, window, sinks)
+    vs[at(1, 470), 0] = math.nan
+    out = torch.where(out.isnan(), out, ref.attention64(q, c, lens, news, scale, window, sinks)[0])
+    vs[at(1, 470), 0] = math.inf
+    before = torch.rand(2, kvh, 1100, device=gpu_device)
+    after = before.clone()
+    got = attend(q, *c.args(), lens, news, scale, window=window, sinks=sinks, weights=before,
+                 out_weights=after)
+    ref.check_out(got, out, bound, dtype)
+    ref.check_weights(before, after, sums, sum_bounds, [0, 1], lens, news)
+
+
+@pytest.mark.parametrize("hq,kvh,d,bs", [(6, 2, 128, 16), (4, 1, 96, 8), (3, 3, 20, 16)])
+def test_fp32_queries_keep_their_bits(gpu_device, hq, kvh, d, bs):
+    """A few positions of alike weight, so that probabilities in 16 bits would show.
+
+    Scores and weights as in ``ref.attention64``: a score off by (D + 16) 2^-24 of its
+    magnitudes A, a weight relatively by twice that and (length + 200) 2^-24; p times
+    the value scale one rounding, the sum over length positions one each, the norm a
+    few: (length + 64) 2^-24."""
+    lens, news = [5, 3, 7], [2, 3, 1]
+    c = ref.Cache(lens, kvh, d, bs, device=gpu_device, seed=43)
+    q = ref.query(sum(news), hq, d, FP32, gpu_device, size=0.1)
+    scale, rep, row = d ** -0.5, hq // kvh, 0
+    got = attend(q, *c.args(), lens, news, scale).double()
+    told = False
+    for b, (length, n) in enumerate(zip(lens, news)):
+        k, v = c.rows(b, length)
+        for i in range(n):
+            m = length - n + i + 1
+            for head in range(hq):
+                kk, vv = k[:m, head // rep], v[:m, head // rep]
+                x = q[row, head].double()
+                p = torch.softmax(kk @ x * scale, 0)
+                a = (kk.abs() @ x.abs()).max() * scale
+                part = (2 * (d + 16) * a + 2 * length + 264) * 2.0 ** -24
+                want, size = p @ vv, p @ vv.abs()
+                limit = 2.0 ** -24 * want.abs() + (1 + 2.0 ** -24) * part * size + 2.0 ** -149
+                assert bool(((got[row, head] - want).abs() <= limit).all())
+                told |= bool(((p.half().double() @ vv - want).abs() > limit).any())
+            row += 1
+    assert told  # the limit is one that 16 bits break
+
+
+def test_captured_evictions_in_place(gpu_device):
+    """Short and long rows, codes, scales and weights moving within their own pages;
+    replays follow what is there."""
+    lens, keep = [40000, 900, 300], 500
+    c = ref.Cache(lens, 2, 64, 64, device=gpu_device, seed=44)
+    w = torch.rand(3, 2, 40000, device=gpu_device)
+    parts = (c.k, c.ks, c.v, c.vs, w)
+    image = [t.clone() for t in parts]
+    kw = dict(sinks=4, recent=50, block_table_host=c.host)
+    evict(*c.args(), lens, w, keep, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, kept = evict(*c.args(), lens, w, keep, **kw)
+    for seed in range(3):
+        new = torch.rand(w.shape, generator=torch.Generator().manual_seed(seed)).to(gpu_device)
+
+        def restore():
+            for t, old in zip(parts, image):
+                t.copy_(old)
+            w.copy_(new)
+
+        restore()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (kept, *parts)]
+        restore()
+        new_lens, again = evict(*c.args(), lens, w, keep, **kw)
+        torch.cuda.synchronize()
+        assert new_lens == [500, 500, 300]
+        for a, b in zip(got, (again, *parts)):
+            assert torch.equal(a, b)
+        ids = ref.kept_rows(new[0, 1].cpu().numpy(), lens[0], keep, 4, 50)
+        np.testing.assert_array_equal(again[0, 1].cpu().numpy(), ids)
