@@ -327,3 +327,29 @@ def test_captured_evictions_in_place(gpu_device):
             assert torch.equal(a, b)
         ids = ref.kept_rows(new[0, 1].cpu().numpy(), lens[0], keep, 4, 50)
         np.testing.assert_array_equal(again[0, 1].cpu().numpy(), ids)
+
+
+# ---- parts of uneven requests ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF16), (64, FP16), (256, BF16), (96, FP16)])
+@pytest.mark.parametrize("long,short,batch", [(1200, 8, 40), (3, 1, 150), (1, 900, 2)])
+def test_joined_parts_of_uneven_requests(gpu_device, d, dtype, long, short, batch):
+    """One request of many rows beside many of few, all of them or some in parts,
+    requests of one part and without rows between them."""
+    lens = [2500] + [(1500, 20, 2300)[b % 3] for b in range(batch)] + [3000]
+    news = [long] + [(short, 1, 0, short)[b % 4] for b in range(batch)] + [short]
+    c = ref.Cache([3000] * 4, 1, d, 16, device=gpu_device, seed=45)
+    c.host = np.stack([c.host[b % 4] for b in range(len(lens))])
+    c.table = torch.from_numpy(c.host).to(gpu_device, torch.int32)
+    c.lens = lens
+    q = ref.query(sum(news), 8, d, dtype, gpu_device)
+    scale = d ** -0.5
+    for window, sinks in ((None, 0), (1700, 3)):
+        out, bound, sums, sum_bounds = ref.attention64(q, c, lens, news, scale, window, sinks)
+        before = torch.rand(len(lens), 1, 3000, device=gpu_device)
+        after = before.clone()
+        got = attend(q, *c.args(), lens, news, scale, window=window, sinks=sinks, weights=before,
+                     out_weights=after, block_table_host=c.host)
+        ref.check_out(got, out, bound, dtype)
+        ref.check_weights(before, after, sums, sum_bounds, list(range(len(lens))), lens, news)

@@ -34,10 +34,16 @@ struct WinArg {
 };
 static_assert(sizeof(WinArg) <= 3584, "kernel arguments end at 4 KB");
 
-// The request whose units [first, first + its own) hold `unit`, read in place:
-// the argument is the kernel's first (indexed by value it would be copied to
-// scratch).  All lanes of the wave ask for the same unit.
+// Request `at` (uniform) of the launch, read in place: the argument is the kernel's
+// first (indexed by value it would be copied to scratch).
 typedef const __attribute__((address_space(4))) int32_t win_cint;
+__device__ __forceinline__ WinReq win_req_at(int at) {
+  win_cint* r = (win_cint*)__builtin_amdgcn_kernarg_segment_ptr() + 8 * at;
+  return WinReq{r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]};
+}
+
+// The request whose units [first, first + its own) hold `unit`.  All lanes of the wave
+// ask for the same unit.
 __device__ __forceinline__ WinReq win_req(int count, int unit) {
   win_cint* a = (win_cint*)__builtin_amdgcn_kernarg_segment_ptr();
   const int lane = threadIdx.x & 63;
@@ -47,8 +53,7 @@ __device__ __forceinline__ WinReq win_req(int count, int unit) {
     at += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on));
   }
   // requests without units share their first with the next one that has some
-  win_cint* r = a + 8 * __builtin_amdgcn_readfirstlane(at - 1);
-  return WinReq{r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]};
+  return win_req_at(__builtin_amdgcn_readfirstlane(at - 1));
 }
 
 // Everything else a kernel needs of the cache.

@@ -271,19 +271,22 @@ win_weights_idle_kernel(WinArg, int count, int kvh, const float* __restrict__ w_
 
 constexpr int kJoinThreads = 256;
 
-// blockIdx.y: the request, blockIdx.x: row * hq + head.  d / 4 threads hold a part's
-// row, the workgroup several parts at once, joined in LDS in a fixed order.  D: d, or 0
-// for any.
+// A unit is a row and head of a request that has parts: blockIdx.x of request blockIdx.y,
+// or, where the grid has one row for several requests, of all of them.  d / 4 threads hold
+// a part's row, the workgroup several parts at once, joined in LDS in a fixed order.
+// D: d, or 0 for any.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-win_join_kernel(WinArg, int hq, int any_d, WinParts parts, T* __restrict__ out,
+win_join_kernel(WinArg, int requests, int hq, int any_d, WinParts parts, T* __restrict__ out,
                 float* __restrict__ lse) {
   const int d = D ? D : any_d, lanes = d / 4, slices = kJoinThreads / lanes;
   __shared__ w_f4 s_o[kJoinThreads];
-  win_cint* a = (win_cint*)__builtin_amdgcn_kernarg_segment_ptr() + 8 * blockIdx.y;
-  const int q0 = a[0], n = a[1], count = a[5], part0 = a[6];
-  const int64_t x = blockIdx.x, stride = static_cast<int64_t>(n) * hq;
-  if (count <= 1 || x >= stride) return;
+  const bool flat = gridDim.y == 1 && requests > 1;
+  const WinReq r = flat ? win_req(requests, blockIdx.x) : win_req_at(blockIdx.y);
+  const int q0 = r.q0, count = r.parts, part0 = r.part0;
+  const int64_t x = static_cast<int>(blockIdx.x) - (flat ? r.first : 0);
+  const int64_t stride = static_cast<int64_t>(r.n) * hq;
+  if (x >= stride) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const w_f2* ml = reinterpret_cast<const w_f2*>(parts.ml) + part0 + x;
   float m = -INFINITY;
@@ -332,15 +335,26 @@ win_join_kernel(WinArg, int hq, int any_d, WinParts parts, T* __restrict__ out,
 namespace kvq {
 
 int launch_win_join(const WinCall& call, const WinArg& arg, int count, WinParts parts) {
-  int64_t rows = 0;
-  for (int i = 0; i < count; ++i)
-    if (arg.r[i].parts > 1) rows = std::max<int64_t>(rows, arg.r[i].n);
-  if (rows == 0) return KVQ_OK;
   const int hq = call.cache.hq;
-  const dim3 grid(static_cast<unsigned>(rows * hq), static_cast<unsigned>(count));
+  WinArg cut;
+  int n = 0;
+  int64_t units = 0, most = 0;  // (at most the call's rows and heads, < 2^31)
+  for (int i = 0; i < count; ++i) {
+    if (arg.r[i].parts <= 1) continue;
+    cut.r[n] = arg.r[i];
+    cut.r[n++].first = static_cast<int32_t>(units);
+    units += static_cast<int64_t>(arg.r[i].n) * hq;
+    most = std::max(most, static_cast<int64_t>(arg.r[i].n) * hq);
+  }
+  if (n == 0) return KVQ_OK;
+  // a grid of requests by the most rows, where half of it has rows (the request is at hand:
+  // 64 of one row each, 104.0 us a call for 104.9), or of all rows in a line (100 requests of
+  // 8 rows beside one of 2000: 204 us for 518, 347 of it in the empty rest of the grid)
+  const dim3 grid = most * n <= 2 * units ? dim3(static_cast<unsigned>(most), static_cast<unsigned>(n))
+                                          : dim3(static_cast<unsigned>(units));
 #define KVQ_WIN_JOIN(T, D)                                                                    \
-  hipLaunchKernelGGL((win_join_kernel<T, D>), grid, dim3(kJoinThreads), 0, call.stream, arg, hq, \
-                     call.cache.d, parts, static_cast<T*>(call.out), call.lse)
+  hipLaunchKernelGGL((win_join_kernel<T, D>), grid, dim3(kJoinThreads), 0, call.stream, cut, n, \
+                     hq, call.cache.d, parts, static_cast<T*>(call.out), call.lse)
 #define KVQ_WIN_JOIN_D(T)                                                              \
   if (call.cache.d == 64) KVQ_WIN_JOIN(T, 64); else if (call.cache.d == 128)           \
   KVQ_WIN_JOIN(T, 128); else if (call.cache.d == 256) KVQ_WIN_JOIN(T, 256); else       \
