@@ -259,11 +259,14 @@ inline int64_t win_part_rows(const WinCall& call, int64_t b, int64_t parts) {
   return parts > 1 ? parts * call.qlens[b] * call.cache.hq : 0;
 }
 // Requests whose decode leaves its scores in the workspace, [kv head][column][positions,
-// a multiple of 16] in the log2 domain, for the weights to be summed from: writing and
-// reading 4 bytes a column and position is less than the keys once more (D + 4 bytes)
-// below this many columns, while all of them stay a small workspace (32 requests of
-// 2048 - 16384 positions, 8 kv heads of 128, 4, 12 and 16 columns: 161, 201 and 227 us a
-// call with the scores, 215, 217 and 215 without).
+// a multiple of 16] in the log2 domain, for the weights to be summed from: below this
+// many columns that takes less than the keys once more and their products, while all of
+// them stay a small workspace.  Written and read, a column's 4 bytes a position are less
+// than the keys' D + 4 up to 15 columns at D = 128 and up to 8 at 64, where the products
+// they spare decide.  32 requests of 2048 - 16384 positions, us a call with the scores
+// and without, 9, 12 and 15 columns: 8 kv heads of 64, 124, 134 and 147 to 146, 147 and
+// 149; 8 of 128, 196, 210 and 227 to 216, 219 and 222; 2 of 256, 89, 94 and 99 to 101, 102
+// and 104.  16 columns, 8 kv heads of 128: 227 to 215.
 constexpr int kScoreCols = 16;
 constexpr int64_t kScoreBytes = 256ll << 20;
 struct WinScores {

@@ -2,8 +2,8 @@
 // Windowed attention over paged E4M3 rows for chunks: tiles of 128 or 256 rows (a row
 // is one query of one head of a kv head's group), 64-position blocks, bound by the
 // matrix units and the softmax beside them: 4 chunks of 2048 queries over 10240
-// positions, 40 heads on 8 of 128, 1.57 ms, 0.98 PFLOP/s, where a plain 8192^3 product
-// reaches 1.28; 6 of 200 - 1500 over 3000 - 9000, 8 heads on 1 of 256, window 2048, 97 us,
+// positions, 40 heads on 8 of 128, 1.55 - 1.61 ms by the card, 0.96 - 1.0 PFLOP/s, where a
+// plain 8192^3 product reaches 1.28; 6 of 200 - 1500 over 3000 - 9000, 8 heads on 1 of 256, window 2048, 97 us,
 // the operands' LDS reads (64 KB a wave and block) being most of it.  Matrix and vector
 // work of a SIMD's waves overlap only in part: 64 products of 16 x 16 x 32 by themselves
 // take 480 ns, 256 fma 478, both, on each of two waves, 690 a wave.
@@ -30,9 +30,11 @@
 // whatever the scales are.  M moves only when a row's maximum outgrows it by 8, so a
 // row's largest p' lies between 2^7 and 2^15 (fp16 ends at 2^16): the rounding is 2^-11
 // of p' at most, or, where fp16 is subnormal, 2^-32 of the row's largest; what is
-// smaller than that counts in l alone (2^20 positions of it: 2^-12).  M closer to the
-// maximum leaves more room below and moves more often (outgrown by 4, less 11: 1647 us
-// for 1612 on the full chunk above and the same card; at every new maximum, less 15: 1691).
+// smaller than that counts in l alone (2^20 positions of it: 2^-12), as l takes p' before
+// its rounding.  (fp16 results lie a quarter farther from exact ones than with p' in fp32,
+// bf16 ones do not; parts of 16 bits each would double the value products.)  M closer to
+// the maximum leaves more room below and moves more often: outgrown by 4, less 11, 1647 us
+// for 1612 on the full chunk above and the same card; at every new maximum, less 15, 1691.
 // lv is that of the scale's magnitude: a negative scale's sign goes to its codes.  One
 // under 2^-90 counts as 0 (codes 0, and 2^-90 stands in for it in lv, which leaves p' and
 // p' / v_scale room in fp32 on either side); one that is not finite makes its row NaN.

@@ -179,7 +179,11 @@ def fp8_per_token_head_window_attention(
     positions (their keys and values are stored already).  A row at position
     ``p`` sees positions ``j <= p``; with ``window``, of those the last
     ``window`` and the first ``sinks``.  A row that sees nothing gives zeros.
+    Positions are places in the cache: after an eviction a window counts the rows
+    that were kept, other ones for each kv head.
     Pages that no row sees any more may be gone from the table (any id).
+    ``block_table_host`` is the host's copy of the table, by which the pages are
+    checked; without it the table is copied from the device and waited for.
     Keys and values are ``code * scale``, whatever the scale's sign (value scales
     under 2^-90 may count as 0; one that is not finite leaves no finite number in
     the rows that see it), not rounded to the query's type, so without a window the result is nearer to that definition than
@@ -196,7 +200,7 @@ def fp8_per_token_head_window_attention(
     ``query`` may have rows behind the last request's (a padded batch), and its
     rows may lie apart (a view of a fused projection); rows of ``out`` behind
     the last request's stay as they were, zeros in a fresh one.  bf16, fp16 or
-    fp32 queries, any head size of the cache.
+    fp32 queries, head sizes up to 512.
     """
     nb, bs, kvh, d = _check_cache(k_data, k_scale, v_data, v_scale)
     if query.dim() != 3 or query.shape[2] != d:
@@ -322,7 +326,9 @@ def fp8_per_token_head_evict(
     new length]`` with -1 behind a request's rows.  Rows behind the new lengths
     stay as they were.  A page that rows move within or to may belong to one
     request only; pages shared between requests (a common prefix) can be read
-    from with ``out_block_table``.
+    from with ``out_block_table``.  The tables' host copies are as in
+    ``fp8_per_token_head_window_attention``; positions, and so windows, count the
+    rows kept from here on.
     """
     nb, bs, kvh, d = _check_cache(k_data, k_scale, v_data, v_scale)
     if kvh == 0 or d == 0:
