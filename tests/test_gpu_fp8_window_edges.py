@@ -353,3 +353,54 @@ def test_joined_parts_of_uneven_requests(gpu_device, d, dtype, long, short, batc
                      out_weights=after, block_table_host=c.host)
         ref.check_out(got, out, bound, dtype)
         ref.check_weights(before, after, sums, sum_bounds, list(range(len(lens))), lens, news)
+
+
+# ---- offsets past 32 bits ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("d,bs,hq,kvh", [(128, 128, 32, 8), (64, 64, 8, 8), (256, 128, 8, 4),
+                                         (96, 128, 8, 8)])
+def test_pages_and_weights_past_32_bits(gpu_device, d, bs, hq, kvh):
+    """Caches of more than 2^32 bytes a side and 2^31 weights: the last pages and rows
+    give what the first ones of a small cache do, bit for bit."""
+    lens, news = [900, 300], [1, 70]
+    c = ref.Cache(lens, kvh, d, bs, device=gpu_device, seed=46, spare=40)
+    pages = (1 << 32) // (bs * kvh * d) + c.nb + 5
+    rows, cols = 2 + (1 << 31) // (kvh * 901), 901
+    base = pages - c.nb
+    big = ref.Cache([1], kvh, d, bs, device=gpu_device)
+    for name in ("k", "ks", "v", "vs"):
+        small = getattr(c, name)
+        t = torch.empty((pages, *small.shape[1:]), dtype=small.dtype, device=gpu_device)
+        t[base:] = small
+        setattr(big, name, t)
+    big.host = c.host + base
+    big.table = torch.from_numpy(big.host).to(gpu_device, torch.int32)
+    w = torch.rand(2, kvh, cols, device=gpu_device)
+    wide = torch.empty((rows, kvh, cols), device=gpu_device)
+    at = [rows - 1, rows - 2]
+    for b in range(2):
+        wide[at[b]] = w[b]
+    for window, sinks in ((None, 0), (200, 4)):
+        for n in ([1, 70], [3, 1], [300, 0]):
+            q = ref.query(sum(n), hq, d, BF16, gpu_device)
+            kw = dict(window=window, sinks=sinks)
+            want = attend(q, *c.args(), lens, n, 0.1, weights=w, **kw)
+            got = attend(q, *big.args(), lens, n, 0.1, weights=wide, weight_rows=at, **kw)
+            assert torch.equal(got, want)
+            assert all(torch.equal(wide[at[b]], w[b]) for b in range(2))
+    free = [i for i in range(c.nb) if i not in set(c.host.reshape(-1).tolist())]
+    dst = np.array(free[:2 * -(-100 // bs)], dtype=np.int64).reshape(2, -1)
+    for fresh in (True, False):
+        for cache, weights, r, off in ((c, w, [0, 1], 0), (big, wide, at, base)):
+            kw = dict(out_block_table=torch.from_numpy(dst + off).to(gpu_device, torch.int32),
+                      out_weights=weights.clone()) if fresh and off == 0 else {}
+            if fresh and off:
+                kw = dict(out_block_table=torch.from_numpy(dst + off).to(gpu_device, torch.int32))
+            evict(*cache.args(), lens, weights, 100, sinks=4, recent=20, weight_rows=r, **kw)
+            if fresh and off:  # (in place, where the small cache's went to a copy)
+                for b in range(2):
+                    wide[at[b]] = w[b]
+        for name in ("k", "ks", "v", "vs"):
+            assert torch.equal(getattr(big, name)[base:], getattr(c, name))
+    assert all(torch.equal(wide[at[b]], w[b]) for b in range(2))
