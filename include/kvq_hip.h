@@ -472,6 +472,8 @@ int kvq_fp8_pth_decode_attn(const void* query, int dtype, int64_t batch, int64_t
  * head] and V likewise, not rounded to `dtype`; softmax in fp32.  A row at position
  * p sees j <= p and, with window > 0, of those j > p - window or j < sinks
  * (window 0: all).  A row that sees nothing gives zeros.
+ * Scales of either sign; value scales under 2^-90 may count as 0, and one that is not
+ * finite leaves no finite number in the rows that see it.
  *   query [>= sum query_lens, num_heads, D] of `dtype`, its rows query_stride
  *   elements apart (heads and dims contiguous); out contiguous; rows behind the
  *   last request's are left alone.  D % 4 == 0, D <= 512, codes on 4-byte bounds.
