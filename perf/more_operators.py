@@ -1,6 +1,7 @@
 # SPDX-License-Identifier: Apache-2.0
-"""Appending rotated keys and values to 8-bit pages, and attention over pages
-with a scale for each block of positions and head, as measurable calls.
+"""Appending rotated rows to 8-bit pages, and attention over pages with a scale
+for each block of positions and head and over pages of shared latent rows, as
+measurable calls.
 
 ``rope``    a step's query, key and value rows, as the projection leaves them:
             queries and keys rotated to their positions, keys and values stored
@@ -9,6 +10,12 @@ with a scale for each block of positions and head, as measurable calls.
             block of positions and head, where a block may hold rows already
 ``attend``  attention of each request's new rows (one token to a whole chunk)
             over such pages, with a sliding window and sinks or without
+``latent_append``  a step's latent rows (one a token, shared by all heads) as
+            E4M3 codes, their position part rotated beside them, and the
+            queries' position part rotated
+``latent``  attention of new rows over those pages, the up-projections absorbed
+            into the queries and the output: a score is over latent and position
+            part, the values are the latent
 
 A state is one layer's view at that moment.  With ``own`` the calls are the
 package's; without, plain torch.
@@ -47,24 +54,15 @@ def listed():
         dict(name="rope_prefill", kind="rope", batch=8, low=0, high=0, new_low=1500, new_high=2048,
              heads=40, kv_heads=8, head=128, block=128, rot=128, interleaved=False, dtype="bf16",
              pad=0, lens=2),
-        # a mixed step padded to its graph's size: interleaved pairs, half of the head
-        # rotated, head size 64, small pages
-        dict(name="rope_mixed_64", kind="rope", batch=23, low=0, high=3000, new_low=1, new_high=111,
-             heads=14, kv_heads=2, head=64, block=16, rot=32, interleaved=True, dtype="fp16",
-             pad=29, lens=3),
-        # a decode batch (32 query / 8 kv heads): one row into every request's last block
-        dict(name="append_decode", kind="append", codes="e4m3", batch=64, low=1, high=16384,
+        # a decode batch (32 query / 8 kv heads): one row into every request's last block,
+        # padded to its graph's size
+        dict(name="append_decode", kind="append", codes="e4m3", batch=59, low=1, high=16384,
              new_low=1, new_high=1, heads=32, kv_heads=8, head=128, block=128, group=128, rot=128,
-             interleaved=False, dtype="bf16", pad=0, lens=4),
+             interleaved=False, dtype="bf16", pad=5, lens=4),
         # chunks of long prompts behind what is cached already, INT8
         dict(name="append_chunks", kind="append", codes="int8", batch=9, low=0, high=9000,
              new_low=700, new_high=2048, heads=40, kv_heads=8, head=128, block=128, group=128,
              rot=128, interleaved=False, dtype="bf16", pad=0, lens=5),
-        # a few rows a request (speculated tokens), head size 256 on one kv head, fp16,
-        # several scales a page
-        dict(name="append_few_256", kind="append", codes="e4m3", batch=19, low=3, high=9000,
-             new_low=1, new_high=8, heads=8, kv_heads=1, head=256, block=128, group=32, rot=256,
-             interleaved=False, dtype="fp16", pad=13, lens=6),
         # one request's next token on one rank of a TP-4 split, INT8: latency alone
         dict(name="attend_one_token", kind="attend", codes="int8", batch=1, low=600, high=600,
              new_low=1, new_high=1, heads=10, kv_heads=2, head=128, block=128, group=128, window=0,
@@ -73,23 +71,27 @@ def listed():
         dict(name="attend_decode", kind="attend", codes="e4m3", batch=32, low=2048, high=16384,
              new_low=1, new_high=1, heads=40, kv_heads=8, head=128, block=128, group=128, window=0,
              sinks=0, dtype="bf16", lens=8),
-        # a decode batch of long contexts through a 4096-token window with 4 sinks, INT8
-        dict(name="attend_decode_window", kind="attend", codes="int8", batch=64, low=4096,
-             high=16384, new_low=1, new_high=1, heads=32, kv_heads=8, head=128, block=128, group=64,
-             window=4096, sinks=4, dtype="bf16", lens=9),
         # a prefill chunk of 2048 tokens over a long prompt's pages, full causal
         dict(name="attend_chunk", kind="attend", codes="e4m3", batch=4, low=10240, high=10240,
              new_low=2048, new_high=2048, heads=40, kv_heads=8, head=128, block=128, group=128,
              window=0, sinks=0, dtype="bf16", lens=10),
-        # ragged chunks of a sliding-window layer at head size 256, fp16, INT8
-        dict(name="attend_chunk_256", kind="attend", codes="int8", batch=6, low=3001, high=9000,
-             new_low=200, new_high=1500, heads=8, kv_heads=1, head=256, block=128, group=128,
-             window=2048, sinks=16, dtype="fp16", lens=11),
-        # a mixed step: anything from one to a few hundred new rows over short histories,
-        # odd sizes, head size 64, small pages
-        dict(name="attend_mixed_64", kind="attend", codes="e4m3", batch=23, low=333, high=3000,
-             new_low=1, new_high=411, heads=14, kv_heads=2, head=64, block=16, group=16,
-             window=1000, sinks=3, dtype="bf16", lens=12),
+        # a decode batch's next rows, 16 heads a rank
+        dict(name="latent_append_decode", kind="latent_append", batch=64, low=600, high=16384,
+             new_low=1, new_high=1, heads=16, rank=512, block=128, rot=64, interleaved=True,
+             dtype="bf16", pad=0, lens=13),
+        # the step of a prefill batch with all of 128 heads
+        dict(name="latent_append_prefill", kind="latent_append", batch=8, low=0, high=3000,
+             new_low=900, new_high=2048, heads=128, rank=512, block=128, rot=64, interleaved=True,
+             dtype="bf16", pad=0, lens=14),
+        # a decode batch of long contexts, 16 heads a rank: the cache streams through once
+        dict(name="latent_decode_16", kind="latent", batch=32, low=2048, high=16384, new_low=1,
+             new_high=1, heads=16, rank=512, block=128, rot=64, dtype="bf16", lens=15),
+        # all of 128 heads on one card, two rows a request (one speculated)
+        dict(name="latent_decode_128", kind="latent", batch=64, low=1000, high=8192, new_low=2,
+             new_high=2, heads=128, rank=512, block=128, rot=64, dtype="bf16", lens=16),
+        # ragged chunks over what is cached, 16 heads a rank, small pages
+        dict(name="latent_chunk", kind="latent", batch=5, low=1111, high=6000, new_low=100,
+             new_high=1024, heads=16, rank=512, block=64, rot=64, dtype="bf16", lens=17),
     ]
 
 
@@ -99,18 +101,25 @@ def _spread(rng, low, high):
 
 
 def draw(rng):
-    kind = rng.choice(["rope", "append", "append", "attend", "attend", "attend"])
-    head = rng.choice([64, 128, 128, 128, 256])
-    kv_heads = rng.choice([1, 2, 4, 8, 8]) if head < 256 else rng.choice([1, 2])
-    case = dict(kind=kind, kv_heads=kv_heads, head=head, heads=kv_heads * rng.choice([1, 2, 4, 5, 7, 8]),
-                block=rng.choice([16, 32, 64, 128, 128]), dtype=rng.choice(["bf16", "fp16"]),
-                lens=rng.randrange(1 << 30))
-    if kind != "rope":
+    kind = rng.choice(["rope", "append", "append", "attend", "attend", "attend", "latent_append",
+                       "latent", "latent"])
+    case = dict(kind=kind, block=rng.choice([16, 32, 64, 128, 128]),
+                dtype=rng.choice(["bf16", "bf16", "fp16"]), lens=rng.randrange(1 << 30))
+    if kind.startswith("latent"):
+        head, kv_heads = 64, 1
+        case.update(heads=rng.choice([8, 16, 16, 32, 64, 128]), rank=rng.choice([256, 512, 512, 512]),
+                    rot=rng.choice([32, 64, 64, 64]))
+    else:
+        head = rng.choice([64, 128, 128, 128, 256])
+        kv_heads = rng.choice([1, 2, 4, 8, 8]) if head < 256 else rng.choice([1, 2])
+        case.update(kv_heads=kv_heads, head=head, heads=kv_heads * rng.choice([1, 2, 4, 5, 7, 8]))
+    if kind in ("append", "attend"):
         case["codes"] = rng.choice(["e4m3", "int8"])
         case["group"] = rng.choice([g for g in (16, 32, 64, 128) if g <= case["block"]])
-    if kind != "attend":
-        case["rot"] = rng.choice([head, head, head // 2])
-        case["interleaved"] = rng.random() < 0.3
+    if kind in ("rope", "append", "latent_append"):
+        if kind != "latent_append":
+            case["rot"] = rng.choice([head, head, head // 2])
+        case["interleaved"] = rng.random() < (0.7 if kind == "latent_append" else 0.3)
         case["pad"] = rng.choice([0, 0, rng.randint(1, 40)])
         case["high"] = _spread(rng, 1, 16384)
         case["low"] = rng.randint(0, case["high"])
@@ -122,9 +131,11 @@ def draw(rng):
         tokens = 14000000 // (head * (case["heads"] + 2 * kv_heads))
         case["batch"] = _spread(rng, 1, max(1, min(200, tokens // case["new_high"])))
         return case
-    case["window"] = rng.choice([0, _spread(rng, 1, 8192)])
-    case["sinks"] = rng.choice([0, 1, 4, 100]) if case["window"] else 0
-    case["high"] = _spread(rng, 1, 16384)
+    if kind == "attend":
+        case["window"] = rng.choice([0, _spread(rng, 1, 8192)])
+        case["sinks"] = rng.choice([0, 1, 4, 100]) if case["window"] else 0
+    longest = 16384 if kind == "attend" else 8192
+    case["high"] = _spread(rng, 1, longest)
     case["low"] = rng.randint(max(1, case["high"] // 4), case["high"])
     if rng.random() < 0.5:  # decode, or a few rows for every request
         case["new_low"] = case["new_high"] = rng.choice([1, 1, 1, 2, 5])
@@ -132,7 +143,8 @@ def draw(rng):
         case["new_high"] = _spread(rng, 1, min(2048, case["high"]))
         case["new_low"] = rng.randint(1, case["new_high"])
     rows = case["new_high"] * case["heads"] * case["high"]  # scores of a request
-    most = min(64, 2000000000 // rows, 2000000 // (case["high"] * kv_heads))
+    most = min(64, (2000000000 if kind == "attend" else 500000000) // rows,
+               2000000 // (case["high"] * kv_heads))
     case["batch"] = _spread(rng, 1, max(1, most))
     return case
 
@@ -142,7 +154,7 @@ def _lengths(case):
     rng = random.Random(case["lens"])
     total = [rng.randint(case["low"], case["high"]) for _ in range(case["batch"])]
     new = [rng.randint(case["new_low"], case["new_high"]) for _ in total]
-    if case["kind"] == "attend":
+    if case["kind"] in ("attend", "latent"):
         return total, [min(t, n) for t, n in zip(total, new)]
     return [t + n for t, n in zip(total, new)], new  # low .. high rows are there before it
 
@@ -161,18 +173,29 @@ def _seen(total, new, window, sinks):
 
 def work(case):
     total, new = _lengths(case)
-    kvh, hq, d = case["kv_heads"], case["heads"], case["head"]
-    if case["kind"] == "attend":
-        seen = [_seen(t, n, case["window"], case["sinks"]) for t, n in zip(total, new)]
-        cols = sum(s[0] for s in seen)
+    hq = case["heads"]
+    if case["kind"] in ("attend", "latent"):
+        seen = [_seen(t, n, case.get("window"), case.get("sinks")) for t, n in zip(total, new)]
+        cols, pairs = sum(s[0] for s in seen), sum(s[1] for s in seen)
+        if case["kind"] == "latent":
+            r, p = case["rank"], case["rot"]
+            return {"bytes": cols * (r + 4 + 2 * p) + 2 * sum(new) * hq * (2 * r + p),
+                    "flops": 2 * hq * pairs * (2 * r + p)}
+        kvh, d = case["kv_heads"], case["head"]
         moved = 2 * cols * kvh * d + 8 * kvh * (cols // case["group"]) + 4 * sum(new) * hq * d
-        return {"bytes": moved, "flops": 4 * d * hq * sum(s[1] for s in seen)}
+        return {"bytes": moved, "flops": 4 * d * hq * pairs}
     rows, live = sum(new) + case["pad"], sum(new)
+    table = rows * (4 * case["rot"] + 16)
+    if case["kind"] == "latent_append":
+        r, p = case["rank"], case["rot"]
+        return {"bytes": 4 * rows * hq * p + live * (3 * r + 4 + 4 * p) + table,
+                "flops": 3 * rows * (hq + 1) * p}
+    kvh, d = case["kv_heads"], case["head"]
     scales = live
     if case["kind"] == "append":
         g = case["group"]
         scales = sum(-(-t // g) - (t - n) // g for t, n in zip(total, new))
-    moved = 4 * rows * hq * d + 6 * live * kvh * d + 8 * kvh * scales + rows * (4 * case["rot"] + 16)
+    moved = 4 * rows * hq * d + 6 * live * kvh * d + 8 * kvh * scales + table
     return {"bytes": moved, "flops": 3 * rows * (hq + kvh) * case["rot"]}
 
 
@@ -181,18 +204,18 @@ def work(case):
 # ---------------------------------------------------------------------------
 
 
-def _pages(gen, dev, pages, bs, kvh, d, group, codes):
+def _pages(gen, dev, pages, bs, kvh, d, group, codes, sides=2):
     """Keys and values as such a cache holds them: (codes, scales) of each.  Keys have
     outlier channels, values rows of different size.  group 0: a scale for each row."""
     e4m3 = codes == "e4m3"
-    data = torch.empty((2, pages, bs, kvh, d), dtype=torch.uint8 if e4m3 else torch.int8, device=dev)
-    shape = (2, pages, bs // group, kvh) if group else (2, pages, bs, kvh, 1)
+    data = torch.empty((sides, pages, bs, kvh, d), dtype=torch.uint8 if e4m3 else torch.int8, device=dev)
+    shape = (sides, pages, bs // group, kvh) if group else (sides, pages, bs, kvh, 1)
     scale = torch.empty(shape, dtype=torch.float32, device=dev)
     channel = torch.exp(0.5 * torch.randn((kvh, d), generator=gen, device=dev))
     step = max(1, (1 << 26) // (bs * kvh * d))
     for p in range(0, pages, step):
         n = min(step, pages - p)
-        for side in (0, 1):
+        for side in range(sides):
             x = torch.randn((n, bs, kvh, d), generator=gen, device=dev)
             if side == 0:
                 x *= channel
@@ -219,16 +242,20 @@ def prepare(case, seed):
     dev = torch.device("cuda")
     gen = torch.Generator(device=dev).manual_seed(seed)
     rng = random.Random(seed)
-    if case["kind"] == "attend":
+    if case["kind"] in ("attend", "latent"):
         return _prepare_attend(case, dev, gen, rng)
     total, new = _lengths(case)
-    hq, kvh, d, bs = case["heads"], case["kv_heads"], case["head"], case["block"]
+    hq, bs, rot = case["heads"], case["block"], case["rot"]
     dtype, pad = DTYPES[case["dtype"]], case["pad"]
+    latent = case["kind"] == "latent_append"
+    kvh, d = (1, case["rank"]) if latent else (case["kv_heads"], case["head"])
     # the pages that the step writes to, anywhere in a cache
     spans = [((t - n) // bs, (t - 1) // bs) for t, n in zip(total, new)]
     ids = list(range(sum(b - a + 1 for a, b in spans) + 3))
     rng.shuffle(ids)
-    data, scale = _pages(gen, dev, len(ids), bs, kvh, d, case.get("group", 0), case.get("codes", "e4m3"))
+    pages = len(ids)
+    data, scale = _pages(gen, dev, pages, bs, kvh, d, case.get("group", 0), case.get("codes", "e4m3"),
+                         sides=1 if latent else 2)
     slots, positions = [], []
     for (a, b), t, n in zip(spans, total, new):
         own_pages = np.array([ids.pop() for _ in range(b - a + 1)], dtype=np.int64)
@@ -238,40 +265,67 @@ def prepare(case, seed):
     slots = np.concatenate([*slots, np.full(pad, -1)])
     positions = np.concatenate([*positions, np.zeros(pad, dtype=np.int64)])
     rows = len(slots)
-    # the fused projection's output, of which queries, keys and values are views
-    qkv = torch.randn((rows, (hq + 2 * kvh), d), generator=gen, device=dev)
-    qkv[:, :hq + kvh] *= torch.exp(0.5 * torch.randn((hq + kvh, d), generator=gen, device=dev))
-    qkv[:, hq:] *= torch.exp(0.3 * torch.randn((rows, 2 * kvh, 1), generator=gen, device=dev))
-    qkv = qkv.to(dtype)
     angle = torch.arange(POSITIONS, dtype=torch.float64, device=dev)[:, None] * torch.pow(
-        10000.0, -torch.arange(0, case["rot"], 2, dtype=torch.float64, device=dev) / case["rot"])
+        10000.0, -torch.arange(0, rot, 2, dtype=torch.float64, device=dev) / rot)
     state = dict(
-        kind=case["kind"], q=qkv[:, :hq], key=qkv[:, hq:hq + kvh], value=qkv[:, hq + kvh:],
-        k=data[0], v=data[1], ks=scale[0], vs=scale[1], group=case.get("group", 0),
-        codes=case.get("codes", "e4m3"), interleaved=case["interleaved"], rot=case["rot"],
-        cos_sin=torch.cat([angle.cos(), angle.sin()], 1).float(), live=rows - pad,
+        kind=case["kind"], interleaved=case["interleaved"], rot=rot, live=rows - pad,
+        cos_sin=torch.cat([angle.cos(), angle.sin()], 1).float(),
         positions=torch.from_numpy(positions).to(dev), slots=torch.from_numpy(slots).to(dev),
     )
+    def projection(*shape):
+        x = torch.randn((rows, *shape), generator=gen, device=dev)
+        x *= torch.exp(0.5 * torch.randn(shape, generator=gen, device=dev))
+        return x
+    if latent:
+        # two projections' outputs: [latent | position part] a token, and the queries,
+        # each [128 dims | position part]
+        down, up = projection(d + rot), projection(hq, 128 + rot).to(dtype)
+        down[:, :d] *= torch.exp(0.3 * torch.randn((rows, 1), generator=gen, device=dev))
+        down = down.to(dtype)
+        state.update(
+            q=up[..., 128:], latent=down[:, :d], part=down[:, d:], data=data[0].view(pages, bs, d),
+            scale=scale[0].view(pages, bs, 1),
+            rope=torch.randn((pages, bs, rot), generator=gen, device=dev).to(dtype))
+        return state
+    # the fused projection's output, of which queries, keys and values are views
+    qkv = projection(hq + 2 * kvh, d)
+    qkv[:, hq:] *= torch.exp(0.3 * torch.randn((rows, 2 * kvh, 1), generator=gen, device=dev))
+    qkv = qkv.to(dtype)
+    state.update(
+        q=qkv[:, :hq], key=qkv[:, hq:hq + kvh], value=qkv[:, hq + kvh:], k=data[0], v=data[1],
+        ks=scale[0], vs=scale[1], group=case.get("group", 0), codes=case.get("codes", "e4m3"))
     return state
 
 
 def _prepare_attend(case, dev, gen, rng):
     total, new = _lengths(case)
-    kvh, d, bs = case["kv_heads"], case["head"], case["block"]
+    bs, dtype = case["block"], DTYPES[case["dtype"]]
+    latent = case["kind"] == "latent"
+    kvh, d = (1, case["rank"]) if latent else (case["kv_heads"], case["head"])
     batch = len(total)
     width = -(-max(total) // bs)
-    order = list(range(batch * width))
+    pages = batch * width
+    order = list(range(pages))
     rng.shuffle(order)
     host = np.array(order, dtype=np.int64).reshape(batch, width)
-    data, scale = _pages(gen, dev, batch * width, bs, kvh, d, case["group"], case["codes"])
-    q = torch.randn((sum(new), case["heads"], d), generator=gen, device=dev)
-    return dict(
-        kind="attend", k=data[0], v=data[1], ks=scale[0], vs=scale[1], total=total, new=new,
-        host=host, table=torch.from_numpy(host.astype(np.int32)).to(dev),
-        lens=torch.tensor(total, device=dev), news=torch.tensor(new, device=dev),
-        q=(1.5 * q).to(DTYPES[case["dtype"]]), group=case["group"], codes=case["codes"],
-        window=case["window"] or None, sinks=case["sinks"], scale=d ** -0.5,
-    )
+    data, scale = _pages(gen, dev, pages, bs, kvh, d, case.get("group", 0), case.get("codes", "e4m3"),
+                         sides=1 if latent else 2)
+    state = dict(
+        kind=case["kind"], total=total, new=new, host=host,
+        table=torch.from_numpy(host.astype(np.int32)).to(dev), lens=torch.tensor(total, device=dev),
+        news=torch.tensor(new, device=dev), window=case.get("window") or None,
+        sinks=case.get("sinks", 0))
+    wide = d + case["rot"] if latent else d
+    q = torch.randn((sum(new), case["heads"], wide), generator=gen, device=dev)
+    if latent:  # (the scale is that of a head before its up-projection was absorbed)
+        q[..., :d] *= 0.5
+        state.update(q=q.to(dtype), data=data[0].view(pages, bs, d), scale_=scale[0].view(pages, bs, 1),
+                     rope=torch.randn((pages, bs, case["rot"]), generator=gen, device=dev).to(dtype),
+                     scale=(128 + case["rot"]) ** -0.5)
+    else:
+        state.update(q=(1.5 * q).to(dtype), k=data[0], v=data[1], ks=scale[0], vs=scale[1],
+                     group=case["group"], codes=case["codes"], scale=d ** -0.5)
+    return state
 
 
 # ---------------------------------------------------------------------------
@@ -282,19 +336,27 @@ def _prepare_attend(case, dev, gen, rng):
 def _package():
     if str(PACKAGE) not in sys.path:
         sys.path.insert(0, str(PACKAGE))
-    from vllm_ascend_quantized_kv_cache.ops import block8, fp8_rotary
+    from vllm_ascend_quantized_kv_cache.ops import block8, fp8_latent, fp8_rotary
 
-    return block8, fp8_rotary
+    return block8, fp8_latent, fp8_rotary
 
 
 def run(s):
     if own:
-        block8, fp8_rotary = _package()
+        block8, fp8_latent, fp8_rotary = _package()
         if s["kind"] == "attend":
             return block8.block8_attention(
                 s["q"], s["k"], s["ks"], s["v"], s["vs"], s["table"], s["total"], s["new"],
                 s["scale"], window=s["window"], sinks=s["sinks"], block_table_host=s["host"])
-        if s["kind"] == "rope":
+        if s["kind"] == "latent":
+            return fp8_latent.fp8_latent_attention(
+                s["q"], s["data"], s["scale_"], s["rope"], s["table"], s["total"], s["new"],
+                s["scale"], block_table_host=s["host"])
+        if s["kind"] == "latent_append":
+            q = fp8_latent.fp8_latent_store(
+                s["latent"], s["part"], s["positions"], s["cos_sin"], s["slots"], s["data"],
+                s["scale"], s["rope"], query=s["q"], interleaved=s["interleaved"])
+        elif s["kind"] == "rope":
             q = fp8_rotary.fp8_per_token_head_rotary_store(
                 s["q"], s["key"], s["value"], s["positions"], s["cos_sin"], s["slots"], s["k"],
                 s["ks"], s["v"], s["vs"], interleaved=s["interleaved"])
@@ -303,14 +365,18 @@ def run(s):
                 s["key"], s["value"], s["slots"], s["k"], s["ks"], s["v"], s["vs"], query=s["q"],
                 positions=s["positions"], cos_sin=s["cos_sin"], interleaved=s["interleaved"])
         return _stored(s, q)
-    if s["kind"] == "attend":
+    if s["kind"] in ("attend", "latent"):
         return _plain_attend(s)
+    if s["kind"] == "latent_append":
+        return _stored(s, _plain_latent_append(s))
     return _stored(s, _plain_rope(s) if s["kind"] == "rope" else _plain_append(s))
 
 
 def _stored(s, q):
     """The rotated queries and what the pages hold: E4M3 codes as the values they stand for,
     of INT8 codes the rows just written."""
+    if s["kind"] == "latent_append":
+        return q, s["data"].view(E4M3), s["scale"], s["rope"]
     if s["codes"] == "e4m3":
         return q, s["k"].view(E4M3), s["ks"], s["v"].view(E4M3), s["vs"]
     slots, (kvh, d) = s["slots"][:s["live"]], s["k"].shape[2:]
@@ -343,6 +409,17 @@ def _plain_rope(s):
         scale = (x.abs().amax(-1, keepdim=True) / 448.0).clamp_min(1e-6)
         codes.view(-1, kvh, d)[slots] = (x / scale).clamp(-448.0, 448.0).to(E4M3).view(torch.uint8)
         scales.view(-1, kvh, 1)[slots] = scale
+    return _rotate(s["q"], s).to(s["q"].dtype)
+
+
+def _plain_latent_append(s):
+    slots, d, p = s["slots"][:s["live"]], s["data"].shape[2], s["rot"]
+    x = s["latent"][:s["live"]].float()
+    scale = (x.abs().amax(-1, keepdim=True) / 448.0).clamp_min(1e-6)
+    s["data"].view(-1, d)[slots] = (x / scale).clamp(-448.0, 448.0).to(E4M3).view(torch.uint8)
+    s["scale"].view(-1, 1)[slots] = scale
+    part = _rotate(s["part"][:, None], s)[:s["live"], 0]
+    s["rope"].view(-1, p)[slots] = part.to(s["rope"].dtype)
     return _rotate(s["q"], s).to(s["q"].dtype)
 
 
@@ -386,23 +463,30 @@ def _plain_append(s):
 
 def _plain_attend(s):
     q, total, new = s["q"], s["lens"], s["news"]
-    nb, bs, kvh, d = s["k"].shape
-    batch, hq = len(s["total"]), q.shape[1]
-    rep, longest, most = hq // kvh, max(s["total"]), max(s["new"])
+    batch, (hq, wide), longest, most = len(s["total"]), q.shape[1:], max(s["total"]), max(s["new"])
+    latent = s["kind"] == "latent"
+    bs, kvh = s["data" if latent else "k"].shape[1], 1 if latent else s["k"].shape[2]
+    rep = hq // kvh
     pos = torch.arange(longest, device=q.device)
     slot = s["table"][:, pos // bs].long() * bs + pos % bs  # [B, L]
-    def dense(codes, scales):
-        x = codes.view(nb * bs, kvh, d)[slot]
-        x = x.view(E4M3).float() if s["codes"] == "e4m3" else x.float()
-        x = x * scales.view(-1, kvh, 1)[slot // s["group"]]
-        return x.transpose(1, 2).reshape(batch * kvh, longest, d)
-    k = dense(s["k"], s["ks"])
+    if latent:
+        d = s["data"].shape[2]
+        v = s["data"].view(-1, d)[slot].view(E4M3).float() * s["scale_"].view(-1, 1)[slot]
+        k = torch.cat([v, s["rope"].view(-1, wide - d)[slot].float()], -1)
+    else:
+        d = wide
+        def dense(codes, scales):
+            x = codes.view(-1, kvh, d)[slot]
+            x = x.view(E4M3).float() if s["codes"] == "e4m3" else x.float()
+            x = x * scales.view(-1, kvh, 1)[slot // s["group"]]
+            return x.transpose(1, 2).reshape(batch * kvh, longest, d)
+        k = dense(s["k"], s["ks"])
     # query rows padded to the longest chunk: row i of request b at cu[b] + i
     cu = torch.cumsum(new, 0) - new
     i = torch.arange(most, device=q.device)
     at = (cu[:, None] + i).clamp_max(q.shape[0] - 1)
-    qp = q.float()[at].view(batch, most, kvh, rep, d).permute(0, 2, 1, 3, 4)
-    scores = torch.bmm(qp.reshape(batch * kvh, most * rep, d),
+    qp = q.float()[at].view(batch, most, kvh, rep, wide).permute(0, 2, 1, 3, 4)
+    scores = torch.bmm(qp.reshape(batch * kvh, most * rep, wide),
                        (k * s["scale"]).transpose(1, 2).contiguous())
     del k
     scores = scores.view(batch, kvh, most, rep, longest)
@@ -417,7 +501,7 @@ def _plain_attend(s):
     del scores
     norm = p.sum(-1, keepdim=True)
     p /= torch.where(norm == 0, torch.ones_like(norm), norm)
-    out = torch.bmm(p.view(batch * kvh, most * rep, longest), dense(s["v"], s["vs"]))
+    out = torch.bmm(p.view(batch * kvh, most * rep, longest), v if latent else dense(s["v"], s["vs"]))
     out = out.view(batch, kvh, most, rep, d).permute(0, 2, 1, 3, 4).reshape(batch, most, hq, d)
     return out[(i < new[:, None])].to(q.dtype)
 
@@ -429,7 +513,7 @@ def _plain_attend(s):
 
 def exact(case, seed):
     s = prepare(case, seed)
-    return _exact_attend(s) if s["kind"] == "attend" else _exact_store(s)
+    return _exact_attend(s) if s["kind"] in ("attend", "latent") else _exact_store(s)
 
 
 def _round_e4m3(x):
@@ -440,8 +524,7 @@ def _round_e4m3(x):
 
 
 def _exact_store(s):
-    e4m3, g, rot = s["codes"] == "e4m3", s["group"], s["rot"]
-    kvh, d = s["k"].shape[2:]
+    e4m3, g, rot = s.get("codes") != "int8", s.get("group"), s["rot"]
     angle = s["cos_sin"].double()[s["positions"]][:, None]
     def rotate(x):
         x = x.double().clone()
@@ -455,6 +538,16 @@ def _exact_store(s):
         return x
     def levels(x):
         return _round_e4m3(x) if e4m3 else torch.round(x).clamp(-127, 127)
+    if s["kind"] == "latent_append":
+        slots, d = s["slots"][:s["live"]], s["data"].shape[2]
+        rows = s["latent"][:s["live"]].double()
+        data, size = s["data"].view(E4M3).double(), s["scale"].double()
+        rope = s["rope"].double()
+        size.view(-1)[slots] = (rows.abs().amax(-1) / 448.0).clamp_min(1e-6)
+        data.view(-1, d)[slots] = levels(rows / size.view(-1, 1)[slots])
+        rope.view(-1, rot)[slots] = rotate(s["part"][:, None])[:s["live"], 0]
+        return rotate(s["q"]), data, size, rope
+    kvh, d = s["k"].shape[2:]
     slots = s["slots"][:s["live"]]
     host = slots.cpu().numpy()
     result = [rotate(s["q"])]
@@ -490,18 +583,25 @@ def _exact_store(s):
 
 def _exact_attend(s):
     q = s["q"].double()
-    hq, d = q.shape[1:]
-    bs, kvh, g = s["k"].shape[1], s["k"].shape[2], s["group"]
+    hq = q.shape[1]
+    latent = s["kind"] == "latent"
+    kvh = 1 if latent else s["k"].shape[2]
     rep = hq // kvh
-    out = torch.zeros_like(q)
+    out = q.new_zeros((*q.shape[:2], s["data"].shape[2] if latent else q.shape[2]))
     row0 = 0
     for b, (total, new) in enumerate(zip(s["total"], s["new"])):
+        bs = s["data" if latent else "k"].shape[1]
         pages = s["table"][b, : -(-total // bs)].long()
-        def values(codes, scales):
-            x = codes[pages].view(E4M3) if s["codes"] == "e4m3" else codes[pages]
-            x = x.double().unflatten(1, (bs // g, g)) * scales[pages].double()[:, :, None, :, None]
-            return x.flatten(0, 2)
-        k, v = values(s["k"], s["ks"]), values(s["v"], s["vs"])
+        if latent:
+            v = s["data"][pages].view(E4M3).double() * s["scale_"][pages]
+            k = torch.cat([v, s["rope"][pages].double()], -1).flatten(0, 1)[:, None]
+            v = v.flatten(0, 1)[:, None]
+        else:
+            def values(codes, scales):
+                x = codes[pages].view(E4M3) if s["codes"] == "e4m3" else codes[pages]
+                x = x.double().unflatten(1, (-1, s["group"]))
+                return (x * scales[pages].double()[:, :, None, :, None]).flatten(0, 2)
+            k, v = values(s["k"], s["ks"]), values(s["v"], s["vs"])
         j = torch.arange(total, device=q.device)
         for h in range(kvh):
             kh, vh = k[:total, h].t().contiguous(), v[:total, h].contiguous()
@@ -512,9 +612,9 @@ def _exact_attend(s):
                 hide = j > i
                 if s["window"]:
                     hide |= (j <= i - s["window"]) & (j >= s["sinks"])
-                x = q[at, h * rep:(h + 1) * rep].reshape(n * rep, d) @ kh * s["scale"]
+                x = q[at, h * rep:(h + 1) * rep].reshape(n * rep, -1) @ kh * s["scale"]
                 x = x.view(n, rep, total).masked_fill(hide[:, None], -math.inf)
                 p = torch.softmax(x, -1)
-                out[at, h * rep:(h + 1) * rep] = (p.view(n * rep, total) @ vh).view(n, rep, d)
+                out[at, h * rep:(h + 1) * rep] = (p.view(n * rep, total) @ vh).view(n, rep, -1)
         row0 += new
     return out
