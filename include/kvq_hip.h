@@ -42,6 +42,12 @@ enum {
   KVQ_INDEX_I64 = 1,
 };
 
+/* 8-bit codes of a cache with a scale for each block (kvq_block8_*). */
+enum {
+  KVQ_CODES_E4M3 = 0,
+  KVQ_CODES_INT8 = 1,
+};
+
 enum {
   KVQ_OK = 0,
   KVQ_ERR_INVALID = -1,     /* bad pointer, dtype or size */
@@ -543,6 +549,80 @@ int64_t kvq_fp8_pth_evict_check(const void* block_table, const void* out_block_t
                                 int block_index_type, int64_t max_blocks, int64_t out_max_blocks,
                                 const int64_t* seq_lens, const int64_t* keep, int64_t batch,
                                 int64_t num_blocks, int block_size);
+
+/* kvq_fp8_pth_store of rows that are rotated to their positions on the way: query
+ * [num_tokens, num_heads, D] (num_heads 0: none) into out_query, which may be query, and
+ * key into the cache, each by the row of cos_sin [table_rows, rot] (cosines, then sines;
+ * rot even, <= D; table_dtype) that positions [num_tokens] (pos_type) names; dims from rot
+ * on stay.  Pairs are dims i and i + rot / 2, or 2 i and 2 i + 1 (interleaved).  fp32, keys
+ * not rounded before they are quantized.  Rows of one token are contiguous, tokens *_stride
+ * elements apart.  Tokens with a slot outside the cache or a position outside the table are
+ * not stored; a query's rotated dims at such a position are NaN.  A row with a NaN or an
+ * infinity reads back as NaN.  D % 4 == 0, D <= 512, codes on 4-byte bounds.  The
+ * arithmetic of pkg/methods/fp8_per_token_head/semantics.py:52-61 behind a rotation that
+ * the reference leaves to its host. */
+int kvq_fp8_pth_rotary_store(const void* query, int64_t query_stride, void* out_query,
+                             int64_t out_stride, const void* key, int64_t key_stride,
+                             const void* value, int64_t value_stride, int dtype,
+                             const void* positions, int pos_type, const void* cos_sin,
+                             int table_dtype, int64_t table_rows, int rot, int interleaved,
+                             const void* slot_mapping, int slot_type, int64_t num_tokens,
+                             int num_heads, int num_kv_heads, int head_size, uint8_t* k_data,
+                             float* k_scale, uint8_t* v_data, float* v_scale, int64_t num_blocks,
+                             int block_size, void* stream);
+
+/* ---- 8-bit codes with a scale for each block of positions and head ------------ */
+
+/* The same (without a rotation where cos_sin is NULL) into codes [NB, Bs, KVH, D] of code_type
+ * (KVQ_CODES_*) with fp32 scales [NB, Bs / group, KVH].  The rows of a block are neighbours
+ * in the call (padding between them is fine), each slot once.  S = s(amax of a block's new
+ * rows), or, where the first of them lies behind the block's start, the larger of that and
+ * the old scale; where it grows, the rows before them are requantized:
+ *   E4M3  s(a) = max(2^-20, the least 2^e with a <= 448 2^e), code = e4m3(y / S),
+ *   INT8  s(a) = max(a / 127, 1e-6), code = rint(y / S) in +-127,
+ * and code * old / S likewise.  Rows of a block behind the last new one are left alone.  No
+ * counterpart in the reference. */
+int kvq_block8_store(const void* query, int64_t query_stride, void* out_query, int64_t out_stride,
+                     const void* key, int64_t key_stride, const void* value, int64_t value_stride,
+                     int dtype, const void* positions, int pos_type, const void* cos_sin,
+                     int table_dtype, int64_t table_rows, int rot, int interleaved,
+                     const void* slot_mapping, int slot_type, int64_t num_tokens, int num_heads,
+                     int num_kv_heads, int head_size, int code_type, void* k_data, float* k_scale,
+                     void* v_data, float* v_scale, int64_t num_blocks, int block_size, int group,
+                     void* stream);
+
+/* kvq_fp8_pth_window_attn (without running weights) over such a cache: K = code * k_scale
+ * [block, head], V likewise, not rounded to `dtype`.  Everything else as there, the page
+ * check (kvq_fp8_pth_window_check) included.  No counterpart in the reference. */
+int64_t kvq_block8_attn_workspace_bytes(const int64_t* seq_lens, const int64_t* query_lens,
+                                        int64_t batch, int dtype, int num_heads, int num_kv_heads,
+                                        int head_size, int block_size, int group, int code_type,
+                                        int64_t window, int64_t sinks);
+int kvq_block8_attn(const void* query, int dtype, int64_t query_stride, const int64_t* seq_lens,
+                    const int64_t* query_lens, int64_t batch, int num_heads, int num_kv_heads,
+                    int head_size, float scale, int64_t window, int64_t sinks, int code_type,
+                    const void* k_data, const float* k_scale, const void* v_data,
+                    const float* v_scale, int64_t num_blocks, int block_size, int group,
+                    const void* block_table, int block_index_type, int64_t max_blocks,
+                    void* workspace, int64_t workspace_bytes, void* out, void* stream);
+
+/* ---- latent rows shared by all heads -------------------------------------------- */
+
+/* Latent rows [num_tokens, rank] (latent_stride elements apart) as E4M3 codes data
+ * [NB, Bs, rank] with scale fp32 [NB, Bs], quantized as kvq_fp8_pth_store does; their position
+ * part [num_tokens, part_size] rotated by all of cos_sin [table_rows, part_size] as
+ * kvq_fp8_pth_rotary_store does, into rope [NB, Bs, part_size] of `dtype`, rounded once;
+ * and the position part of the queries [num_tokens, num_heads, part_size] (strides of tokens
+ * and heads) likewise into out_query.  Padding as there.  rank % 4 == 0, rank and part_size
+ * <= 512, part_size even.  No counterpart in the reference. */
+int kvq_fp8_latent_store(const void* query, int64_t query_stride, int64_t query_head_stride,
+                         void* out_query, int64_t out_stride, int64_t out_head_stride,
+                         const void* latent, int64_t latent_stride, const void* part,
+                         int64_t part_stride, int dtype, const void* positions, int pos_type,
+                         const void* cos_sin, int table_dtype, int64_t table_rows, int interleaved,
+                         const void* slot_mapping, int slot_type, int64_t num_tokens, int num_heads,
+                         int rank, int part_size, uint8_t* data, float* scale, void* rope,
+                         int64_t num_blocks, int block_size, void* stream);
 
 /* ---- self-test ---------------------------------------------------------- */
 

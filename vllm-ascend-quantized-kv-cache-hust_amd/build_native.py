@@ -59,6 +59,7 @@ EXTRA_FLAGS = {
     "decode_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     # likewise
     "fp8_window_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "block8_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -138,7 +138,33 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
          _P, _P, _I64, _P, _I64, _P, _I64, _P],
     ),
     "kvq_fp8_pth_evict_check": (_I64, [_P, _P, _I, _I64, _I64, _P, _P, _I64, _I64, _I]),
+    "kvq_fp8_pth_rotary_store": (
+        _I,
+        [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _P, _I, _P, _I, _I64, _I, _I, _P, _I, _I64,
+         _I, _I, _I, _P, _P, _P, _P, _I64, _I, _P],
+    ),
+    "kvq_block8_store": (
+        _I,
+        [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _P, _I, _P, _I, _I64, _I, _I, _P, _I, _I64,
+         _I, _I, _I, _I, _P, _P, _P, _P, _I64, _I, _I, _P],
+    ),
+    "kvq_block8_attn_workspace_bytes": (
+        _I64, [_P, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _I64, _I64]
+    ),
+    "kvq_block8_attn": (
+        _I,
+        [_P, _I, _I64, _P, _P, _I64, _I, _I, _I, _F, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I, _I,
+         _P, _I, _I64, _P, _I64, _P, _P],
+    ),
+    "kvq_fp8_latent_store": (
+        _I,
+        [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I, _P, _I, _P, _I, _I64, _I, _P, _I,
+         _I64, _I, _I, _I, _P, _P, _P, _I64, _I, _P],
+    ),
 }
+
+#: kinds of 8-bit codes of a cache with a scale for each block
+KVQ_CODES_E4M3, KVQ_CODES_INT8 = 0, 1
 
 KVQ_ERR_INVALID = -1
 KVQ_ERR_GEOMETRY = -2
