@@ -624,6 +624,24 @@ int kvq_fp8_latent_store(const void* query, int64_t query_stride, int64_t query_
                          int rank, int part_size, uint8_t* data, float* scale, void* rope,
                          int64_t num_blocks, int block_size, void* stream);
 
+/* Causal attention of each request's last query_lens[b] of its seq_lens[b] cached positions
+ * over such a cache, the up-projections absorbed: query [>= sum query_lens, num_heads, rank +
+ * part_size] of `dtype` (that of rope; rows query_stride elements apart), out [.., num_heads,
+ * rank] contiguous.  A row at position p sees j <= p; with c_j = code * row_scale, score
+ * scale (q[:rank] . c_j + q[rank:] . rope_j), value c_j; softmax in fp32.  A row that sees
+ * nothing gives zeros; rows behind the last request's are left alone.  rank % 4 == 0, <= 512,
+ * part_size <= 256, codes on 4-byte bounds; num_blocks to block_table, lengths and workspace
+ * as for kvq_fp8_pth_window_attn.  No counterpart in the reference. */
+int64_t kvq_fp8_latent_attn_workspace_bytes(const int64_t* seq_lens, const int64_t* query_lens,
+                                            int64_t batch, int dtype, int num_heads, int rank,
+                                            int part_size, int block_size);
+int kvq_fp8_latent_attn(const void* query, int dtype, int64_t query_stride, const int64_t* seq_lens,
+                        const int64_t* query_lens, int64_t batch, int num_heads, int rank,
+                        int part_size, float scale, const uint8_t* data, const float* row_scale,
+                        const void* rope, int64_t num_blocks, int block_size,
+                        const void* block_table, int block_index_type, int64_t max_blocks,
+                        void* workspace, int64_t workspace_bytes, void* out, void* stream);
+
 /* ---- self-test ---------------------------------------------------------- */
 
 /* One v_mfma_f32_16x16x32_f16 with the operand/result lane mapping the decode

@@ -191,3 +191,66 @@ class Pages:
 
     def args(self):
         return self.data[0], self.scale[0], self.data[1], self.scale[1], self.table
+
+
+class Latents:
+    """Latent rows and position parts of requests of these lengths, quantized as the store does."""
+
+    def __init__(self, lens, rank, dims, bs, dtype, *, device="cpu", seed=0, index=torch.int32,
+                 spare=2):
+        self.host, pages = paged(lens, bs, seed, spare)
+        self.host = self.host.astype(np.int64)
+        self.table = torch.from_numpy(self.host).to(device, index)
+        g = torch.Generator().manual_seed(seed)
+        x = torch.randn(pages * bs, rank, generator=g) * torch.exp(
+            0.5 * torch.randn(rank, generator=g)) * torch.exp(torch.randn(pages * bs, 1, generator=g))
+        s = (x.abs().amax(-1, keepdim=True) / 448.0).clamp_min(1e-6)
+        self.data = (x / s).clamp(-448, 448).to(E4M3).view(torch.uint8).view(pages, bs, rank).to(device)
+        self.scale = s.view(pages, bs, 1).to(device)
+        self.rope = torch.randn(pages, bs, dims, generator=g).to(dtype).to(device)
+        self.rank, self.dims, self.bs = rank, dims, bs
+
+    def rows(self, b, length):
+        """64-bit ([length, R], [length, P])."""
+        at = torch.from_numpy(slots_of(self.host, b, np.arange(length), self.bs)).to(
+            self.table.device)
+        c = self.data.view(E4M3).double().view(-1, self.rank)[at]
+        return c * self.scale.double().view(-1, 1)[at], self.rope.double().view(-1, self.dims)[at]
+
+    def args(self):
+        return self.data, self.scale, self.rope, self.table
+
+
+def latent64(q, cache, lens, news, scale):
+    """(out, bound) in 64 bits; the bound as ``_fp8_window.attention64`` derives it: a score is
+    R + P exact products summed in fp32, two products, two sums and a logarithm behind them,
+    a weight goes through the matrix units in 16 bits."""
+    heads, wide = q.shape[1:]
+    rank = cache.rank
+    out, bound = q.new_zeros((2, q.shape[0], heads, rank), dtype=torch.float64)
+    row0 = 0
+    for b, (length, n) in enumerate(zip(lens, news)):
+        if n and length:
+            c, r = cache.rows(b, length)
+            k = torch.cat([c, r], 1).T.contiguous()
+            pos = (length - n + torch.arange(n, device=q.device))[:, None]
+            mask = (torch.arange(length, device=q.device) <= pos).repeat_interleave(heads, 0)
+            x = q[row0:row0 + n].double().reshape(n * heads, wide)
+            s = (x @ k * scale).masked_fill(~mask, -math.inf)
+            size = torch.where(mask, (x.abs() @ k.abs() * scale).nan_to_num(0.0, 0.0, 0.0), 0.0)
+            a = size.amax(-1, keepdim=True)
+            top = s.amax(-1, keepdim=True)
+            p = torch.where(mask, torch.exp(s - torch.where(top == -math.inf, 0.0, top)), 0.0)
+            norm = p.sum(-1, keepdim=True)
+            p = torch.where(mask, p / torch.where(norm == 0, 1.0, norm), 0.0)
+            bad = (mask.double() @ c.isnan().double()) > 0
+            v = torch.where(c.isfinite(), c, 0.0)
+            o = torch.where(bad, math.nan, p @ v)
+            o = torch.where(norm.isnan(), math.nan, o)
+            off = 2 * (wide + 16) * 2.0 ** -24 * a + (length + 200) * 2.0 ** -24
+            peak = (p * v.abs().amax(-1)).amax(-1, keepdim=True)
+            ob = (off + 2.0 ** -11) * (p @ v.abs()) + length * 2.0 ** -24 * peak
+            out[row0:row0 + n] = o.view(n, heads, rank)
+            bound[row0:row0 + n] = ob.view(n, heads, rank)
+        row0 += n
+    return out, bound

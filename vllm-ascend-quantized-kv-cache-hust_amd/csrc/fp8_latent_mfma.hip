@@ -1,0 +1,479 @@
+// SPDX-License-Identifier: Apache-2.0
+// Attention over latent rows that all heads share, on the matrix units: decodes, where the
+// rows stream through once, and chunks.
+//
+// One workgroup of eight waves per tile of 16 or 32 columns (row, head), request and part of
+// its positions, 128 positions at a time.  The latent is key and value at once, so a stage's
+// codes are read from memory once, by DMA into LDS (64 KB at R = 512, two stages, 16-byte
+// chunk c of row t at c ^ t % 16), and converted to 16 bits on their way to the matrix units:
+//   S^T = C * Q^T: wave w takes positions 16 w ..; A = codes in the query's type, exact: lane
+//     (g, n) holds dims R/4 g .. of position n; B = the queries, all R dims of the tile's
+//     columns in every wave's registers.  The position part beside it, from global memory
+//     straight into the operand.
+//   softmax: the waves put their positions' maxima into LDS; with t = (S s_j + S_r) scale
+//     log2(e) + log2(s_j) and m its running maximum, p' = 2^(t - m + 14) = p s_j fits fp16
+//     whatever the scales are: rounded by 2^-11 of it, or, where fp16 is subnormal, 2^-38 of
+//     the row's largest; the sum takes p' / s_j in fp32 before that rounding.  p' goes
+//     through LDS to all waves.
+//   O^T += C^T * p'^T: wave w takes dims R/8 w ..; A = codes in fp16, exact, by the transposing
+//     reads of bytes (16 lanes read 8 rows of 16 bytes, lane s gets column s).
+//
+// Positions that a column does not see: weights by selection; in stages that some column
+// does not wholly see, NaN codes become zeros in LDS between the two products (a row that
+// sees one is NaN by its score).
+#include <algorithm>
+
+#include "fp8_latent.h"
+#include "block8.h"
+
+namespace {
+
+using namespace kvq;
+
+constexpr int kWaves = 8;
+constexpr int kStage = 16 * kWaves;  // positions
+constexpr float kRaise = 14.0f;      // log2 of the largest p'
+
+typedef const __attribute__((address_space(4))) int32_t lat_ci32;
+typedef const __attribute__((address_space(4))) int64_t lat_ci64;
+typedef int lat_i2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) lat_i2* lat_lds2;
+
+template <int R, int NG>
+struct LatLds {
+  static constexpr int STAGE = kStage * R;
+  static constexpr int PROW = 2 * kStage + 16;        // bytes of a column's p', padded
+  static constexpr int P = 2 * STAGE;                 // [16 NG][PROW]
+  static constexpr int MAX = P + 16 * NG * PROW;      // [16 NG][kWaves] floats
+  static constexpr int BYTES = MAX + 16 * NG * kWaves * 4;
+};
+
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+template <typename T, int R, int PART, int NG>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
+latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query,
+                     int64_t q_stride, int wide, float qscale, T* __restrict__ out, WinParts parts) {
+  using L = LatLds<R, NG>;
+  constexpr int KS = R / 32;      // k-steps of a score
+  constexpr int RS = PART / 32;   // and of its position part
+  constexpr int DB = R / 128;     // 16-dim blocks of a wave's dims
+  constexpr int CH = R / 16;      // 16-byte chunks of a row
+  constexpr int RPI = 64 / CH;    // rows a DMA instruction brings
+  constexpr int DMAS = 16 / RPI;  // of a wave's 16 rows
+  extern __shared__ __align__(16) char lds[];
+  const WinReq r = win_req(count, blockIdx.x);
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int heads = c.hq, cols = r.n * heads;
+  const int tiles = (cols + 16 * NG - 1) / (16 * NG);
+  // tiles of a part lie 8 workgroups apart, on one XCD, whose L2 then holds its codes once
+  int u = static_cast<int>(blockIdx.x) - r.first;
+  const int set = u / (8 * tiles);
+  u -= set * 8 * tiles;
+  const int across = min(8, r.parts - 8 * set);
+  const int tile = tiles - 1 - u / across, seg = 8 * set + u % across;
+  const int col0 = 16 * NG * tile;
+  auto row_of = [&](int col) { return static_cast<int>(c.rep.div(static_cast<uint32_t>(col))); };
+  const int base = r.len - r.n;  // position of the request's first row
+  const int tile_first = base + row_of(col0);
+  const int tile_last = base + row_of(min(col0 + 16 * NG, cols) - 1);
+  // the lane's columns; one past the last sees nothing
+  int row[NG], head[NG], pos[NG];
+  bool live[NG];
+#pragma unroll
+  for (int x = 0; x < NG; ++x) {
+    const int col = col0 + 16 * x + n;
+    live[x] = col < cols;
+    row[x] = row_of(live[x] ? col : 0);
+    head[x] = (live[x] ? col : 0) - row[x] * heads;
+    pos[x] = live[x] ? base + row[x] : -1;
+  }
+  const int stages = tile_last >= 0 ? (tile_last + kStage) / kStage : 0;
+  const int s0 = static_cast<int>(static_cast<int64_t>(stages) * seg / r.parts);
+  const int s1 = static_cast<int>(static_cast<int64_t>(stages) * (seg + 1) / r.parts);
+  if (s0 >= s1) {  // uniform: a part without positions, or columns that see nothing
+    for (int x = tid; x < 16 * NG * (R / 4); x += 64 * kWaves) {
+      const int col = col0 + x / (R / 4);
+      if (col >= cols) break;
+      const int i = row_of(col);
+      const int64_t at = (static_cast<int64_t>(r.q0) + i) * heads + col - i * heads;
+      if (r.parts > 1) {
+        const int64_t part = r.part0 + static_cast<int64_t>(seg) * r.n * heads + col;
+        if (x % (R / 4) == 0) *reinterpret_cast<w_f2*>(parts.ml + 2 * part) = w_f2{-INFINITY, 0.0f};
+      } else {
+        for (int e = 0; e < 4; ++e) out[at * R + 4 * (x % (R / 4)) + e] = from_f32<T>(0.0f);
+      }
+    }
+    return;
+  }
+
+  // ---- a stage on its way ----
+  const uint32_t lds0 = win_lds(lds);
+  uint32_t off[DMAS];
+#pragma unroll
+  for (int j = 0; j < DMAS; ++j) {
+    const int t = RPI * j + lane / CH;
+    off[j] = static_cast<uint32_t>(t) * R + 16 * ((lane % CH) ^ t);
+  }
+  const int groups = (r.len + 15) / 16;  // 16-position groups, each in one page
+  struct Beside {
+    w_u4 rope[RS];
+    w_f4 scale;
+  };
+  auto issue = [&](int stage) {
+    const int p = 16 * min(stage * kWaves + wave, groups - 1);
+    const uint32_t i = c.bs.div(static_cast<uint32_t>(p));
+    const int64_t at = __builtin_amdgcn_readfirstlane(
+        static_cast<int>(i) < c.maxb ? static_cast<int>(i) : static_cast<int>(c.maxb - 1));
+    const int64_t e = static_cast<int64_t>(r.table) * c.maxb + at;
+    const int64_t id = c.bt64 ? ((lat_ci64*)(const void*)c.table)[e]
+                              : static_cast<int64_t>(((lat_ci32*)(const void*)c.table)[e]);
+    const int64_t page = id < 0 ? 0 : (id >= c.nb ? c.nb - 1 : id);
+    const int64_t slot = page * c.bs.d + (static_cast<uint32_t>(p) - i * c.bs.d);
+    const uint32_t to = lds0 + stage % 2 * L::STAGE + wave * 16 * R;
+#pragma unroll
+    for (int j = 0; j < DMAS; ++j) win_dma16(c.kd + slot * R, off[j], to + j * 1024);
+    Beside b;
+    const T* rope = static_cast<const T*>(c.rope) + (slot + n) * PART + 8 * g;
+#pragma unroll
+    for (int s = 0; s < RS; ++s) b.rope[s] = *reinterpret_cast<const w_u4*>(rope + 32 * s);
+    b.scale = *reinterpret_cast<const w_f4*>(c.ks + slot + 4 * g);
+    return b;
+  };
+
+  Beside next = issue(s0);
+  w_u4 q[NG][KS], qr[NG][RS];
+#pragma unroll
+  for (int x = 0; x < NG; ++x) {
+    const T* qrow = query + (static_cast<int64_t>(r.q0) + row[x]) * q_stride +
+                    static_cast<int64_t>(head[x]) * (R + PART);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[x][s] = load_op8(qrow + (R / 4) * g + 8 * s, wide & 1);
+#pragma unroll
+    for (int s = 0; s < RS; ++s) qr[x][s] = load_op8(qrow + R + 32 * s + 8 * g, wide & 1);
+    if (!live[x]) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[x][s] = w_u4{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < RS; ++s) qr[x][s] = w_u4{0, 0, 0, 0};
+    }
+  }
+  float m[NG], l[NG];
+  w_f4 o[DB][NG];
+#pragma unroll
+  for (int x = 0; x < NG; ++x) {
+    m[x] = -INFINITY;
+    l[x] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d][x] = w_f4{0.f, 0.f, 0.f, 0.f};
+  }
+  float* const smax = reinterpret_cast<float*>(lds + L::MAX);
+
+  for (int st = s0; st < s1; ++st) {
+    wait_vmcnt<0>();  // this wave's part of the stage
+    lds_barrier();    // everybody's; and the last stage's other buffer is read
+    Beside b = next;
+#pragma unroll
+    for (int s = 0; s < RS; ++s) asm volatile("" : "+v"(b.rope[s]));
+    asm volatile("" : "+v"(b.scale));
+    if (st + 1 < s1) next = issue(st + 1);
+    char* const codes = lds + st % 2 * L::STAGE;
+    const int p0 = st * kStage + 16 * wave;  // of this wave's positions
+    const bool edge = st * kStage + kStage - 1 > tile_first;  // uniform
+
+    // ---- scores ----
+    w_f4 s[NG], sr[NG];
+#pragma unroll
+    for (int x = 0; x < NG; ++x) s[x] = sr[x] = w_f4{0.f, 0.f, 0.f, 0.f};
+    const char* kr = codes + (16 * wave + n) * R;
+#pragma unroll
+    for (int w = 0; w < KS / 2; ++w) {
+      const w_u4 k = *reinterpret_cast<const w_u4*>(kr + 16 * ((CH / 4 * g + w) ^ n));
+      const w_u4 k0 = code_op8<T>(k[0], k[1]), k1 = code_op8<T>(k[2], k[3]);
+#pragma unroll
+      for (int x = 0; x < NG; ++x) s[x] = mfma_op(k0, q[x][2 * w], s[x], T{});
+#pragma unroll
+      for (int x = 0; x < NG; ++x) s[x] = mfma_op(k1, q[x][2 * w + 1], s[x], T{});
+    }
+#pragma unroll
+    for (int i = 0; i < RS; ++i)
+#pragma unroll
+      for (int x = 0; x < NG; ++x) sr[x] = mfma_op(b.rope[i], qr[x][i], sr[x], T{});
+    B8Value val[4];
+    bool signs = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      val[e] = b8_value(b.scale[e]);
+      signs = signs || val[e].sign != 1.0f;
+    }
+    uint32_t seen[NG];
+#pragma unroll
+    for (int x = 0; x < NG; ++x) {
+      seen[x] = 0xf;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        s[x][e] = __builtin_fmaf(s[x][e], b.scale[e] * qscale,
+                                 __builtin_fmaf(sr[x][e], qscale, val[e].lv));
+      if (edge) {
+        seen[x] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool on = p0 + 4 * g + e <= pos[x];
+          seen[x] |= on ? 1u << e : 0u;
+          s[x][e] = on ? s[x][e] : -INFINITY;
+        }
+      }
+      const float mx = max_rows4(fmaxf(fmaxf(s[x][0], s[x][1]), fmaxf(s[x][2], s[x][3])));
+      if (g == 0) smax[(16 * x + n) * kWaves + wave] = mx;
+    }
+    lds_barrier();  // the maxima; and the codes are read as keys
+
+    // ---- weights ----
+    float alpha[NG];
+#pragma unroll
+    for (int x = 0; x < NG; ++x) {
+      const w_f4* y = reinterpret_cast<const w_f4*>(smax + (16 * x + n) * kWaves);
+      const w_f4 a = y[0], z = y[1];
+      const float mx = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
+                             fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
+      const float m_new = fmaxf(m[x], mx);
+      const float top = m_new == -INFINITY ? 0.0f : m_new;
+      alpha[x] = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - top);
+      m[x] = m_new;
+      float pv[4], sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pv[e] = __builtin_amdgcn_exp2f(s[x][e] - (top - kRaise));
+        sum = __builtin_fmaf(pv[e], val[e].iv, sum);
+      }
+      if (__any(signs)) {  // (none that the store writes)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pv[e] = (seen[x] >> e) & 1 ? pv[e] * val[e].sign : 0.0f;
+      }
+      l[x] = l[x] * alpha[x] + sum;
+      *reinterpret_cast<uint2*>(lds + L::P + (16 * x + n) * L::PROW + 2 * (16 * wave + 4 * g)) =
+          make_uint2(pack_pair(pv[0], pv[1], f16{}), pack_pair(pv[2], pv[3], f16{}));
+    }
+    if (edge) {  // NaN codes of this wave's rows
+#pragma unroll
+      for (int j = 0; j < DMAS; ++j) {
+        w_u4* p = reinterpret_cast<w_u4*>(codes + wave * 16 * R + j * 1024 + 16 * lane);
+        w_u4 w = *p;
+        const uint32_t odd = nan_codes(w[0]) | nan_codes(w[1]) | nan_codes(w[2]) | nan_codes(w[3]);
+        if (odd) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] &= ~((nan_codes(w[k]) >> 7) * 0xffu);
+          *p = w;
+        }
+      }
+    }
+    lds_barrier();
+
+    // ---- values ----
+#pragma unroll
+    for (int x = 0; x < NG; ++x)
+      if (__any(alpha[x] != 1.0f)) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d][x] *= alpha[x];
+      }
+#pragma unroll
+    for (int k = 0; k < kStage / 32; ++k) {
+      w_u4 p[NG];
+#pragma unroll
+      for (int x = 0; x < NG; ++x)
+        p[x] = *reinterpret_cast<const w_u4*>(lds + L::P + (16 * x + n) * L::PROW +
+                                              2 * (32 * k + 8 * g));
+      const int t = 32 * k + 8 * g + n / 2;  // the row this lane addresses
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const int chunk = (DB * wave + d) ^ (t % 16);
+        const lat_i2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lat_lds2)(codes + t * R + 16 * chunk + 8 * (n % 2)));
+        const w_u4 a = code_op8<f16>(static_cast<uint32_t>(v[0]), static_cast<uint32_t>(v[1]));
+#pragma unroll
+        for (int x = 0; x < NG; ++x) o[d][x] = mfma_op(a, p[x], o[d][x], f16{});
+      }
+    }
+  }
+
+  // ---- results: o[d][x][e] is dim R/8 wave + 16 d + 4 g + e of the column ----
+  lds_barrier();  // the maxima's place is read
+#pragma unroll
+  for (int x = 0; x < NG; ++x) {
+    const float sum = sum_rows4(l[x]);
+    if (g == 0) smax[(16 * x + n) * kWaves + wave] = sum;
+  }
+  lds_barrier();
+#pragma unroll
+  for (int x = 0; x < NG; ++x) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += smax[(16 * x + n) * kWaves + w];
+    if (!live[x]) continue;
+    const int dim = R / 8 * wave + 4 * g;
+    if (r.parts > 1) {
+      const int64_t part =
+          r.part0 + (static_cast<int64_t>(seg) * r.n + row[x]) * heads + head[x];
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        *reinterpret_cast<w_f4*>(parts.o + part * R + dim + 16 * d) = o[d][x];
+      if (g == 0 && wave == 0)  // a NaN score leaves m without it, but not l
+        *reinterpret_cast<w_f2*>(parts.ml + 2 * part) = w_f2{sum != sum ? INFINITY : m[x], sum};
+      continue;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* dst = out + ((static_cast<int64_t>(r.q0) + row[x]) * heads + head[x]) * R + dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const uint32_t lo = pack_pair(o[d][x][0] * inv, o[d][x][1] * inv, T{});
+      const uint32_t hi = pack_pair(o[d][x][2] * inv, o[d][x][3] * inv, T{});
+      if (wide & 2) {
+        *reinterpret_cast<uint2*>(dst + 16 * d) = make_uint2(lo, hi);
+      } else {
+        uint16_t* d16 = reinterpret_cast<uint16_t*>(dst + 16 * d);
+        d16[0] = static_cast<uint16_t>(lo);
+        d16[1] = static_cast<uint16_t>(lo >> 16);
+        d16[2] = static_cast<uint16_t>(hi);
+        d16[3] = static_cast<uint16_t>(hi >> 16);
+      }
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------
+
+int64_t lat_tiles(const LatentCall& call, int64_t b, int cols) {
+  return (call.win.qlens[b] * call.cache.hq + cols - 1) / cols;
+}
+int64_t lat_stages(const LatentCall& call, int64_t b) {
+  return std::max<int64_t>(1, (call.win.lens[b] + kStage - 1) / kStage);
+}
+// Columns of a tile: 32, or 16 where no request has more.
+int lat_cols(const LatentCall& call) {
+  for (int64_t b = 0; b < call.win.batch; ++b)
+    if (call.win.qlens[b] * call.cache.hq > 16) return 32;
+  return 16;
+}
+
+// Stages of a part: what ends soonest, in stages of one workgroup, when the CUs take one
+// workgroup each at a time, a workgroup costs two stages beside its own (queries in, results
+// out), and the partial results go through memory and back (a stage per 6 MB of them).
+int64_t lat_split(const LatentCall& call, int cols, int cus) {
+  int64_t longest = 1;
+  for (int64_t b = 0; b < call.win.batch; ++b)
+    if (call.win.qlens[b] > 0) longest = std::max(longest, lat_stages(call, b));
+  int64_t best = longest, cost = INT64_MAX;
+  for (int64_t split = longest; split >= 1;
+       split = split > 64 ? split - split / 8 : (split > 16 ? split - 4 : split - 1)) {
+    int64_t work = 0, groups = 0, rows = 0;
+    for (int64_t b = 0; b < call.win.batch; ++b) {
+      if (call.win.qlens[b] <= 0) continue;
+      const int64_t tiles = lat_tiles(call, b, cols), n = lat_stages(call, b);
+      const int64_t parts = (n + split - 1) / split;
+      work += tiles * (n + 2 * parts);
+      groups += tiles * parts;
+      rows += win_part_rows(call.win, b, parts);
+    }
+    // (what is left over when the CUs come out unevenly: half of a workgroup's time)
+    const int64_t each = split + 2;
+    int64_t time = groups <= cus ? each : std::max(each, work / cus + each / 2);
+    if (rows > 0) time += 3 + rows * call.cache.d * 4 / 6000000;
+    if (time < cost) {
+      best = split;
+      cost = time;
+    }
+  }
+  return best;
+}
+
+template <typename G>
+int lat_launches(const LatentCall& call, int* cols_out, G&& go) {
+  int cus = 0;
+  const int rc = device_cu_count(&cus);
+  if (rc != KVQ_OK) return rc;
+  if (cus <= 0) cus = 256;
+  const int cols = lat_cols(call);
+  if (cols_out) *cols_out = cols;
+  const int64_t split = lat_split(call, cols, cus);
+  return win_launches(
+      call.win,
+      [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
+        parts = (lat_stages(call, b) + split - 1) / split;
+        rows = win_part_rows(call.win, b, parts);
+        units = lat_tiles(call, b, cols) * parts;
+        return true;
+      },
+      go);
+}
+
+}  // namespace
+
+namespace kvq {
+
+bool latent_matrix(const LatentCall& call) {
+  const LatentCache& c = call.cache;
+  return (call.win.dtype == KVQ_DTYPE_BF16 || call.win.dtype == KVQ_DTYPE_F16) &&
+         (c.d == 256 || c.d == 512) && (c.part == 32 || c.part == 64) && c.bs.d % 16 == 0 &&
+         aligned16(c.kd, c.ks) && aligned16(c.rope, nullptr);
+}
+
+int64_t latent_matrix_bytes(const LatentCall& call, int* rc) {
+  int64_t most = 0;
+  *rc = KVQ_OK;
+  if (!latent_matrix(call)) return 0;
+  *rc = lat_launches(call, nullptr, [&](const WinArg&, int, int64_t, int64_t rows) -> int {
+    most = std::max(most, win_parts_bytes(rows, call.cache.d));
+    return KVQ_OK;
+  });
+  return most;
+}
+
+int latent_matrix_attend(const LatentCall& call, void* workspace) {
+  const WinCall& win = call.win;
+  const LatentCache& c = call.cache;
+  const int wide = (win.q_wide() ? 1 : 0) | (aligned16(win.out, nullptr) ? 2 : 0);
+  int cols = 0;
+  return lat_launches(call, &cols, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
+    const WinParts parts{static_cast<float*>(workspace),
+                         static_cast<float*>(workspace) + rows * c.d};
+#define KVQ_LATENT(T, R, P, NG)                                                                \
+  hipLaunchKernelGGL((latent_matrix_kernel<T, R, P, NG>), dim3(static_cast<unsigned>(units)),  \
+                     dim3(64 * kWaves), (LatLds<R, NG>::BYTES), win.stream, arg, count, c,     \
+                     static_cast<const T*>(win.query), win.q_stride, wide, win.qscale,         \
+                     static_cast<T*>(win.out), parts)
+#define KVQ_LATENT_N(T, R, P)   \
+  if (cols == 32)               \
+    KVQ_LATENT(T, R, P, 2);     \
+  else                          \
+    KVQ_LATENT(T, R, P, 1)
+#define KVQ_LATENT_P(T, R)      \
+  if (c.part == 64) {           \
+    KVQ_LATENT_N(T, R, 64);     \
+  } else {                      \
+    KVQ_LATENT_N(T, R, 32);     \
+  }
+#define KVQ_LATENT_R(T)         \
+  if (c.d == 512) {             \
+    KVQ_LATENT_P(T, 512)        \
+  } else {                      \
+    KVQ_LATENT_P(T, 256)        \
+  }
+    if (win.dtype == KVQ_DTYPE_BF16) {
+      KVQ_LATENT_R(bf16)
+    } else {
+      KVQ_LATENT_R(f16)
+    }
+#undef KVQ_LATENT_R
+#undef KVQ_LATENT_P
+#undef KVQ_LATENT_N
+#undef KVQ_LATENT
+    KVQ_LAUNCH_CHECK();
+    return rows > 0 ? launch_win_join(win, arg, count, parts) : KVQ_OK;
+  });
+}
+
+}  // namespace kvq

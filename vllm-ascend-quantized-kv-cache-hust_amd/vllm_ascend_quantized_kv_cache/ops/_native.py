@@ -161,6 +161,12 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I, _P, _I, _P, _I, _I64, _I, _P, _I,
          _I64, _I, _I, _I, _P, _P, _P, _I64, _I, _P],
     ),
+    "kvq_fp8_latent_attn_workspace_bytes": (_I64, [_P, _P, _I64, _I, _I, _I, _I, _I]),
+    "kvq_fp8_latent_attn": (
+        _I,
+        [_P, _I, _I64, _P, _P, _I64, _I, _I, _I, _F, _P, _P, _P, _I64, _I, _P, _I, _I64, _P, _I64,
+         _P, _P],
+    ),
 }
 
 #: kinds of 8-bit codes of a cache with a scale for each block

@@ -1,6 +1,7 @@
 # SPDX-License-Identifier: Apache-2.0
 """A paged E4M3 cache of latent rows that all heads share (``kvq_fp8_latent_*``):
-the store, with the position rotation applied on the way.
+the store, with the position rotation applied on the way, and causal attention
+straight over it, the up-projections absorbed.
 
 A token keeps one latent row of ``R`` dims as E4M3 codes ``data [NB, Bs, R]`` (uint8)
 with a scale ``scale [NB, Bs, 1]`` fp32, the quantization of
@@ -10,13 +11,25 @@ with a scale ``scale [NB, Bs, 1]`` fp32, the quantization of
 
 from __future__ import annotations
 
+from collections.abc import Sequence
+
 import torch
 
 from . import _native
-from .fp8_rotary import _check_devices, _check_query, _check_rotation, _same_view, _storage
-from .fp8_window import _on_device
+from .block8 import _checked_table
+from .fp8_rotary import (
+    _check_devices,
+    _check_query,
+    _check_rotation,
+    _rows,
+    _same_view,
+    _storage,
+    _token_stride,
+)
+from .fp8_window import _lengths, _on_device
 
 _STORE = "fp8_latent_store"
+_ATTENTION = "fp8_latent_attention"
 
 
 def _check_cache(what: str, data, scale, rope):
@@ -134,4 +147,98 @@ def fp8_latent_store(
     return target
 
 
-__all__ = ["fp8_latent_store"]
+def fp8_latent_attention(
+    query: torch.Tensor,
+    data: torch.Tensor,
+    scale: torch.Tensor,
+    rope: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: Sequence[int],
+    query_lens: Sequence[int],
+    softmax_scale: float,
+    *,
+    out: torch.Tensor | None = None,
+    block_table_host=None,
+) -> torch.Tensor:
+    """Causal attention of TND ``query [sum query_lens, H, R + P]`` over the latent
+    rows, with the up-projections absorbed: ``[..., :R]`` is a head's query through
+    its key up-projection, ``[..., R:]`` its rotated position part, and the result
+    ``[.., H, R]`` is for the caller to take through the value up-projection.
+
+    With ``c_j = code * scale`` of position ``j`` (not rounded to the query's type)
+    and ``r_j`` its position part, a score is ``softmax_scale * (q[:R] . c_j + q[R:] .
+    r_j)`` and a value is ``c_j``.  ``softmax_scale`` is that of the heads before
+    absorption.  Each request's rows are its last ``query_lens[b]`` of
+    ``seq_lens[b]`` cached positions (stored already); a row at position ``p`` sees
+    ``j <= p``, one that sees nothing gives zeros.  Scales under 2^-90 may count as 0
+    in the values; one that is not finite makes the rows that see it NaN.
+
+    ``block_table_host`` is the host's copy of the table, by which the pages are
+    checked; without it the table is copied from the device and waited for.  The
+    lengths are host values that travel with the launches: a call captured in a
+    graph replays the lengths it was captured with.
+
+    ``query`` may have rows behind the last request's (a padded batch), and its
+    rows may lie apart; rows of ``out`` behind the last request's stay as they were,
+    zeros in a fresh one.  Queries are of ``rope``'s type, ``R`` up to 512 and ``P`` up
+    to 256; bf16 and fp16 with ``R`` 256 or 512, ``P`` 32 or 64 and pages of whole
+    16-position groups run on the matrix units.
+    """
+    nb, bs, rank, dims = _check_cache(_ATTENTION, data, scale, rope)
+    if query.dim() != 3 or query.shape[2] != rank + dims or query.shape[1] == 0:
+        raise RuntimeError(
+            f"{_ATTENTION}: query must be [tokens, heads, {rank + dims}], got "
+            f"{tuple(query.shape)}.")
+    tokens, heads = query.shape[:2]
+    if query.dtype != rope.dtype:
+        raise RuntimeError(f"{_ATTENTION}: query is {query.dtype}, rope {rope.dtype}.")
+    dtype = _native.dtype_code(query.dtype)
+    if not 0 < softmax_scale < float("inf"):
+        raise RuntimeError(f"{_ATTENTION}: softmax_scale must be positive, got {softmax_scale}.")
+    lens, totals = _lengths(_ATTENTION, seq_lens, "seq_lens")
+    news, counts = _lengths(_ATTENTION, query_lens, "query_lens")
+    batch = len(totals)
+    if len(counts) != batch:
+        raise RuntimeError(f"{_ATTENTION}: {len(counts)} query_lens for {batch} seq_lens.")
+    rows = sum(counts)
+    if rows > tokens:
+        raise RuntimeError(f"{_ATTENTION}: query_lens sum to {rows}, the query has {tokens} rows.")
+    _check_devices(_ATTENTION, data, query=query, block_table=block_table)
+    shape = (tokens, heads, rank)
+    if out is not None:
+        if out.shape != shape:
+            raise RuntimeError(f"{_ATTENTION}: out must be {shape}, got {tuple(out.shape)}.")
+        _check_devices(_ATTENTION, data, out=out)
+    table = _checked_table(_ATTENTION, block_table, block_table_host, totals, lens, news, nb, bs, 0, 0)
+    # straight into `out` unless it is laid out otherwise or is the query's own memory
+    direct = out is None or (out.is_contiguous() and out.dtype == query.dtype
+                             and _storage(out) != _storage(query))
+    if rows:
+        _native.require_gpu_tensors(_ATTENTION, query, data)
+    q = _rows(query)
+    result = out if out is not None and direct else torch.empty(
+        shape, dtype=q.dtype, device=q.device)
+    if rows < tokens and out is None:
+        result[rows:].zero_()
+    if rows == 0:
+        return result if out is None else out
+    lib = _native.lib()
+    with _on_device(data):
+        nbytes = lib.kvq_fp8_latent_attn_workspace_bytes(
+            lens, news, batch, dtype, heads, rank, dims, bs)
+        _native.check(nbytes if nbytes < 0 else 0, "kvq_fp8_latent_attn_workspace_bytes")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        rc = lib.kvq_fp8_latent_attn(
+            q.data_ptr(), dtype, _token_stride(q), lens, news, batch, heads, rank, dims,
+            softmax_scale, data.data_ptr(), scale.data_ptr(), rope.data_ptr(), nb, bs,
+            table.data_ptr(), _native.index_code(table.dtype), table.shape[1], _native.ptr(ws),
+            nbytes, result.data_ptr(), _native.stream_of(data),
+        )
+    _native.check(rc, "kvq_fp8_latent_attn")
+    if not direct:
+        out[:rows].copy_(result[:rows])
+        return out
+    return result
+
+
+__all__ = ["fp8_latent_attention", "fp8_latent_store"]
