@@ -8,8 +8,7 @@
 // chunk c of row t at c ^ t % 16), and converted to 16 bits on their way to the matrix units:
 //   S^T = C * Q^T: wave w takes positions 16 w ..; A = codes in the query's type, exact: lane
 //     (g, n) holds dims R/4 g .. of position n; B = the queries, all R dims of the tile's
-//     columns in every wave's registers.  The position part beside it, from global memory
-//     straight into the operand.
+//     columns in every wave's registers.  The position part beside it, from 16 KB of its own.
 //   softmax: the waves put their positions' maxima into LDS; with t = (S s_j + S_r) scale
 //     log2(e) + log2(s_j) and m its running maximum, p' = 2^(t - m + 14) = p s_j fits fp16
 //     whatever the scales are: rounded by 2^-11 of it, or, where fp16 is subnormal, 2^-38 of
@@ -38,12 +37,14 @@ typedef const __attribute__((address_space(4))) int32_t lat_ci32;
 typedef const __attribute__((address_space(4))) int64_t lat_ci64;
 typedef int lat_i2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) lat_i2* lat_lds2;
+typedef const __attribute__((address_space(3))) w_u4* lat_cu4;
 
-template <int R, int NG>
+template <int R, int PART, int NG>
 struct LatLds {
   static constexpr int STAGE = kStage * R;
+  static constexpr int ROPE = 2 * STAGE;              // [kStage][PART] of 16 bits
   static constexpr int PROW = 2 * kStage + 16;        // bytes of a column's p', padded
-  static constexpr int P = 2 * STAGE;                 // [16 NG][PROW]
+  static constexpr int P = ROPE + 2 * kStage * PART;  // [16 NG][PROW]
   static constexpr int MAX = P + 16 * NG * PROW;      // [16 NG][kWaves] floats
   static constexpr int BYTES = MAX + 16 * NG * kWaves * 4;
 };
@@ -56,7 +57,7 @@ template <typename T, int R, int PART, int NG>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
 latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query,
                      int64_t q_stride, int wide, float qscale, T* __restrict__ out, WinParts parts) {
-  using L = LatLds<R, NG>;
+  using L = LatLds<R, PART, NG>;
   constexpr int KS = R / 32;      // k-steps of a score
   constexpr int RS = PART / 32;   // and of its position part
   constexpr int DB = R / 128;     // 16-dim blocks of a wave's dims
@@ -81,17 +82,22 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
   const int base = r.len - r.n;  // position of the request's first row
   const int tile_first = base + row_of(col0);
   const int tile_last = base + row_of(min(col0 + 16 * NG, cols) - 1);
-  // the lane's columns; one past the last sees nothing
-  int row[NG], head[NG], pos[NG];
-  bool live[NG];
-#pragma unroll
-  for (int x = 0; x < NG; ++x) {
-    const int col = col0 + 16 * x + n;
-    live[x] = col < cols;
-    row[x] = row_of(live[x] ? col : 0);
-    head[x] = (live[x] ? col : 0) - row[x] * heads;
-    pos[x] = live[x] ? base + row[x] : -1;
-  }
+  // the lane's column of group x, found where it is needed (held, these would cost registers);
+  // one past the last sees nothing
+  struct Col {
+    bool live;
+    int row, head, pos;
+  };
+  auto col_at = [&](int x) {
+    int col = col0 + 16 * x + n;
+    asm volatile("" : "+v"(col));  // found anew
+    Col y;
+    y.live = col < cols;
+    y.row = row_of(y.live ? col : 0);
+    y.head = (y.live ? col : 0) - y.row * heads;
+    y.pos = y.live ? base + y.row : -1;
+    return y;
+  };
   const int stages = tile_last >= 0 ? (tile_last + kStage) / kStage : 0;
   const int s0 = static_cast<int>(static_cast<int64_t>(stages) * seg / r.parts);
   const int s1 = static_cast<int>(static_cast<int64_t>(stages) * (seg + 1) / r.parts);
@@ -113,18 +119,16 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
 
   // ---- a stage on its way ----
   const uint32_t lds0 = win_lds(lds);
-  uint32_t off[DMAS];
-#pragma unroll
-  for (int j = 0; j < DMAS; ++j) {
-    const int t = RPI * j + lane / CH;
-    off[j] = static_cast<uint32_t>(t) * R + 16 * ((lane % CH) ^ t);
-  }
+  // instruction j brings rows RPI j + lane / CH: off ^ 16 RPI j from its first one's start
+  const uint32_t off = static_cast<uint32_t>(lane / CH) * R + 16 * ((lane % CH) ^ (lane / CH));
+  // position parts: chunk c of row t at c ^ t % RC, a wave's own rows
+  constexpr int RC = PART / 8;
+  const uint32_t rope_off =
+      static_cast<uint32_t>(lane / RC) * 2 * PART + 16 * ((lane % RC) ^ (lane / RC % RC));
+  const uint32_t rope_lds = lds0 + L::ROPE + wave * 32 * PART;
   const int groups = (r.len + 15) / 16;  // 16-position groups, each in one page
-  struct Beside {
-    w_u4 rope[RS];
-    w_f4 scale;
-  };
-  auto issue = [&](int stage) {
+  // slot of this wave's positions
+  auto slot_of = [&](int stage) -> int64_t {
     const int p = 16 * min(stage * kWaves + wave, groups - 1);
     const uint32_t i = c.bs.div(static_cast<uint32_t>(p));
     const int64_t at = __builtin_amdgcn_readfirstlane(
@@ -133,29 +137,35 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
     const int64_t id = c.bt64 ? ((lat_ci64*)(const void*)c.table)[e]
                               : static_cast<int64_t>(((lat_ci32*)(const void*)c.table)[e]);
     const int64_t page = id < 0 ? 0 : (id >= c.nb ? c.nb - 1 : id);
-    const int64_t slot = page * c.bs.d + (static_cast<uint32_t>(p) - i * c.bs.d);
+    return page * c.bs.d + (static_cast<uint32_t>(p) - i * c.bs.d);
+  };
+  auto issue = [&](int stage, int64_t slot) {
     const uint32_t to = lds0 + stage % 2 * L::STAGE + wave * 16 * R;
 #pragma unroll
-    for (int j = 0; j < DMAS; ++j) win_dma16(c.kd + slot * R, off[j], to + j * 1024);
-    Beside b;
-    const T* rope = static_cast<const T*>(c.rope) + (slot + n) * PART + 8 * g;
+    for (int j = 0; j < DMAS; ++j)
+      win_dma16(c.kd + slot * R + j * 1024, off ^ (16 * RPI * j), to + j * 1024);
+    return *reinterpret_cast<const w_f4*>(c.ks + slot + 4 * g);
+  };
+  auto issue_rope = [&](int64_t slot) {
 #pragma unroll
-    for (int s = 0; s < RS; ++s) b.rope[s] = *reinterpret_cast<const w_u4*>(rope + 32 * s);
-    b.scale = *reinterpret_cast<const w_f4*>(c.ks + slot + 4 * g);
-    return b;
+    for (int s = 0; s < RS; ++s)
+      win_dma16(static_cast<const T*>(c.rope) + slot * PART + 512 * s, rope_off, rope_lds + 1024 * s);
   };
 
-  Beside next = issue(s0);
+  int64_t slot = slot_of(s0);
+  w_f4 next = issue(s0, slot);
+  issue_rope(slot);
   w_u4 q[NG][KS], qr[NG][RS];
 #pragma unroll
   for (int x = 0; x < NG; ++x) {
-    const T* qrow = query + (static_cast<int64_t>(r.q0) + row[x]) * q_stride +
-                    static_cast<int64_t>(head[x]) * (R + PART);
+    const Col y = col_at(x);
+    const T* qrow = query + (static_cast<int64_t>(r.q0) + y.row) * q_stride +
+                    static_cast<int64_t>(y.head) * (R + PART);
 #pragma unroll
     for (int s = 0; s < KS; ++s) q[x][s] = load_op8(qrow + (R / 4) * g + 8 * s, wide & 1);
 #pragma unroll
     for (int s = 0; s < RS; ++s) qr[x][s] = load_op8(qrow + R + 32 * s + 8 * g, wide & 1);
-    if (!live[x]) {
+    if (!y.live) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) q[x][s] = w_u4{0, 0, 0, 0};
 #pragma unroll
@@ -176,11 +186,12 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
   for (int st = s0; st < s1; ++st) {
     wait_vmcnt<0>();  // this wave's part of the stage
     lds_barrier();    // everybody's; and the last stage's other buffer is read
-    Beside b = next;
-#pragma unroll
-    for (int s = 0; s < RS; ++s) asm volatile("" : "+v"(b.rope[s]));
-    asm volatile("" : "+v"(b.scale));
-    if (st + 1 < s1) next = issue(st + 1);
+    w_f4 scale = next;
+    asm volatile("" : "+v"(scale));
+    if (st + 1 < s1) {
+      slot = slot_of(st + 1);
+      next = issue(st + 1, slot);
+    }
     char* const codes = lds + st % 2 * L::STAGE;
     const int p0 = st * kStage + 16 * wave;  // of this wave's positions
     const bool edge = st * kStage + kStage - 1 > tile_first;  // uniform
@@ -189,26 +200,38 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
     w_f4 s[NG], sr[NG];
 #pragma unroll
     for (int x = 0; x < NG; ++x) s[x] = sr[x] = w_f4{0.f, 0.f, 0.f, 0.f};
-    const char* kr = codes + (16 * wave + n) * R;
+#pragma unroll
+    for (int i = 0; i < RS; ++i) {
+      const w_u4 k = *(lat_cu4)(rope_lds + n * 2 * PART + 16 * ((4 * i + g) ^ (n % RC)));
+#pragma unroll
+      for (int x = 0; x < NG; ++x) sr[x] = mfma_op(k, qr[x][i], sr[x], T{});
+    }
+    const uint32_t kr = win_lds(codes) + (16 * wave + n) * R + 16 * ((CH / 4 * g) ^ n);
 #pragma unroll
     for (int w = 0; w < KS / 2; ++w) {
-      const w_u4 k = *reinterpret_cast<const w_u4*>(kr + 16 * ((CH / 4 * g + w) ^ n));
+      const w_u4 k = *(lat_cu4)(kr ^ (16 * w));
       const w_u4 k0 = code_op8<T>(k[0], k[1]), k1 = code_op8<T>(k[2], k[3]);
 #pragma unroll
       for (int x = 0; x < NG; ++x) s[x] = mfma_op(k0, q[x][2 * w], s[x], T{});
 #pragma unroll
       for (int x = 0; x < NG; ++x) s[x] = mfma_op(k1, q[x][2 * w + 1], s[x], T{});
     }
-#pragma unroll
-    for (int i = 0; i < RS; ++i)
-#pragma unroll
-      for (int x = 0; x < NG; ++x) sr[x] = mfma_op(b.rope[i], qr[x][i], sr[x], T{});
-    B8Value val[4];
-    bool signs = false;
+    w_f4 lv, iv;
+    bool odd = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      val[e] = b8_value(b.scale[e]);
-      signs = signs || val[e].sign != 1.0f;
+      lv[e] = __builtin_amdgcn_logf(scale[e]);
+      iv[e] = __builtin_amdgcn_rcpf(scale[e]);
+      odd = odd || !(scale[e] >= 0x1p-90f && scale[e] < INFINITY);
+    }
+    const bool odds = __any(odd);  // (none that the store writes)
+    if (odds) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const B8Value v = b8_value(scale[e]);
+        lv[e] = v.lv;
+        iv[e] = v.iv;
+      }
     }
     uint32_t seen[NG];
 #pragma unroll
@@ -216,13 +239,14 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
       seen[x] = 0xf;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        s[x][e] = __builtin_fmaf(s[x][e], b.scale[e] * qscale,
-                                 __builtin_fmaf(sr[x][e], qscale, val[e].lv));
+        s[x][e] = __builtin_fmaf(s[x][e], scale[e] * qscale,
+                                 __builtin_fmaf(sr[x][e], qscale, lv[e]));
       if (edge) {
         seen[x] = 0;
+        const int pos = col_at(x).pos;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool on = p0 + 4 * g + e <= pos[x];
+          const bool on = p0 + 4 * g + e <= pos;
           seen[x] |= on ? 1u << e : 0u;
           s[x][e] = on ? s[x][e] : -INFINITY;
         }
@@ -231,6 +255,7 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
       if (g == 0) smax[(16 * x + n) * kWaves + wave] = mx;
     }
     lds_barrier();  // the maxima; and the codes are read as keys
+    if (st + 1 < s1) issue_rope(slot);
 
     // ---- weights ----
     float alpha[NG];
@@ -248,11 +273,12 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         pv[e] = __builtin_amdgcn_exp2f(s[x][e] - (top - kRaise));
-        sum = __builtin_fmaf(pv[e], val[e].iv, sum);
+        sum = __builtin_fmaf(pv[e], iv[e], sum);
       }
-      if (__any(signs)) {  // (none that the store writes)
+      if (odds) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pv[e] = (seen[x] >> e) & 1 ? pv[e] * val[e].sign : 0.0f;
+        for (int e = 0; e < 4; ++e)
+          pv[e] = (seen[x] >> e) & 1 ? pv[e] * b8_value(scale[e]).sign : 0.0f;
       }
       l[x] = l[x] * alpha[x] + sum;
       *reinterpret_cast<uint2*>(lds + L::P + (16 * x + n) * L::PROW + 2 * (16 * wave + 4 * g)) =
@@ -313,11 +339,12 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
     float sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) sum += smax[(16 * x + n) * kWaves + w];
-    if (!live[x]) continue;
+    const Col y = col_at(x);
+    if (!y.live) continue;
     const int dim = R / 8 * wave + 4 * g;
     if (r.parts > 1) {
       const int64_t part =
-          r.part0 + (static_cast<int64_t>(seg) * r.n + row[x]) * heads + head[x];
+          r.part0 + (static_cast<int64_t>(seg) * r.n + y.row) * heads + y.head;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
         *reinterpret_cast<w_f4*>(parts.o + part * R + dim + 16 * d) = o[d][x];
@@ -326,7 +353,7 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
       continue;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* dst = out + ((static_cast<int64_t>(r.q0) + row[x]) * heads + head[x]) * R + dim;
+    T* dst = out + ((static_cast<int64_t>(r.q0) + y.row) * heads + y.head) * R + dim;
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
       const uint32_t lo = pack_pair(o[d][x][0] * inv, o[d][x][1] * inv, T{});
@@ -442,7 +469,7 @@ int latent_matrix_attend(const LatentCall& call, void* workspace) {
                          static_cast<float*>(workspace) + rows * c.d};
 #define KVQ_LATENT(T, R, P, NG)                                                                \
   hipLaunchKernelGGL((latent_matrix_kernel<T, R, P, NG>), dim3(static_cast<unsigned>(units)),  \
-                     dim3(64 * kWaves), (LatLds<R, NG>::BYTES), win.stream, arg, count, c,     \
+                     dim3(64 * kWaves), (LatLds<R, P, NG>::BYTES), win.stream, arg, count, c,     \
                      static_cast<const T*>(win.query), win.q_stride, wide, win.qscale,         \
                      static_cast<T*>(win.out), parts)
 #define KVQ_LATENT_N(T, R, P)   \
