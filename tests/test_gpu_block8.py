@@ -217,6 +217,17 @@ def test_large_scores(gpu_device):
 
 
 @pytest.mark.parametrize("codes", ["e4m3", "int8"])
+@pytest.mark.parametrize("size", [2.0 ** 22, 2.0 ** 25, 2.0 ** 28, 2.0 ** 40])
+def test_scores_beyond_their_steps(gpu_device, codes, size):
+    """Where a score's step is 4, 16 and more, the weights of 16 bits stay finite."""
+    lens, d = [300], 128
+    c = ref.Pages(lens, 2, d, 64, 64, codes, device=gpu_device, seed=18)
+    for news in (1, 60):
+        q = win.query(news, 8, d, BF16, gpu_device, size=size)
+        _check(gpu_device, lens, [news], 8, 2, d, 64, 64, codes, BF16, cache=c, q=q)
+
+
+@pytest.mark.parametrize("codes", ["e4m3", "int8"])
 @pytest.mark.parametrize("shift", [1, 8])
 def test_rows_off_their_bounds(gpu_device, codes, shift):
     """Queries and outputs at odd addresses; caches off a 16-byte bound."""

@@ -253,7 +253,8 @@ b8_decode_kernel(WinArg, int count, B8Cache c, const T* __restrict__ query, int6
       const float m_new = fmaxf(m[x], mx);
       const float base = m_new == -INFINITY ? 0.0f : m_new;
       const float alpha = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - base);
-      const float low = base - kRaise;
+      // (among scores of 2^26 and more the difference rounds up: p' stays within fp16 all the same)
+      const float raised = base - kRaise, low = base - raised > kRaise + 1.0f ? base : raised;
       m[x] = m_new;
       float sum = 0.0f;
 #pragma unroll
