@@ -142,6 +142,29 @@ def test_large_scores(gpu_device):
         _check(gpu_device, [700], [news], 8, 512, 64, 64, FP16, size=12.0)
 
 
+@pytest.mark.parametrize("heads", [4, 32, 33, 64, 65, 96])
+@pytest.mark.parametrize("growth", [2.0 ** 0.1, 2.0 ** -0.1, 64.0])
+def test_scores_that_grow(gpu_device, heads, growth):
+    """Maxima that outgrow the offsets again and again, or stay the first ones, by rows that
+    get larger or smaller from position to position."""
+    lens, news = [500, 129], [1, 2]
+    for rank, dims in ((512, 64), (256, 32)):
+        c = ref.Latents(lens, rank, dims, 64, BF16, device=gpu_device, seed=14)
+        for b, n in enumerate(lens):
+            at = torch.from_numpy(ref.slots_of(c.host, b, torch.arange(n).numpy(), 64))
+            steps = torch.arange(n) // 48 if growth == 64.0 else torch.arange(n) % 300
+            size = torch.exp2(torch.log2(torch.tensor(growth)) * steps).clamp(2.0 ** -40, 2.0 ** 40)
+            c.scale.view(-1)[at.to(gpu_device)] = (2.0 ** -6 * size).to(gpu_device)
+        _check(gpu_device, lens, news, heads, rank, dims, 64, BF16, cache=c, size=0.1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_few_and_many_columns(gpu_device, dtype):
+    """Requests of both kernels in one call, between those without rows."""
+    lens, news = [70, 2000, 0, 300, 900, 64, 5], [1, 3, 0, 2, 40, 0, 1]
+    _check(gpu_device, lens, news, 16, 512, 64, 16, dtype, seed=15)
+
+
 @pytest.mark.parametrize("shift", [1, 8])
 def test_rows_off_their_bounds(gpu_device, shift):
     lens, news = [130, 20], [9, 1]

@@ -239,9 +239,14 @@ LatentCall make_call(const void* query, int dtype, int64_t query_stride, const i
 }
 
 int64_t workspace_of(const LatentCall& call, int* rc) {
-  const int64_t matrix = latent_matrix_bytes(call, rc);
-  if (*rc != KVQ_OK) return 0;
-  return (std::max(matrix, general_bytes(call.win)) + 15) / 16 * 16;
+  int64_t most = general_bytes(call.win);
+  *rc = KVQ_OK;
+  if (latent_matrix(call)) {
+    most = std::max(most, latent_few_bytes(call, rc));
+    if (*rc == KVQ_OK) most = std::max(most, latent_tile_bytes(call, rc));
+    if (*rc != KVQ_OK) return 0;
+  }
+  return (most + 15) / 16 * 16;
 }
 
 }  // namespace
@@ -296,7 +301,10 @@ extern "C" int kvq_fp8_latent_attn(const void* query, int dtype, int64_t query_s
   if (rc != KVQ_OK) return rc;
   if (bytes > 0 && (!workspace || !aligned16(workspace, nullptr) || workspace_bytes < bytes))
     return KVQ_ERR_INVALID;
-  if (latent_matrix(call)) return latent_matrix_attend(call, workspace);
+  if (latent_matrix(call)) {
+    const int done = latent_few_attend(call, workspace);
+    return done != KVQ_OK ? done : latent_tile_attend(call, workspace);
+  }
   KVQ_DISPATCH_FLOAT(dtype, T, { rc = attend_general<T>(call, workspace); });
   return rc;
 }

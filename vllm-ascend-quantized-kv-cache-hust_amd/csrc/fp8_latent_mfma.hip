@@ -1,6 +1,6 @@
 // SPDX-License-Identifier: Apache-2.0
-// Attention over latent rows that all heads share, on the matrix units: decodes, where the
-// rows stream through once, and chunks.
+// Attention over latent rows that all heads share, on the matrix units, where a request has
+// few columns: decodes of few heads, where memory bounds it and the rows stream through once.
 //
 // One workgroup of eight waves per tile of 16 or 32 columns (row, head), request and part of
 // its positions, 128 positions at a time.  The latent is key and value at once, so a stage's
@@ -16,6 +16,8 @@
 //     through LDS to all waves.
 //   O^T += C^T * p'^T: wave w takes dims R/8 w ..; A = codes in fp16, exact, by the transposing
 //     reads of bytes (16 lanes read 8 rows of 16 bytes, lane s gets column s).
+//
+// 32 requests of 2048 - 16384 positions, 16 heads, R = 512, P = 64 (177 MB): 46 us, 3.8 TB/s.
 //
 // Positions that a column does not see: weights by selection; in stages that some column
 // does not wholly see, NaN codes become zeros in LDS between the two products (a row that
@@ -55,7 +57,7 @@ __device__ __forceinline__ void lds_barrier() {
 
 template <typename T, int R, int PART, int NG>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
-latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query,
+latent_few_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query,
                      int64_t q_stride, int wide, float qscale, T* __restrict__ out, WinParts parts) {
   using L = LatLds<R, PART, NG>;
   constexpr int KS = R / 32;      // k-steps of a score
@@ -269,10 +271,12 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
       const float top = m_new == -INFINITY ? 0.0f : m_new;
       alpha[x] = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - top);
       m[x] = m_new;
+      // (among scores of 2^26 and more the difference rounds up: p' stays within fp16 all the same)
+      const float low = top - kRaise, from = top - low > kRaise + 1.0f ? top : low;
       float pv[4], sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        pv[e] = __builtin_amdgcn_exp2f(s[x][e] - (top - kRaise));
+        pv[e] = __builtin_amdgcn_exp2f(s[x][e] - from);
         sum = __builtin_fmaf(pv[e], iv[e], sum);
       }
       if (odds) {
@@ -373,68 +377,12 @@ latent_matrix_kernel(WinArg, int count, LatentCache c, const T* __restrict__ que
 
 // ---- host -----------------------------------------------------------------------
 
-int64_t lat_tiles(const LatentCall& call, int64_t b, int cols) {
-  return (call.win.qlens[b] * call.cache.hq + cols - 1) / cols;
-}
-int64_t lat_stages(const LatentCall& call, int64_t b) {
-  return std::max<int64_t>(1, (call.win.lens[b] + kStage - 1) / kStage);
-}
 // Columns of a tile: 32, or 16 where no request has more.
-int lat_cols(const LatentCall& call) {
+LatentShape few_shape(const LatentCall& call) {
+  int cols = 16;
   for (int64_t b = 0; b < call.win.batch; ++b)
-    if (call.win.qlens[b] * call.cache.hq > 16) return 32;
-  return 16;
-}
-
-// Stages of a part: what ends soonest, in stages of one workgroup, when the CUs take one
-// workgroup each at a time, a workgroup costs two stages beside its own (queries in, results
-// out), and the partial results go through memory and back (a stage per 6 MB of them).
-int64_t lat_split(const LatentCall& call, int cols, int cus) {
-  int64_t longest = 1;
-  for (int64_t b = 0; b < call.win.batch; ++b)
-    if (call.win.qlens[b] > 0) longest = std::max(longest, lat_stages(call, b));
-  int64_t best = longest, cost = INT64_MAX;
-  for (int64_t split = longest; split >= 1;
-       split = split > 64 ? split - split / 8 : (split > 16 ? split - 4 : split - 1)) {
-    int64_t work = 0, groups = 0, rows = 0;
-    for (int64_t b = 0; b < call.win.batch; ++b) {
-      if (call.win.qlens[b] <= 0) continue;
-      const int64_t tiles = lat_tiles(call, b, cols), n = lat_stages(call, b);
-      const int64_t parts = (n + split - 1) / split;
-      work += tiles * (n + 2 * parts);
-      groups += tiles * parts;
-      rows += win_part_rows(call.win, b, parts);
-    }
-    // (what is left over when the CUs come out unevenly: half of a workgroup's time)
-    const int64_t each = split + 2;
-    int64_t time = groups <= cus ? each : std::max(each, work / cus + each / 2);
-    if (rows > 0) time += 3 + rows * call.cache.d * 4 / 6000000;
-    if (time < cost) {
-      best = split;
-      cost = time;
-    }
-  }
-  return best;
-}
-
-template <typename G>
-int lat_launches(const LatentCall& call, int* cols_out, G&& go) {
-  int cus = 0;
-  const int rc = device_cu_count(&cus);
-  if (rc != KVQ_OK) return rc;
-  if (cus <= 0) cus = 256;
-  const int cols = lat_cols(call);
-  if (cols_out) *cols_out = cols;
-  const int64_t split = lat_split(call, cols, cus);
-  return win_launches(
-      call.win,
-      [&](int64_t b, int64_t& units, int64_t& parts, int64_t& rows) {
-        parts = (lat_stages(call, b) + split - 1) / split;
-        rows = win_part_rows(call.win, b, parts);
-        units = lat_tiles(call, b, cols) * parts;
-        return true;
-      },
-      go);
+    if (latent_few(call, b) && call.win.qlens[b] * call.cache.hq > 16) cols = 32;
+  return LatentShape{true, cols, kStage, 2, 3, 6000000};
 }
 
 }  // namespace
@@ -448,27 +396,27 @@ bool latent_matrix(const LatentCall& call) {
          aligned16(c.kd, c.ks) && aligned16(c.rope, nullptr);
 }
 
-int64_t latent_matrix_bytes(const LatentCall& call, int* rc) {
+int64_t latent_few_bytes(const LatentCall& call, int* rc) {
   int64_t most = 0;
-  *rc = KVQ_OK;
-  if (!latent_matrix(call)) return 0;
-  *rc = lat_launches(call, nullptr, [&](const WinArg&, int, int64_t, int64_t rows) -> int {
-    most = std::max(most, win_parts_bytes(rows, call.cache.d));
-    return KVQ_OK;
-  });
+  *rc = latent_launches(call, few_shape(call),
+                        [&](const WinArg&, int, int64_t, int64_t rows) -> int {
+                          most = std::max(most, win_parts_bytes(rows, call.cache.d));
+                          return KVQ_OK;
+                        });
   return most;
 }
 
-int latent_matrix_attend(const LatentCall& call, void* workspace) {
+int latent_few_attend(const LatentCall& call, void* workspace) {
   const WinCall& win = call.win;
   const LatentCache& c = call.cache;
   const int wide = (win.q_wide() ? 1 : 0) | (aligned16(win.out, nullptr) ? 2 : 0);
-  int cols = 0;
-  return lat_launches(call, &cols, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
+  const LatentShape shape = few_shape(call);
+  const int cols = shape.cols;
+  return latent_launches(call, shape, [&](const WinArg& arg, int count, int64_t units, int64_t rows) -> int {
     const WinParts parts{static_cast<float*>(workspace),
                          static_cast<float*>(workspace) + rows * c.d};
 #define KVQ_LATENT(T, R, P, NG)                                                                \
-  hipLaunchKernelGGL((latent_matrix_kernel<T, R, P, NG>), dim3(static_cast<unsigned>(units)),  \
+  hipLaunchKernelGGL((latent_few_kernel<T, R, P, NG>), dim3(static_cast<unsigned>(units)),  \
                      dim3(64 * kWaves), (LatLds<R, P, NG>::BYTES), win.stream, arg, count, c,     \
                      static_cast<const T*>(win.query), win.q_stride, wide, win.qscale,         \
                      static_cast<T*>(win.out), parts)
