@@ -94,13 +94,12 @@ def fp8_latent_store(
     A slot is given once.  A latent row that is not finite reads back as NaN.
     """
     nb, bs, rank, dims = _check_cache(_STORE, data, scale, rope)
-    tokens = latent.shape[0]
-    if latent.dim() != 2 or latent.shape[1] != rank or part.shape != (tokens, dims):
+    if latent.dim() != 2 or latent.shape[1] != rank or part.shape != (latent.shape[0], dims):
         raise RuntimeError(
             f"{_STORE}: latent and part must be [tokens, {rank}] and [tokens, {dims}], got "
             f"{tuple(latent.shape)} and {tuple(part.shape)}."
         )
-    dtype = _native.dtype_code(latent.dtype)
+    tokens, dtype = latent.shape[0], _native.dtype_code(latent.dtype)
     if part.dtype != latent.dtype or rope.dtype != latent.dtype:
         raise RuntimeError(
             f"{_STORE}: latent is {latent.dtype}, part {part.dtype}, rope {rope.dtype}.")
