@@ -392,7 +392,11 @@ __device__ __forceinline__ uint32_t requantize(uint32_t w, float old, float scal
   return MODE == kBlockInt8 ? int8_word(x) : e4m3x4(x[0], x[1], x[2], x[3]);
 }
 
-constexpr int kKeep = 4;  // rows of a lane that stay in registers between maximum and codes
+// Rows of a lane that stay in registers between maximum and codes: the wave has to leave room
+// for the waves that rotate queries beside it.  Nine chunks of 11503 tokens, 40 + 16 heads of
+// 128 (306 MB), us a call: four rows in 166 registers 105, two in 128 97; 512 decodes 49 and
+// 39.  One row, in 96 registers: 114 and 57.
+constexpr int kKeep = 2;
 
 // The run of tokens that begins at t0 and shares its block.
 template <typename T, bool FAST, int MODE>
@@ -609,7 +613,7 @@ __device__ __forceinline__ void rotate_rows(const Step& s, int64_t block) {
 }
 
 template <typename T, bool FAST, int MODE, int HEADS>
-__global__ void __launch_bounds__(256) rotary_store_kernel(Step s) {
+__global__ void __launch_bounds__(256, 4) rotary_store_kernel(Step s) {
   if (blockIdx.x >= s.store_blocks) {
     rotate_rows<T, FAST, HEADS>(s, static_cast<int64_t>(blockIdx.x) - s.store_blocks);
     return;
@@ -681,8 +685,11 @@ int launch_store(Step& s, int dtype, hipStream_t stream) {
   if (MODE == kToken) {
     s.store_blocks = ((rows << s.shift) + 255) / 256;
   } else {
-    // a workgroup a token while those that find no block's first row cost little
-    s.chunk = s.tokens <= 1024 ? 1 : 16;
+    // A workgroup takes the blocks that begin in its tokens one after another, and one that
+    // finds none is time lost.  us a call at 1, 4, 16, 32 and 64 tokens: 11503 tokens of nine
+    // chunks 271, 139, 94, 85 and 82 in blocks of 128, 324, 193, 111, 101 and 95 in blocks of
+    // 16; 1100 decodes 77, 65, 88, 95 and 172, 1100 tokens of one chunk 32, 23, 22, 22 and 22.
+    s.chunk = s.tokens <= 1024 ? 1 : (s.tokens <= 2048 ? 4 : 32);
     s.store_blocks = (s.tokens + s.chunk - 1) / s.chunk * s.sides * s.kvh;
   }
   KVQ_DISPATCH_FLOAT(dtype, T, {
