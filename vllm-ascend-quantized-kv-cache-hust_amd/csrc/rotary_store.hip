@@ -28,6 +28,11 @@
 // wave a row, a lane up to four pairs, element by element.
 // A block's new rows are one workgroup's (a head and side): maximum, then codes, rows past
 // the first kKeep of a lane read twice (from L2).
+//
+// Bound by HBM: eight prompts of 14911 tokens, 40 + 16 heads of 128 (406 MB) 81 us, 5.0 TB/s; 12300
+// latent rows of 512 with 128 heads of 64 (428 MB) 89 us, 4.8 TB/s.  Blocks of 128 in nine chunks
+// (306 MB) 88 us, 3.5 TB/s: a block's maximum comes before its codes, and its tokens before
+// both, three latencies in a row.
 #include <algorithm>
 
 #include "fp8_codes.h"
