@@ -216,6 +216,24 @@ def test_block_scales(gpu_device, requests, pad, hq, kvh, d, bs, group, rot, int
     ref.check_block_store(before, after, rows, slots, [0 <= s < pages * bs for s in slots])
 
 
+@pytest.mark.parametrize("gaps", [(3, 200, 700), (0, 40, 1300), (1000, 70, 2500)])
+def test_block_scales_among_padding(gpu_device, gaps):
+    """Runs of a block whose rows lie far apart in the call, past a workgroup's tokens."""
+    dev = gpu_device
+    d, kvh, bs, group = 64, 1, 32, 32
+    slots = []
+    for i in range(9):  # two and a half blocks, cut by padding wherever it falls
+        slots += [-1] * gaps[i % 3] + list(range(100 + 9 * i, 100 + 9 * (i + 1)))
+    slots += [-1] * gaps[0]
+    tokens = len(slots)
+    _, k, v = _rows(tokens, 1, kvh, d, BF16, dev, 17)
+    before = ref.BlockCache(8, bs, kvh, d, group, "int8", dev)
+    after = before.clone()
+    block8_store(k, v, torch.tensor(slots, device=dev), *after.args())
+    rows = [(x.double(), x.double().abs()) for x in (k, v)]
+    ref.check_block_store(before, after, rows, slots, [x >= 0 for x in slots])
+
+
 @pytest.mark.parametrize("codes", ["e4m3", "int8"])
 @pytest.mark.parametrize("steps", [[1] * 40, [16, 1, 30, 2, 100], [7, 70, 3]])
 def test_a_block_in_several_calls(gpu_device, codes, steps):

@@ -217,31 +217,31 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
 
   if (scorer) {
     // ---- scores and weights ----
-  w_u4 q[2 * KW], qr[RS];
-  {
-    const Col y = col_at(ch);
-    const T* qrow = query + (static_cast<int64_t>(r.q0) + y.row) * q_stride +
-                    static_cast<int64_t>(y.head) * (R + PART);
-    if (wide & 1) {
+    w_u4 q[2 * KW], qr[RS];
+    {
+      const Col y = col_at(ch);
+      const T* qrow = query + (static_cast<int64_t>(r.q0) + y.row) * q_stride +
+                      static_cast<int64_t>(y.head) * (R + PART);
+      if (wide & 1) {
 #pragma unroll
-      for (int s = 0; s < 2 * KW; ++s)
-        q[s] = load_op8(qrow + 32 * (s / 2) + 16 * g + 8 * (s % 2), true);
+        for (int s = 0; s < 2 * KW; ++s)
+          q[s] = load_op8(qrow + 32 * (s / 2) + 16 * g + 8 * (s % 2), true);
 #pragma unroll
-      for (int s = 0; s < RS; ++s) qr[s] = load_op8(qrow + R + 16 * s + 8 * g, true);
-    } else {
+        for (int s = 0; s < RS; ++s) qr[s] = load_op8(qrow + R + 16 * s + 8 * g, true);
+      } else {
 #pragma unroll
-      for (int s = 0; s < 2 * KW; ++s)
-        q[s] = load_op8(qrow + 32 * (s / 2) + 16 * g + 8 * (s % 2), false);
+        for (int s = 0; s < 2 * KW; ++s)
+          q[s] = load_op8(qrow + 32 * (s / 2) + 16 * g + 8 * (s % 2), false);
 #pragma unroll
-      for (int s = 0; s < RS; ++s) qr[s] = load_op8(qrow + R + 16 * s + 8 * g, false);
+        for (int s = 0; s < RS; ++s) qr[s] = load_op8(qrow + R + 16 * s + 8 * g, false);
+      }
+      if (!y.live) {
+#pragma unroll
+        for (int s = 0; s < 2 * KW; ++s) q[s] = w_u4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < RS; ++s) qr[s] = w_u4{0, 0, 0, 0};
+      }
     }
-    if (!y.live) {
-#pragma unroll
-      for (int s = 0; s < 2 * KW; ++s) q[s] = w_u4{0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < RS; ++s) qr[s] = w_u4{0, 0, 0, 0};
-    }
-  }
     float m = kNone, l = 0.0f;
     const uint32_t k_row = 32 * ph + n;
     const uint32_t k_off = k_row * R + 16 * (g ^ (n % 16));
@@ -253,153 +253,155 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
     // domain, their largest, and the sum
     float t[16], top, l_stage = 0.0f;
     bool odds = false;  // scales that the store does not write
-  // the rows' constants, by way of the wave's own place
-  auto row_values = [&](float scale) {
-    const B8Value b = b8_value(scale);
-    odds = !(scale >= 0x1p-90f && scale < INFINITY);
-    rows[n] = scale * qscale;
-    rows[32 + n] = b.lv;
-    rows[64 + n] = b.iv;
-    rows[96 + n] = b.sign;
-    asm volatile("" ::: "memory");
-  };
-  auto row4 = [&](int which, int i) -> w_f4 {  // of rows 8 i + 4 g ..
-    return *(lat_cf4)(rows_lds + 128 * which + 32 * i + 16 * g);
-  };
-  // all weights again, where there are masks, odd scales or another offset
-  auto weigh_again = [&](int st, bool edge, float was, float now, char* to) {
-    const int rel = (edge ? col_at(ch).pos : 0x7fffffff) - (edge ? st * kStage + 32 * ph + 4 * g : 0);
-    l_stage = 0.0f;
-    top = -INFINITY;
+    // the rows' constants, by way of the wave's own place
+    auto row_values = [&](float scale) {
+      const B8Value b = b8_value(scale);
+      odds = !(scale >= 0x1p-90f && scale < INFINITY);
+      rows[n] = scale * qscale;
+      rows[32 + n] = b.lv;
+      rows[64 + n] = b.iv;
+      rows[96 + n] = b.sign;
+      asm volatile("" ::: "memory");
+    };
+    auto row4 = [&](int which, int i) -> w_f4 {  // of rows 8 i + 4 g ..
+      return *(lat_cf4)(rows_lds + 128 * which + 32 * i + 16 * g);
+    };
+    // all weights again, where there are masks, odd scales or another offset
+    auto weigh_again = [&](int st, bool edge, float was, float now, char* to) {
+      const int rel = (edge ? col_at(ch).pos : 0x7fffffff) - (edge ? st * kStage + 32 * ph + 4 * g : 0);
+      l_stage = 0.0f;
+      top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const w_f4 iv = row4(2, i);
-      float pv[4];
-      w_f4 sign = w_f4{1.f, 1.f, 1.f, 1.f};
-      if (odds) sign = row4(3, i);
+      for (int i = 0; i < 4; ++i) {
+        const w_f4 iv = row4(2, i);
+        float pv[4];
+        w_f4 sign = w_f4{1.f, 1.f, 1.f, 1.f};
+        if (odds) sign = row4(3, i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool on = 8 * i + e <= rel;
-        float& x = t[4 * i + e];
-        x = on ? x + (was - now) : -INFINITY;
-        top = fmaxf(top, x);
-        pv[e] = __builtin_amdgcn_exp2f(x);
-        l_stage = __builtin_fmaf(pv[e], iv[e], l_stage);
-        pv[e] = on ? pv[e] * sign[e] : 0.0f;
+        for (int e = 0; e < 4; ++e) {
+          const bool on = 8 * i + e <= rel;
+          float& x = t[4 * i + e];
+          x = on ? x + (was - now) : -INFINITY;
+          top = fmaxf(top, x);
+          pv[e] = __builtin_amdgcn_exp2f(x);
+          l_stage = __builtin_fmaf(pv[e], iv[e], l_stage);
+          pv[e] = on ? pv[e] * sign[e] : 0.0f;
+        }
+        *reinterpret_cast<uint2*>(to + 16 * i) =
+            make_uint2(pack_pair(pv[0], pv[1], f16{}), pack_pair(pv[2], pv[3], f16{}));
       }
-      *reinterpret_cast<uint2*>(to + 16 * i) =
-          make_uint2(pack_pair(pv[0], pv[1], f16{}), pack_pair(pv[2], pv[3], f16{}));
-    }
-  };
-  lat_f16 sv, srv;
-  w_u4 k[KW], kp[RS];
-  float scale;
-  w_f4 sq[4], lv[4], iv[4];
-  auto scores_ahead = [&](uint32_t stage) {
-    const uint32_t kr = stage + k_off;
+    };
+    lat_f16 sv, srv;
+    w_u4 k[KW], kp[RS];
+    float scale;
+    w_f4 sq[4], lv[4], iv[4];
+    auto scores_ahead = [&](uint32_t stage) {
+      const uint32_t kr = stage + k_off;
 #pragma unroll
-    for (int w = 0; w < AHEAD; ++w) k[w] = *(lat_cu4)(kr ^ (32 * w));
-    scale = *(const __attribute__((address_space(3))) float*)(stage + L::SCALE + 4 * k_row);
-  };
-  auto scores = [&](uint32_t stage) {
+      for (int w = 0; w < AHEAD; ++w) k[w] = *(lat_cu4)(kr ^ (32 * w));
+      scale = *(const __attribute__((address_space(3))) float*)(stage + L::SCALE + 4 * k_row);
+    };
+    auto scores = [&](uint32_t stage) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sv[e] = srv[e] = 0.0f;
-    const uint32_t kr = stage + k_off, rr = stage + r_off;
+      for (int e = 0; e < 16; ++e) sv[e] = srv[e] = 0.0f;
+      const uint32_t kr = stage + k_off, rr = stage + r_off;
 #pragma unroll
-    for (int w = 0; w < KW; ++w) {
-      if (w + AHEAD < KW)
-        k[w + AHEAD] = *(lat_cu4)(kr ^ (32 * (w + AHEAD)));
-      else if (w + AHEAD - KW < RS)
-        kp[w + AHEAD - KW] = *(lat_cu4)(rr ^ (32 * (w + AHEAD - KW)));
-      sv = mfma32(code_op8<T>(k[w][0], k[w][1]), q[2 * w], sv, T{});
-      sv = mfma32(code_op8<T>(k[w][2], k[w][3]), q[2 * w + 1], sv, T{});
-      if (w == KW / 2) row_values(scale);
+      for (int w = 0; w < KW; ++w) {
+        if (w + AHEAD < KW)
+          k[w + AHEAD] = *(lat_cu4)(kr ^ (32 * (w + AHEAD)));
+        else if (w + AHEAD - KW < RS)
+          kp[w + AHEAD - KW] = *(lat_cu4)(rr ^ (32 * (w + AHEAD - KW)));
+        sv = mfma32(code_op8<T>(k[w][0], k[w][1]), q[2 * w], sv, T{});
+        sv = mfma32(code_op8<T>(k[w][2], k[w][3]), q[2 * w + 1], sv, T{});
+        if (w == KW / 2) row_values(scale);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sq[i] = row4(0, i);
+        lv[i] = row4(1, i);
+      }
       __builtin_amdgcn_sched_barrier(0);
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sq[i] = row4(0, i);
-      lv[i] = row4(1, i);
-    }
-    __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < RS; ++i) srv = mfma32(kp[i], qr[i], srv, T{});
+    };
+    // (In one run of instructions with the products: behind a branch the compiler has not always
+    // kept the distance that their results need.)
+    auto weigh = [&](float mine, char* to) {
+      top = -INFINITY;
+      l_stage = 0.0f;
 #pragma unroll
-    for (int i = 0; i < RS; ++i) srv = mfma32(kp[i], qr[i], srv, T{});
-  };
-  auto weigh = [&](float mine, char* to) {
-    top = -INFINITY;
-    l_stage = 0.0f;
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float& x = t[4 * i + e];
-        x = __builtin_fmaf(sv[4 * i + e], sq[i][e],
-                           __builtin_fmaf(srv[4 * i + e], qscale, lv[i][e] - mine));
-        top = fmaxf(top, x);
+        for (int e = 0; e < 4; ++e) {
+          float& x = t[4 * i + e];
+          x = __builtin_fmaf(sv[4 * i + e], sq[i][e],
+                             __builtin_fmaf(srv[4 * i + e], qscale, lv[i][e] - mine));
+          top = fmaxf(top, x);
+        }
+        iv[i] = row4(2, i);
       }
-      iv[i] = row4(2, i);
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float pv[4];
+      for (int i = 0; i < 4; ++i) {
+        float pv[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pv[e] = __builtin_amdgcn_exp2f(t[4 * i + e]);
-        l_stage = __builtin_fmaf(pv[e], iv[i][e], l_stage);
+        for (int e = 0; e < 4; ++e) {
+          pv[e] = __builtin_amdgcn_exp2f(t[4 * i + e]);
+          l_stage = __builtin_fmaf(pv[e], iv[i][e], l_stage);
+        }
+        *reinterpret_cast<uint2*>(to + 16 * i) =
+            make_uint2(pack_pair(pv[0], pv[1], f16{}), pack_pair(pv[2], pv[3], f16{}));
       }
-      *reinterpret_cast<uint2*>(to + 16 * i) =
-          make_uint2(pack_pair(pv[0], pv[1], f16{}), pack_pair(pv[2], pv[3], f16{}));
-    }
-  };
-  // masks, and whether a maximum has outgrown its offset
-  auto settle = [&](int st, float mine, char* to) {
-    const bool edge = is_edge(st);
-    odds = __any(odds);
-    if (edge || odds) weigh_again(st, edge, mine, mine, to);
-    const bool grown = __any(top > (m == kNone ? -0x1p126f : kRaise + kOutgrow));
-    if (lane == 0) flags[st % 2 * 4 + w4] = grown;
-  };
-  auto offset = [&]() { return m == kNone ? 0.0f : m; };  // nothing seen: from zero
+    };
+    // masks, and whether a maximum has outgrown its offset
+    auto settle = [&](int st, float mine, char* to) {
+      const bool edge = is_edge(st);
+      odds = __any(odds);
+      if (edge || odds) weigh_again(st, edge, mine, mine, to);
+      const bool grown = __any(top > (m == kNone ? -0x1p126f : kRaise + kOutgrow));
+      if (lane == 0) flags[st % 2 * 4 + w4] = grown;
+    };
+    auto offset = [&]() { return m == kNone ? 0.0f : m; };  // nothing seen: from zero
 
-  lds_barrier();  // the first stage
-  {
-    scores_ahead(stage_at(0));
-    scores(stage_at(0));
-    char* const to = p_write + s0 % 2 * L::PBUF;
-    weigh(0.0f, to);
-    settle(s0, 0.0f, to);
-  }
-  int at = 0;  // the stage's place in the ring
-  for (int st = s0; st < s1; ++st) {
-    lds_barrier();  // the weights are there, and the next stage
-    const int next = st + 1 < s1 ? stage_after(at) : at;
-    scores_ahead(stage_at(next));
-    if (outgrown(st)) {
-      const float was = offset(), mx = max_halves(top) + was;
-      if (g == 0) smax[2 * (32 * ch + n) + ph] = mx;
-      lds_barrier();
-      const float m_new = moved(ch, m);
-      l *= __builtin_amdgcn_exp2f(m - m_new);
-      m = m_new;
-      weigh_again(st, is_edge(st), was, offset(), p_write + st % 2 * L::PBUF);
-      lds_barrier();
+    lds_barrier();  // the first stage
+    {
+      scores_ahead(stage_at(0));
+      scores(stage_at(0));
+      char* const to = p_write + s0 % 2 * L::PBUF;
+      weigh(0.0f, to);
+      settle(s0, 0.0f, to);
     }
-    l += l_stage;
-    if (is_edge(st)) lds_barrier();  // NaN codes are out of the values
-    if (st + 1 < s1) {
-      scores(stage_at(next));
-      char* const to = p_write + (st + 1) % 2 * L::PBUF;
-      const float mine = offset();
-      weigh(mine, to);
-      settle(st + 1, mine, to);
+    int at = 0;  // the stage's place in the ring
+    for (int st = s0; st < s1; ++st) {
+      lds_barrier();  // the weights are there, and the next stage
+      const int next = st + 1 < s1 ? stage_after(at) : at;
+      scores_ahead(stage_at(next));
+      if (outgrown(st)) {
+        const float was = offset(), mx = max_halves(top) + was;
+        if (g == 0) smax[2 * (32 * ch + n) + ph] = mx;
+        lds_barrier();
+        const float m_new = moved(ch, m);
+        l *= __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        weigh_again(st, is_edge(st), was, offset(), p_write + st % 2 * L::PBUF);
+        lds_barrier();
+      }
+      l += l_stage;
+      if (is_edge(st)) lds_barrier();  // NaN codes are out of the values
+      if (st + 1 < s1) {
+        scores(stage_at(next));
+        char* const to = p_write + (st + 1) % 2 * L::PBUF;
+        const float mine = offset();
+        weigh(mine, to);
+        settle(st + 1, mine, to);
+      }
+      at = next;
     }
-    at = next;
-  }
-  lds_barrier();  // the maxima's place is read
-  const float sum = sum_halves(l);
-  if (g == 0) smax[2 * (32 * ch + n) + ph] = sum;
-  lds_barrier();
-  return;
+    lds_barrier();  // the maxima's place is read
+    const float sum = sum_halves(l);
+    if (g == 0) smax[2 * (32 * ch + n) + ph] = sum;
+    lds_barrier();
+    return;
   }
 
   // ---- values ----

@@ -510,16 +510,26 @@ __device__ __forceinline__ void store_blocks(const Step& s) {
   int h = static_cast<int>(blockIdx.x - rest * s.per_token.d);
   const int side = h >= s.kvh ? 1 : 0;
   h -= side * s.kvh;
-  const int64_t c0 = static_cast<int64_t>(rest) * s.chunk, t = c0 + (threadIdx.x & 63);
-  bool start = false;
-  if (static_cast<int>(threadIdx.x & 63) < s.chunk && t < s.tokens) {
-    const int64_t x = live_slot(s, t);
-    if (x >= 0) {
-      int64_t before = -1;  // slot of the last token before it that is stored
-      for (int64_t p = t - 1; p >= 0 && before < 0; --p) before = live_slot(s, p);
-      start = before < 0 || block_of(s, before) != block_of(s, x);
-    }
+  const int64_t c0 = static_cast<int64_t>(rest) * s.chunk;
+  const int lane = threadIdx.x & 63;
+  const int64_t x = lane < s.chunk && c0 + lane < s.tokens ? live_slot(s, c0 + lane) : -1;
+  const int64_t block = x < 0 ? -1 : block_of(s, x);
+  // the block of the last token before it that is stored, among these or before them
+  const uint64_t lives = __builtin_amdgcn_ballot_w64(x >= 0);
+  if (!lives) return;
+  const uint64_t below = lives & ((1ull << lane) - 1);
+  int64_t before = __shfl(block, below ? 63 - __builtin_clzll(below) : lane, 64);
+  if (!below) before = -1;
+  for (int64_t end = c0; end > 0; end -= 64) {
+    const int64_t p = end - 1 - lane;
+    const int64_t y = p < 0 ? -1 : live_slot(s, p);
+    const uint64_t found = __builtin_amdgcn_ballot_w64(y >= 0);
+    if (!found) continue;
+    const int64_t last = __shfl(y, __builtin_ctzll(found), 64);
+    if (!below) before = block_of(s, last);
+    break;
   }
+  const bool start = x >= 0 && before != block;
   uint64_t starts = __builtin_amdgcn_ballot_w64(start);
   while (starts) {  // the same in every wave
     store_run<T, FAST, MODE>(s, c0 + __builtin_ctzll(starts), side, h, red);
