@@ -257,6 +257,19 @@ def test_latent_store_refuses(kw, match):
     _refused(fp8_latent_store, _latent(), kw, match)
 
 
+def test_rows_that_share_elements_are_seen():
+    from vllm_ascend_quantized_kv_cache.ops.fp8_latent import _apart
+
+    x = torch.zeros(5, 4, 48)
+    for t in (x, x[..., 32:], x.transpose(0, 1), x[::2, 1:3], x[:1], x[:, :1, 8:24],
+              x[:1].expand(1, 4, 48), x[:, :1].transpose(0, 1), torch.zeros(1, 1, 8)):
+        assert _apart(t), (t.shape, t.stride())
+    for t in (x[:1].expand(5, 4, 48), x[:, :1].expand(5, 4, 48), x[..., ::2],
+              x.flatten().as_strided((5, 4, 48), (16, 240, 1)),
+              x.flatten().as_strided((2, 4, 48), (100, 48, 1))):
+        assert not _apart(t), (t.shape, t.stride())
+
+
 def _latents():
     c = ref.Latents([40, 17], 32, 16, 16, BF16)
     return dict(query=torch.zeros(4, 4, 48, dtype=BF16), data=c.data, scale=c.scale, rope=c.rope,

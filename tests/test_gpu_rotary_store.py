@@ -343,6 +343,29 @@ def test_latent_store(gpu_device, tokens, heads, rank, dims, inter, dtype, shift
     assert (rope.view(-1, dims)[rest] == 4.0).all()
 
 
+def test_latent_out_query(gpu_device):
+    """Heads first, in place, rows of two tensors' memory; rows that share elements are refused."""
+    dev, tokens, heads, dims = gpu_device, 6, 3, 16
+    g = torch.Generator().manual_seed(18)
+    latent, part, q = (torch.randn(shape, generator=g).to(BF16).to(dev) for shape in (
+        (tokens, 32), (tokens, dims), (tokens, heads, dims)))
+    cache = (torch.zeros(1, 16, 32, dtype=torch.uint8, device=dev), torch.zeros(1, 16, 1, device=dev),
+             torch.zeros(1, 16, dims, dtype=BF16, device=dev))
+    at = torch.arange(tokens, device=dev)
+    args = (latent, part, at, ref.table(tokens, dims).to(dev), at, *cache)
+    want = fp8_latent_store(*args, query=q)
+    first = torch.zeros(heads, tokens, dims, dtype=BF16, device=dev).transpose(0, 1)
+    assert fp8_latent_store(*args, query=q, out_query=first) is first and torch.equal(first, want)
+    shared = torch.zeros(tokens, 1, dims, dtype=BF16, device=dev).expand(tokens, heads, dims)
+    with pytest.raises(RuntimeError):
+        fp8_latent_store(*args, query=q, out_query=shared)
+    buf = torch.zeros(tokens, heads, dims + 8, dtype=BF16, device=dev)
+    buf[..., :dims] = q
+    fp8_latent_store(*args, query=buf[..., :dims], out_query=buf[..., 8:])
+    assert torch.equal(buf[..., 8:], want)
+    assert fp8_latent_store(*args, query=q, out_query=q) is q and torch.equal(q, want)
+
+
 @pytest.mark.parametrize("which", ["token", "block", "latent"])
 def test_captured_and_replayed(gpu_device, which):
     """The slots and positions are the device's: a replay takes what they hold then."""

@@ -64,6 +64,15 @@ def _strides(t: torch.Tensor) -> tuple[int, int]:
     return t.stride(0), t.stride(1)
 
 
+def _apart(t: torch.Tensor) -> bool:
+    """Whether the rows of [tokens, heads, dims] are runs that share no element."""
+    (tokens, heads, dims), (token, head, dim) = t.shape, t.stride()
+    if dim != 1 or min(token if tokens > 1 else dims, head if heads > 1 else dims) < dims:
+        return False
+    (n, near), (m, far) = sorted(((tokens, token), (heads, head)), key=lambda x: x[1])
+    return n == 1 or m == 1 or far >= (n - 1) * near + dims
+
+
 def fp8_latent_store(
     latent: torch.Tensor,
     part: torch.Tensor,
@@ -123,7 +132,7 @@ def fp8_latent_store(
     q = target = None
     if query is not None:
         q = query if query.stride(2) == 1 else query.contiguous()
-        fits = out_query is not None and out_query.stride(2) == 1 and (
+        fits = out_query is not None and _apart(out_query) and (
             _same_view(out_query, query)
             or all(_storage(out_query) != _storage(t) for t in (query, latent, part)))
         target = out_query if fits else torch.empty(query.shape, dtype=query.dtype,
