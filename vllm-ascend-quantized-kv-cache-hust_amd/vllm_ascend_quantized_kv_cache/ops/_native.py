@@ -209,6 +209,7 @@ def lib() -> ctypes.CDLL:
 
 
 _DTYPE_CODES: dict = {}
+_INDEX_CODES: dict = {}
 
 
 def dtype_code(dtype) -> int:
@@ -225,13 +226,16 @@ def dtype_code(dtype) -> int:
 
 
 def index_code(dtype) -> int:
+    code = _INDEX_CODES.get(dtype)
+    if code is not None:
+        return code
     import torch
 
-    if dtype == torch.int32:
-        return 0
-    if dtype == torch.int64:
-        return 1
-    raise RuntimeError(f"index tensors must be int32/int64, got {dtype}")
+    codes = {torch.int32: 0, torch.int64: 1}
+    if dtype not in codes:
+        raise RuntimeError(f"index tensors must be int32/int64, got {dtype}")
+    _INDEX_CODES[dtype] = codes[dtype]
+    return codes[dtype]
 
 
 def ptr(t) -> int | None:

@@ -56,12 +56,13 @@ def _check_cache(what: str, k_data, k_scale, v_data, v_scale):
     if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
         raise RuntimeError(
             f"{what}: scale caches must be float32, got {k_scale.dtype} and {v_scale.dtype}.")
+    device = k_data.device
     for name, t in (("key data", k_data), ("key scale", k_scale), ("value data", v_data),
                     ("value scale", v_scale)):
         if not t.is_contiguous():
             raise RuntimeError(f"{what}: {name} must be contiguous.")
-        if t.device != k_data.device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, key data on {k_data.device}.")
+        if t.device != device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, key data on {device}.")
     return nb, bs, kvh, d, bs // scales[1], _CODES[dtype]
 
 

@@ -28,22 +28,23 @@ def _check_rotation(what: str, positions, cos_sin, interleaved, tokens: int, wid
     if positions.shape != (tokens,):
         raise RuntimeError(
             f"{what}: positions must be 1D of {tokens} tokens, got {tuple(positions.shape)}.")
-    if cos_sin.dim() != 2 or cos_sin.shape[0] == 0 or not cos_sin.is_contiguous():
+    shape = cos_sin.shape
+    if len(shape) != 2 or shape[0] == 0 or not cos_sin.is_contiguous():
         raise RuntimeError(
-            f"{what}: cos_sin must be contiguous [positions, rotated dims], got "
-            f"{tuple(cos_sin.shape)}.")
-    rot = cos_sin.shape[1]
+            f"{what}: cos_sin must be contiguous [positions, rotated dims], got {tuple(shape)}.")
+    rot = shape[1]
     if rot == 0 or rot % 2 or rot > width:
         raise RuntimeError(f"{what}: cos_sin rotates {rot} dims of {width}; an even number of them.")
     _check_devices(what, like, positions=positions, cos_sin=cos_sin)
     return (_native.index_code(positions.dtype), _native.dtype_code(cos_sin.dtype),
-            cos_sin.shape[0], rot)
+            shape[0], rot)
 
 
 def _check_devices(what: str, like, **tensors) -> None:
+    device = like.device
     for name, t in tensors.items():
-        if t.device != like.device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, the rows on {like.device}.")
+        if t.device != device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, the rows on {device}.")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -69,13 +70,18 @@ def _storage(t: torch.Tensor) -> int:
 
 
 def _check_query(what: str, query, out_query, tokens: int, width: int, like) -> None:
-    for name, t in (("query", query), ("out_query", query if out_query is None else out_query)):
-        if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != width or t.shape[1] == 0:
+    dtype, device = like.dtype, like.device
+    for name, t in (("query", query), ("out_query", out_query)):
+        if t is None:
+            continue
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != width or shape[1] == 0:
             raise RuntimeError(
-                f"{what}: {name} must be [{tokens}, heads, {width}], got {tuple(t.shape)}.")
-        if t.dtype != like.dtype:
-            raise RuntimeError(f"{what}: {name} is {t.dtype}, the rows are {like.dtype}.")
-        _check_devices(what, like, **{name: t})
+                f"{what}: {name} must be [{tokens}, heads, {width}], got {tuple(shape)}.")
+        if t.dtype != dtype:
+            raise RuntimeError(f"{what}: {name} is {t.dtype}, the rows are {dtype}.")
+        if t.device != device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, the rows on {device}.")
     if out_query is not None and out_query.shape != query.shape:
         raise RuntimeError(
             f"{what}: out_query {tuple(out_query.shape)} does not match query {tuple(query.shape)}.")
