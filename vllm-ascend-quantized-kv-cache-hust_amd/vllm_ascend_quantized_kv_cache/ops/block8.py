@@ -129,18 +129,19 @@ def block8_store(
     if tokens == 0:
         return query if out_query is None else out_query
     _native.require_gpu_tensors(_STORE, key)
-    k, v = _rows(key), _rows(value)
-    q = target = None
+    k, k_stride = _rows(key)
+    v, v_stride = _rows(value)
+    q, q_stride, target = None, 0, None
     if query is not None:
-        q = _rows(query)
+        q, q_stride = _rows(query)
         target = _target(query, out_query, (key, value))
     slots = slot_mapping.contiguous()
     places = None if positions is None else positions.contiguous()
     with _on_device(k_data):
         rc = _native.lib().kvq_block8_store(
-            _native.ptr(q), 0 if q is None else _token_stride(q), _native.ptr(target),
-            0 if q is None else _token_stride(target), k.data_ptr(), _token_stride(k), v.data_ptr(),
-            _token_stride(v), dtype, _native.ptr(places), pos_type, _native.ptr(cos_sin), table_type,
+            _native.ptr(q), q_stride, _native.ptr(target),
+            0 if q is None else _token_stride(target), k.data_ptr(), k_stride, v.data_ptr(),
+            v_stride, dtype, _native.ptr(places), pos_type, _native.ptr(cos_sin), table_type,
             table_rows, rot, 1 if interleaved else 0, slots.data_ptr(), slot_type, tokens,
             0 if q is None else q.shape[1], kvh, d, codes, k_data.data_ptr(), k_scale.data_ptr(),
             v_data.data_ptr(), v_scale.data_ptr(), nb, bs, group, _native.stream_of(k_data),
@@ -228,7 +229,7 @@ def block8_attention(
         and out.untyped_storage().data_ptr() != query.untyped_storage().data_ptr())
     if rows:
         _native.require_gpu_tensors(_ATTENTION, query, k_data)
-    q = _rows(query)
+    q, q_stride = _rows(query)
     result = out if out is not None and direct else torch.empty(
         query.shape, dtype=q.dtype, device=q.device)
     if rows < tokens and out is None:
@@ -242,7 +243,7 @@ def block8_attention(
         _native.check(nbytes if nbytes < 0 else 0, "kvq_block8_attn_workspace_bytes")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib.kvq_block8_attn(
-            q.data_ptr(), dtype, _token_stride(q), lens, news, batch, hq, kvh, d, scale, win, sinks,
+            q.data_ptr(), dtype, q_stride, lens, news, batch, hq, kvh, d, scale, win, sinks,
             codes, k_data.data_ptr(), k_scale.data_ptr(), v_data.data_ptr(), v_scale.data_ptr(), nb,
             bs, group, table.data_ptr(), _native.index_code(table.dtype), width, _native.ptr(ws),
             nbytes, result.data_ptr(), _native.stream_of(k_data),

@@ -24,7 +24,6 @@ from .fp8_rotary import (
     _rows,
     _same_view,
     _storage,
-    _token_stride,
 )
 from .fp8_window import _lengths, _on_device
 
@@ -223,7 +222,7 @@ def fp8_latent_attention(
                              and _storage(out) != _storage(query))
     if rows:
         _native.require_gpu_tensors(_ATTENTION, query, data)
-    q = _rows(query)
+    q, q_stride = _rows(query)
     result = out if out is not None and direct else torch.empty(
         shape, dtype=q.dtype, device=q.device)
     if rows < tokens and out is None:
@@ -237,7 +236,7 @@ def fp8_latent_attention(
         _native.check(nbytes if nbytes < 0 else 0, "kvq_fp8_latent_attn_workspace_bytes")
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib.kvq_fp8_latent_attn(
-            q.data_ptr(), dtype, _token_stride(q), lens, news, batch, heads, rank, dims,
+            q.data_ptr(), dtype, q_stride, lens, news, batch, heads, rank, dims,
             softmax_scale, data.data_ptr(), scale.data_ptr(), rope.data_ptr(), nb, bs,
             table.data_ptr(), _native.index_code(table.dtype), table.shape[1], _native.ptr(ws),
             nbytes, result.data_ptr(), _native.stream_of(data),

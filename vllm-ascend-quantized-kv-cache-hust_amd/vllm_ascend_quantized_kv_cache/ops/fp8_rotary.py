@@ -47,14 +47,15 @@ def _check_devices(what: str, like, **tensors) -> None:
             raise RuntimeError(f"{what}: {name} is on {t.device}, the rows on {device}.")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [tokens, heads, dims] with its heads and dims in one run, copied if need be."""
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` [tokens, heads, dims] with its heads and dims in one run, copied if need be, and the
+    stride of its tokens."""
     tokens, heads, dims = t.shape
-    strides = t.stride()
-    if strides[2] != 1 or (heads > 1 and strides[1] != dims) or (
-            tokens > 1 and strides[0] < heads * dims):
-        return t.contiguous()
-    return t
+    token, head, dim = t.stride()
+    run = heads * dims
+    if dim != 1 or (heads > 1 and head != dims) or (tokens > 1 and token < run):
+        return t.contiguous(), run
+    return t, token if tokens > 1 else run
 
 
 def _token_stride(t: torch.Tensor) -> int:
@@ -152,17 +153,18 @@ def fp8_per_token_head_rotary_store(
             return query if out_query is None else out_query
         raise RuntimeError(f"{_STORE}: keys and values have no heads.")
     _native.require_gpu_tensors(_STORE, key)
-    k, v = _rows(key), _rows(value)
-    q = target = None
+    k, k_stride = _rows(key)
+    v, v_stride = _rows(value)
+    q, q_stride, target = None, 0, None
     if query is not None:
-        q = _rows(query)
+        q, q_stride = _rows(query)
         target = _target(query, out_query, (key, value))
     slots, places = slot_mapping.contiguous(), positions.contiguous()
     with _on_device(k_data):
         rc = _native.lib().kvq_fp8_pth_rotary_store(
-            _native.ptr(q), 0 if q is None else _token_stride(q), _native.ptr(target),
-            0 if q is None else _token_stride(target), k.data_ptr(), _token_stride(k), v.data_ptr(),
-            _token_stride(v), dtype, places.data_ptr(), pos_type, cos_sin.data_ptr(), table_type,
+            _native.ptr(q), q_stride, _native.ptr(target),
+            0 if q is None else _token_stride(target), k.data_ptr(), k_stride, v.data_ptr(),
+            v_stride, dtype, places.data_ptr(), pos_type, cos_sin.data_ptr(), table_type,
             table_rows, rot, 1 if interleaved else 0, slots.data_ptr(),
             _native.index_code(slots.dtype), tokens, 0 if q is None else q.shape[1], kvh, d,
             k_data.data_ptr(), k_scale.data_ptr(), v_data.data_ptr(), v_scale.data_ptr(),
