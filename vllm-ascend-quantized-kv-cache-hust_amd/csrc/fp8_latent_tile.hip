@@ -13,8 +13,8 @@
 //   four form scores, wave (p, c) of positions 32 p .. and columns 32 c .. of the NEXT stage:
 //     S^T = C * Q^T in products of 32 x 32 x 16; A = codes in the query's type, exact, lane
 //     (n, g) dims 32 w + 16 g .. of position n; B = the queries, all R + P dims of its columns
-//     in registers (144 of them).  Then t = (S s_j + S_r) scale log2(e) + log2(s_j) - m, S_r
-//     the position parts' product and m the column's offset, and p' = 2^t = p s_j, within
+//     in registers (144 of them).  Then t = (S s_j + S_r) scale log2(e) + log2(s_j), S_r the
+//     position parts' product, and with m the column's offset p' = 2^(t - m) = p s_j, within
 //     fp16's range whatever the scales are, goes through LDS to the others.
 //   four sum values, R / 4 dims of all 64 columns each: O^T += C^T * p'^T; A = codes in fp16,
 //     exact, by the transposing reads of bytes (16 lanes read 8 rows of 16 bytes, lane s gets
@@ -22,7 +22,9 @@
 // m moves only when some column's maximum outgrows it by kOutgrow, which all waves learn with
 // the weights and then settle together; it leaves the largest p' between 2^7 and 2^15, so p' is
 // rounded by 2^-11 of itself, or, where fp16 is subnormal, by 2^-32 of the column's largest.
-// The sum takes p' / s_j in fp32 before that rounding.
+// The sum takes p' / s_j in fp32 before that rounding.  t is rounded before m is taken off: m
+// then follows from scores as they are compared, and t - m stays under 16 also where scores
+// have steps of 16 and more (the largest p' is 1 there).
 // 16-byte chunk c of row t lies at c ^ t % 16, a position part's at c ^ t % 8, so that the rows
 // of an operand are in different banks.
 //
@@ -249,8 +251,8 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
     char* const p_write = lds + L::P + (32 * ch + n) * L::PROW + 2 * (32 * ph + 4 * g);
     float* const rows = reinterpret_cast<float*>(lds + L::ROWS) + w4 * 128;
     const uint32_t rows_lds = win_lds(rows);
-    // of the stage whose weights come next: scores over the column's offset in the log2
-    // domain, their largest, and the sum
+    // of the stage whose weights come next: scores in the log2 domain, their largest, and the
+    // sum
     float t[16], top, l_stage = 0.0f;
     bool odds = false;  // scales that the store does not write
     // the rows' constants, by way of the wave's own place
@@ -267,7 +269,7 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
       return *(lat_cf4)(rows_lds + 128 * which + 32 * i + 16 * g);
     };
     // all weights again, where there are masks, odd scales or another offset
-    auto weigh_again = [&](int st, bool edge, float was, float now, char* to) {
+    auto weigh_again = [&](int st, bool edge, char* to) {
       const int rel = (edge ? col_at(ch).pos : 0x7fffffff) - (edge ? st * kStage + 32 * ph + 4 * g : 0);
       l_stage = 0.0f;
       top = -INFINITY;
@@ -281,9 +283,9 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
         for (int e = 0; e < 4; ++e) {
           const bool on = 8 * i + e <= rel;
           float& x = t[4 * i + e];
-          x = on ? x + (was - now) : -INFINITY;
+          x = on ? x : -INFINITY;
           top = fmaxf(top, x);
-          pv[e] = __builtin_amdgcn_exp2f(x);
+          pv[e] = __builtin_amdgcn_exp2f(x - m);
           l_stage = __builtin_fmaf(pv[e], iv[e], l_stage);
           pv[e] = on ? pv[e] * sign[e] : 0.0f;
         }
@@ -327,7 +329,7 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
     };
     // (In one run of instructions with the products: behind a branch the compiler has not always
     // kept the distance that their results need.)
-    auto weigh = [&](float mine, char* to) {
+    auto weigh = [&](char* to) {
       top = -INFINITY;
       l_stage = 0.0f;
 #pragma unroll
@@ -336,7 +338,7 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
         for (int e = 0; e < 4; ++e) {
           float& x = t[4 * i + e];
           x = __builtin_fmaf(sv[4 * i + e], sq[i][e],
-                             __builtin_fmaf(srv[4 * i + e], qscale, lv[i][e] - mine));
+                             __builtin_fmaf(srv[4 * i + e], qscale, lv[i][e]));
           top = fmaxf(top, x);
         }
         iv[i] = row4(2, i);
@@ -346,7 +348,7 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
         float pv[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pv[e] = __builtin_amdgcn_exp2f(t[4 * i + e]);
+          pv[e] = __builtin_amdgcn_exp2f(t[4 * i + e] - m);
           l_stage = __builtin_fmaf(pv[e], iv[i][e], l_stage);
         }
         *reinterpret_cast<uint2*>(to + 16 * i) =
@@ -354,22 +356,21 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
       }
     };
     // masks, and whether a maximum has outgrown its offset
-    auto settle = [&](int st, float mine, char* to) {
+    auto settle = [&](int st, char* to) {
       const bool edge = is_edge(st);
       odds = __any(odds);
-      if (edge || odds) weigh_again(st, edge, mine, mine, to);
-      const bool grown = __any(top > (m == kNone ? -0x1p126f : kRaise + kOutgrow));
+      if (edge || odds) weigh_again(st, edge, to);
+      const bool grown = __any(top - m > kRaise + kOutgrow);
       if (lane == 0) flags[st % 2 * 4 + w4] = grown;
     };
-    auto offset = [&]() { return m == kNone ? 0.0f : m; };  // nothing seen: from zero
 
     lds_barrier();  // the first stage
     {
       scores_ahead(stage_at(0));
       scores(stage_at(0));
       char* const to = p_write + s0 % 2 * L::PBUF;
-      weigh(0.0f, to);
-      settle(s0, 0.0f, to);
+      weigh(to);
+      settle(s0, to);
     }
     int at = 0;  // the stage's place in the ring
     for (int st = s0; st < s1; ++st) {
@@ -377,13 +378,13 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
       const int next = st + 1 < s1 ? stage_after(at) : at;
       scores_ahead(stage_at(next));
       if (outgrown(st)) {
-        const float was = offset(), mx = max_halves(top) + was;
+        const float mx = max_halves(top);
         if (g == 0) smax[2 * (32 * ch + n) + ph] = mx;
         lds_barrier();
         const float m_new = moved(ch, m);
         l *= __builtin_amdgcn_exp2f(m - m_new);
         m = m_new;
-        weigh_again(st, is_edge(st), was, offset(), p_write + st % 2 * L::PBUF);
+        weigh_again(st, is_edge(st), p_write + st % 2 * L::PBUF);
         lds_barrier();
       }
       l += l_stage;
@@ -391,9 +392,8 @@ latent_tile_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query
       if (st + 1 < s1) {
         scores(stage_at(next));
         char* const to = p_write + (st + 1) % 2 * L::PBUF;
-        const float mine = offset();
-        weigh(mine, to);
-        settle(st + 1, mine, to);
+        weigh(to);
+        settle(st + 1, to);
       }
       at = next;
     }
