@@ -23,6 +23,7 @@ import torch
 
 from tests import _eight_bit as ref
 from tests import _fp8_window as win
+from vllm_ascend_quantized_kv_cache.ops.block8 import block8_attention
 from vllm_ascend_quantized_kv_cache.ops.fp8_latent import fp8_latent_attention
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +108,28 @@ def test_latent_rows_of_any_scores(gpu_device, size, heads):
         want, bound = ref.latent64(q, c, lens, news, scale)
         got = fp8_latent_attention(q, *c.args(), lens, news, scale, block_table_host=c.host)
         win.check_out(got, want, bound, BF16)
+
+
+@pytest.mark.parametrize("codes,dtype", [("e4m3", BF16), ("int8", BF16), ("e4m3", FP32)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("size", SIZES)
+def test_block_scales(gpu_device, size, d, codes, dtype):
+    dev, hq, kvh, bs = gpu_device, 8, 2, 64
+    for length, n in ((700, 1), (700, 41), (6000, 2)):
+        c = ref.Pages([length], kvh, d, bs, 16, codes, device=dev, seed=2)
+        for scale in c.scale:
+            scale.fill_(1.0)
+        q = _queries(n, hq, d, size, dtype, dev)
+        at = torch.from_numpy(ref.slots_of(c.host, 0, np.arange(length), bs)).to(dev)
+        for seed, pattern in enumerate(PATTERNS):
+            k = _steps(length, pattern, seed)
+            if codes == "e4m3":
+                rows = _codes(length * kvh, d, k.repeat_interleave(kvh), seed)
+            else:
+                rows = torch.zeros(length * kvh, d, dtype=torch.int8)
+                rows[:, 0], rows[:, 1] = 1, k.repeat_interleave(kvh)
+            c.data[0].view(-1, kvh, d)[at] = rows.view(length, kvh, d).to(dev)
+            _, values = c.rows(0, length)
+            want, bound = _expected(k, values.repeat_interleave(hq // kvh, 1), q, n)
+            got = block8_attention(q, *c.args(), [length], [n], LN2, block_table_host=c.host)
+            win.check_out(got, want, bound, dtype)

@@ -10,10 +10,13 @@
 //   S^T = K * Q^T: A = key codes, exact in the query's type; INT8 in fp16 times 2^-9, with
 //     bf16 queries raised by a power of two for each row into fp16's range (exact too).
 //   softmax: a group of 16 positions has one key scale and one value scale, so the scales
-//     are one fma a score, t = S ks' + log2(vs), and the running maximum of t leaves
-//     p' = 2^(t - m + 14) = p vs within fp16's range whatever the scales are: rounded by
-//     2^-11 of it, or, where fp16 is subnormal, 2^-38 of the row's largest.  The sum takes
-//     p' / vs in fp32, before that rounding.
+//     are one fma a score, t = S ks' + log2(vs), and an offset m 14 below the running maximum
+//     of t leaves p' = 2^(t - m) = p vs within fp16's range whatever the scales are: rounded
+//     by 2^-11 of it, or, where fp16 is subnormal, 2^-38 of the row's largest.  Where t has
+//     steps of 4 and more, m is what 14 below rounds to, or the maximum itself if that is
+//     more than 15 away (2^-24 of the largest then).  Tiles and parts are joined by m, which
+//     is what their sums are relative to.  The sum takes p' / vs in fp32, before that
+//     rounding.
 //   O^T += V^T * p'^T: A = value codes, exact in fp16; one product where the scales of
 //     single positions need p' in two parts.
 //
@@ -251,11 +254,10 @@ b8_decode_kernel(WinArg, int count, B8Cache c, const T* __restrict__ query, int6
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[j][x][e]);
       mx = max_rows4(mx);
-      const float m_new = fmaxf(m[x], mx);
-      const float base = m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - base);
-      // (among scores of 2^26 and more the difference rounds up: p' stays within fp16 all the same)
-      const float raised = base - kRaise, low = base - raised > kRaise + 1.0f ? base : raised;
+      const float raised = mx - kRaise;
+      const float m_new = fmaxf(m[x], mx - raised > kRaise + 1.0f ? mx : raised);
+      const float low = m_new == -INFINITY ? 0.0f : m_new;
+      const float alpha = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - low);
       m[x] = m_new;
       float sum = 0.0f;
 #pragma unroll
