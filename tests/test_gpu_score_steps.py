@@ -79,7 +79,8 @@ def _codes(rows, dims, k, seed):
     return x.to(ref.E4M3).view(torch.uint8)
 
 
-@pytest.mark.parametrize("heads,dtype", [(33, BF16), (64, BF16), (96, BF16), (3, FP32)])
+@pytest.mark.parametrize("heads,dtype", [(4, BF16), (16, BF16), (33, BF16), (64, BF16), (96, BF16),
+                                         (3, FP32)])
 @pytest.mark.parametrize("size", SIZES)
 def test_latent_rows(gpu_device, size, heads, dtype):
     dev, rank, dims, bs = gpu_device, 512, 64, 64

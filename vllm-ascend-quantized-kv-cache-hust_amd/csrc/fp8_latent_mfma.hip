@@ -10,10 +10,12 @@
 //     (g, n) holds dims R/4 g .. of position n; B = the queries, all R dims of the tile's
 //     columns in every wave's registers.  The position part beside it, from 16 KB of its own.
 //   softmax: the waves put their positions' maxima into LDS; with t = (S s_j + S_r) scale
-//     log2(e) + log2(s_j) and m its running maximum, p' = 2^(t - m + 14) = p s_j fits fp16
-//     whatever the scales are: rounded by 2^-11 of it, or, where fp16 is subnormal, 2^-38 of
-//     the row's largest; the sum takes p' / s_j in fp32 before that rounding.  p' goes
-//     through LDS to all waves.
+//     log2(e) + log2(s_j) and an offset m 14 below its running maximum, p' = 2^(t - m) = p s_j
+//     fits fp16 whatever the scales are: rounded by 2^-11 of it, or, where fp16 is subnormal,
+//     2^-38 of the row's largest; the sum takes p' / s_j in fp32 before that rounding.  Where
+//     t has steps of 4 and more, m is what 14 below rounds to, or the maximum itself if that
+//     is more than 15 away (2^-24 of the largest then).  Stages and parts are joined by m,
+//     which is what their sums are relative to.  p' goes through LDS to all waves.
 //   O^T += C^T * p'^T: wave w takes dims R/8 w ..; A = codes in fp16, exact, by the transposing
 //     reads of bytes (16 lanes read 8 rows of 16 bytes, lane s gets column s).
 //
@@ -267,12 +269,11 @@ latent_few_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query,
       const w_f4 a = y[0], z = y[1];
       const float mx = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
                              fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
-      const float m_new = fmaxf(m[x], mx);
-      const float top = m_new == -INFINITY ? 0.0f : m_new;
-      alpha[x] = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - top);
+      const float raised = mx - kRaise;
+      const float m_new = fmaxf(m[x], mx - raised > kRaise + 1.0f ? mx : raised);
+      const float from = m_new == -INFINITY ? 0.0f : m_new;
+      alpha[x] = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - from);
       m[x] = m_new;
-      // (among scores of 2^26 and more the difference rounds up: p' stays within fp16 all the same)
-      const float low = top - kRaise, from = top - low > kRaise + 1.0f ? top : low;
       float pv[4], sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
