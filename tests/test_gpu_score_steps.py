@@ -25,6 +25,7 @@ from tests import _eight_bit as ref
 from tests import _fp8_window as win
 from vllm_ascend_quantized_kv_cache.ops.block8 import block8_attention
 from vllm_ascend_quantized_kv_cache.ops.fp8_latent import fp8_latent_attention
+from vllm_ascend_quantized_kv_cache.ops.fp8_window import fp8_per_token_head_window_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -133,4 +134,26 @@ def test_block_scales(gpu_device, size, d, codes, dtype):
             _, values = c.rows(0, length)
             want, bound = _expected(k, values.repeat_interleave(hq // kvh, 1), q, n)
             got = block8_attention(q, *c.args(), [length], [n], LN2, block_table_host=c.host)
+            win.check_out(got, want, bound, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("size", SIZES)
+def test_windowed_attention(gpu_device, size, d, dtype):
+    dev, hq, kvh, bs = gpu_device, 8, 2, 64
+    for length, n in ((700, 1), (700, 41), (6000, 2), (1200, 300)):
+        c = win.Cache([length], kvh, d, bs, device=dev, seed=3)
+        c.ks.fill_(1.0)
+        c.vs.fill_(1.0)
+        q = _queries(n, hq, d, size, dtype, dev)
+        at = torch.from_numpy(c.slots(0, np.arange(length))).to(dev)
+        for seed, pattern in enumerate(PATTERNS):
+            k = _steps(length, pattern, seed)
+            rows = _codes(length * kvh, d, k.repeat_interleave(kvh), seed)
+            c.k.view(-1, kvh, d)[at] = rows.view(length, kvh, d).to(dev)
+            _, values = c.rows(0, length)
+            want, bound = _expected(k, values.repeat_interleave(hq // kvh, 1), q, n)
+            got = fp8_per_token_head_window_attention(q, *c.args(), [length], [n], LN2,
+                                                      block_table_host=c.host)
             win.check_out(got, want, bound, dtype)

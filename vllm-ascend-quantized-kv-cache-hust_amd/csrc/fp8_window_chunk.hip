@@ -393,11 +393,11 @@ win_chunk_kernel(WinArg, int count, WinCache c, const T* __restrict__ query, int
     }
     bool rescale = false;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) rescale = rescale || tmax[g] - (kRaise + kOutgrow) > m[g];
+    for (int g = 0; g < NG; ++g) rescale = rescale || tmax[g] - m[g] > kRaise + kOutgrow;
     if (__any(rescale)) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const float mn = tmax[g] - (kRaise + kOutgrow) > m[g] ? tmax[g] - kRaise : m[g];
+        const float mn = tmax[g] - m[g] > kRaise + kOutgrow ? tmax[g] - kRaise : m[g];
         const float alpha = __builtin_amdgcn_exp2f(m[g] - mn);
         l[g] *= alpha;
 #pragma unroll
