@@ -220,31 +220,23 @@ latent_few_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query,
 #pragma unroll
       for (int x = 0; x < NG; ++x) s[x] = mfma_op(k1, q[x][2 * w + 1], s[x], T{});
     }
-    w_f4 lv, iv;
-    bool odd = false;
+    // b8_value's logarithms without a branch: behind one, the compiler has not always kept the
+    // distance that a product's result needs (a scale that is not finite spoils its rows anyway)
+    w_f4 lv;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      lv[e] = __builtin_amdgcn_logf(scale[e]);
-      iv[e] = __builtin_amdgcn_rcpf(scale[e]);
-      odd = odd || !(scale[e] >= 0x1p-90f && scale[e] < INFINITY);
-    }
-    const bool odds = __any(odd);  // (none that the store writes)
-    if (odds) {
+    for (int e = 0; e < 4; ++e)
+      lv[e] = __builtin_amdgcn_logf(
+          __builtin_amdgcn_fmed3f(fabsf(scale[e]), 0x1p-90f, 0x1.fffffep127f));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const B8Value v = b8_value(scale[e]);
-        lv[e] = v.lv;
-        iv[e] = v.iv;
-      }
-    }
-    uint32_t seen[NG];
-#pragma unroll
-    for (int x = 0; x < NG; ++x) {
-      seen[x] = 0xf;
+    for (int x = 0; x < NG; ++x)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         s[x][e] = __builtin_fmaf(s[x][e], scale[e] * qscale,
                                  __builtin_fmaf(sr[x][e], qscale, lv[e]));
+    uint32_t seen[NG];
+#pragma unroll
+    for (int x = 0; x < NG; ++x) {
+      seen[x] = 0xf;
       if (edge) {
         seen[x] = 0;
         const int pos = col_at(x).pos;
@@ -262,6 +254,18 @@ latent_few_kernel(WinArg, int count, LatentCache c, const T* __restrict__ query,
     if (st + 1 < s1) issue_rope(slot);
 
     // ---- weights ----
+    w_f4 iv;
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      iv[e] = __builtin_amdgcn_rcpf(scale[e]);
+      odd = odd || !(scale[e] >= 0x1p-90f && scale[e] < INFINITY);
+    }
+    const bool odds = __any(odd);  // (none that the store writes)
+    if (odds) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) iv[e] = b8_value(scale[e]).iv;
+    }
     float alpha[NG];
 #pragma unroll
     for (int x = 0; x < NG; ++x) {
