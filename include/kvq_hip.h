@@ -580,8 +580,9 @@ int kvq_fp8_pth_rotary_store(const void* query, int64_t query_stride, void* out_
  * the old scale; where it grows, the rows before them are requantized:
  *   E4M3  s(a) = max(2^-20, the least 2^e with a <= 448 2^e), code = e4m3(y / S),
  *   INT8  s(a) = max(a / 127, 1e-6), code = rint(y / S) in +-127,
- * and code * old / S likewise.  Rows of a block behind the last new one are left alone.  No
- * counterpart in the reference. */
+ * and code * old / S likewise.  Rows of a block behind the last new one are left alone; the
+ * scale does not shrink, and a NaN stays, until a row at the block's start.  No counterpart
+ * in the reference. */
 int kvq_block8_store(const void* query, int64_t query_stride, void* out_query, int64_t out_stride,
                      const void* key, int64_t key_stride, const void* value, int64_t value_stride,
                      int dtype, const void* positions, int pos_type, const void* cos_sin,

@@ -3,8 +3,12 @@
 // query of one head of a kv head's group), 64-position blocks, bound by the matrix units and
 // the softmax beside them.
 //
-// Four chunks of 2048 rows over 10240 positions, 40 heads on 8 of 128 (1.546 TFLOP): 1620 us, 0.95 PFLOP/s; the vector units
-// are busy for 50% of it, the matrix units for 38%, one after the other in a wave.
+// Four chunks of 2048 rows over 10240 positions, 40 heads on 8 of 128 (1.546 TFLOP): 1630 us,
+// 0.95 PFLOP/s, INT8 1687; the vector units are busy for 50% of it, the matrix units for 38%:
+// a step converts and stages a block ahead of its products, and the softmax stands between
+// them, so that the two kinds of work overlap across the SIMD's two waves only.
+// (prefill_attn.hip, whose rows need no conversion and whose softmax runs beside the next
+// block's products, reaches 1.0 - 1.15.)
 //
 // As fp8_window_chunk.hip: one workgroup of four or eight waves (chk_shape) per tile, kv head
 // and segment of the tile's blocks.  Codes come from their pages into registers two blocks
@@ -29,7 +33,9 @@
 // whatever the scales are.  M moves only when a row's maximum outgrows it by 8, so a
 // row's largest p' lies between 2^7 and 2^15 (fp16 ends at 2^16): the rounding is 2^-11
 // of p' at most, or, where fp16 is subnormal, 2^-32 of the row's largest; what is
-// smaller than that counts in l alone, as l takes p' before its rounding.
+// smaller than that counts in l alone, as l takes p' before its rounding.  (fp16 results lie
+// up to 1.4 times as far off as their own rounding puts them, bf16 ones 1.01.)  Where t has
+// steps of 16 and more, M is the maximum itself.
 //
 // Positions a row does not see: weights by selection; in blocks that some row does not
 // wholly see, NaN codes of values (and rows of a scale that is not finite) are staged as

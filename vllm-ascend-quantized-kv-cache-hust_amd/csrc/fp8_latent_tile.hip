@@ -28,8 +28,11 @@
 // 16-byte chunk c of row t lies at c ^ t % 16, a position part's at c ^ t % 8, so that the rows
 // of an operand are in different banks.
 //
-// 64 requests of 1000 - 8192 positions, 256 columns, R = 512, P = 64 (157 GFLOP): 220 us; five
-// chunks of 100 - 1024 rows by 16 heads over 1111 - 6000 positions (444 GFLOP): 460 us, 0.96
+// (In 16 bits p' puts fp16 results up to 1.4 times as far off as their own rounding does, bf16
+// ones 1.01.)
+//
+// 64 requests of 1000 - 8192 positions, 256 columns, R = 512, P = 64 (157 GFLOP): 207 us; five
+// chunks of 100 - 1024 rows by 16 heads over 1111 - 6000 positions (444 GFLOP): 455 us, 0.98
 // PFLOP/s.  The tiles of 32 columns of fp8_latent_mfma.hip take 306 and 693 for them; these
 // tiles with all eight waves doing both kinds of work, half the dims of a score each, 270 and
 // 535; with four such waves of 512 registers 270 and 520.

@@ -10,7 +10,10 @@ for each head and side where ``fp8_per_token_head`` keeps 512.  The reference ha
 no counterpart.
 
 A block's rows may come in several calls (a token a step): its scale grows with
-them, and the rows that are there are requantized when it does.
+them, and the rows that are there are requantized when it does.  That costs E4M3
+codes nothing but subnormals; INT8 codes are rounded once more each time (rows of
+one size, a token a call: 1.25 times the error of one call, rms, in blocks of 16
+positions, 1.30 in blocks of 128).
 """
 
 from __future__ import annotations
@@ -96,10 +99,12 @@ def block8_store(
 
     The rows of one block are neighbours in the call and each slot is given once.
     A row written at a block's start begins it anew; rows behind the last one
-    written (a speculation taken back) stay as they were and count as gone.
+    written (a speculation taken back) stay as they were and count as gone.  What
+    they did to the scale stays: it grows only, until a row at the block's start.
     Negative slots, and slots outside the cache, are padding; so are rows whose
     position is outside the table.  A row that is not finite makes its block
-    NaN (INT8: its scale).  bf16, fp16 or fp32 rows, which may lie apart.
+    NaN (INT8: its scale), for good likewise.  bf16, fp16 or fp32 rows, which may
+    lie apart.
     """
     nb, bs, kvh, d, group, codes = _check_cache(_STORE, k_data, k_scale, v_data, v_scale)
     if key.dim() != 3 or key.shape != value.shape or key.shape[1:] != (kvh, d):
@@ -178,7 +183,9 @@ def block8_attention(
     first ``sinks``.  A row that sees nothing gives zeros.  Keys and values are
     ``code * scale`` of their block, not rounded to the query's type (value scales
     under 2^-90 may count as 0; one that is not finite leaves no finite number in
-    the rows that see its block).
+    the rows that see its block).  Sums are fp32; with bf16 and fp16 queries a
+    weight times its value's scale is rounded to fp16 once, which puts fp16 results
+    up to 1.4 times as far off as their own rounding does (bf16: 1.01).
 
     Pages that no row sees any more may be gone from the table (any id).
     ``block_table_host`` is the host's copy of the table, by which the pages are

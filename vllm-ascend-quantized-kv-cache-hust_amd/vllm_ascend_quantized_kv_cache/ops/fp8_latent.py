@@ -178,7 +178,8 @@ def fp8_latent_attention(
     absorption.  Each request's rows are its last ``query_lens[b]`` of
     ``seq_lens[b]`` cached positions (stored already); a row at position ``p`` sees
     ``j <= p``, one that sees nothing gives zeros.  Scales under 2^-90 may count as 0
-    in the values; one that is not finite makes the rows that see it NaN.
+    in the values; one that is not finite makes the rows that see it NaN.  Weights on
+    the matrix units are rounded as in ``block8_attention``.
 
     ``block_table_host`` is the host's copy of the table, by which the pages are
     checked; without it the table is copied from the device and waited for.  The
